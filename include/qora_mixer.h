@@ -5,7 +5,8 @@
  * MI355X (gfx950) with hand-written HIP kernels loaded from code objects:
  *   - Gated DeltaNet: recurrent decode step and chunked prefill;
  *   - full-attention GQA: decode step over an f16 KV cache and causal
- *     prefill that writes that cache.
+ *     prefill that writes that cache; the decode step also over a paged
+ *     4-bit KV cache, with what keeps its pages.
  * Each mixer entry replaces the middle of one reference layer-forward
  * (cited per entry).  Around the mixer the library also exports the
  * neighbouring steps of a decode or prefill layer, each a separate entry
@@ -281,6 +282,117 @@ int32_t qm_gqa_prefill(qm_context* ctx, qm_stream stream, int32_t seq_len,
                        const float* rope_sin_dev, int32_t rope_len,
                        uint16_t* k_cache_dev, uint16_t* v_cache_dev,
                        int64_t cache_capacity, uint16_t* out_dev);
+
+/* ---- paged 4-bit KV cache ---------------------------------------------- */
+/* A KV cache in 4 bits, in pages that sequences can share: no counterpart in
+ * the reference, whose cache is f32 and one per run.  It takes 1152 bytes a
+ * token and layer where the f16 cache takes 4096, so a decode step over long
+ * contexts reads 3.6 times fewer bytes, and sequences with a common prompt
+ * hold one copy of it.
+ *
+ * Values.  Per token, kv head and group of 64 dims (group 0 are the rotary
+ * dims) the f16 values x are kept as a minimum, a scale and 64 codes:
+ *   lo = min x,  s = f16(f32((max x - min x) / 15)),
+ *   q = clamp(round((x - lo) / s), 0, 15), ties to even (0 where s = 0),
+ * and stand for lo + s q: within s / 2 of x (within 15 2^-25 where that is
+ * more, s being subnormal or 0).  A group with an infinity or a NaN reads
+ * back as NaN.
+ *
+ * Pages.  A page holds QM_KV4_PAGE_TOKENS tokens of the four kv heads' K and
+ * V of one layer, QM_KV4_PAGE_BYTES; what stands where in it is the library's
+ * (qm_kv4_store / _load convert).  Row r of the table lists the pages of a
+ * sequence of lens[r] tokens in order; entries past them are ignored.  All
+ * layers share the table: page p of layer l is page l * num_pages + p of the
+ * pool.  refs counts the rows that hold a page.  A new cache has lens and
+ * refs zero (qm_memset); pages and table need no initial value.
+ *
+ * The caller keeps the buffers; qm_kv4_resize, _fork and _compact keep table,
+ * lens and refs, on the device, in stream order, so a captured step can
+ * replay without the host.  pages_dev must be 16-byte aligned, the int32
+ * arrays here and below 4-byte.  Table entries that are no page of the pool
+ * are skipped, never followed. */
+enum { QM_KV4_PAGE_TOKENS = 64, QM_KV4_PAGE_BYTES = 73728 };
+typedef struct {
+    uint8_t* pages_dev;        /* [layers][num_pages][QM_KV4_PAGE_BYTES] */
+    int32_t* table_dev;        /* [rows][max_pages] */
+    int32_t* lens_dev;         /* [rows] */
+    int32_t* refs_dev;         /* [num_pages] */
+    int32_t layers;
+    int32_t num_pages;
+    int32_t rows;              /* at most 65536 */
+    int32_t max_pages;         /* pages of a row, at most 33554431 */
+} qm_kv4_cache;
+
+/* The `count` rows rows_dev (NULL: rows 0 .. count - 1), all different, at
+ * most 1024, take the lengths lens_dev [count] (flags QM_KV4_ADD: their
+ * present lengths plus lens_dev).  A row that shrinks gives up the pages past
+ * its end; to 0 frees it.  A row that grows gets free pages, lowest ids
+ * first, in list order; if its last page is partly filled and other rows
+ * hold it too, the row gets a copy of that page (every layer's), unless all
+ * its holders grow in this call and this is the first of them.  So the
+ * tokens a row grows by are its own to write.  Pages given up in a call are
+ * free from the next call on.
+ * result_dev int32 [1]: 0; or, with nothing changed, the number of free
+ * pages lacking, or -1 where a row is out of range or listed twice, a length
+ * is negative or needs more than max_pages pages, or the table, lens and refs
+ * contradict each other. */
+enum { QM_KV4_LENS = 0, QM_KV4_ADD = 1 };
+int32_t qm_kv4_resize(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache,
+                      int32_t count, const int32_t* rows_dev, const int32_t* lens_dev,
+                      int32_t flags, int32_t* result_dev);
+
+/* Row dst_dev[i] becomes row src_dev[i] as it was before the call (i < count,
+ * at most 1024; the destinations all different, a row may be both source and
+ * destination): its own pages are given up, the source's shared, none copied
+ * (qm_kv4_resize copies the last one when a holder grows).  Sampling several
+ * answers to one prompt, beam search.  result_dev int32 [1]: 0, or -1 with
+ * nothing changed where a row is out of range or a destination listed twice. */
+int32_t qm_kv4_fork(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache,
+                    int32_t count, const int32_t* src_dev, const int32_t* dst_dev,
+                    int32_t* result_dev);
+
+/* Move the pages in use to the front of the pool (every layer's; the k-th of
+ * those past the bound to the k-th free one before it), so that pages live ..
+ * are free; table and refs follow.  live_dev int32 [1]: the pages in use. */
+int32_t qm_kv4_compact(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache,
+                       int32_t* live_dev);
+
+/* Tokens first .. first + n - 1 of the table rows row .. row + batch - 1 of a
+ * layer from f16 rows k_dev, v_dev [batch][4][capacity][256] (rows 0 .. n - 1
+ * of each head; the layout of qm_gqa_prefill's and qm_gqa_decode's caches).
+ * first_dev int32 [batch], or NULL: 0.  Tokens at or past a row's length are
+ * left out, as are sequences whose first is negative: grow the row with
+ * qm_kv4_resize first. */
+int32_t qm_kv4_store(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
+                     int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
+                     const uint16_t* k_dev, const uint16_t* v_dev, int64_t capacity);
+
+/* The other way: f16(lo + s q), the sum rounded to f32 first.  f16 rows of
+ * tokens left out stay as they were. */
+int32_t qm_kv4_load(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
+                    int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
+                    uint16_t* k_dev, uint16_t* v_dev, int64_t capacity);
+
+/* qm_gqa_decode over a layer of such a cache.  Batch row b steps table row
+ * slots_dev[b] (NULL: b); its position is lens - 1, the last of the tokens
+ * that qm_kv4_resize has grown it by: k (in 64 bits, rounded to f32 and f16)
+ * and v are written there in 4 bits, and attention reads lens tokens, the new
+ * one as it is kept.  A batch row whose slot is outside the table (-1) or
+ * whose length is 0 writes nothing and its output is 0.  One whose length is
+ * over max_len, or whose slot an earlier batch row has, writes nothing and its
+ * output is NaN.
+ * max_len  upper bound of the lengths: at most rope_len (else
+ *          QM_ERR_ROPE_RANGE) and QM_KV4_PAGE_TOKENS * max_pages
+ *          (QM_ERR_CAPACITY)
+ * result_dev  NULL, or a resize's result: where it is not 0 (the rows did not
+ *          grow) nothing is written and every output is 0
+ * q_gate_dev .. rope_len and out_dev as for qm_gqa_decode. */
+int32_t qm_gqa_decode_kv4(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache,
+                          int32_t layer, int32_t batch, const int32_t* slots_dev,
+                          const float* q_gate_dev, const float* k_new_dev, const float* v_new_dev,
+                          const uint16_t* q_norm_dev, const uint16_t* k_norm_dev,
+                          const float* rope_cos_dev, const float* rope_sin_dev, int32_t rope_len,
+                          int32_t max_len, const int32_t* result_dev, float* out_dev);
 
 /* ---- Q4 projections --------------------------------------------------- */
 /* A Q4Weight (gemv.rs:29-34, written by quantize_q4, convert.rs:437-467)

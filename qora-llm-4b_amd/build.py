@@ -32,7 +32,8 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-parameter",
 ]
 
-KERNELS = ["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample"]
+KERNELS = ["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample",
+           "kv4_cache", "gqa_decode_kv4"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -108,6 +109,13 @@ def build_dispatch_test() -> None:
           str(ROOT / "tests" / "cpp" / "dispatch_test.cpp"), "-o", str(LIB / "dispatch_test")])
 
 
+def build_kv4_test() -> None:
+    """tests/cpp/kv4_test.cpp: the 4-bit KV cache's layout and checks on the CPU
+    (g++ only, no device code; test infrastructure)."""
+    _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-I", str(ROOT / "include"), "-I", str(CSRC),
+          str(ROOT / "tests" / "cpp" / "kv4_test.cpp"), "-o", str(LIB / "kv4_test")])
+
+
 if __name__ == "__main__":
     build()
     if "--no-oracle" not in sys.argv:
@@ -116,4 +124,5 @@ if __name__ == "__main__":
         build_file_test()
         build_plan_test()
         build_dispatch_test()
+        build_kv4_test()
     print("built:", ", ".join(sorted(p.name for p in LIB.iterdir())))

@@ -1,0 +1,565 @@
+// kv4_cache.hip -- the paged 4-bit KV cache (qm_kv4.h) for gfx950: f16 rows
+// into the pages and back, and the pages themselves: growing, shrinking and
+// freeing rows, forking them, and moving the live pages together.
+#include "qm_kv4_device.h"
+
+// ---- f16 rows <-> pages ---------------------------------------------------
+// A workgroup takes half a page (32 tokens) of one sequence and head.  A
+// token's row is 32 lanes x 8 dims, so a group of 64 dims is 8 lanes and a
+// lane's 8 codes are one K word; V words hold 8 tokens of one dim, so V's
+// codes turn in LDS.
+#define KV4_ROWS_THREADS 256
+
+struct HalfAt {
+    bool some, whole;        // any / all of the half page's tokens taken
+    int lo, hi;              // tokens of the half page taken: [lo, hi)
+    int64_t src0;            // row of the f16 side of token 0
+    uint8_t* page;
+};
+QM_DEV HalfAt half_at(const Kv4RowsArgs& A, int b, int head, int tile) {
+    HalfAt h;
+    const int first = A.first ? A.first[b] : 0;
+    const int row = A.row + b;
+    const int t0 = ((first >> 5) + tile) << 5;
+    const int64_t end = min((int64_t)first + A.n, (int64_t)A.c.lens[row]);
+    h.src0 = (int64_t)t0 - first;
+    h.lo = max(0, first - t0);
+    h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, max(end - t0, (int64_t)0));
+    h.some = first >= 0 && h.lo < h.hi && (t0 >> 6) < A.c.max_pages;
+    h.whole = h.lo == 0 && h.hi == QMK_KV4_HALF_TOKENS;
+    h.page = nullptr;
+    if (h.some) {
+        const int id = A.c.table[(size_t)row * A.c.max_pages + (t0 >> 6)];
+        h.some = kv4_is_page(A.c, id);
+        if (h.some) h.page = kv4_half(A.c, A.layer, id, head, (t0 >> 5) & 1);
+    }
+    return h;
+}
+
+// Smallest / largest over the 8 lanes of a group.
+QM_DEV float min_of8(float x) {
+    x = fminf(x, dpp_f32<0xB1>(x));
+    x = fminf(x, dpp_f32<0x4E>(x));
+    return fminf(x, dpp_f32<0x141>(x));
+}
+QM_DEV float max_of8(float x) {
+    x = fmaxf(x, dpp_f32<0xB1>(x));
+    x = fmaxf(x, dpp_f32<0x4E>(x));
+    return fmaxf(x, dpp_f32<0x141>(x));
+}
+
+// Eight f16 values of a lane -> their codes in a word (element e as in
+// kv4_nibble), and the group's scale and minimum.
+struct Coded {
+    uint32_t word;
+    uint16_t s, lo;
+};
+QM_DEV Coded code8(uint4 raw) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[8];
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xffffu));
+        x[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
+        big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+    }
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+    }
+    lo = min_of8(lo);
+    hi = max_of8(hi);
+    const bool bad = max_of8(big >= 0x7c00u ? 1.0f : 0.0f) > 0.0f;     // an infinity or a NaN
+    Coded c;
+    c.s = bad ? (uint16_t)0x7e00u : kv4_scale(lo, hi);
+    c.lo = bad ? (uint16_t)0x7e00u : f32_to_f16(lo);
+    const float s = f16_to_f32(c.s), inv = s > 0.0f ? 1.0f / s : 0.0f;
+    c.word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c.word |= kv4_code(x[e], lo, s, inv) << (4 * kv4_nibble(e));
+    return c;
+}
+
+extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
+    __shared__ __attribute__((aligned(16))) uint32_t kw[1024];          // K words, in the page's order
+    __shared__ __attribute__((aligned(16))) uint32_t vt[32][33];        // V words of token t, dims 8 i ..
+    __shared__ uint16_t meta[4][128];                                   // sK, loK, sV, loV
+    const int tid = threadIdx.x;
+    const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
+    const int head = bh & 3, b = bh >> 2;
+    const HalfAt h = half_at(A, b, head, tile);
+    if (!h.some) return;
+    const int i = tid & 31;                       // dims 8 i .. 8 i + 7
+    const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = (tid >> 5) + 8 * r;
+        const bool in = t >= h.lo && t < h.hi;
+        const size_t at = (base + (size_t)(in ? h.src0 + t : h.src0 + h.lo)) * 256 + 8 * i;
+        const Coded ck = code8(*reinterpret_cast<const uint4*>(A.k + at));
+        const Coded cv = code8(*reinterpret_cast<const uint4*>(A.v + at));
+        kw[kv4_k_word(t, 8 * i)] = ck.word;
+        vt[t][i] = cv.word;
+        if ((i & 7) == 0) {
+            meta[0][kv4_s_at(t, i >> 3)] = ck.s;
+            meta[1][kv4_lo_at(t, i >> 3)] = ck.lo;
+            meta[2][kv4_s_at(t, i >> 3)] = cv.s;
+            meta[3][kv4_lo_at(t, i >> 3)] = cv.lo;
+        }
+    }
+    __syncthreads();
+    uint4* out = reinterpret_cast<uint4*>(h.page);
+    {   // K: chunk tid is four words of one token
+        const int t = (tid >> 7) * 16 + (tid & 15);
+        if (t >= h.lo && t < h.hi) out[tid] = *reinterpret_cast<const uint4*>(&kw[4 * tid]);
+    }
+    {   // V: chunk tid is dims 64 group + 16 word + c of eight tokens
+        const int group = tid >> 6, g = (tid >> 4) & 3, c = tid & 15;
+        uint32_t w[4], keep = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int t = 16 * (e >> 2) + 4 * g + (e & 3);
+            if (t < h.lo || t >= h.hi) keep |= 15u << (4 * kv4_nibble(e));
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const int d = 64 * group + 16 * m + c;
+            w[m] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int t = 16 * (e >> 2) + 4 * g + (e & 3);
+                w[m] |= ((vt[t][d >> 3] >> (4 * kv4_nibble(d & 7))) & 15u) << (4 * kv4_nibble(e));
+            }
+        }
+        uint4 old = make_uint4(0, 0, 0, 0);
+        if (keep && keep != 0xffffffffu) old = out[256 + tid];
+        if (keep != 0xffffffffu)
+            out[256 + tid] = make_uint4((w[0] & ~keep) | (old.x & keep), (w[1] & ~keep) | (old.y & keep),
+                                        (w[2] & ~keep) | (old.z & keep), (w[3] & ~keep) | (old.w & keep));
+    }
+    uint16_t* mo = reinterpret_cast<uint16_t*>(h.page + QMK_KV4_META);
+    if (h.whole) {
+        reinterpret_cast<uint32_t*>(mo)[tid] = reinterpret_cast<const uint32_t*>(&meta[0][0])[tid];
+    } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int j = tid + 256 * r, which = j >> 7, t = (j & 127) >> 2, group = j & 3;
+            if (t >= h.lo && t < h.hi) {
+                const int at = (which & 1) ? kv4_lo_at(t, group) : kv4_s_at(t, group);
+                mo[which * 128 + at] = meta[which][at];
+            }
+        }
+    }
+}
+
+QM_DEV float kv4_read(uint32_t word, int e, float s, float lo) {
+    return __builtin_fmaf((float)((word >> (4 * kv4_nibble(e))) & 15u), s, lo);
+}
+
+extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4RowsArgs A) {
+    __shared__ __attribute__((aligned(16))) uint32_t w[QMK_KV4_HALF_BYTES / 4];
+    const int tid = threadIdx.x;
+    const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
+    const int head = bh & 3, b = bh >> 2;
+    const HalfAt h = half_at(A, b, head, tile);
+    if (!h.some) return;
+    for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
+        reinterpret_cast<uint4*>(w)[j] = reinterpret_cast<const uint4*>(h.page)[j];
+    __syncthreads();
+    const uint16_t* meta = reinterpret_cast<const uint16_t*>(&w[QMK_KV4_META / 4]);
+    const int i = tid & 31, group = i >> 3;
+    const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = (tid >> 5) + 8 * r;
+        if (t < h.lo || t >= h.hi) continue;
+        const int sa = kv4_s_at(t, group), la = kv4_lo_at(t, group);
+        const float sk = f16_to_f32(meta[sa]), lk = f16_to_f32(meta[128 + la]);
+        const float sv = f16_to_f32(meta[256 + sa]), lv = f16_to_f32(meta[384 + la]);
+        const uint32_t kw = w[kv4_k_word(t, 8 * i)];
+        const int shift = 4 * kv4_v_nibble(t);
+        uint32_t ko[4], vo[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            ko[p] = (uint32_t)f32_to_f16(kv4_read(kw, 2 * p, sk, lk)) | (uint32_t)f32_to_f16(kv4_read(kw, 2 * p + 1, sk, lk)) << 16;
+            uint32_t o = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t q = (w[kv4_v_word(t, 8 * i + 2 * p + e)] >> shift) & 15u;
+                o |= (uint32_t)f32_to_f16(__builtin_fmaf((float)q, sv, lv)) << (16 * e);
+            }
+            vo[p] = o;
+        }
+        const size_t at = (base + (size_t)(h.src0 + t)) * 256 + 8 * i;
+        *reinterpret_cast<uint4*>(A.k + at) = make_uint4(ko[0], ko[1], ko[2], ko[3]);
+        *reinterpret_cast<uint4*>(A.v + at) = make_uint4(vo[0], vo[1], vo[2], vo[3]);
+    }
+}
+
+// ---- the pages ------------------------------------------------------------
+#define KV4_PLAN_THREADS 1024
+#define KV4_BLOCK_PAGES (64 * KV4_PLAN_THREADS)     // pages whose state one pass holds, 64 a thread
+#define KV4_WINDOW 4096                              // free pages handed out at a time
+
+// Exclusive sum over the workgroup's 1024 threads, and the total.
+QM_DEV uint64_t plan_scan(uint64_t x, uint64_t* sums, uint64_t& total) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    uint64_t incl = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint64_t o = __shfl_up(incl, off);
+        if (lane >= off) incl += o;
+    }
+    __syncthreads();
+    if (lane == 63) sums[w] = incl;
+    __syncthreads();
+    uint64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int j = 0; j < KV4_PLAN_THREADS / 64; ++j) {
+        if (j < w) before += sums[j];
+        total += sums[j];
+    }
+    return before + incl - x;
+}
+
+// Bit j: page block + 64 tid + j is free (reference count 0).  Ids past the
+// pool are not free.
+QM_DEV uint64_t free_pages(const Kv4Cache& c, int64_t block) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint64_t mine = 0;
+    const int64_t at = block + (int64_t)w * 4096;
+    for (int r0 = 0; r0 < 64; r0 += 16) {
+        if (at + r0 * 64 >= c.num_pages) break;
+        int v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int64_t p = at + (r0 + j) * 64 + lane;
+            v[j] = p < c.num_pages ? c.refs[p] : 1;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint64_t m = __ballot(v[j] == 0);
+            if (lane == r0 + j) mine = m;
+        }
+    }
+    return mine;
+}
+
+// 16-byte copy of a third of a page by a workgroup of 256.
+#define KV4_COPY_PARTS 3
+#define KV4_COPY_THREADS 256
+QM_DEV void copy_part(const Kv4Cache& c, int layer, int src, int dst, int part) {
+    constexpr int N = QMK_KV4_PAGE_BYTES / 16 / KV4_COPY_PARTS / KV4_COPY_THREADS;
+    static_assert(N * 16 * KV4_COPY_PARTS * KV4_COPY_THREADS == QMK_KV4_PAGE_BYTES, "a page in whole vectors");
+    const uint4* s = reinterpret_cast<const uint4*>(c.pages + ((size_t)layer * c.num_pages + src) * QMK_KV4_PAGE_BYTES);
+    uint4* d = reinterpret_cast<uint4*>(c.pages + ((size_t)layer * c.num_pages + dst) * QMK_KV4_PAGE_BYTES);
+    const int at = part * (N * KV4_COPY_THREADS) + threadIdx.x;
+    uint4 v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = s[at + j * KV4_COPY_THREADS];
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[at + j * KV4_COPY_THREADS] = v[j];
+}
+
+// Rows take new lengths (one workgroup, thread i has list row i).  A row that
+// grows gets pages for the new tokens, and its partly filled last page, if
+// other rows hold it too, is replaced by a copy: written pages have one
+// holder.  When every holder of such a page grows in this call, the first of
+// them keeps it.  Fresh pages are the lowest free ids before the call, in
+// list order.  Nothing is changed unless all of it can be.
+extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4ResizeArgs A) {
+    __shared__ uint64_t sums[KV4_PLAN_THREADS / 64];
+    __shared__ uint32_t seen[QMK_KV4_MAX_ROWS / 32];
+    __shared__ int last[QMK_KV4_MAX_COUNT];
+    __shared__ uint32_t off[QMK_KV4_MAX_COUNT];
+    __shared__ int row_of[QMK_KV4_MAX_COUNT], begin_of[QMK_KV4_MAX_COUNT];
+    __shared__ int list[KV4_WINDOW];
+    __shared__ uint32_t copies;
+    const int tid = threadIdx.x;
+    const Kv4Cache& c = A.c;
+    for (int j = tid; j < (c.rows + 31) / 32; j += KV4_PLAN_THREADS) seen[j] = 0;
+    if (tid == 0) copies = 0;
+    __syncthreads();
+
+    // the list, checked
+    const bool mine = tid < A.count;
+    int row = -1, old = 0, want = 0, page = -1, held = 0;
+    bool bad = false, grow = false;
+    if (mine) {
+        row = A.list ? A.list[tid] : tid;
+        bad = (uint32_t)row >= (uint32_t)c.rows;
+        if (!bad) {
+            const uint32_t bit = 1u << (row & 31);
+            bad = (atomicOr(&seen[row >> 5], bit) & bit) != 0;
+            old = c.lens[row];
+            const int64_t to = (int64_t)A.lens[tid] + (A.add ? old : 0);
+            const int64_t most = (int64_t)c.max_pages * QMK_KV4_PAGE_TOKENS;
+            bad = bad || old < 0 || old > most || to < 0 || to > most;
+            want = bad ? 0 : (int)to;
+            grow = !bad && want > old;
+            if (grow && (old & (QMK_KV4_PAGE_TOKENS - 1))) {
+                page = c.table[(size_t)row * c.max_pages + old / QMK_KV4_PAGE_TOKENS];
+                if (kv4_is_page(c, page)) held = c.refs[page];
+                bad = held < 1;
+            }
+        }
+    }
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) {
+            A.result[0] = -1;
+            A.state[0] = 1;
+        }
+        return;
+    }
+    last[tid] = page;
+    __syncthreads();
+    bool copy = false;
+    if (page >= 0) {
+        int growing = 0;
+        bool first = true;
+        for (int j = 0; j < A.count; ++j) {
+            const bool same = last[j] == page;
+            growing += same;
+            first = first && !(same && j < tid);
+        }
+        copy = !(growing == held && first);
+    }
+    const int had = kv4_pages_of(old), pages = kv4_pages_of(want);
+    const int begin = copy ? old / QMK_KV4_PAGE_TOKENS : had;
+    uint64_t need;
+    const uint64_t before = plan_scan(grow ? (uint64_t)(pages - begin) : 0, sums, need);
+    off[tid] = (uint32_t)min(before, (uint64_t)0xffffffffu);
+    row_of[tid] = row;
+    begin_of[tid] = copy ? ~begin : begin;             // the sign: its first fresh page is a copy
+
+    // enough free pages?
+    uint64_t mask = 0, ahead = 0, found = 0;
+    int64_t block = 0;
+    for (; block < c.num_pages && found < need; block += KV4_BLOCK_PAGES) {
+        mask = free_pages(c, block);
+        uint64_t total;
+        ahead = plan_scan((uint64_t)__popcll(mask), sums, total);
+        found += total;
+    }
+    if (found < need) {
+        if (tid == 0) {
+            A.result[0] = (int)min(need - found, (uint64_t)0x7fffffff);
+            A.state[0] = 1;
+        }
+        return;
+    }
+
+    // hand them out, KV4_WINDOW at a time
+    const bool kept = block <= KV4_BLOCK_PAGES;          // the first pass saw them all
+    int32_t* job = A.state + 4;
+    uint64_t done = 0;
+    for (int64_t blk = 0; done < need; blk += KV4_BLOCK_PAGES) {
+        uint64_t total = found;
+        if (!kept) {
+            mask = free_pages(c, blk);
+            ahead = plan_scan((uint64_t)__popcll(mask), sums, total);
+        }
+        const uint64_t take = min(total, need - done);
+        for (uint64_t w0 = 0; w0 < take; w0 += KV4_WINDOW) {
+            __syncthreads();
+            uint64_t k = ahead;
+            for (uint64_t m = mask; m && k < w0 + KV4_WINDOW; m &= m - 1, ++k)
+                if (k >= w0) list[k - w0] = (int)(blk + 64 * tid + __builtin_ctzll(m));
+            __syncthreads();
+            const int n = (int)min((uint64_t)KV4_WINDOW, take - w0);
+            for (int j = tid; j < n; j += KV4_PLAN_THREADS) {
+                const uint32_t at = (uint32_t)(done + w0 + j);
+                int lo = 0, hi = A.count;               // the last list row that begins at or before `at`
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (off[mid] <= at) lo = mid;
+                    else hi = mid;
+                }
+                const int from = begin_of[lo], index = (from < 0 ? ~from : from) + (int)(at - off[lo]);
+                const int id = list[j];
+                int32_t* entry = c.table + (size_t)row_of[lo] * c.max_pages + index;
+                if (from < 0 && at == off[lo]) {
+                    const uint32_t slot = atomicAdd(&copies, 1u);
+                    job[2 * slot] = last[lo];
+                    job[2 * slot + 1] = id;
+                }
+                *entry = id;
+                c.refs[id] = 1;
+            }
+        }
+        done += take;
+    }
+    if (copy) atomicSub(&c.refs[page], 1);
+    if (mine) {
+        c.lens[row] = want;
+        job[2 * A.count + 2 * tid] = pages;
+        job[2 * A.count + 2 * tid + 1] = had;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        A.state[0] = 0;
+        A.state[1] = (int)copies;
+        A.result[0] = 0;
+    }
+}
+
+// The second half of a resize: the pages to copy, in every layer, and the
+// references that shrunk rows give up.
+extern "C" __global__ __launch_bounds__(KV4_COPY_THREADS) void qm_kv4_resize_pages(Kv4ResizeArgs A) {
+    if (A.state[0]) return;
+    const Kv4Cache& c = A.c;
+    const int32_t* job = A.state + 4;
+    for (int i = blockIdx.x; i < A.count; i += gridDim.x) {
+        const int2 gone = *reinterpret_cast<const int2*>(job + 2 * A.count + 2 * i);
+        const int row = A.list ? A.list[i] : i;
+        for (int j = gone.x + threadIdx.x; j < gone.y; j += KV4_COPY_THREADS) {
+            const int id = c.table[(size_t)row * c.max_pages + j];
+            if (kv4_is_page(c, id)) atomicSub(&c.refs[id], 1);
+        }
+    }
+    const int64_t parts = (int64_t)A.state[1] * c.layers * KV4_COPY_PARTS;
+    for (int64_t p = blockIdx.x; p < parts; p += gridDim.x) {
+        const int part = (int)(p % KV4_COPY_PARTS);
+        const int64_t q = p / KV4_COPY_PARTS;
+        const int layer = (int)(q % c.layers), i = (int)(q / c.layers);
+        copy_part(c, layer, job[2 * i], job[2 * i + 1], part);
+    }
+}
+
+// Rows become copies of rows as they were before the call, page by page in
+// the table only: references to the new pages are counted and the new entries
+// set aside (first half), then the old ones' given up and the entries
+// written.  Workgroup i has pair i; each checks the whole list.
+extern "C" __global__ __launch_bounds__(256) void qm_kv4_fork(Kv4ForkArgs A) {
+    __shared__ uint32_t seen[QMK_KV4_MAX_ROWS / 32];
+    const int tid = threadIdx.x, i = blockIdx.x;
+    const Kv4Cache& c = A.c;
+    for (int j = tid; j < (c.rows + 31) / 32; j += 256) seen[j] = 0;
+    __syncthreads();
+    bool bad = false;
+    for (int j = tid; j < A.count; j += 256) {
+        const int src = A.src[j], dst = A.dst[j];
+        if ((uint32_t)src >= (uint32_t)c.rows || (uint32_t)dst >= (uint32_t)c.rows) {
+            bad = true;
+        } else {
+            const uint32_t bit = 1u << (dst & 31);
+            bad = bad || (atomicOr(&seen[dst >> 5], bit) & bit) != 0;
+        }
+    }
+    bad = __syncthreads_or(bad);
+    if (i == 0 && tid == 0) {
+        A.state[0] = bad;
+        A.result[0] = bad ? -1 : 0;
+    }
+    if (bad) return;
+    const int src = A.src[i], len = c.lens[src];
+    const int n = min(max(kv4_pages_of(len), 0), c.max_pages);
+    int32_t* aside = A.state + 4 + A.count + (size_t)i * c.max_pages;
+    for (int j = tid; j < n; j += 256) {
+        const int id = c.table[(size_t)src * c.max_pages + j];
+        aside[j] = id;
+        if (kv4_is_page(c, id)) atomicAdd(&c.refs[id], 1);
+    }
+    if (tid == 0) A.state[4 + i] = len;
+}
+
+extern "C" __global__ __launch_bounds__(256) void qm_kv4_fork_rows(Kv4ForkArgs A) {
+    if (A.state[0]) return;
+    const int tid = threadIdx.x, i = blockIdx.x;
+    const Kv4Cache& c = A.c;
+    const int dst = A.dst[i], len = A.state[4 + i];
+    const int n = min(max(kv4_pages_of(len), 0), c.max_pages);
+    const int had = min(max(kv4_pages_of(c.lens[dst]), 0), c.max_pages);
+    const int32_t* aside = A.state + 4 + A.count + (size_t)i * c.max_pages;
+    int32_t* row = c.table + (size_t)dst * c.max_pages;
+    for (int j = tid; j < max(n, had); j += 256) {
+        if (j < had) {
+            const int id = row[j];
+            if (kv4_is_page(c, id)) atomicSub(&c.refs[id], 1);
+        }
+        if (j < n) row[j] = aside[j];
+    }
+    __syncthreads();
+    if (tid == 0) c.lens[dst] = len;
+}
+
+// Live pages move down to [0, live): the k-th live page past that bound goes
+// to the k-th free page below it.  First the plan (one workgroup), then the
+// moves.
+extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_compact(Kv4CompactArgs A) {
+    __shared__ uint64_t sums[KV4_PLAN_THREADS / 64];
+    const int tid = threadIdx.x;
+    const Kv4Cache& c = A.c;
+    int64_t free = 0;
+    uint64_t mask = 0;
+    for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
+        mask = free_pages(c, block);
+        uint64_t total;
+        plan_scan((uint64_t)__popcll(mask), sums, total);
+        free += (int64_t)total;
+    }
+    const int64_t live = c.num_pages - free;
+    int32_t* movers = A.state + 4;
+    int32_t* holes = movers + c.num_pages;
+    int32_t* to = holes + c.num_pages;
+    uint64_t moves = 0, gaps = 0;
+    for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
+        if (c.num_pages > KV4_BLOCK_PAGES) mask = free_pages(c, block);
+        // bits of this thread's pages: in the pool, and below the bound
+        const int64_t p0 = block + 64 * tid;
+        const int in = (int)min(max(c.num_pages - p0, (int64_t)0), (int64_t)64);
+        const int low = (int)min(max(live - p0, (int64_t)0), (int64_t)64);
+        const uint64_t pool = in == 64 ? ~0ull : (1ull << in) - 1, below = low == 64 ? ~0ull : (1ull << low) - 1;
+        const uint64_t hole = mask & below, move = ~mask & pool & ~below;
+        // both counts in one scan (at most 65536 each)
+        uint64_t total;
+        const uint64_t at = plan_scan((uint64_t)__popcll(hole) << 32 | (uint64_t)__popcll(move), sums, total);
+        uint64_t k = gaps + (at >> 32);
+        for (uint64_t m = hole; m; m &= m - 1) holes[k++] = (int)(p0 + __builtin_ctzll(m));
+        k = moves + (at & 0xffffffffu);
+        for (uint64_t m = move; m; m &= m - 1) movers[k++] = (int)(p0 + __builtin_ctzll(m));
+        gaps += total >> 32;
+        moves += total & 0xffffffffu;
+    }
+    __syncthreads();
+    for (int64_t p = live + tid; p < c.num_pages; p += KV4_PLAN_THREADS) to[p] = (int)p;
+    __syncthreads();
+    for (uint64_t k = tid; k < moves; k += KV4_PLAN_THREADS) to[movers[k]] = holes[k];
+    if (tid == 0) {
+        A.state[0] = (int)live;
+        A.state[1] = (int)moves;
+        A.live[0] = (int)live;
+    }
+}
+
+extern "C" __global__ __launch_bounds__(KV4_COPY_THREADS) void qm_kv4_compact_pages(Kv4CompactArgs A) {
+    const Kv4Cache& c = A.c;
+    const int live = A.state[0], moves = A.state[1];
+    const int32_t* movers = A.state + 4;
+    const int32_t* holes = movers + c.num_pages;
+    const int32_t* to = holes + c.num_pages;
+    const int tid = threadIdx.x;
+    for (int64_t k = (int64_t)blockIdx.x * KV4_COPY_THREADS + tid; k < moves; k += (int64_t)gridDim.x * KV4_COPY_THREADS) {
+        c.refs[holes[k]] = c.refs[movers[k]];
+        c.refs[movers[k]] = 0;
+    }
+    for (int r = blockIdx.x; r < c.rows; r += gridDim.x) {
+        const int n = min(max(kv4_pages_of(c.lens[r]), 0), c.max_pages);
+        int32_t* row = c.table + (size_t)r * c.max_pages;
+        for (int j = tid; j < n; j += KV4_COPY_THREADS) {
+            const int id = row[j];
+            if (kv4_is_page(c, id) && id >= live) row[j] = to[id];
+        }
+    }
+    const int64_t parts = (int64_t)moves * c.layers * KV4_COPY_PARTS;
+    for (int64_t p = blockIdx.x; p < parts; p += gridDim.x) {
+        const int part = (int)(p % KV4_COPY_PARTS);
+        const int64_t q = p / KV4_COPY_PARTS;
+        const int layer = (int)(q % c.layers), k = (int)(q / c.layers);
+        copy_part(c, layer, movers[k], holes[k], part);
+    }
+}

@@ -11,6 +11,7 @@
 #include "qora_mixer.h"
 #include "qm_kernel_args.h"
 #include "qm_gqa_plan.h"
+#include "qm_kv4_check.h"
 #include "qm_noalloc.h"
 #include "qm_q4_tiles.h"
 
@@ -63,6 +64,11 @@ struct qm_context {
     hipFunction_t f_sample_select = nullptr;
     hipFunction_t f_sample_slices = nullptr;
     hipFunction_t f_sample_draw = nullptr;
+    hipFunction_t f_kv4_store = nullptr, f_kv4_load = nullptr;
+    hipFunction_t f_kv4_resize = nullptr, f_kv4_resize_pages = nullptr;
+    hipFunction_t f_kv4_fork = nullptr, f_kv4_fork_rows = nullptr;
+    hipFunction_t f_kv4_compact = nullptr, f_kv4_compact_pages = nullptr;
+    hipFunction_t f_gqa_kv4_append = nullptr, f_gqa_kv4_split = nullptr, f_gqa_kv4_merge = nullptr;
     int lm_head_hidden = 0;              // the hidden size lm_head_wg_per_cu was computed for
     int lm_head_wg_per_cu = 1;
     int dnp_chunk_threads = 0;     // the DeltaNet prefill chunk kernel's workgroup size (its launch bounds)
@@ -330,8 +336,8 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     std::string dir = code_object_dir ? code_object_dir : library_dir();
     const char* files[] = {"qm_dn_decode.hsaco", "qm_gqa_decode.hsaco", "qm_util.hsaco",
                            "qm_dn_prefill.hsaco", "qm_gqa_prefill.hsaco", "qm_q4_proj.hsaco",
-                           "qm_q4_vocab.hsaco", "qm_sample.hsaco"};
-    constexpr int kModules = 8;
+                           "qm_q4_vocab.hsaco", "qm_sample.hsaco", "qm_kv4_cache.hsaco", "qm_gqa_decode_kv4.hsaco"};
+    constexpr int kModules = 10;
     hipModule_t mods[kModules] = {};
     for (int i = 0; i < kModules; ++i) {
         std::string path = dir + "/" + files[i];
@@ -385,6 +391,17 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     if (st == QM_OK) st = load_function(c, mods[7], "qm_sample_select", &c->f_sample_select);
     if (st == QM_OK) st = load_function(c, mods[7], "qm_sample_slices", &c->f_sample_slices);
     if (st == QM_OK) st = load_function(c, mods[7], "qm_sample_draw", &c->f_sample_draw);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_store", &c->f_kv4_store);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_load", &c->f_kv4_load);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_resize", &c->f_kv4_resize);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_resize_pages", &c->f_kv4_resize_pages);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_fork", &c->f_kv4_fork);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_fork_rows", &c->f_kv4_fork_rows);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_compact", &c->f_kv4_compact);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_compact_pages", &c->f_kv4_compact_pages);
+    if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_append", &c->f_gqa_kv4_append);
+    if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_split", &c->f_gqa_kv4_split);
+    if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_merge", &c->f_gqa_kv4_merge);
     if (st == QM_OK &&
         (hipFuncGetAttribute(&c->q4_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gemv) != hipSuccess ||
          hipFuncGetAttribute(&c->q4_gu_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gate_up) !=
@@ -789,6 +806,7 @@ int32_t qm_reserve(qm_context* c, int32_t max_batch, int32_t max_kv_len, int32_t
             bn = std::min<int64_t>(B * per_seq, std::max<int64_t>(512 + B, B * ((L + 2047) / 2048)));
         }
         ws = std::max(ws, static_cast<size_t>(bn) * QM_GQA_KV_HEADS * 4 * 260 * sizeof(float));
+        ws = std::max(ws, qm_kv4::reserve_ws(max_batch, max_kv_len));
     }
     if (max_prefill_tokens > 0) {
         ws = std::max(ws, dn_prefill_layout(max_prefill_tokens).total);
@@ -1193,6 +1211,132 @@ int32_t qm_q4_gemm_gate_up(qm_context* c, qm_stream stream, int32_t m, int32_t k
     Q4GemmArgs ga{x, gate_codes, gate_gscales, up_codes, up_gscales, nullptr, out_bf16, nullptr, m, k, n,
                   QM_Q4_TILE(n)};
     return q4_gemm_launch(c, stream, ga, x_dtype, true, "qm_q4_gemm_gate_up");
+}
+
+// ---- paged 4-bit KV cache ----------------------------------------------------------
+}  // extern "C"
+
+namespace {
+// The context's device is the current one while a call enqueues (its
+// workspace may grow), whichever the caller's thread had.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const qm_context* c) {
+        int now = c->device;
+        if (hipGetDevice(&now) == hipSuccess && now != c->device && hipSetDevice(c->device) == hipSuccess) before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) hipSetDevice(before);
+    }
+};
+
+Kv4Cache kv4_of(const qm_kv4_cache& c) {
+    return Kv4Cache{c.pages_dev, c.table_dev, c.lens_dev, c.refs_dev, c.layers, c.num_pages, c.rows, c.max_pages};
+}
+
+int32_t kv4_rows(qm_context* c, qm_stream stream, hipFunction_t f, const char* who, const qm_kv4_cache* cache,
+                 int32_t layer, int32_t row, int32_t batch, const int32_t* first, int32_t n, uint16_t* k, uint16_t* v,
+                 int64_t capacity) {
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_rows(who, cache, layer, row, batch, first, n, k, v, capacity);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    // half pages that n tokens can touch: one more where they begin anywhere
+    const int64_t halves = (static_cast<int64_t>(n) + QMK_KV4_HALF_TOKENS - 1 + (first ? QMK_KV4_HALF_TOKENS - 1 : 0)) /
+                           QMK_KV4_HALF_TOKENS;
+    const int64_t grid = halves * batch * QM_GQA_KV_HEADS;
+    if (grid > 0x7fffffff) return fail(c, QM_ERR_INVALID_ARG, "%s: grid too large", who);
+    Kv4RowsArgs a{kv4_of(*cache), first, k, v, capacity, layer, row, batch, n, static_cast<int32_t>(halves)};
+    return launch(c, f, static_cast<uint32_t>(grid), 256, a, pick(c, stream), who);
+}
+}  // namespace
+
+extern "C" {
+
+int32_t qm_kv4_store(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t row,
+                     int32_t batch, const int32_t* first, int32_t n, const uint16_t* k, const uint16_t* v,
+                     int64_t capacity) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    return kv4_rows(c, stream, c->f_kv4_store, "qm_kv4_store", cache, layer, row, batch, first, n,
+                    const_cast<uint16_t*>(k), const_cast<uint16_t*>(v), capacity);
+}
+
+int32_t qm_kv4_load(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t row,
+                    int32_t batch, const int32_t* first, int32_t n, uint16_t* k, uint16_t* v, int64_t capacity) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    return kv4_rows(c, stream, c->f_kv4_load, "qm_kv4_load", cache, layer, row, batch, first, n, k, v, capacity);
+}
+
+int32_t qm_kv4_resize(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t count, const int32_t* rows,
+                      const int32_t* lens, int32_t flags, int32_t* result) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_resize(cache, count, rows, lens, flags, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    int32_t st = ensure(c, s, qm_kv4::resize_ws(count));
+    if (st != QM_OK) return st;
+    Kv4ResizeArgs a{kv4_of(*cache), rows, lens, result, static_cast<int32_t*>(c->ws), count, flags == QM_KV4_ADD};
+    st = launch(c, c->f_kv4_resize, 1, 1024, a, s, "qm_kv4_resize");
+    if (st != QM_OK) return st;
+    const int64_t parts = static_cast<int64_t>(count) * cache->layers * 3;
+    return launch(c, c->f_kv4_resize_pages, static_cast<uint32_t>(std::min<int64_t>(parts, 8 * c->num_cu)), 256, a, s,
+                  "qm_kv4_resize_pages");
+}
+
+int32_t qm_kv4_fork(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t count, const int32_t* src,
+                    const int32_t* dst, int32_t* result) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_list("qm_kv4_fork", cache, count, {src, dst}, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    int32_t st = ensure(c, s, qm_kv4::fork_ws(count, cache->max_pages));
+    if (st != QM_OK) return st;
+    Kv4ForkArgs a{kv4_of(*cache), src, dst, result, static_cast<int32_t*>(c->ws), count};
+    st = launch(c, c->f_kv4_fork, static_cast<uint32_t>(count), 256, a, s, "qm_kv4_fork");
+    if (st != QM_OK) return st;
+    return launch(c, c->f_kv4_fork_rows, static_cast<uint32_t>(count), 256, a, s, "qm_kv4_fork_rows");
+}
+
+int32_t qm_kv4_compact(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t* live) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_list("qm_kv4_compact", cache, 1, {}, live);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    int32_t st = ensure(c, s, qm_kv4::compact_ws(cache->num_pages));
+    if (st != QM_OK) return st;
+    Kv4CompactArgs a{kv4_of(*cache), live, static_cast<int32_t*>(c->ws)};
+    st = launch(c, c->f_kv4_compact, 1, 1024, a, s, "qm_kv4_compact");
+    if (st != QM_OK) return st;
+    const int64_t parts = static_cast<int64_t>(cache->num_pages) * cache->layers * 3;
+    return launch(c, c->f_kv4_compact_pages, static_cast<uint32_t>(std::min<int64_t>(parts, 8 * c->num_cu)), 256, a, s,
+                  "qm_kv4_compact_pages");
+}
+
+int32_t qm_gqa_decode_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t batch,
+                          const int32_t* slots, const float* q_gate, const float* k_new, const float* v_new,
+                          const uint16_t* q_norm, const uint16_t* k_norm, const float* rope_cos, const float* rope_sin,
+                          int32_t rope_len, int32_t max_len, const int32_t* result, float* out) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_decode(
+        cache, layer, batch, slots, {q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, out}, rope_len, max_len, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    const int64_t chunk = qm_kv4::split_tokens(max_len, batch), nsplit = qm_kv4::splits(max_len, batch);
+    const uint64_t grid = static_cast<uint64_t>(batch) * QM_GQA_KV_HEADS * nsplit;
+    if (grid > 0x7fffffffull || static_cast<uint64_t>(batch) * QM_GQA_HEADS > 0x7fffffffull)
+        return fail(c, QM_ERR_INVALID_ARG, "qm_gqa_decode_kv4: grid too large");
+    int32_t st = ensure(c, s, qm_kv4::decode_ws(batch, nsplit));
+    if (st != QM_OK) return st;
+    GqaKv4Args a{kv4_of(*cache), slots, q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, result, out,
+                 static_cast<float*>(c->ws), layer, batch, max_len, static_cast<int32_t>(chunk), static_cast<int32_t>(nsplit)};
+    st = launch(c, c->f_gqa_kv4_append, static_cast<uint32_t>(batch) * QM_GQA_KV_HEADS, 64, a, s, "qm_gqa_kv4_append");
+    if (st != QM_OK) return st;
+    st = launch(c, c->f_gqa_kv4_split, static_cast<uint32_t>(grid), 256, a, s, "qm_gqa_kv4_split");
+    if (st != QM_OK) return st;
+    return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(batch) * QM_GQA_HEADS, 256, a, s, "qm_gqa_kv4_merge");
 }
 
 }  // extern "C"

@@ -51,6 +51,16 @@ class QmSampleParams(C.Structure):
                 ("banned_id", C.c_int32), ("flags", C.c_int32)]
 
 
+QM_KV4_PAGE_TOKENS, QM_KV4_PAGE_BYTES = 64, 73728
+QM_KV4_LENS, QM_KV4_ADD = 0, 1
+
+
+class QmKv4Cache(C.Structure):
+    _fields_ = [("pages_dev", C.c_void_p), ("table_dev", C.c_void_p), ("lens_dev", C.c_void_p),
+                ("refs_dev", C.c_void_p), ("layers", C.c_int32), ("num_pages", C.c_int32),
+                ("rows", C.c_int32), ("max_pages", C.c_int32)]
+
+
 class QmConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "num_qk_heads", "num_v_heads", "dn_head_dim", "conv_kernel",
@@ -100,6 +110,12 @@ _SIGNATURES = {
     "qm_gqa_decode": [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _I32, _P, _P, _I64, _P],
     "qm_gqa_decode_noalloc": [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _I32, _P, _P, _I64, _P],
     "qm_gqa_prefill": [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _I64, _P],
+    "qm_kv4_resize": [_P, _P, C.POINTER(QmKv4Cache), _I32, _P, _P, _I32, _P],
+    "qm_kv4_fork": [_P, _P, C.POINTER(QmKv4Cache), _I32, _P, _P, _P],
+    "qm_kv4_compact": [_P, _P, C.POINTER(QmKv4Cache), _P],
+    "qm_kv4_store": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _I32, _P, _I32, _P, _P, _I64],
+    "qm_kv4_load": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _I32, _P, _I32, _P, _P, _I64],
+    "qm_gqa_decode_kv4": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P],
     "qm_q4_repack": [_P, _P, _I32, _I32, _P, _P, _P, _P],
     "qm_q4_gemv": [_P, _P, _I32, _I32, _P, _P, _P, _P],
     "qm_q4_gemv_multi": [_P, _P, _I32, _P, _P, _I32, _P],
@@ -190,6 +206,27 @@ class DeviceBuffer:
             self.close()
         except Exception:
             pass
+
+
+class Kv4Cache:
+    """A paged 4-bit KV cache: its buffers and what the library's calls take of them (qm_kv4_cache)."""
+
+    def __init__(self, ctx: "Context", layers: int, num_pages: int, rows: int, max_pages: int):
+        """A new, empty cache in buffers of its own."""
+        self.pages = ctx.alloc(layers * num_pages * QM_KV4_PAGE_BYTES)
+        self.table = ctx.alloc(rows * max_pages * 4)
+        self.lens, self.refs = ctx.alloc(rows * 4), ctx.alloc(num_pages * 4)
+        for buf in (self.lens, self.refs):
+            ctx.memset(buf, 0, buf.nbytes)
+        self.c = QmKv4Cache(self.pages.ptr, self.table.ptr, self.lens.ptr, self.refs.ptr, layers, num_pages, rows, max_pages)
+
+    @classmethod
+    def of(cls, pages, table, lens, refs, layers: int, num_pages: int, rows: int, max_pages: int) -> "Kv4Cache":
+        """A cache in device buffers that the caller keeps."""
+        self = cls.__new__(cls)
+        self.pages, self.table, self.lens, self.refs = pages, table, lens, refs
+        self.c = QmKv4Cache(_addr(pages), _addr(table), _addr(lens), _addr(refs), layers, num_pages, rows, max_pages)
+        return self
 
 
 class Context:
@@ -313,6 +350,37 @@ class Context:
             self.h, self.stream, batch, _addr(q_gate), _addr(k_new), _addr(v_new), _addr(q_norm),
             _addr(k_norm), _addr(rope_cos), _addr(rope_sin), rope_len, _addr(pos), max_pos,
             _addr(k_cache), _addr(v_cache), cap, _addr(out)))
+
+    def kv4_resize(self, cache, count, rows, lens, result, flags=QM_KV4_LENS):
+        """Rows (int32 [count]; None: 0 .. count - 1) take the lengths lens (QM_KV4_ADD: added to theirs);
+        result int32 [1]: 0, pages lacking, or -1."""
+        self._check(self.lib.qm_kv4_resize(self.h, self.stream, C.byref(cache.c), count, _addr(rows), _addr(lens), flags,
+                                           _addr(result)))
+
+    def kv4_fork(self, cache, count, src, dst, result):
+        """Rows dst become rows src as they were (int32 [count] each), sharing their pages."""
+        self._check(self.lib.qm_kv4_fork(self.h, self.stream, C.byref(cache.c), count, _addr(src), _addr(dst), _addr(result)))
+
+    def kv4_compact(self, cache, live):
+        """The pages in use move to the front of the pool; live int32 [1] is their number."""
+        self._check(self.lib.qm_kv4_compact(self.h, self.stream, C.byref(cache.c), _addr(live)))
+
+    def kv4_store(self, cache, layer, row, batch, first, n, k, v, cap):
+        """f16 rows k, v [batch][4][cap][256] become tokens first .. first + n - 1 of table rows row .."""
+        self._check(self.lib.qm_kv4_store(self.h, self.stream, C.byref(cache.c), layer, row, batch, _addr(first), n,
+                                          _addr(k), _addr(v), cap))
+
+    def kv4_load(self, cache, layer, row, batch, first, n, k, v, cap):
+        """The inverse: tokens of the cache as f16 rows k, v."""
+        self._check(self.lib.qm_kv4_load(self.h, self.stream, C.byref(cache.c), layer, row, batch, _addr(first), n,
+                                         _addr(k), _addr(v), cap))
+
+    def gqa_decode_kv4(self, cache, layer, batch, slots, q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin,
+                       rope_len, max_len, result, out):
+        """qm_gqa_decode over a layer of a 4-bit cache; batch row b steps table row slots[b] (None: b)."""
+        self._check(self.lib.qm_gqa_decode_kv4(
+            self.h, self.stream, C.byref(cache.c), layer, batch, _addr(slots), _addr(q_gate), _addr(k_new), _addr(v_new),
+            _addr(q_norm), _addr(k_norm), _addr(rope_cos), _addr(rope_sin), rope_len, max_len, _addr(result), _addr(out)))
 
     def gqa_prefill(self, seq_len, q_gate, k, v, q_norm, k_norm, rope_cos, rope_sin, rope_len,
                     k_cache, v_cache, cap, out):

@@ -10,7 +10,8 @@ use std::env;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const KERNELS: &[&str] = &["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample"];
+const KERNELS: &[&str] = &["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample",
+                         "kv4_cache", "gqa_decode_kv4"];
 
 // hipcc flags of every device compile: gfx950 only; no packed-fp32 VALU ops;
 // MFMA results in arch VGPRs.

@@ -56,6 +56,10 @@ pub mod raw {
     pub const QM_DN_POSTACT: i32 = 0;
     pub const QM_DN_PREACT: i32 = 1;
     pub const QM_SAMPLE_WGPU: i32 = 1;
+    pub const QM_KV4_PAGE_TOKENS: i32 = 64;
+    pub const QM_KV4_PAGE_BYTES: i32 = 73728;
+    pub const QM_KV4_LENS: i32 = 0;
+    pub const QM_KV4_ADD: i32 = 1;
 
     /// Qor4bConfig's mixer fields (config.rs:4-32).
     #[repr(C)]
@@ -94,6 +98,20 @@ pub mod raw {
         pub presence_penalty: f32,
         pub banned_id: i32,
         pub flags: i32,
+    }
+
+    /// A paged 4-bit KV cache: the caller's buffers.
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct qm_kv4_cache {
+        pub pages_dev: *mut u8,
+        pub table_dev: *mut i32,
+        pub lens_dev: *mut i32,
+        pub refs_dev: *mut i32,
+        pub layers: i32,
+        pub num_pages: i32,
+        pub rows: i32,
+        pub max_pages: i32,
     }
 
     #[link(name = "qora_mixer")]
@@ -165,6 +183,25 @@ pub mod raw {
                               rope_cos_dev: *const f32, rope_sin_dev: *const f32, rope_len: i32,
                               k_cache_dev: *mut u16, v_cache_dev: *mut u16, cache_capacity: i64,
                               out_dev: *mut u16) -> i32;
+
+        // ---- paged 4-bit KV cache
+        pub fn qm_kv4_resize(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, count: i32,
+                             rows_dev: *const i32, lens_dev: *const i32, flags: i32, result_dev: *mut i32) -> i32;
+        pub fn qm_kv4_fork(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, count: i32,
+                           src_dev: *const i32, dst_dev: *const i32, result_dev: *mut i32) -> i32;
+        pub fn qm_kv4_compact(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache,
+                              live_dev: *mut i32) -> i32;
+        pub fn qm_kv4_store(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, layer: i32,
+                            row: i32, batch: i32, first_dev: *const i32, n: i32, k_dev: *const u16,
+                            v_dev: *const u16, capacity: i64) -> i32;
+        pub fn qm_kv4_load(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, layer: i32,
+                           row: i32, batch: i32, first_dev: *const i32, n: i32, k_dev: *mut u16, v_dev: *mut u16,
+                           capacity: i64) -> i32;
+        pub fn qm_gqa_decode_kv4(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, layer: i32,
+                                 batch: i32, slots_dev: *const i32, q_gate_dev: *const f32, k_new_dev: *const f32,
+                                 v_new_dev: *const f32, q_norm_dev: *const u16, k_norm_dev: *const u16,
+                                 rope_cos_dev: *const f32, rope_sin_dev: *const f32, rope_len: i32, max_len: i32,
+                                 result_dev: *const i32, out_dev: *mut f32) -> i32;
 
         // ---- Q4 projections
         pub fn qm_q4_repack(ctx: *mut qm_context, stream: qm_stream, k: i32, n: i32, packed_dev: *const u8,
