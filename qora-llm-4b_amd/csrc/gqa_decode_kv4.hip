@@ -1,6 +1,31 @@
 // gqa_decode_kv4.hip -- the GQA decode step over the paged 4-bit KV cache
 // (qm_kv4.h) for gfx950: the mixer slice of qm_gqa_decode (gemv.rs:927-1011)
 // with the cache's rows read as lo + s * code.
+//
+// Split-K flash decode: workgroup (b, g, split) has `chunk` tokens of kv head
+// g and g's four query heads; qm_gqa_kv4_merge joins the splits (a single one
+// finishes by itself).  A wave takes half a page (32 tokens) a round.
+//
+// Mathematics.  With K = lo + s c per group of 64 dims,
+//   q . K = sum_groups s (q . c) + lo (sum of q over the group),
+//   sum_t p V = sum_groups sum_t (p s) c + (sum_t p lo),
+// so both products run on v_mfma_f32_16x16x32_bf16 over the codes themselves,
+// and scales and minima enter in f32 on 1/64 of the values.
+//   A code c in bits 0..3 (4..7) of a half is the bf16 subnormal c 2^-133
+//   (16 c 2^-133): masks alone make operands of a word (5 instructions for 8
+//   codes).  The other operand carries 2^90 (2^86 for the elements of bits
+//   4..7), which keeps products normal: for p down to 2^-216, q up to 2^37.
+//   That operand is f32 and enters as three bf16 parts, 24 bits, exactly:
+//   four heads x three parts are 12 of the 16 rows (columns) that a matrix
+//   instruction has anyway.
+//   QK: A = 16 tokens' codes, B = q (column 4 part + head).  Lane (g, c) ends
+//   with tokens 4 g .. + 3 of column c; the parts' scores are summed over
+//   columns c & 3 by two DPP adds, so that every lane holds its head's.
+//   PV: A = p s (row 4 part + head; the same lane has the same head's p),
+//   B = the codes of 16 dims, one instruction per 16 dims and 32 tokens.
+//   The minimum terms are the lanes' own: the lane of part j adds group j's.
+// Softmax in base 2; a running maximum is raised only where a score passes it
+// by 2^8, so the accumulators are seldom rescaled.
 #include "qm_kv4_device.h"
 #include "qm_kernel_args.h"
 #include "qm_gqa_common.h"
@@ -86,130 +111,467 @@ QM_DEV CodedRow code_row(const uint16_t (&h)[4]) {
     return c;
 }
 
-// The new token's K and V rows into the cache: one wave per (batch row, kv
-// head).
-extern "C" __global__ __launch_bounds__(64) void qm_gqa_kv4_append(GqaKv4Args A) {
-    const int lane = threadIdx.x, g = blockIdx.x & 3, b = blockIdx.x >> 2;
-    const StepRow r = step_row(A, b);
-    if (r.len == 0) return;
-    const int pos = r.len - 1, t = pos & 31;
-    if ((pos >> 6) >= A.c.max_pages) return;
-    const int id = A.c.table[(size_t)r.row * A.c.max_pages + (pos >> 6)];
-    if (!kv4_is_page(A.c, id)) return;
-    const size_t src = ((size_t)b * QM_GQA_KV_HEADS + g) * QM_GQA_HD + 4 * lane;
-    float4 rc, rs;
-    rope_row_loads(A.rope_cos + (size_t)pos * (QM_GQA_ROT / 2), A.rope_sin + (size_t)pos * (QM_GQA_ROT / 2), lane, rc, rs);
-    uint16_t kh[4];
-    new_k(ld4(A.k_new + src), *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane), rc, rs, lane, kh);
-    const float4 v = ld4(A.v_new + src);
-    const uint16_t vh[4] = {f32_to_f16(v.x), f32_to_f16(v.y), f32_to_f16(v.z), f32_to_f16(v.w)};
-    const CodedRow ck = code_row(kh), cv = code_row(vh);
-    uint32_t* words = reinterpret_cast<uint32_t*>(kv4_half(A.c, A.layer, id, g, (pos >> 5) & 1));
-    uint32_t kw = 0;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+#define KV4_WAVES 4
+#define KV4_Q_STRIDE (QM_GQA_HD + 8)   // bf16 of a q row in LDS: 16 rows 528 bytes apart fall into different banks
+#define KV4_P_BIAS 90.0f               // p and q carry 2^90: codes are bf16 subnormals
+
+// What a wave loads of half a page: lane (g, c) = (lane >> 4, lane & 15).
+struct HalfK {
+    uint4 w[2][2];           // codes of token 16 u + c, dims 32 s + 8 g .. + 7 in word s = 4 h + i of [u][h]
+    uint4 s[4];              // scales of tokens 16 u + 4 g + i, four groups each
+    uint4 lo;                // minima of those eight tokens, group c >> 2
+};
+struct HalfV {
+    uint4 w[4];              // codes of dims 64 j + 16 m + c in word m of [j], tokens 16 u + 4 g + i
+    uint4 s[4];
+    uint4 lo;
+};
+QM_DEV void load_meta(uint4 (&s)[4], uint4& lo, const uint8_t* meta, int lane) {
+    const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kw |= ck.q[i] << (4 * kv4_nibble(4 * (lane & 1) + i));
-    kw |= __shfl_xor(kw, 1);
-    if ((lane & 1) == 0) words[kv4_k_word(t, 4 * lane)] = kw;
-    const int shift = 4 * kv4_v_nibble(t);
+    for (int i = 0; i < 4; ++i) s[i] = *reinterpret_cast<const uint4*>(meta + 64 * g + 16 * i);
+    lo = *reinterpret_cast<const uint4*>(meta + 256 + (4 * (c >> 2) + g) * 16);
+}
+QM_DEV void load_k(HalfK& k, const uint8_t* half, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k.w[i >> 1][i & 1] = *reinterpret_cast<const uint4*>(half + 1024 * i + 16 * lane);
+    load_meta(k.s, k.lo, half + QMK_KV4_META, lane);
+}
+QM_DEV void load_v(HalfV& v, const uint8_t* half, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.w[j] = *reinterpret_cast<const uint4*>(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
+    load_meta(v.s, v.lo, half + QMK_KV4_META + 512, lane);
+}
+QM_DEV uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+QM_DEV void set_word(uint4& v, int i, uint32_t x) {
+    if (i == 0) v.x = x;
+    else if (i == 1) v.y = x;
+    else if (i == 2) v.z = x;
+    else v.w = x;
+}
+
+// The eight codes of a word as bf16 subnormals, elements 2, 3, 6, 7 times 16.
+QM_DEV bf16x8 codes_bf16(uint32_t w) {
+    const uint32_t v = w >> 8;
+    uint4 m = make_uint4(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u);
+    // opaque to the optimiser, which would otherwise fold each mask into a
+    // per-nibble bit-field extract
+    asm("" : "+v"(m.x), "+v"(m.y), "+v"(m.z), "+v"(m.w));
+    return __builtin_bit_cast(bf16x8, m);
+}
+
+// Part j of an f32: its upper 8, middle 8 or lower 8 bits of significand as a
+// bf16 in the upper half (j = 3: nothing).  hi, lo: the masks of part_masks.
+struct PartMasks {
+    uint32_t hi, lo;
+};
+QM_DEV PartMasks part_masks(int j) {
+    return PartMasks{j == 0 ? 0xffff0000u : j == 1 ? 0xffffff00u : 0xffffffffu,
+                     j == 0 ? 0u : j == 1 ? 0xffff0000u : j == 2 ? 0xffffff00u : 0xffffffffu};
+}
+QM_DEV uint32_t part_of(float x, PartMasks m) {
+    const uint32_t u = __float_as_uint(x);
+    return __float_as_uint(__uint_as_float(u & m.hi) - __uint_as_float(u & m.lo));
+}
+QM_DEV uint32_t pack_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+QM_DEV half2_t halves(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
+
+// Per-wave softmax state and accumulators.  o[m]: dims 16 m + c, element e of
+// lane group g: part g of head e, in units of 2^-43; lo: the lane's share of
+// its head's and group's minimum terms, l of its head's sum (elements 2, 3, 6,
+// 7 apart), in units of 2^90.
+struct WaveKv4 {
+    float m, l, l16, lo;
+    floatx4 o[16];
+};
+
+struct SplitKv4Lds {
+    __attribute__((aligned(16))) uint16_t q[13][KV4_Q_STRIDE];       // row 4 part + head; row 12 zero
+    float qsum[4][4];                                                // [head][group]
+    __attribute__((aligned(16))) float acc[KV4_WAVES][4][QM_GQA_HD];
+    float m[KV4_WAVES][4], l[KV4_WAVES][4];
+    // the new token: K words [dims / 128][g], V codes as bytes [c][4 j + m], scales and minima by group
+    __attribute__((aligned(16))) uint32_t kw[2][4][4];
+    __attribute__((aligned(16))) uint8_t vq[16][16];
+    uint32_t ks[2], vs[2];
+    uint16_t klo[4], vlo[4];
+};
+
+// The new token t (0 .. 31 of the half page) into the loaded operands, and
+// from them to the page.
+QM_DEV void put_k(HalfK& k, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
+    const int c = lane & 15, g = lane >> 4, u = t >> 4;
+    if (c == (t & 15)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 w = *reinterpret_cast<const uint4*>(sh.kw[h][g]);
+            k.w[0][h] = u == 0 ? w : k.w[0][h];
+            k.w[1][h] = u == 1 ? w : k.w[1][h];
+            *reinterpret_cast<uint4*>(half + 1024 * (2 * u + h) + 16 * lane) = w;
+        }
+    }
+}
+QM_DEV void put_meta(uint4 (&s)[4], uint4& lo, const uint32_t (&ns)[2], const uint16_t (&nlo)[4], int t, uint8_t* meta, int lane) {
+    const int c = lane & 15, g = lane >> 4, e = 4 * (t >> 4) + (t & 3);
+    if (g != ((t >> 2) & 3)) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t* w = words + kv4_v_word(t, 4 * lane + i);
-        *w = (*w & ~(15u << shift)) | (cv.q[i] << shift);
+        if (i == e >> 1) {
+            if (e & 1) { s[i].z = ns[0]; s[i].w = ns[1]; }
+            else { s[i].x = ns[0]; s[i].y = ns[1]; }
+        }
     }
-    if ((lane & 15) == 0) {
-        uint16_t* meta = reinterpret_cast<uint16_t*>(words) + QMK_KV4_META / 2;
-        const int sa = kv4_s_at(t, lane >> 4), la = kv4_lo_at(t, lane >> 4);
-        meta[sa] = ck.s;
-        meta[128 + la] = ck.lo;
-        meta[256 + sa] = cv.s;
-        meta[384 + la] = cv.lo;
+    const uint32_t n = nlo[c >> 2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i == e >> 1) {
+            const uint32_t w = word_of(lo, i);
+            set_word(lo, i, e & 1 ? (w & 0xffffu) | n << 16 : (w & 0xffff0000u) | n);
+        }
+    }
+    if (c == 0) *reinterpret_cast<uint2*>(meta + 64 * g + 8 * e) = make_uint2(ns[0], ns[1]);
+    if ((c & 3) == 0) *reinterpret_cast<uint16_t*>(meta + 256 + (4 * (c >> 2) + g) * 16 + 2 * e) = (uint16_t)n;
+}
+QM_DEV void put_v(HalfV& v, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    if (g != ((t >> 2) & 3)) return;
+    const int shift = 4 * kv4_v_nibble(t);
+    const uint4 q = *reinterpret_cast<const uint4*>(sh.vq[c]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const uint32_t code = (word_of(q, j) >> (8 * m)) & 15u;
+            set_word(v.w[j], m, (word_of(v.w[j], m) & ~(15u << shift)) | (code << shift));
+        }
+        *reinterpret_cast<uint4*>(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane) = v.w[j];
     }
 }
 
-// Attention of one split: `chunk` tokens of one (batch row, kv head), all
-// four query heads, half a page at a time through LDS in f32.
-extern "C" __global__ __launch_bounds__(256) void qm_gqa_kv4_split(GqaKv4Args A) {
-    __shared__ __attribute__((aligned(16))) uint32_t w[QMK_KV4_HALF_BYTES / 4];
-    __shared__ float tile[32][257];
-    __shared__ float q[4][256], p[4][32], top[4], total[4], corr[4];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int split = blockIdx.x % A.nsplit, bg = blockIdx.x / A.nsplit;
-    const int g = bg & 3, b = bg >> 2;
-    const StepRow r = step_row(A, b);
-    const int t_begin = split * A.chunk, t_end = min(t_begin + A.chunk, r.len);
-    float acc[4] = {0, 0, 0, 0};
-    {
-        const int pos = max(r.len - 1, 0);
-        float4 rc, rs;
-        rope_row_loads(A.rope_cos + (size_t)pos * (QM_GQA_ROT / 2), A.rope_sin + (size_t)pos * (QM_GQA_ROT / 2), lane, rc, rs);
-        const float4 x = norm_rope_head(ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + 4 * g + wv) * (2 * QM_GQA_HD) + 4 * lane),
-                                        *reinterpret_cast<const uint2*>(A.q_norm + 4 * lane), rc, rs, lane);
-        *reinterpret_cast<float4*>(&q[wv][4 * lane]) = x;
-        if (tid < 4) { top[tid] = -INFINITY; total[tid] = 0.0f; }
+// Scores of the half page's 32 tokens: x[4 u + i] of token 16 u + 4 g + i and
+// head c & 3, in units of log2 e / 16.
+QM_DEV void scores(float (&x)[8], const HalfK& k, const uint16_t* qsrc, float qsum) {
+    floatx4 acc[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[u][n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        const bf16x8 q = *reinterpret_cast<const bf16x8*>(qsrc + 32 * s);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            acc[u][s >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(word_of(k.w[u][s >> 2], s & 3)), q, acc[u][s >> 1], 0, 0, 0);
     }
-    for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-        if ((t0 >> 6) >= A.c.max_pages) break;
-        const int id = A.c.table[(size_t)r.row * A.c.max_pages + (t0 >> 6)];
-        if (!kv4_is_page(A.c, id)) continue;
-        const uint4* src = reinterpret_cast<const uint4*>(kv4_half(A.c, A.layer, id, g, (t0 >> 5) & 1));
-        __syncthreads();
-        for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += 256) reinterpret_cast<uint4*>(w)[j] = src[j];
-        __syncthreads();
-        const uint16_t* meta = reinterpret_cast<const uint16_t*>(&w[QMK_KV4_META / 4]);
-        const int d = tid, group = d >> 6;
-        for (int t = 0; t < 32; ++t)
-            tile[t][d] = fmaf((float)((w[kv4_k_word(t, d)] >> (4 * kv4_k_nibble(d))) & 15u),
-                              f16_to_f32(meta[kv4_s_at(t, group)]), f16_to_f32(meta[128 + kv4_lo_at(t, group)]));
-        __syncthreads();
-        if (tid < 128) {
-            const int h = tid >> 5, t = tid & 31;
-            float s = 0.0f;
-            for (int j = 0; j < 256; ++j) s = fmaf(q[h][j], tile[t][j], s);
-            s = t0 + t < t_end ? s * (1.4426950408889634f / 16.0f) : -INFINITY;
-            float m = s;
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            const float mn = fmaxf(top[h], m), co = top[h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[h] - mn);
-            const float e = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
-            float l = e;
-            for (int o = 16; o; o >>= 1) l += __shfl_xor(l, o);
-            p[h][t] = e;
-            if (t == 0) { total[h] = total[h] * co + l; corr[h] = co; top[h] = mn; }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4& s = k.s[2 * u + (i >> 1)];
+            const half2_t s01 = halves(i & 1 ? s.z : s.x), s23 = halves(i & 1 ? s.w : s.y);
+            float t = fmaf(acc[u][0][i], (float)s01[0], 0.0f);
+            t = fmaf(acc[u][1][i], (float)s01[1], t);
+            t = fmaf(acc[u][2][i], (float)s23[0], t);
+            t = fmaf(acc[u][3][i], (float)s23[1], t);
+            const float lo = (float)halves(word_of(k.lo, 2 * u + (i >> 1)))[i & 1];
+            t = fmaf(t, 0x1p43f, lo * qsum);
+            t += dpp_f32<0x128>(t);                  // the parts: columns 8 and 4 apart
+            x[4 * u + i] = t + dpp_f32<0x124>(t);
         }
-        __syncthreads();
+    }
+}
+
+// The softmax weights of a round, and their products with V.
+QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, int lane) {
+    const int g = lane >> 4;
+    if (left < QMK_KV4_HALF_TOKENS) {                // uniform: tokens from `left` on are none
 #pragma unroll
-        for (int h = 0; h < 4; ++h) acc[h] *= corr[h];
-        for (int t = 0; t < 32; ++t) {
-            if (t0 + t >= t_end) break;
-            const float v = fmaf((float)((w[kv4_v_word(t, d)] >> (4 * kv4_v_nibble(t))) & 15u),
-                                 f16_to_f32(meta[256 + kv4_s_at(t, group)]), f16_to_f32(meta[384 + kv4_lo_at(t, group)]));
+        for (int e = 0; e < 8; ++e) {
+            if (16 * (e >> 2) + 4 * g + (e & 3) < left) continue;
+            x[e] = -INFINITY;
+            // whatever stands there: a weight of zero times it must be zero
+            if (e & 1) { v.s[e >> 1].z = 0; v.s[e >> 1].w = 0; }
+            else { v.s[e >> 1].x = 0; v.s[e >> 1].y = 0; }
+            const uint32_t w = word_of(v.lo, e >> 1);
+            set_word(v.lo, e >> 1, e & 1 ? w & 0xffffu : w & 0xffff0000u);
+        }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    mx = max_xor32(max_xor16(mx));
+    if (__ballot(mx > st.m + 8.0f)) {                // uniform
+        const float m = mx > st.m + 8.0f ? mx : st.m;
+        const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+        st.m = m;
+        st.l *= f;
+        st.l16 *= f;
+        st.lo *= f;
+        const float f0 = readlane_f32(f, 0), f1 = readlane_f32(f, 1), f2 = readlane_f32(f, 2), f3 = readlane_f32(f, 3);
 #pragma unroll
-            for (int h = 0; h < 4; ++h) acc[h] = fmaf(p[h][t], v, acc[h]);
+        for (int m4 = 0; m4 < 16; ++m4) {
+            st.o[m4][0] *= f0;
+            st.o[m4][1] *= f1;
+            st.o[m4][2] *= f2;
+            st.o[m4][3] *= f3;
+        }
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - (st.m - (e & 2 ? KV4_P_BIAS - 4.0f : KV4_P_BIAS)));
+    st.l += (p[0] + p[1]) + (p[4] + p[5]);
+    st.l16 += (p[2] + p[3]) + (p[6] + p[7]);
+    float lo = 0.0f, lo16 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float w = (float)halves(word_of(v.lo, e >> 1))[e & 1];
+        if (e & 2) lo16 = fmaf(p[e], w, lo16);
+        else lo = fmaf(p[e], w, lo);
+    }
+    st.lo += fmaf(lo16, 16.0f, lo);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t part[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4& s = v.s[i];
+                const float sc = (float)halves(h ? (j < 2 ? s.z : s.w) : (j < 2 ? s.x : s.y))[j & 1];
+                part[h] = part_of(fmaf(p[2 * i + h], sc, 0.0f), pm);
+            }
+            a[i] = pack_hi(part[0], part[1]);
+        }
+        const bf16x8 w = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(word_of(v.w[j], m)), st.o[4 * j + m], 0, 0, 0);
+    }
+}
+
+// The gated output of head h of g, dims 4 lane .. + 3; l = 0: no tokens.
+QM_DEV void kv4_out(const GqaKv4Args& A, int b, int h, int lane, float4 o, float l, float4 gate, bool refused) {
+    const float inv = l != 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
+    float4 r = make_float4(o.x * inv * sigmoid_fast(gate.x), o.y * inv * sigmoid_fast(gate.y), o.z * inv * sigmoid_fast(gate.z),
+                           o.w * inv * sigmoid_fast(gate.w));
+    if (refused) r.x = r.y = r.z = r.w = __builtin_nanf("");
+    st4(A.out + ((size_t)b * QM_GQA_HEADS + h) * QM_GQA_HD + 4 * lane, r);
+}
+QM_DEV float4 kv4_gate(const GqaKv4Args& A, int b, int h, int lane) {
+    return ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + h) * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
+}
+
+extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(GqaKv4Args A) {
+    __shared__ SplitKv4Lds sh;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int split = blockIdx.x % A.nsplit, bg = blockIdx.x / A.nsplit;
+    const int kvh = bg & 3, b = bg >> 2;
+    const int t_begin = split * A.chunk;
+    const StepRow r = step_row(A, b);
+    const int t_end = min(t_begin + A.chunk, r.len);
+    if (t_begin >= t_end && A.nsplit > 1) return;        // uniform: the merge reads the splits of the row's tokens
+    const int h0 = __builtin_amdgcn_readfirstlane(t_begin / QMK_KV4_HALF_TOKENS + w);
+    const int h_end = __builtin_amdgcn_readfirstlane((t_end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
+    // page ids of the split, one a lane (a split has at most 64 pages)
+    const int page0 = t_begin / QMK_KV4_PAGE_TOKENS;
+    int ids = -1;
+    if (t_begin < t_end) {
+        const int at = page0 + lane;
+        if (at < A.c.max_pages && at * (int64_t)QMK_KV4_PAGE_TOKENS < t_end) ids = A.c.table[(size_t)r.row * A.c.max_pages + at];
+    }
+    auto half_of = [&](int h, bool& there) {
+        const int id = __builtin_amdgcn_readlane(ids, (h >> 1) - page0);
+        there = kv4_is_page(A.c, id);
+        return kv4_half(A.c, A.layer, there ? id : 0, kvh, h & 1);
+    };
+
+    HalfK k;
+    HalfV v;
+    bool there = false;
+    uint8_t* half = nullptr;
+    if (h0 < h_end) {
+        half = half_of(h0, there);
+        load_k(k, half, lane);
+        load_v(v, half, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // q of head 4 kvh + w: norm, RoPE, the softmax's scale, and the parts
+    const int pos = max(r.len - 1, 0);
+    float4 rc, rs;
+    rope_row_loads(A.rope_cos + (size_t)pos * (QM_GQA_ROT / 2), A.rope_sin + (size_t)pos * (QM_GQA_ROT / 2), lane, rc, rs);
+    const bool appends = pos >= t_begin && pos < t_end;
+    {
+        float4 x = norm_rope_head(ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + 4 * kvh + w) * (2 * QM_GQA_HD) + 4 * lane),
+                                  *reinterpret_cast<const uint2*>(A.q_norm + 4 * lane), rc, rs, lane);
+        const float scale = 1.4426950408889634f / 16.0f;
+        x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+        const float sum = row_sum16((x.x + x.y) + (x.z + x.w));
+        if (c == 0) sh.qsum[w][g] = sum;
+        const float y[4] = {x.x * 0x1p90f, x.y * 0x1p90f, x.z * 0x1p86f, x.w * 0x1p86f};
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const PartMasks pm = part_masks(j);
+            *reinterpret_cast<uint2*>(&sh.q[4 * j + w][4 * lane]) =
+                make_uint2(pack_hi(part_of(y[0], pm), part_of(y[1], pm)), pack_hi(part_of(y[2], pm), part_of(y[3], pm)));
+        }
+        if (w == 3) *reinterpret_cast<uint2*>(&sh.q[12][4 * lane]) = make_uint2(0, 0);
+    }
+    if (appends && w < 2) {                                // uniform per wave
+        const size_t src = ((size_t)b * QM_GQA_KV_HEADS + kvh) * QM_GQA_HD + 4 * lane;
+        uint16_t x[4];
+        if (w == 0) {
+            new_k(ld4(A.k_new + src), *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane), rc, rs, lane, x);
+        } else {
+            const float4 n = ld4(A.v_new + src);
+            x[0] = f32_to_f16(n.x), x[1] = f32_to_f16(n.y), x[2] = f32_to_f16(n.z), x[3] = f32_to_f16(n.w);
+        }
+        const CodedRow q = code_row(x);
+        if (w == 0) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word |= q.q[i] << (4 * kv4_nibble(4 * (lane & 1) + i));
+            word |= __shfl_xor(word, 1);
+            const int d = 4 * lane;
+            if ((lane & 1) == 0) sh.kw[d >> 7][(d >> 3) & 3][(d >> 5) & 3] = word;
+            if (c == 0) {
+                reinterpret_cast<uint16_t*>(sh.ks)[g] = q.s;
+                sh.klo[g] = q.lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 4 * lane + i;                // dim 64 j + 16 m + c
+                sh.vq[d & 15][d >> 4] = (uint8_t)q.q[i];
+            }
+            if (c == 0) {
+                reinterpret_cast<uint16_t*>(sh.vs)[g] = q.s;
+                sh.vlo[g] = q.lo;
+            }
         }
     }
     __syncthreads();
+
+    WaveKv4 st;
+    st.m = -INFINITY;
+    st.l = st.l16 = st.lo = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        float* P = A.partial + ((size_t)(bg * (size_t)A.nsplit + split) * 4 + h) * KV4_PART_STRIDE;
-        P[tid] = acc[h];
-        if (tid == 0) { P[256] = top[h]; P[257] = total[h]; }
+    for (int m = 0; m < 16; ++m) st.o[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const PartMasks pm = part_masks(c >> 2);
+    const uint16_t* qsrc = &sh.q[min(c, 12)][8 * g];
+    const float qsum = sh.qsum[c & 3][c >> 2];
+    const int new_half = __builtin_amdgcn_readfirstlane(appends ? pos / QMK_KV4_HALF_TOKENS : -1);
+    for (int h = h0; h < h_end; h += KV4_WAVES) {
+        const bool more = h + KV4_WAVES < h_end;
+        bool next_there = false;
+        uint8_t* next = nullptr;
+        if (more) next = half_of(h + KV4_WAVES, next_there);
+        float x[8];
+        if (there) {
+            if (h == new_half) {
+                const int t = pos & (QMK_KV4_HALF_TOKENS - 1);
+                put_k(k, sh, t, half, lane);
+                put_meta(k.s, k.lo, sh.ks, sh.klo, t, half + QMK_KV4_META, lane);
+                put_v(v, sh, t, half, lane);
+                put_meta(v.s, v.lo, sh.vs, sh.vlo, t, half + QMK_KV4_META + 512, lane);
+            }
+            scores(x, k, qsrc, qsum);
+        }
+        if (more) load_k(k, next, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        if (there) weigh(st, x, v, pm, t_end - h * QMK_KV4_HALF_TOKENS, lane);
+        if (more) load_v(v, next, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        half = next;
+        there = next_there;
+    }
+
+    // Join the parts (lane groups) of each head: after both swaps lane group g
+    // has head {0, 2, 1, 3}[g] of dims 16 m + c.  Its minimum term stands in
+    // the lanes of that head and group.
+    {
+        const float l = sum_xor32(sum_xor16(fmaf(st.l16, 16.0f, st.l))), lo = sum_xor32(sum_xor16(st.lo));
+        if (lane < 4) {
+            sh.m[w][lane] = st.m;
+            sh.l[w][lane] = l * 0x1p-90f;
+        }
+        const int head = ((g & 1) << 1) | (g >> 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float base = __shfl(lo, 4 * j + head) * 0x1p-90f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const floatx4 o = st.o[4 * j + m];
+                const auto s01 = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[0]), __float_as_uint(o[1]), false, false);
+                const auto s23 = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[2]), __float_as_uint(o[3]), false, false);
+                const float a = __uint_as_float(s01[0]) + __uint_as_float(s01[1]), d = __uint_as_float(s23[0]) + __uint_as_float(s23[1]);
+                const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(d), false, false);
+                sh.acc[w][head][64 * j + 16 * m + c] = fmaf(__uint_as_float(s[0]) + __uint_as_float(s[1]), 0x1p43f, base);
+            }
+        }
+    }
+    __syncthreads();
+    {
+        const int h = w;                                    // head 4 kvh + h, dims 4 lane .. + 3
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KV4_WAVES; ++i) M = fmaxf(M, sh.m[i][h]);
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < KV4_WAVES; ++i) {
+            if (sh.l[i][h] == 0.0f) continue;               // uniform: no tokens
+            const float f = sh.m[i][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sh.m[i][h] - M);
+            l = fmaf(sh.l[i][h], f, l);
+            const float4 a = *reinterpret_cast<const float4*>(&sh.acc[i][h][4 * lane]);
+            o.x = fmaf(a.x, f, o.x);
+            o.y = fmaf(a.y, f, o.y);
+            o.z = fmaf(a.z, f, o.z);
+            o.w = fmaf(a.w, f, o.w);
+        }
+        if (A.nsplit == 1) {
+            kv4_out(A, b, 4 * kvh + h, lane, o, l, kv4_gate(A, b, 4 * kvh + h, lane), r.refused);
+        } else {
+            float* P = A.partial + (((size_t)bg * A.nsplit + split) * 4 + h) * KV4_PART_STRIDE;
+            st4(P + 4 * lane, o);
+            if (lane == 0) *reinterpret_cast<float2*>(P + 256) = make_float2(M, l);
+        }
     }
 }
 
-// The splits' partials of one query head, joined, and the gate.
-extern "C" __global__ __launch_bounds__(256) void qm_gqa_kv4_merge(GqaKv4Args A) {
-    const int d = threadIdx.x, h = blockIdx.x % QM_GQA_HEADS, b = blockIdx.x / QM_GQA_HEADS;
-    const StepRow r = step_row(A, b);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int s = 0; s < A.nsplit; ++s) {
-        const float* P = A.partial + ((size_t)((b * 4 + (h >> 2)) * (size_t)A.nsplit + s) * 4 + (h & 3)) * KV4_PART_STRIDE;
-        const float ms = P[256];
-        if (P[257] == 0.0f) continue;                 // no tokens
-        const float mn = fmaxf(m, ms), c0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), c1 = __builtin_amdgcn_exp2f(ms - mn);
-        l = l * c0 + P[257] * c1;
-        o = o * c0 + P[d] * c1;
-        m = mn;
-    }
+// The splits' partials of query head h of batch row b, joined, and the gate:
+// one wave per (b, h, 64 dims), 32 splits' loads in flight at a time.
+#define KV4_MERGE_BATCH 32
+extern "C" __global__ __launch_bounds__(64) void qm_gqa_kv4_merge(GqaKv4Args A) {
+    const int lane = threadIdx.x, d = 64 * (blockIdx.x & 3) + lane;
+    const int h = (blockIdx.x >> 2) % QM_GQA_HEADS, b = blockIdx.x / (4 * QM_GQA_HEADS);
     const float gate = A.q_gate[((size_t)b * QM_GQA_HEADS + h) * (2 * QM_GQA_HD) + QM_GQA_HD + d];
+    const float* P = A.partial + ((size_t)(b * QM_GQA_KV_HEADS + (h >> 2)) * A.nsplit * 4 + (h & 3)) * KV4_PART_STRIDE;
+    const size_t step = 4 * KV4_PART_STRIDE;
+    const StepRow r = step_row(A, b);
+    const int n = (r.len + A.chunk - 1) / A.chunk;
+    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    for (int s0 = 0; s0 < n; s0 += KV4_MERGE_BATCH) {       // uniform
+        float a[KV4_MERGE_BATCH];
+#pragma unroll
+        for (int j = 0; j < KV4_MERGE_BATCH; ++j) a[j] = P[(size_t)min(s0 + j, n - 1) * step + d];
+        float2 ml = *reinterpret_cast<const float2*>(P + (size_t)min(s0 + lane, n - 1) * step + 256);
+        const bool some = lane < KV4_MERGE_BATCH && s0 + lane < n && ml.y != 0.0f;     // a split of tokens
+        const float mb = fmaxf(m, max_xor32(max_xor16(row_max16(some ? ml.x : -INFINITY))));
+        const float c = m == mb ? 1.0f : __builtin_amdgcn_exp2f(m - mb);
+        const float f = !some ? 0.0f : ml.x == mb ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mb);
+        l = l * c + wave_sum64(some ? ml.y * f : 0.0f);
+        o *= c;
+#pragma unroll
+        for (int j = 0; j < KV4_MERGE_BATCH; ++j) {
+            const float fj = readlane_f32(f, j);
+            o = fj != 0.0f ? fmaf(a[j], fj, o) : o;
+        }
+        m = mb;
+    }
     float y = l != 0.0f ? (o * __builtin_amdgcn_rcpf(l)) * sigmoid_fast(gate) : 0.0f;
     if (r.refused) y = __builtin_nanf("");
     A.out[((size_t)b * QM_GQA_HEADS + h) * QM_GQA_HD + d] = y;

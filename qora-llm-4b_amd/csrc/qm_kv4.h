@@ -32,6 +32,7 @@
 #define QMK_KV4_META 8192           // first byte of the scales and minima
 #define QMK_KV4_MAX_COUNT 1024      // rows of one resize or fork: one thread each
 #define QMK_KV4_MAX_ROWS 65536      // table rows: the LDS bitmap of those seen
+#define QMK_KV4_MAX_SPLIT 4096      // tokens of a decode workgroup: 64 pages
 #define QMK_KV4_LEN_PAGES 33554431  // pages of a row: its length is an int32
 
 #ifdef __HIPCC__
@@ -123,6 +124,6 @@ struct GqaKv4Args {
     float* out;              // [B][16][256]
     float* partial;          // [B][4][nsplit][4 heads][260]: acc[256], m, l, pad
     int32_t layer, batch, max_len;
-    int32_t chunk;           // tokens per split, a multiple of 64
+    int32_t chunk;           // tokens per split, a multiple of 128, at most QMK_KV4_MAX_SPLIT
     int32_t nsplit;
 };

@@ -111,14 +111,16 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
     return Fault{};
 }
 
-// Tokens per split workgroup, whole pages: as many splits as give the chip
-// about eight workgroups per CU, at most 64 per sequence and head (the merge
-// folds them in one pass).
+// Tokens per split workgroup: a multiple of 128 (a round of its four waves),
+// at most QMK_KV4_MAX_SPLIT (its page ids are one a lane), and within that at
+// most 64 splits per sequence and head and about kSplitGroups workgroups.
+constexpr int64_t kSplitGroups = 2048;
 inline int64_t split_tokens(int64_t len, int32_t batch) {
     int64_t want = (len + 63) / 64;
-    const int64_t fill = (len * batch * 4 + 2047) / 2048;
+    const int64_t fill = (len * batch * 4 + kSplitGroups - 1) / kSplitGroups;
     if (fill > want) want = fill;
-    return (want + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS * QMK_KV4_PAGE_TOKENS;
+    want = (want + 127) / 128 * 128;
+    return want < QMK_KV4_MAX_SPLIT ? want : QMK_KV4_MAX_SPLIT;
 }
 inline int64_t splits(int64_t len, int32_t batch) {
     const int64_t t = split_tokens(len, batch);
@@ -135,13 +137,16 @@ inline size_t decode_ws(int32_t batch, int64_t nsplit) { return static_cast<size
 
 // A bound of all of them for batches up to `batch` over lengths up to `len`,
 // a pool of no more pages than those need, forks and resizes of at most
-// `batch` rows (decode: splits are whole pages, at most 64 per sequence, and
-// batch * splits at most 512 + batch).
+// `batch` rows.  Decode: below the cap a split holds at least len / 64 and
+// len batch 4 / kSplitGroups tokens; at the cap there are ceil(len / 4096).
 inline size_t reserve_ws(int32_t batch, int32_t len) {
     const int64_t pages = (static_cast<int64_t>(len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
-    const int64_t each = pages < 64 ? pages : 64;
-    int64_t all = each * batch;
-    if (all > 512 + static_cast<int64_t>(batch)) all = 512 + static_cast<int64_t>(batch);
+    const int64_t capped = (static_cast<int64_t>(len) + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT;
+    int64_t each = capped > 64 ? capped : 64;
+    if (pages < each) each = pages;
+    int64_t all = kSplitGroups / 4 + batch;
+    if (capped * batch > all) all = capped * batch;
+    if (each * batch < all) all = each * batch;
     size_t ws = static_cast<size_t>(all) * 4 * 4 * 260 * 4;
     const size_t lists = resize_ws(batch), forks = fork_ws(batch, static_cast<int32_t>(pages));
     const size_t pool = 4 * (4 + 3 * static_cast<size_t>(pages) * static_cast<size_t>(batch));

@@ -68,7 +68,7 @@ struct qm_context {
     hipFunction_t f_kv4_resize = nullptr, f_kv4_resize_pages = nullptr;
     hipFunction_t f_kv4_fork = nullptr, f_kv4_fork_rows = nullptr;
     hipFunction_t f_kv4_compact = nullptr, f_kv4_compact_pages = nullptr;
-    hipFunction_t f_gqa_kv4_append = nullptr, f_gqa_kv4_split = nullptr, f_gqa_kv4_merge = nullptr;
+    hipFunction_t f_gqa_kv4_split = nullptr, f_gqa_kv4_merge = nullptr;
     int lm_head_hidden = 0;              // the hidden size lm_head_wg_per_cu was computed for
     int lm_head_wg_per_cu = 1;
     int dnp_chunk_threads = 0;     // the DeltaNet prefill chunk kernel's workgroup size (its launch bounds)
@@ -399,7 +399,6 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_fork_rows", &c->f_kv4_fork_rows);
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_compact", &c->f_kv4_compact);
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_compact_pages", &c->f_kv4_compact_pages);
-    if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_append", &c->f_gqa_kv4_append);
     if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_split", &c->f_gqa_kv4_split);
     if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_merge", &c->f_gqa_kv4_merge);
     if (st == QM_OK &&
@@ -1326,17 +1325,15 @@ int32_t qm_gqa_decode_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* c
     hipStream_t s = pick(c, stream);
     const int64_t chunk = qm_kv4::split_tokens(max_len, batch), nsplit = qm_kv4::splits(max_len, batch);
     const uint64_t grid = static_cast<uint64_t>(batch) * QM_GQA_KV_HEADS * nsplit;
-    if (grid > 0x7fffffffull || static_cast<uint64_t>(batch) * QM_GQA_HEADS > 0x7fffffffull)
+    if (grid > 0x7fffffffull || static_cast<uint64_t>(batch) * QM_GQA_HEADS * 4 > 0x7fffffffull)
         return fail(c, QM_ERR_INVALID_ARG, "qm_gqa_decode_kv4: grid too large");
-    int32_t st = ensure(c, s, qm_kv4::decode_ws(batch, nsplit));
+    int32_t st = ensure(c, s, nsplit > 1 ? qm_kv4::decode_ws(batch, nsplit) : 0);
     if (st != QM_OK) return st;
     GqaKv4Args a{kv4_of(*cache), slots, q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, result, out,
                  static_cast<float*>(c->ws), layer, batch, max_len, static_cast<int32_t>(chunk), static_cast<int32_t>(nsplit)};
-    st = launch(c, c->f_gqa_kv4_append, static_cast<uint32_t>(batch) * QM_GQA_KV_HEADS, 64, a, s, "qm_gqa_kv4_append");
-    if (st != QM_OK) return st;
     st = launch(c, c->f_gqa_kv4_split, static_cast<uint32_t>(grid), 256, a, s, "qm_gqa_kv4_split");
-    if (st != QM_OK) return st;
-    return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(batch) * QM_GQA_HEADS, 256, a, s, "qm_gqa_kv4_merge");
+    if (st != QM_OK || nsplit == 1) return st;
+    return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(batch) * QM_GQA_HEADS * 4, 64, a, s, "qm_gqa_kv4_merge");
 }
 
 }  // extern "C"

@@ -183,8 +183,8 @@ def test_splits_cover_the_length_in_whole_pages_and_fit_the_reserve():
     sizes = [(n, b) for n in (1, 63, 64, 65, 4097, 20000, 32769, 131072, 2 ** 20, 2 ** 31 - 1) for b in (1, 2, 7, 19, 64, 200, 1024)]
     got = [[int(x) for x in a.split()] for a in ask([f"split {n} {b}" for n, b in sizes] + [f"ws {n} {b}" for n, b in sizes])]
     for (n, b), (tokens, splits), (ws, reserve) in zip(sizes, got, got[len(sizes):]):
-        assert tokens % 64 == 0 and (splits - 1) * tokens < n <= splits * tokens
-        assert splits <= 64 and b * splits <= 512 + b
+        assert tokens % 128 == 0 and tokens <= 4096 and (splits - 1) * tokens < n <= splits * tokens
+        assert tokens == 4096 or (splits <= 64 and b * splits <= 512 + b)
         assert ws <= reserve, (n, b)
     # a reserve for the largest covers the smaller
     reserve = int(ask(["ws 32769 64"])[0].split()[1])
