@@ -119,39 +119,41 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 #define KV4_Q_STRIDE (QM_GQA_HD + 8)   // bf16 of a q row in LDS: 16 rows 528 bytes apart fall into different banks
 #define KV4_P_BIAS 90.0f               // p and q carry 2^90: codes are bf16 subnormals
 
-// What a wave loads of half a page: lane (g, c) = (lane >> 4, lane & 15).
+// What a wave loads of half a page, dword by dword: lane (g, c) = (lane >> 4,
+// lane & 15).
 struct HalfK {
-    uint4 w[2][2];           // codes of token 16 u + c, dims 32 s + 8 g .. + 7 in word s = 4 h + i of [u][h]
-    uint4 s[4];              // scales of tokens 16 u + 4 g + i, four groups each
-    uint4 lo;                // minima of those eight tokens, group c >> 2
+    uint32_t w[2][8];        // codes of token 16 u + c, dims 32 s + 8 g .. + 7 in [u][s]
+    uint32_t s[8][2];        // scales of token 16 u + 4 g + i, groups 2 n and 2 n + 1, in [4 u + i][n]
+    uint32_t lo[4];          // minima of those tokens, group c >> 2: tokens 2 n and 2 n + 1 in [n]
 };
 struct HalfV {
-    uint4 w[4];              // codes of dims 64 j + 16 m + c in word m of [j], tokens 16 u + 4 g + i
-    uint4 s[4];
-    uint4 lo;
+    uint32_t w[16];          // codes of dim 16 m + c, tokens 16 u + 4 g + i, in [m]
+    uint32_t s[8][2];
+    uint32_t lo[4];
 };
-QM_DEV void load_meta(uint4 (&s)[4], uint4& lo, const uint8_t* meta, int lane) {
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+QM_DEV void load4(uint32_t* into, const uint8_t* from) {
+    const uintx4 v = *reinterpret_cast<const uintx4*>(from);
+    into[0] = v[0], into[1] = v[1], into[2] = v[2], into[3] = v[3];
+}
+QM_DEV void store4(uint8_t* into, const uint32_t* v) {
+    *reinterpret_cast<uintx4*>(into) = uintx4{v[0], v[1], v[2], v[3]};
+}
+QM_DEV void load_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint8_t* meta, int lane) {
     const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = *reinterpret_cast<const uint4*>(meta + 64 * g + 16 * i);
-    lo = *reinterpret_cast<const uint4*>(meta + 256 + (4 * (c >> 2) + g) * 16);
+    for (int i = 0; i < 4; ++i) load4(&s[2 * i][0], meta + 64 * g + 16 * i);
+    load4(lo, meta + 256 + (4 * (c >> 2) + g) * 16);
 }
 QM_DEV void load_k(HalfK& k, const uint8_t* half, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) k.w[i >> 1][i & 1] = *reinterpret_cast<const uint4*>(half + 1024 * i + 16 * lane);
+    for (int i = 0; i < 4; ++i) load4(&k.w[i >> 1][4 * (i & 1)], half + 1024 * i + 16 * lane);
     load_meta(k.s, k.lo, half + QMK_KV4_META, lane);
 }
 QM_DEV void load_v(HalfV& v, const uint8_t* half, int lane) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v.w[j] = *reinterpret_cast<const uint4*>(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
+    for (int j = 0; j < 4; ++j) load4(&v.w[4 * j], half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
     load_meta(v.s, v.lo, half + QMK_KV4_META + 512, lane);
-}
-QM_DEV uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-QM_DEV void set_word(uint4& v, int i, uint32_t x) {
-    if (i == 0) v.x = x;
-    else if (i == 1) v.y = x;
-    else if (i == 2) v.z = x;
-    else v.w = x;
 }
 
 // The eight codes of a word as bf16 subnormals, elements 2, 3, 6, 7 times 16.
@@ -205,50 +207,49 @@ struct SplitKv4Lds {
 // from them to the page.
 QM_DEV void put_k(HalfK& k, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
     const int c = lane & 15, g = lane >> 4, u = t >> 4;
-    if (c == (t & 15)) {
+    const bool mine = c == (t & 15);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sh.kw[h][g]);
-            k.w[0][h] = u == 0 ? w : k.w[0][h];
-            k.w[1][h] = u == 1 ? w : k.w[1][h];
-            *reinterpret_cast<uint4*>(half + 1024 * (2 * u + h) + 16 * lane) = w;
+    for (int h = 0; h < 2; ++h) {
+        uint32_t n[4];
+        load4(n, reinterpret_cast<const uint8_t*>(sh.kw[h][g]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k.w[0][4 * h + i] = mine && u == 0 ? n[i] : k.w[0][4 * h + i];
+            k.w[1][4 * h + i] = mine && u == 1 ? n[i] : k.w[1][4 * h + i];
         }
+        if (mine) store4(half + 1024 * (2 * u + h) + 16 * lane, n);
     }
 }
-QM_DEV void put_meta(uint4 (&s)[4], uint4& lo, const uint32_t (&ns)[2], const uint16_t (&nlo)[4], int t, uint8_t* meta, int lane) {
+QM_DEV void put_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint32_t (&ns)[2], const uint16_t (&nlo)[4], int t,
+                     uint8_t* meta, int lane) {
     const int c = lane & 15, g = lane >> 4, e = 4 * (t >> 4) + (t & 3);
-    if (g != ((t >> 2) & 3)) return;
+    const bool mine = g == ((t >> 2) & 3);
+    const uint32_t s01 = ns[0], s23 = ns[1], n = nlo[c >> 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s[i][0] = mine && i == e ? s01 : s[i][0];
+        s[i][1] = mine && i == e ? s23 : s[i][1];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (i == e >> 1) {
-            if (e & 1) { s[i].z = ns[0]; s[i].w = ns[1]; }
-            else { s[i].x = ns[0]; s[i].y = ns[1]; }
-        }
+        lo[i] = mine && e == 2 * i ? (lo[i] & 0xffff0000u) | n : lo[i];
+        lo[i] = mine && e == 2 * i + 1 ? (lo[i] & 0xffffu) | n << 16 : lo[i];
     }
-    const uint32_t n = nlo[c >> 2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i == e >> 1) {
-            const uint32_t w = word_of(lo, i);
-            set_word(lo, i, e & 1 ? (w & 0xffffu) | n << 16 : (w & 0xffff0000u) | n);
-        }
-    }
-    if (c == 0) *reinterpret_cast<uint2*>(meta + 64 * g + 8 * e) = make_uint2(ns[0], ns[1]);
-    if ((c & 3) == 0) *reinterpret_cast<uint16_t*>(meta + 256 + (4 * (c >> 2) + g) * 16 + 2 * e) = (uint16_t)n;
+    if (mine && c == 0) *reinterpret_cast<uint2*>(meta + 64 * g + 8 * e) = make_uint2(s01, s23);
+    if (mine && (c & 3) == 0) *reinterpret_cast<uint16_t*>(meta + 256 + (4 * (c >> 2) + g) * 16 + 2 * e) = (uint16_t)n;
 }
 QM_DEV void put_v(HalfV& v, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
     const int c = lane & 15, g = lane >> 4;
-    if (g != ((t >> 2) & 3)) return;
+    const bool mine = g == ((t >> 2) & 3);
     const int shift = 4 * kv4_v_nibble(t);
-    const uint4 q = *reinterpret_cast<const uint4*>(sh.vq[c]);
+    const uint32_t keep = mine ? ~(15u << shift) : ~0u;
+    uint32_t q[4];
+    load4(q, sh.vq[c]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int m = 0; m < 16; ++m) v.w[m] = (v.w[m] & keep) | (((q[m >> 2] >> (8 * (m & 3))) & 15u) << shift & ~keep);
+    if (mine) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const uint32_t code = (word_of(q, j) >> (8 * m)) & 15u;
-            set_word(v.w[j], m, (word_of(v.w[j], m) & ~(15u << shift)) | (code << shift));
-        }
-        *reinterpret_cast<uint4*>(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane) = v.w[j];
+        for (int j = 0; j < 4; ++j) store4(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane, &v.w[4 * j]);
     }
 }
 
@@ -265,19 +266,18 @@ QM_DEV void scores(float (&x)[8], const HalfK& k, const uint16_t* qsrc, float qs
         const bf16x8 q = *reinterpret_cast<const bf16x8*>(qsrc + 32 * s);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            acc[u][s >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(word_of(k.w[u][s >> 2], s & 3)), q, acc[u][s >> 1], 0, 0, 0);
+            acc[u][s >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(k.w[u][s]), q, acc[u][s >> 1], 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4& s = k.s[2 * u + (i >> 1)];
-            const half2_t s01 = halves(i & 1 ? s.z : s.x), s23 = halves(i & 1 ? s.w : s.y);
+            const half2_t s01 = halves(k.s[4 * u + i][0]), s23 = halves(k.s[4 * u + i][1]);
             float t = fmaf(acc[u][0][i], (float)s01[0], 0.0f);
             t = fmaf(acc[u][1][i], (float)s01[1], t);
             t = fmaf(acc[u][2][i], (float)s23[0], t);
             t = fmaf(acc[u][3][i], (float)s23[1], t);
-            const float lo = (float)halves(word_of(k.lo, 2 * u + (i >> 1)))[i & 1];
+            const float lo = (float)halves(k.lo[2 * u + (i >> 1)])[i & 1];
             t = fmaf(t, 0x1p43f, lo * qsum);
             t += dpp_f32<0x128>(t);                  // the parts: columns 8 and 4 apart
             x[4 * u + i] = t + dpp_f32<0x124>(t);
@@ -291,13 +291,12 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
     if (left < QMK_KV4_HALF_TOKENS) {                // uniform: tokens from `left` on are none
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (16 * (e >> 2) + 4 * g + (e & 3) < left) continue;
-            x[e] = -INFINITY;
+            const bool none = 16 * (e >> 2) + 4 * g + (e & 3) >= left;
+            x[e] = none ? -INFINITY : x[e];
             // whatever stands there: a weight of zero times it must be zero
-            if (e & 1) { v.s[e >> 1].z = 0; v.s[e >> 1].w = 0; }
-            else { v.s[e >> 1].x = 0; v.s[e >> 1].y = 0; }
-            const uint32_t w = word_of(v.lo, e >> 1);
-            set_word(v.lo, e >> 1, e & 1 ? w & 0xffffu : w & 0xffff0000u);
+            v.s[e][0] = none ? 0u : v.s[e][0];
+            v.s[e][1] = none ? 0u : v.s[e][1];
+            v.lo[e >> 1] = none ? v.lo[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u) : v.lo[e >> 1];
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -326,7 +325,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
     float lo = 0.0f, lo16 = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float w = (float)halves(word_of(v.lo, e >> 1))[e & 1];
+        const float w = (float)halves(v.lo[e >> 1])[e & 1];
         if (e & 2) lo16 = fmaf(p[e], w, lo16);
         else lo = fmaf(p[e], w, lo);
     }
@@ -339,8 +338,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
             uint32_t part[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint4& s = v.s[i];
-                const float sc = (float)halves(h ? (j < 2 ? s.z : s.w) : (j < 2 ? s.x : s.y))[j & 1];
+                const float sc = (float)halves(v.s[2 * i + h][j >> 1])[j & 1];
                 part[h] = part_of(fmaf(p[2 * i + h], sc, 0.0f), pm);
             }
             a[i] = pack_hi(part[0], part[1]);
@@ -348,7 +346,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
         const bf16x8 w = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(word_of(v.w[j], m)), st.o[4 * j + m], 0, 0, 0);
+            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(v.w[4 * j + m]), st.o[4 * j + m], 0, 0, 0);
     }
 }
 
