@@ -59,11 +59,25 @@ QM_DEV StepRow step_row(const GqaKv4Args& A, int b) {
     return r;
 }
 
+template <int CTRL>
+QM_DEV double dpp_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+QM_DEV double readlane_f64(double x, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 // Sum over the wave in 64 bits.
 QM_DEV double wave_sum64_f64(double x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
-    return x;
+    x += dpp_f64<0xB1>(x);
+    x += dpp_f64<0x4E>(x);
+    x += dpp_f64<0x141>(x);
+    x += dpp_f64<0x140>(x);
+    return (readlane_f64(x, 0) + readlane_f64(x, 16)) + (readlane_f64(x, 32) + readlane_f64(x, 48));
 }
 
 // The new k row of a head as the f16 cache holds it: per-head RMSNorm
@@ -74,12 +88,16 @@ QM_DEV void new_k(const float4 x, uint2 gw, float4 c, float4 s, int lane, uint16
     const double v[4] = {x.x, x.y, x.z, x.w};
     const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
     const uint16_t g[4] = {(uint16_t)(gw.x & 0xffffu), (uint16_t)(gw.x >> 16), (uint16_t)(gw.y & 0xffffu), (uint16_t)(gw.y >> 16)};
-    const double sum = wave_sum64_f64((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
-    const double inv = 1.0 / __builtin_sqrt(sum / QM_GQA_HD + 1e-6);
+    const double mean = wave_sum64_f64((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3])) * (1.0 / QM_GQA_HD) + 1e-6;
+    // v_rsq_f64 is good to about 2^-24; each step of Newton's squares the error
+    double inv = __builtin_amdgcn_rsq(mean);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) inv = inv * __builtin_fma(-0.5 * mean * inv, inv, 1.5);
+    if (!(mean < __builtin_inf())) inv = mean == mean ? 0.0 : mean;      // rsq's own 0 for an infinity, NaN for NaN
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const double y = v[i] * inv * (1.0 + (double)f16_to_f32(g[i]));
-        const double partner = __shfl_xor(y, 8);
+        const double partner = dpp_f64<0x128>(y);
         const double turned = lane < 8 ? y * cc[i] - partner * ss[i] : y * cc[i] + partner * ss[i];
         out[i] = f64_to_f16_by_f32(lane < 16 ? turned : y);
     }
@@ -105,7 +123,7 @@ QM_DEV CodedRow code_row(const uint16_t (&h)[4]) {
     CodedRow c;
     c.s = bad ? (uint16_t)0x7e00u : kv4_scale(lo, hi);
     c.lo = bad ? (uint16_t)0x7e00u : f32_to_f16(lo);
-    const float s = f16_to_f32(c.s), inv = s > 0.0f ? 1.0f / s : 0.0f;
+    const float s = f16_to_f32(c.s), inv = __builtin_amdgcn_rcpf(s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) c.q[i] = kv4_code(x[i], lo, s, inv);
     return c;
@@ -119,41 +137,26 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 #define KV4_Q_STRIDE (QM_GQA_HD + 8)   // bf16 of a q row in LDS: 16 rows 528 bytes apart fall into different banks
 #define KV4_P_BIAS 90.0f               // p and q carry 2^90: codes are bf16 subnormals
 
-// What a wave loads of half a page, dword by dword: lane (g, c) = (lane >> 4,
-// lane & 15).
-struct HalfK {
-    uint32_t w[2][8];        // codes of token 16 u + c, dims 32 s + 8 g .. + 7 in [u][s]
-    uint32_t s[8][2];        // scales of token 16 u + 4 g + i, groups 2 n and 2 n + 1, in [4 u + i][n]
-    uint32_t lo[4];          // minima of those tokens, group c >> 2: tokens 2 n and 2 n + 1 in [n]
-};
-struct HalfV {
-    uint32_t w[16];          // codes of dim 16 m + c, tokens 16 u + 4 g + i, in [m]
-    uint32_t s[8][2];
-    uint32_t lo[4];
-};
+// A wave's half pages come by LDS DMA, as they stand, into one of its two
+// buffers, the one after the next in flight; lane (g, c) = (lane >> 4,
+// lane & 15) reads its operands from there.
+#define KV4_DMA (QMK_KV4_HALF_BYTES / 1024)
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
-QM_DEV void load4(uint32_t* into, const uint8_t* from) {
+QM_DEV void lds4(uint32_t* into, const uint8_t* from) {
     const uintx4 v = *reinterpret_cast<const uintx4*>(from);
     into[0] = v[0], into[1] = v[1], into[2] = v[2], into[3] = v[3];
 }
-QM_DEV void store4(uint8_t* into, const uint32_t* v) {
-    *reinterpret_cast<uintx4*>(into) = uintx4{v[0], v[1], v[2], v[3]};
+QM_DEV void fetch_half(const uint8_t* half, uint32_t buf, int lane) {
+#pragma unroll
+    for (int i = 0; i < KV4_DMA; ++i) dma16_off(half + 1024 * i, 16 * lane, buf + 1024 * i);
 }
-QM_DEV void load_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint8_t* meta, int lane) {
+// Scales of token 16 u + 4 g + i, groups 2 n and 2 n + 1, in s[4 u + i][n];
+// minima of those tokens, group c >> 2: tokens 2 n and 2 n + 1 in lo[n].
+QM_DEV void read_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint8_t* meta, int lane) {
     const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load4(&s[2 * i][0], meta + 64 * g + 16 * i);
-    load4(lo, meta + 256 + (4 * (c >> 2) + g) * 16);
-}
-QM_DEV void load_k(HalfK& k, const uint8_t* half, int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load4(&k.w[i >> 1][4 * (i & 1)], half + 1024 * i + 16 * lane);
-    load_meta(k.s, k.lo, half + QMK_KV4_META, lane);
-}
-QM_DEV void load_v(HalfV& v, const uint8_t* half, int lane) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) load4(&v.w[4 * j], half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
-    load_meta(v.s, v.lo, half + QMK_KV4_META + 512, lane);
+    for (int i = 0; i < 4; ++i) lds4(&s[2 * i][0], meta + 64 * g + 16 * i);
+    lds4(lo, meta + 256 + (4 * (c >> 2) + g) * 16);
 }
 
 // The eight codes of a word as bf16 subnormals, elements 2, 3, 6, 7 times 16.
@@ -192,93 +195,72 @@ struct WaveKv4 {
 };
 
 struct SplitKv4Lds {
+    __attribute__((aligned(16))) uint8_t ring[KV4_WAVES][2][QMK_KV4_HALF_BYTES];   // later acc: [wave][head][dim] f32
     __attribute__((aligned(16))) uint16_t q[13][KV4_Q_STRIDE];       // row 4 part + head; row 12 zero
     float qsum[4][4];                                                // [head][group]
-    __attribute__((aligned(16))) float acc[KV4_WAVES][4][QM_GQA_HD];
     float m[KV4_WAVES][4], l[KV4_WAVES][4];
-    // the new token: K words [dims / 128][g], V codes as bytes [c][4 j + m], scales and minima by group
+    // the new token: K words [dims / 128][g], V codes as bytes [c][4 j + m], scales and minima [s, lo of K, of V][group]
     __attribute__((aligned(16))) uint32_t kw[2][4][4];
     __attribute__((aligned(16))) uint8_t vq[16][16];
-    uint32_t ks[2], vs[2];
-    uint16_t klo[4], vlo[4];
+    uint16_t meta[4][4];
 };
 
-// The new token t (0 .. 31 of the half page) into the loaded operands, and
-// from them to the page.
-QM_DEV void put_k(HalfK& k, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
-    const int c = lane & 15, g = lane >> 4, u = t >> 4;
-    const bool mine = c == (t & 15);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t n[4];
-        load4(n, reinterpret_cast<const uint8_t*>(sh.kw[h][g]));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            k.w[0][4 * h + i] = mine && u == 0 ? n[i] : k.w[0][4 * h + i];
-            k.w[1][4 * h + i] = mine && u == 1 ? n[i] : k.w[1][4 * h + i];
-        }
-        if (mine) store4(half + 1024 * (2 * u + h) + 16 * lane, n);
+// The new token t (0 .. 31 of the half page) into the fetched half page and
+// into the cache's.
+QM_DEV void put_token(uint8_t* buf, uint8_t* half, const SplitKv4Lds& sh, int t, int lane) {
+    if (lane < 8) {
+        const uintx4 w = *reinterpret_cast<const uintx4*>(sh.kw[lane >> 2][lane & 3]);
+        const int at = 4 * kv4_k_word(t, 128 * (lane >> 2) + 8 * (lane & 3));
+        *reinterpret_cast<uintx4*>(buf + at) = w;
+        *reinterpret_cast<uintx4*>(half + at) = w;
     }
-}
-QM_DEV void put_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint32_t (&ns)[2], const uint16_t (&nlo)[4], int t,
-                     uint8_t* meta, int lane) {
-    const int c = lane & 15, g = lane >> 4, e = 4 * (t >> 4) + (t & 3);
-    const bool mine = g == ((t >> 2) & 3);
-    const uint32_t s01 = ns[0], s23 = ns[1], n = nlo[c >> 2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        s[i][0] = mine && i == e ? s01 : s[i][0];
-        s[i][1] = mine && i == e ? s23 : s[i][1];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        lo[i] = mine && e == 2 * i ? (lo[i] & 0xffff0000u) | n : lo[i];
-        lo[i] = mine && e == 2 * i + 1 ? (lo[i] & 0xffffu) | n << 16 : lo[i];
-    }
-    if (mine && c == 0) *reinterpret_cast<uint2*>(meta + 64 * g + 8 * e) = make_uint2(s01, s23);
-    if (mine && (c & 3) == 0) *reinterpret_cast<uint16_t*>(meta + 256 + (4 * (c >> 2) + g) * 16 + 2 * e) = (uint16_t)n;
-}
-QM_DEV void put_v(HalfV& v, const SplitKv4Lds& sh, int t, uint8_t* half, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-    const bool mine = g == ((t >> 2) & 3);
     const int shift = 4 * kv4_v_nibble(t);
-    const uint32_t keep = mine ? ~(15u << shift) : ~0u;
-    uint32_t q[4];
-    load4(q, sh.vq[c]);
+    const int at = 4 * kv4_v_word(t, 64 * (lane >> 4) + (lane & 15));
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(&sh.vq[lane & 15][4 * (lane >> 4)]);
+    uint32_t w[4];
+    lds4(w, buf + at);
 #pragma unroll
-    for (int m = 0; m < 16; ++m) v.w[m] = (v.w[m] & keep) | (((q[m >> 2] >> (8 * (m & 3))) & 15u) << shift & ~keep);
-    if (mine) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store4(half + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane, &v.w[4 * j]);
+    for (int m = 0; m < 4; ++m) w[m] = (w[m] & ~(15u << shift)) | ((q >> (8 * m)) & 15u) << shift;
+    *reinterpret_cast<uintx4*>(buf + at) = uintx4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<uintx4*>(half + at) = uintx4{w[0], w[1], w[2], w[3]};
+    if (lane < 16) {
+        const int which = lane >> 2, group = lane & 3;
+        const int m = QMK_KV4_META + 256 * which + 2 * (which & 1 ? kv4_lo_at(t, group) : kv4_s_at(t, group));
+        const uint16_t x = sh.meta[which][group];
+        *reinterpret_cast<uint16_t*>(buf + m) = x;
+        *reinterpret_cast<uint16_t*>(half + m) = x;
     }
 }
 
 // Scores of the half page's 32 tokens: x[4 u + i] of token 16 u + 4 g + i and
 // head c & 3, in units of log2 e / 16.
-QM_DEV void scores(float (&x)[8], const HalfK& k, const uint16_t* qsrc, float qsum) {
+QM_DEV void scores(float (&x)[8], const uint8_t* buf, const uint16_t* qsrc, float qsum, int lane) {
+    uint32_t w[2][8], s[8][2], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds4(&w[i >> 1][4 * (i & 1)], buf + 1024 * i + 16 * lane);
+    read_meta(s, lo, buf + QMK_KV4_META, lane);
     floatx4 acc[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[u][n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const bf16x8 q = *reinterpret_cast<const bf16x8*>(qsrc + 32 * s);
+    for (int n = 0; n < 8; ++n) {
+        const bf16x8 q = *reinterpret_cast<const bf16x8*>(qsrc + 32 * n);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            acc[u][s >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(k.w[u][s]), q, acc[u][s >> 1], 0, 0, 0);
+            acc[u][n >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(w[u][n]), q, acc[u][n >> 1], 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const half2_t s01 = halves(k.s[4 * u + i][0]), s23 = halves(k.s[4 * u + i][1]);
+            const half2_t s01 = halves(s[4 * u + i][0]), s23 = halves(s[4 * u + i][1]);
             float t = fmaf(acc[u][0][i], (float)s01[0], 0.0f);
             t = fmaf(acc[u][1][i], (float)s01[1], t);
             t = fmaf(acc[u][2][i], (float)s23[0], t);
             t = fmaf(acc[u][3][i], (float)s23[1], t);
-            const float lo = (float)halves(k.lo[2 * u + (i >> 1)])[i & 1];
-            t = fmaf(t, 0x1p43f, lo * qsum);
+            t = fmaf(t, 0x1p43f, (float)halves(lo[2 * u + (i >> 1)])[i & 1] * qsum);
             t += dpp_f32<0x128>(t);                  // the parts: columns 8 and 4 apart
             x[4 * u + i] = t + dpp_f32<0x124>(t);
         }
@@ -286,17 +268,21 @@ QM_DEV void scores(float (&x)[8], const HalfK& k, const uint16_t* qsrc, float qs
 }
 
 // The softmax weights of a round, and their products with V.
-QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, int lane) {
+QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, PartMasks pm, int left, int lane) {
     const int g = lane >> 4;
+    uint32_t vw[16], vs[8][2], vlo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds4(&vw[4 * j], buf + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
+    read_meta(vs, vlo, buf + QMK_KV4_META + 512, lane);
     if (left < QMK_KV4_HALF_TOKENS) {                // uniform: tokens from `left` on are none
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool none = 16 * (e >> 2) + 4 * g + (e & 3) >= left;
             x[e] = none ? -INFINITY : x[e];
             // whatever stands there: a weight of zero times it must be zero
-            v.s[e][0] = none ? 0u : v.s[e][0];
-            v.s[e][1] = none ? 0u : v.s[e][1];
-            v.lo[e >> 1] = none ? v.lo[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u) : v.lo[e >> 1];
+            vs[e][0] = none ? 0u : vs[e][0];
+            vs[e][1] = none ? 0u : vs[e][1];
+            vlo[e >> 1] = none ? vlo[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u) : vlo[e >> 1];
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -325,7 +311,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
     float lo = 0.0f, lo16 = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float w = (float)halves(v.lo[e >> 1])[e & 1];
+        const float w = (float)halves(vlo[e >> 1])[e & 1];
         if (e & 2) lo16 = fmaf(p[e], w, lo16);
         else lo = fmaf(p[e], w, lo);
     }
@@ -338,7 +324,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
             uint32_t part[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float sc = (float)halves(v.s[2 * i + h][j >> 1])[j & 1];
+                const float sc = (float)halves(vs[2 * i + h][j >> 1])[j & 1];
                 part[h] = part_of(fmaf(p[2 * i + h], sc, 0.0f), pm);
             }
             a[i] = pack_hi(part[0], part[1]);
@@ -346,7 +332,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], HalfV& v, PartMasks pm, int left, 
         const bf16x8 w = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(v.w[4 * j + m]), st.o[4 * j + m], 0, 0, 0);
+            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(vw[4 * j + m]), st.o[4 * j + m], 0, 0, 0);
     }
 }
 
@@ -362,49 +348,68 @@ QM_DEV float4 kv4_gate(const GqaKv4Args& A, int b, int h, int lane) {
     return ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + h) * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
 }
 
-extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(GqaKv4Args A) {
+QM_DEV uint32_t lds_of(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split(GqaKv4Args A) {
     __shared__ SplitKv4Lds sh;
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % A.nsplit, bg = blockIdx.x / A.nsplit;
     const int kvh = bg & 3, b = bg >> 2;
     const int t_begin = split * A.chunk;
     const StepRow r = step_row(A, b);
-    const int t_end = min(t_begin + A.chunk, r.len);
-    if (t_begin >= t_end && A.nsplit > 1) return;        // uniform: the merge reads the splits of the row's tokens
-    const int h0 = __builtin_amdgcn_readfirstlane(t_begin / QMK_KV4_HALF_TOKENS + w);
-    const int h_end = __builtin_amdgcn_readfirstlane((t_end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
-    // page ids of the split, one a lane (a split has at most 64 pages)
+
+    // The loads that depend on no other: q, the new token's row (wave 0 k, wave
+    // 1 v) and the split's page ids, one a lane (a split has at most 64 pages).
+    const float4 qx = ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + 4 * kvh + w) * (2 * QM_GQA_HD) + 4 * lane);
+    const uint2 qn = *reinterpret_cast<const uint2*>(A.q_norm + 4 * lane);
+    const float4 nx = ld4((w == 0 ? A.k_new : A.v_new) + ((size_t)b * QM_GQA_KV_HEADS + kvh) * QM_GQA_HD + 4 * lane);
+    const uint2 kn = *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane);
     const int page0 = t_begin / QMK_KV4_PAGE_TOKENS;
     int ids = -1;
-    if (t_begin < t_end) {
-        const int at = page0 + lane;
-        if (at < A.c.max_pages && at * (int64_t)QMK_KV4_PAGE_TOKENS < t_end) ids = A.c.table[(size_t)r.row * A.c.max_pages + at];
-    }
+    if (lane < A.chunk / QMK_KV4_PAGE_TOKENS && page0 + lane < A.c.max_pages)
+        ids = A.c.table[(size_t)max(r.row, 0) * A.c.max_pages + page0 + lane];
+
+    const int t_end = min(t_begin + A.chunk, r.len);
+    if (t_begin >= t_end && A.nsplit > 1) return;        // uniform: the merge reads the splits of the row's tokens
+    const int h0 = t_begin / QMK_KV4_HALF_TOKENS + w;
+    const int h_end = __builtin_amdgcn_readfirstlane((t_end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
     auto half_of = [&](int h, bool& there) {
         const int id = __builtin_amdgcn_readlane(ids, (h >> 1) - page0);
         there = kv4_is_page(A.c, id);
         return kv4_half(A.c, A.layer, there ? id : 0, kvh, h & 1);
     };
+    // The compiler does not count the DMA below: what it loads has to be here
+    // before that starts, or its waits would take the DMA's for its own.
+    asm volatile("" ::"v"(qx.x), "v"(qn.x), "v"(nx.x), "v"(kn.x), "v"(ids));
 
-    HalfK k;
-    HalfV v;
-    bool there = false;
-    uint8_t* half = nullptr;
-    if (h0 < h_end) {
-        half = half_of(h0, there);
-        load_k(k, half, lane);
-        load_v(v, half, lane);
+    // The RoPE rows of the new position (to LDS, a q row that this wave writes
+    // later), then the wave's first two half pages.
+    const int pos = max(r.len - 1, 0);
+    uint16_t* rope = sh.q[8 + w];
+    dma4((lane < 32 ? A.rope_cos : A.rope_sin) + (size_t)pos * (QM_GQA_ROT / 2) + (lane & 31), lds_of(rope));
+    bool there[2] = {false, false};
+    uint8_t* half[2] = {nullptr, nullptr};
+    const uint32_t ring = lds_of(sh.ring[w]);
+    int ahead = 0;                                         // DMA instructions after the RoPE rows'
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (h0 + KV4_WAVES * i < h_end) {
+            half[i] = half_of(h0 + KV4_WAVES * i, there[i]);
+            fetch_half(half[i], ring + QMK_KV4_HALF_BYTES * i, lane);
+            ahead += KV4_DMA;
+        }
     }
-    __builtin_amdgcn_sched_barrier(0);
+    if (ahead == 2 * KV4_DMA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KV4_DMA) : "memory");
+    else if (ahead == KV4_DMA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KV4_DMA) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const float4 rc = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rope) + 4 * (lane & 7));
+    const float4 rs = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rope) + 32 + 4 * (lane & 7));
 
     // q of head 4 kvh + w: norm, RoPE, the softmax's scale, and the parts
-    const int pos = max(r.len - 1, 0);
-    float4 rc, rs;
-    rope_row_loads(A.rope_cos + (size_t)pos * (QM_GQA_ROT / 2), A.rope_sin + (size_t)pos * (QM_GQA_ROT / 2), lane, rc, rs);
     const bool appends = pos >= t_begin && pos < t_end;
     {
-        float4 x = norm_rope_head(ld4(A.q_gate + ((size_t)b * QM_GQA_HEADS + 4 * kvh + w) * (2 * QM_GQA_HD) + 4 * lane),
-                                  *reinterpret_cast<const uint2*>(A.q_norm + 4 * lane), rc, rs, lane);
+        float4 x = norm_rope_head(qx, qn, rc, rs, lane);
         const float scale = 1.4426950408889634f / 16.0f;
         x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
         const float sum = row_sum16((x.x + x.y) + (x.z + x.w));
@@ -419,39 +424,30 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(Gq
         if (w == 3) *reinterpret_cast<uint2*>(&sh.q[12][4 * lane]) = make_uint2(0, 0);
     }
     if (appends && w < 2) {                                // uniform per wave
-        const size_t src = ((size_t)b * QM_GQA_KV_HEADS + kvh) * QM_GQA_HD + 4 * lane;
-        uint16_t x[4];
-        if (w == 0) {
-            new_k(ld4(A.k_new + src), *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane), rc, rs, lane, x);
-        } else {
-            const float4 n = ld4(A.v_new + src);
-            x[0] = f32_to_f16(n.x), x[1] = f32_to_f16(n.y), x[2] = f32_to_f16(n.z), x[3] = f32_to_f16(n.w);
-        }
+        uint16_t x[4] = {f32_to_f16(nx.x), f32_to_f16(nx.y), f32_to_f16(nx.z), f32_to_f16(nx.w)};
+        if (w == 0) new_k(nx, kn, rc, rs, lane, x);
         const CodedRow q = code_row(x);
         if (w == 0) {
             uint32_t word = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) word |= q.q[i] << (4 * kv4_nibble(4 * (lane & 1) + i));
-            word |= __shfl_xor(word, 1);
+            word |= __builtin_amdgcn_mov_dpp((int)word, 0xB1, 0xF, 0xF, false);
             const int d = 4 * lane;
             if ((lane & 1) == 0) sh.kw[d >> 7][(d >> 3) & 3][(d >> 5) & 3] = word;
-            if (c == 0) {
-                reinterpret_cast<uint16_t*>(sh.ks)[g] = q.s;
-                sh.klo[g] = q.lo;
-            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 4 * lane + i;                // dim 64 j + 16 m + c
                 sh.vq[d & 15][d >> 4] = (uint8_t)q.q[i];
             }
-            if (c == 0) {
-                reinterpret_cast<uint16_t*>(sh.vs)[g] = q.s;
-                sh.vlo[g] = q.lo;
-            }
+        }
+        if (c == 0) {
+            sh.meta[2 * w][g] = q.s;
+            sh.meta[2 * w + 1][g] = q.lo;
         }
     }
-    __syncthreads();
+    // every wave's q and the new token; the DMA stays in flight
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
     WaveKv4 st;
     st.m = -INFINITY;
@@ -461,30 +457,26 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(Gq
     const PartMasks pm = part_masks(c >> 2);
     const uint16_t* qsrc = &sh.q[min(c, 12)][8 * g];
     const float qsum = sh.qsum[c & 3][c >> 2];
-    const int new_half = __builtin_amdgcn_readfirstlane(appends ? pos / QMK_KV4_HALF_TOKENS : -1);
-    for (int h = h0; h < h_end; h += KV4_WAVES) {
-        const bool more = h + KV4_WAVES < h_end;
-        bool next_there = false;
-        uint8_t* next = nullptr;
-        if (more) next = half_of(h + KV4_WAVES, next_there);
-        float x[8];
-        if (there) {
-            if (h == new_half) {
-                const int t = pos & (QMK_KV4_HALF_TOKENS - 1);
-                put_k(k, sh, t, half, lane);
-                put_meta(k.s, k.lo, sh.ks, sh.klo, t, half + QMK_KV4_META, lane);
-                put_v(v, sh, t, half, lane);
-                put_meta(v.s, v.lo, sh.vs, sh.vlo, t, half + QMK_KV4_META + 512, lane);
-            }
-            scores(x, k, qsrc, qsum);
+    const int new_half = appends ? pos / QMK_KV4_HALF_TOKENS : -1;
+    int i = 0;
+    for (int h = h0; h < h_end; h += KV4_WAVES, i ^= 1) {
+        // this round's half page is here when only the next one's DMA is out
+        if (h + KV4_WAVES < h_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KV4_DMA) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        uint8_t* buf = sh.ring[w][i];
+        if (there[0]) {
+            if (h == new_half) put_token(buf, half[0], sh, pos & (QMK_KV4_HALF_TOKENS - 1), lane);
+            float x[8];
+            scores(x, buf, qsrc, qsum, lane);
+            weigh(st, x, buf, pm, t_end - h * QMK_KV4_HALF_TOKENS, lane);
         }
-        if (more) load_k(k, next, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        if (there) weigh(st, x, v, pm, t_end - h * QMK_KV4_HALF_TOKENS, lane);
-        if (more) load_v(v, next, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        half = next;
-        there = next_there;
+        half[0] = half[1];
+        there[0] = there[1];
+        if (h + 2 * KV4_WAVES < h_end) {
+            half[1] = half_of(h + 2 * KV4_WAVES, there[1]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the buffer's reads are done
+            fetch_half(half[1], ring + QMK_KV4_HALF_BYTES * i, lane);
+        }
     }
 
     // Join the parts (lane groups) of each head: after both swaps lane group g
@@ -497,6 +489,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(Gq
             sh.l[w][lane] = l * 0x1p-90f;
         }
         const int head = ((g & 1) << 1) | (g >> 1);
+        float* acc = reinterpret_cast<float*>(sh.ring[w]);          // the wave's own buffers, all read
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float base = __shfl(lo, 4 * j + head) * 0x1p-90f;
@@ -507,7 +500,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(Gq
                 const auto s23 = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[2]), __float_as_uint(o[3]), false, false);
                 const float a = __uint_as_float(s01[0]) + __uint_as_float(s01[1]), d = __uint_as_float(s23[0]) + __uint_as_float(s23[1]);
                 const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(d), false, false);
-                sh.acc[w][head][64 * j + 16 * m + c] = fmaf(__uint_as_float(s[0]) + __uint_as_float(s[1]), 0x1p43f, base);
+                acc[head * QM_GQA_HD + 64 * j + 16 * m + c] = fmaf(__uint_as_float(s[0]) + __uint_as_float(s[1]), 0x1p43f, base);
             }
         }
     }
@@ -524,7 +517,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES) void qm_gqa_kv4_split(Gq
             if (sh.l[i][h] == 0.0f) continue;               // uniform: no tokens
             const float f = sh.m[i][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sh.m[i][h] - M);
             l = fmaf(sh.l[i][h], f, l);
-            const float4 a = *reinterpret_cast<const float4*>(&sh.acc[i][h][4 * lane]);
+            const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.ring[i]) + h * QM_GQA_HD + 4 * lane);
             o.x = fmaf(a.x, f, o.x);
             o.y = fmaf(a.y, f, o.y);
             o.z = fmaf(a.z, f, o.z);
