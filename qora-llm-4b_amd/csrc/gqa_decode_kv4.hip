@@ -15,15 +15,20 @@
 //   (16 c 2^-133): masks alone make operands of a word (5 instructions for 8
 //   codes).  The other operand carries 2^90 (2^86 for the elements of bits
 //   4..7), which keeps products normal: for p down to 2^-216, q up to 2^37.
-//   That operand is f32 and enters as three bf16 parts, 24 bits, exactly:
-//   four heads x three parts are 12 of the 16 rows (columns) that a matrix
-//   instruction has anyway.
-//   QK: A = 16 tokens' codes, B = q (column 4 part + head).  Lane (g, c) ends
-//   with tokens 4 g .. + 3 of column c; the parts' scores are summed over
-//   columns c & 3 by two DPP adds, so that every lane holds its head's.
-//   PV: A = p s (row 4 part + head; the same lane has the same head's p),
-//   B = the codes of 16 dims, one instruction per 16 dims and 32 tokens.
-//   The minimum terms are the lanes' own: the lane of part j adds group j's.
+//   Products are in units of 2^-43.
+//   That operand is f32 and enters as three bf16 parts, 24 bits, exactly.
+//   QK: A = 16 tokens' codes, B = q (column 4 part + head: 12 of the 16
+//   columns that the instruction has anyway).  Lane (g, c) ends with tokens
+//   4 g .. + 3 of column c; the parts' scores are summed over columns c & 3 by
+//   two DPP adds, so that every lane holds its head's.
+//   PV: A = p s (row 4 group + head, so a lane weighs its head's tokens for
+//   one group only), B = the codes of 16 dims, an instruction per part; of the
+//   result the rows of the dims' own group count.  With the parts as rows each
+//   lane would weigh all four groups: a third of the instructions, but 144
+//   vector instructions a round to make the operands instead of 52, and the
+//   vector unit is what the kernel waits for.
+//   The minimum terms are the lanes' own: the lane of column 4 j + head adds
+//   group j's.
 // Softmax in base 2; a running maximum is raised only where a score passes it
 // by 2^8, so the accumulators are seldom rescaled.
 #include "qm_kv4_device.h"
@@ -150,15 +155,6 @@ QM_DEV void fetch_half(const uint8_t* half, uint32_t buf, int lane) {
 #pragma unroll
     for (int i = 0; i < KV4_DMA; ++i) dma16_off(half + 1024 * i, 16 * lane, buf + 1024 * i);
 }
-// Scales of token 16 u + 4 g + i, groups 2 n and 2 n + 1, in s[4 u + i][n];
-// minima of those tokens, group c >> 2: tokens 2 n and 2 n + 1 in lo[n].
-QM_DEV void read_meta(uint32_t (&s)[8][2], uint32_t (&lo)[4], const uint8_t* meta, int lane) {
-    const int c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lds4(&s[2 * i][0], meta + 64 * g + 16 * i);
-    lds4(lo, meta + 256 + (4 * (c >> 2) + g) * 16);
-}
-
 // The eight codes of a word as bf16 subnormals, elements 2, 3, 6, 7 times 16.
 QM_DEV bf16x8 codes_bf16(uint32_t w) {
     const uint32_t v = w >> 8;
@@ -169,26 +165,17 @@ QM_DEV bf16x8 codes_bf16(uint32_t w) {
     return __builtin_bit_cast(bf16x8, m);
 }
 
-// Part j of an f32: its upper 8, middle 8 or lower 8 bits of significand as a
-// bf16 in the upper half (j = 3: nothing).  hi, lo: the masks of part_masks.
-struct PartMasks {
-    uint32_t hi, lo;
-};
-QM_DEV PartMasks part_masks(int j) {
-    return PartMasks{j == 0 ? 0xffff0000u : j == 1 ? 0xffffff00u : 0xffffffffu,
-                     j == 0 ? 0u : j == 1 ? 0xffff0000u : j == 2 ? 0xffffff00u : 0xffffffffu};
-}
-QM_DEV uint32_t part_of(float x, PartMasks m) {
-    const uint32_t u = __float_as_uint(x);
-    return __float_as_uint(__uint_as_float(u & m.hi) - __uint_as_float(u & m.lo));
-}
+// An f32 with the upper 8 bits of its significand: what a bf16 of its upper
+// half holds.
+QM_DEV float upper8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 QM_DEV uint32_t pack_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 QM_DEV half2_t halves(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
 
-// Per-wave softmax state and accumulators.  o[m]: dims 16 m + c, element e of
-// lane group g: part g of head e, in units of 2^-43; lo: the lane's share of
-// its head's and group's minimum terms, l of its head's sum (elements 2, 3, 6,
-// 7 apart), in units of 2^90.
+// Per-wave softmax state and accumulators.  m: the maximum, in the scores'
+// units.  o[m]: dims 16 m + c; in lane group g = m >> 2, whose group of dims
+// that is, element e is head e's sum, in units of 2^-43; lo: the lane's share
+// of its head's and group's minimum terms, l of its head's sum (elements 2, 3,
+// 6, 7 apart), in units of 2^90.
 struct WaveKv4 {
     float m, l, l16, lo;
     floatx4 o[16];
@@ -233,12 +220,19 @@ QM_DEV void put_token(uint8_t* buf, uint8_t* half, const SplitKv4Lds& sh, int t,
 }
 
 // Scores of the half page's 32 tokens: x[4 u + i] of token 16 u + 4 g + i and
-// head c & 3, in units of log2 e / 16.
+// head c & 3, in units of 2^-43 ln 2 / 16 (as qsum).
+template <int CTRL>
+QM_DEV float add_dpp(float x) {      // update_dpp, unlike mov_dpp, is folded into the add
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
 QM_DEV void scores(float (&x)[8], const uint8_t* buf, const uint16_t* qsrc, float qsum, int lane) {
     uint32_t w[2][8], s[8][2], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) lds4(&w[i >> 1][4 * (i & 1)], buf + 1024 * i + 16 * lane);
-    read_meta(s, lo, buf + QMK_KV4_META, lane);
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds4(&s[2 * i][0], buf + QMK_KV4_META + 64 * g + 16 * i);
+    lds4(lo, buf + QMK_KV4_META + 256 + (4 * (c >> 2) + g) * 16);
     floatx4 acc[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -252,44 +246,43 @@ QM_DEV void scores(float (&x)[8], const uint8_t* buf, const uint16_t* qsrc, floa
             acc[u][n >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(w[u][n]), q, acc[u][n >> 1], 0, 0, 0);
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const half2_t s01 = halves(s[4 * u + i][0]), s23 = halves(s[4 * u + i][1]);
-            float t = fmaf(acc[u][0][i], (float)s01[0], 0.0f);
-            t = fmaf(acc[u][1][i], (float)s01[1], t);
-            t = fmaf(acc[u][2][i], (float)s23[0], t);
-            t = fmaf(acc[u][3][i], (float)s23[1], t);
-            t = fmaf(t, 0x1p43f, (float)halves(lo[2 * u + (i >> 1)])[i & 1] * qsum);
-            t += dpp_f32<0x128>(t);                  // the parts: columns 8 and 4 apart
-            x[4 * u + i] = t + dpp_f32<0x124>(t);
-        }
+    for (int e = 0; e < 8; ++e) {
+        const int u = e >> 2, i = e & 3;
+        const half2_t s01 = halves(s[e][0]), s23 = halves(s[e][1]);
+        float t = fmaf((float)halves(lo[e >> 1])[e & 1], qsum, 0.0f);
+        t = fmaf(acc[u][0][i], (float)s01[0], t);
+        t = fmaf(acc[u][1][i], (float)s01[1], t);
+        t = fmaf(acc[u][2][i], (float)s23[0], t);
+        t = fmaf(acc[u][3][i], (float)s23[1], t);
+        x[e] = add_dpp<0x124>(add_dpp<0x128>(t));                    // the parts: columns 8 and 4 apart
     }
 }
 
 // The softmax weights of a round, and their products with V.
-QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, PartMasks pm, int left, int lane) {
-    const int g = lane >> 4;
-    uint32_t vw[16], vs[8][2], vlo[4];
+QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    uint32_t vw[16], lo[4];
+    uint16_t sv[8];                                      // scales of the lane's eight tokens, group c >> 2
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sv[e] = *reinterpret_cast<const uint16_t*>(buf + QMK_KV4_META + 512 + 64 * g + 8 * e + 2 * (c >> 2));
+    lds4(lo, buf + QMK_KV4_META + 768 + (4 * (c >> 2) + g) * 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) lds4(&vw[4 * j], buf + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
-    read_meta(vs, vlo, buf + QMK_KV4_META + 512, lane);
-    if (left < QMK_KV4_HALF_TOKENS) {                // uniform: tokens from `left` on are none
+    if (left < QMK_KV4_HALF_TOKENS) {                    // uniform: tokens from `left` on are none
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool none = 16 * (e >> 2) + 4 * g + (e & 3) >= left;
             x[e] = none ? -INFINITY : x[e];
             // whatever stands there: a weight of zero times it must be zero
-            vs[e][0] = none ? 0u : vs[e][0];
-            vs[e][1] = none ? 0u : vs[e][1];
-            vlo[e >> 1] = none ? vlo[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u) : vlo[e >> 1];
+            sv[e] = none ? (uint16_t)0 : sv[e];
+            lo[e >> 1] = none ? lo[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u) : lo[e >> 1];
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     mx = max_xor32(max_xor16(mx));
-    if (__ballot(mx > st.m + 8.0f)) {                // uniform
-        const float m = mx > st.m + 8.0f ? mx : st.m;
-        const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+    if (__ballot(mx > st.m + 0x1p-40f)) {                // uniform: 2^8
+        const float m = mx > st.m + 0x1p-40f ? mx : st.m;
+        const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f((st.m - m) * 0x1p43f);
         st.m = m;
         st.l *= f;
         st.l16 *= f;
@@ -303,36 +296,43 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, PartMasks pm, 
             st.o[m4][3] *= f3;
         }
     }
+    const float bias = fmaf(-st.m, 0x1p43f, KV4_P_BIAS), bias16 = fmaf(-st.m, 0x1p43f, KV4_P_BIAS - 4.0f);
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - (st.m - (e & 2 ? KV4_P_BIAS - 4.0f : KV4_P_BIAS)));
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], 0x1p43f, e & 2 ? bias16 : bias));
     st.l += (p[0] + p[1]) + (p[4] + p[5]);
     st.l16 += (p[2] + p[3]) + (p[6] + p[7]);
-    float lo = 0.0f, lo16 = 0.0f;
+    float lo1 = 0.0f, lo16 = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float w = (float)halves(vlo[e >> 1])[e & 1];
+        const float w = (float)halves(lo[e >> 1])[e & 1];
         if (e & 2) lo16 = fmaf(p[e], w, lo16);
-        else lo = fmaf(p[e], w, lo);
+        else lo1 = fmaf(p[e], w, lo1);
     }
-    st.lo += fmaf(lo16, 16.0f, lo);
+    st.lo += fmaf(lo16, 16.0f, lo1);
+    // the three parts of p s: upper 8, middle 8 and lower 8 bits of its significand
+    uint32_t part[3][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t a[4];
+    for (int i = 0; i < 4; ++i) {
+        float a[2], r[2], q[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t part[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float sc = (float)halves(vs[2 * i + h][j >> 1])[j & 1];
-                part[h] = part_of(fmaf(p[2 * i + h], sc, 0.0f), pm);
-            }
-            a[i] = pack_hi(part[0], part[1]);
+        for (int h = 0; h < 2; ++h) {
+            a[h] = fmaf(p[2 * i + h], (float)__builtin_bit_cast(_Float16, sv[2 * i + h]), 0.0f);
+            r[h] = a[h] - upper8(a[h]);
+            q[h] = r[h] - upper8(r[h]);
         }
-        const bf16x8 w = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
+        part[0][i] = pack_hi(__float_as_uint(a[0]), __float_as_uint(a[1]));
+        part[1][i] = pack_hi(__float_as_uint(r[0]), __float_as_uint(r[1]));
+        part[2][i] = pack_hi(__float_as_uint(q[0]), __float_as_uint(q[1]));
+    }
+    bf16x8 a[3];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-            st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, codes_bf16(vw[4 * j + m]), st.o[4 * j + m], 0, 0, 0);
+    for (int n = 0; n < 3; ++n) a[n] = __builtin_bit_cast(bf16x8, uintx4{part[n][0], part[n][1], part[n][2], part[n][3]});
+#pragma unroll
+    for (int m = 0; m < 16; ++m) {
+        const bf16x8 v = codes_bf16(vw[m]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) st.o[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n], v, st.o[m], 0, 0, 0);
     }
 }
 
@@ -413,13 +413,14 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
         const float scale = 1.4426950408889634f / 16.0f;
         x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
         const float sum = row_sum16((x.x + x.y) + (x.z + x.w));
-        if (c == 0) sh.qsum[w][g] = sum;
-        const float y[4] = {x.x * 0x1p90f, x.y * 0x1p90f, x.z * 0x1p86f, x.w * 0x1p86f};
+        if (c == 0) sh.qsum[w][g] = sum * 0x1p-43f;
+        float y[4] = {x.x * 0x1p90f, x.y * 0x1p90f, x.z * 0x1p86f, x.w * 0x1p86f};
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
-            const PartMasks pm = part_masks(j);
             *reinterpret_cast<uint2*>(&sh.q[4 * j + w][4 * lane]) =
-                make_uint2(pack_hi(part_of(y[0], pm), part_of(y[1], pm)), pack_hi(part_of(y[2], pm), part_of(y[3], pm)));
+                make_uint2(pack_hi(__float_as_uint(y[0]), __float_as_uint(y[1])), pack_hi(__float_as_uint(y[2]), __float_as_uint(y[3])));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] -= upper8(y[i]);
         }
         if (w == 3) *reinterpret_cast<uint2*>(&sh.q[12][4 * lane]) = make_uint2(0, 0);
     }
@@ -454,7 +455,6 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     st.l = st.l16 = st.lo = 0.0f;
 #pragma unroll
     for (int m = 0; m < 16; ++m) st.o[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    const PartMasks pm = part_masks(c >> 2);
     const uint16_t* qsrc = &sh.q[min(c, 12)][8 * g];
     const float qsum = sh.qsum[c & 3][c >> 2];
     const int new_half = appends ? pos / QMK_KV4_HALF_TOKENS : -1;
@@ -468,7 +468,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
             if (h == new_half) put_token(buf, half[0], sh, pos & (QMK_KV4_HALF_TOKENS - 1), lane);
             float x[8];
             scores(x, buf, qsrc, qsum, lane);
-            weigh(st, x, buf, pm, t_end - h * QMK_KV4_HALF_TOKENS, lane);
+            weigh(st, x, buf, t_end - h * QMK_KV4_HALF_TOKENS, lane);
         }
         half[0] = half[1];
         there[0] = there[1];
@@ -479,28 +479,22 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
         }
     }
 
-    // Join the parts (lane groups) of each head: after both swaps lane group g
-    // has head {0, 2, 1, 3}[g] of dims 16 m + c.  Its minimum term stands in
-    // the lanes of that head and group.
+    // Lane group g has group g of the dims, for its four heads.  A head's
+    // minimum term of that group stands in the lanes of column 4 g + head.
     {
         const float l = sum_xor32(sum_xor16(fmaf(st.l16, 16.0f, st.l))), lo = sum_xor32(sum_xor16(st.lo));
         if (lane < 4) {
             sh.m[w][lane] = st.m;
             sh.l[w][lane] = l * 0x1p-90f;
         }
-        const int head = ((g & 1) << 1) | (g >> 1);
         float* acc = reinterpret_cast<float*>(sh.ring[w]);          // the wave's own buffers, all read
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float base = __shfl(lo, 4 * j + head) * 0x1p-90f;
+        for (int head = 0; head < 4; ++head) {
+            const float base = __shfl(lo, 4 * g + head) * 0x1p-90f;
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const floatx4 o = st.o[4 * j + m];
-                const auto s01 = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[0]), __float_as_uint(o[1]), false, false);
-                const auto s23 = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[2]), __float_as_uint(o[3]), false, false);
-                const float a = __uint_as_float(s01[0]) + __uint_as_float(s01[1]), d = __uint_as_float(s23[0]) + __uint_as_float(s23[1]);
-                const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(d), false, false);
-                acc[head * QM_GQA_HD + 64 * j + 16 * m + c] = fmaf(__uint_as_float(s[0]) + __uint_as_float(s[1]), 0x1p43f, base);
+                const float a = g & 1 ? st.o[4 + m][head] : st.o[m][head], d = g & 1 ? st.o[12 + m][head] : st.o[8 + m][head];
+                acc[head * QM_GQA_HD + 64 * g + 16 * m + c] = fmaf(g & 2 ? d : a, 0x1p43f, base);
             }
         }
     }
@@ -515,7 +509,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
 #pragma unroll
         for (int i = 0; i < KV4_WAVES; ++i) {
             if (sh.l[i][h] == 0.0f) continue;               // uniform: no tokens
-            const float f = sh.m[i][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sh.m[i][h] - M);
+            const float f = sh.m[i][h] == M ? 1.0f : __builtin_amdgcn_exp2f((sh.m[i][h] - M) * 0x1p43f);
             l = fmaf(sh.l[i][h], f, l);
             const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.ring[i]) + h * QM_GQA_HD + 4 * lane);
             o.x = fmaf(a.x, f, o.x);
@@ -528,7 +522,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
         } else {
             float* P = A.partial + (((size_t)bg * A.nsplit + split) * 4 + h) * KV4_PART_STRIDE;
             st4(P + 4 * lane, o);
-            if (lane == 0) *reinterpret_cast<float2*>(P + 256) = make_float2(M, l);
+            if (lane == 0) *reinterpret_cast<float2*>(P + 256) = make_float2(M * 0x1p43f, l);
         }
     }
 }
