@@ -239,7 +239,8 @@ QM_DEV void scores(float (&x)[8], const uint8_t* buf, const uint16_t* qsrc, floa
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[u][n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
+    for (int i = 0; i < 8; ++i) {
+        const int n = 2 * (i & 3) + (i >> 2);                // both halves of a group four steps apart
         const bf16x8 q = *reinterpret_cast<const bf16x8*>(qsrc + 32 * n);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -329,10 +330,14 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
 #pragma unroll
     for (int n = 0; n < 3; ++n) a[n] = __builtin_bit_cast(bf16x8, uintx4{part[n][0], part[n][1], part[n][2], part[n][3]});
 #pragma unroll
-    for (int m = 0; m < 16; ++m) {
-        const bf16x8 v = codes_bf16(vw[m]);
+    for (int j = 0; j < 4; ++j) {
+        bf16x8 v[4];
 #pragma unroll
-        for (int n = 0; n < 3; ++n) st.o[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n], v, st.o[m], 0, 0, 0);
+        for (int m = 0; m < 4; ++m) v[m] = codes_bf16(vw[4 * j + m]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) st.o[4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n], v[m], st.o[4 * j + m], 0, 0, 0);
     }
 }
 
