@@ -37,31 +37,123 @@
 
 #define KV4_PART_STRIDE 260   // acc[256], m, l, pad[2]
 
-// What a batch row of the step is: a table row of `len` tokens, the last of
-// them new; none (len 0: the output is zero); or one that is refused (its
-// output is NaN): longer than max_len, or a table row that an earlier batch
-// row has.
+// A batch row of the step: its table row and the tokens to read there, the
+// last of them new (0: none, the output is zero).  A row that is refused (its
+// output is NaN) is longer than max_len, or steps a table row that an earlier
+// batch row has.
 struct StepRow {
     int row, len;
     bool refused;
 };
-QM_DEV StepRow step_row(const GqaKv4Args& A, int b) {
+// Lane l's batch row b, but for repeats (whose length counts here).
+QM_DEV StepRow lane_row(const GqaKv4Args& A, int b) {
     StepRow r{-1, 0, false};
-    if (A.result && A.result[0] != 0) return r;
+    if (b >= A.batch) return r;
     const int row = A.slots ? A.slots[b] : b;
     if ((uint32_t)row >= (uint32_t)A.c.rows) return r;
     r.row = row;
-    r.len = max(A.c.lens[row], 0);
-    r.refused = r.len > A.max_len;
-    if (A.slots) {
-        const int lane = threadIdx.x & 63;
-        for (int j0 = 0; j0 < b; j0 += 64) {          // uniform
-            const int j = j0 + lane;
-            if (__ballot(j < b && A.slots[min(j, b - 1)] == row)) r.refused = true;
-        }
-    }
-    if (r.refused) r.len = 0;
+    const int len = max(A.c.lens[row], 0);
+    r.refused = len > A.max_len;
+    r.len = r.refused ? 0 : len;
     return r;
+}
+// Whether a batch row before b has table row `row`.  All lanes call it.
+QM_DEV bool repeated(const GqaKv4Args& A, int b, int row, int lane) {
+    bool found = false;
+    if (A.slots)
+        for (int j0 = 0; j0 < b; j0 += 64) {               // uniform
+            const int j = j0 + lane;
+            if (__ballot(j < b && A.slots[min(j, b - 1)] == row)) found = true;
+        }
+    return found;
+}
+// Inclusive sum over the wave's lanes: within the rows of 16, then the last
+// lane of a row into the next row, and of the lower half into the upper.
+template <int CTRL, int ROWS>
+QM_DEV int scan_step(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
+QM_DEV int wave_scan(int x) {
+    x = scan_step<0x111, 0xF>(x);
+    x = scan_step<0x112, 0xF>(x);
+    x = scan_step<0x114, 0xF>(x);
+    x = scan_step<0x118, 0xF>(x);
+    x = scan_step<0x142, 0xA>(x);
+    return scan_step<0x143, 0xC>(x);
+}
+// ceil(len / chunk), chunk a multiple of 128: the f32 quotient is off by two at
+// most, and put right.
+QM_DEV int splits_of(int len, int chunk) {
+    const uint32_t all = (uint32_t)len, each = (uint32_t)chunk;
+    uint32_t n = (uint32_t)((float)len * __builtin_amdgcn_rcpf((float)chunk));
+    n -= n * each >= all && n > 0;
+    n -= n * each >= all && n > 0;
+    n += n * each < all;
+    return (int)(n + (n * each < all));
+}
+
+// How the step's tokens are dealt to workgroups: splits of `chunk` tokens of
+// each row, the rows one after the other.  The chunk follows from the lengths
+// that the rows have now, so that a ragged batch fills the chip as evenly as
+// an equal one, and a captured step whose max_len is the capacity as one whose
+// max_len is its length.  Every workgroup finds the same chunk: one workgroup
+// per CU, or two where that makes the chunk enough shorter, and not a few more
+// than that, which would be a round of their own; at most QMK_KV4_MAX_SPLIT
+// tokens.  Two workgroups on a CU take 1.7 times as long as one (a round of a
+// lone wave is bound by its own chain of vector and matrix instructions, of
+// two by the vector unit).  Measured, the step in us, one per CU / two: 1 x
+// 32769 tokens 17.5 / 19.2, 8 x 4097 15.6 / 18.0, 16 ragged rows of up to 7001
+// 20.8 / 19.8, 64 x 2049 34.4 / 34.6.
+struct Deal {
+    int chunk;
+    int b, first;            // a batch row, and the splits before its own
+    StepRow r;
+};
+QM_DEV int chunk_for(const GqaKv4Args& A, float total, int groups, int len) {
+    const float want = fminf(total * __builtin_amdgcn_rcpf((float)groups), (float)(QMK_KV4_MAX_SPLIT - 1));
+    int chunk = __builtin_amdgcn_readfirstlane(((int)want + 128) / 128 * 128);      // more than `want`
+    if (A.batch <= 64)
+        for (int tries = 0; tries < 4 && chunk < QMK_KV4_MAX_SPLIT; ++tries, chunk += 128)
+            if (QM_GQA_KV_HEADS * __builtin_amdgcn_readlane(wave_scan(splits_of(len, chunk)), 63) <= groups) break;
+    return chunk;
+}
+QM_DEV int deal_chunk(const GqaKv4Args& A, const StepRow& mine, int lane) {
+    float total = (float)mine.len;                         // the first 64 rows stay in the lanes
+    for (int b0 = 64; b0 < A.batch; b0 += 64) total += (float)lane_row(A, b0 + lane).len;
+    total = wave_sum64(total) * QM_GQA_KV_HEADS;
+    const int one = chunk_for(A, total, A.cus, mine.len);
+    if (one == 128) return one;
+    const int two = chunk_for(A, total, 2 * A.cus, mine.len);
+    return 10 * one <= 17 * two && one < QMK_KV4_MAX_SPLIT ? one : two;
+}
+// The row of split k (all lanes agree), false past the last split; and, where
+// `note`, batch row k's splits to the merge: {first, splits}, -1 splits where
+// it is refused.
+QM_DEV bool deal_split(const GqaKv4Args& A, Deal& d, int k, bool note, int lane) {
+    StepRow mine = lane_row(A, lane);
+    d.chunk = deal_chunk(A, mine, lane);
+    d.first = 0;
+    bool found = false;
+    int first = 0;
+    for (int b0 = 0; b0 < A.batch; b0 += 64) {             // uniform
+        if (b0) mine = lane_row(A, b0 + lane);
+        const int n = splits_of(mine.len, d.chunk), incl = wave_scan(n), all = __builtin_amdgcn_readlane(incl, 63);
+        if (!found && k < first + all) {
+            const int at = __popcll(__ballot(first + incl <= k));
+            found = true;
+            d.b = b0 + at;
+            d.first = first + __builtin_amdgcn_readlane(incl - n, at);
+            d.r.row = __builtin_amdgcn_readlane(mine.row, at);
+            d.r.len = __builtin_amdgcn_readlane(mine.len, at);
+            d.r.refused = repeated(A, d.b, d.r.row, lane);
+        }
+        if (note && k >= b0 && k < b0 + 64) {
+            const int row = __builtin_amdgcn_readlane(mine.row, k - b0);
+            const bool refused = __builtin_amdgcn_readlane(mine.refused, k - b0) || (row >= 0 && repeated(A, k, row, lane));
+            if (lane == k - b0) reinterpret_cast<int2*>(A.splits)[k] = make_int2(first + incl - n, refused ? -1 : n);
+        }
+        if (found && (!note || k < b0 + 64)) break;
+        first += all;
+    }
+    return found;
 }
 
 template <int CTRL>
@@ -359,10 +451,24 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     __shared__ SplitKv4Lds sh;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int split = blockIdx.x % A.nsplit, bg = blockIdx.x / A.nsplit;
-    const int kvh = bg & 3, b = bg >> 2;
-    const int t_begin = split * A.chunk;
-    const StepRow r = step_row(A, b);
+    const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2;
+    if (A.result && A.result[0] != 0 && !A.single) return;
+    // A workgroup for each (split, head); with A.single one for each (batch
+    // row, head), which then finishes by itself.
+    Deal deal;
+    if (A.single) {
+        deal.chunk = QMK_KV4_MAX_SPLIT;
+        deal.b = deal.first = index;
+        deal.r = lane_row(A, index);
+        deal.r.refused = deal.r.refused || (deal.r.row >= 0 && repeated(A, index, deal.r.row, lane));
+        if (A.result && A.result[0] != 0) deal.r = StepRow{-1, 0, false};
+    } else if (!deal_split(A, deal, index, kvh == 0 && index < A.batch && w == 0, lane) || deal.r.refused) {
+        return;                                            // uniform, as are all values of `deal`
+    }
+    const int b = __builtin_amdgcn_readfirstlane(deal.b), chunk = deal.chunk;
+    StepRow r = deal.r;
+    if (r.refused) r.len = 0;
+    const int split = index - deal.first, t_begin = split * chunk;
 
     // The loads that depend on no other: q, the new token's row (wave 0 k, wave
     // 1 v) and the split's page ids, one a lane (a split has at most 64 pages).
@@ -372,11 +478,10 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     const uint2 kn = *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane);
     const int page0 = t_begin / QMK_KV4_PAGE_TOKENS;
     int ids = -1;
-    if (lane < A.chunk / QMK_KV4_PAGE_TOKENS && page0 + lane < A.c.max_pages)
+    if (lane < chunk / QMK_KV4_PAGE_TOKENS && page0 + lane < A.c.max_pages)
         ids = A.c.table[(size_t)max(r.row, 0) * A.c.max_pages + page0 + lane];
 
-    const int t_end = min(t_begin + A.chunk, r.len);
-    if (t_begin >= t_end && A.nsplit > 1) return;        // uniform: the merge reads the splits of the row's tokens
+    const int t_end = min(t_begin + chunk, r.len);
     const int h0 = t_begin / QMK_KV4_HALF_TOKENS + w;
     const int h_end = __builtin_amdgcn_readfirstlane((t_end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
     auto half_of = [&](int h, bool& there) {
@@ -522,10 +627,10 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
             o.z = fmaf(a.z, f, o.z);
             o.w = fmaf(a.w, f, o.w);
         }
-        if (A.nsplit == 1) {
+        if (A.single) {
             kv4_out(A, b, 4 * kvh + h, lane, o, l, kv4_gate(A, b, 4 * kvh + h, lane), r.refused);
         } else {
-            float* P = A.partial + (((size_t)bg * A.nsplit + split) * 4 + h) * KV4_PART_STRIDE;
+            float* P = A.partial + ((size_t)blockIdx.x * 4 + h) * KV4_PART_STRIDE;
             st4(P + 4 * lane, o);
             if (lane == 0) *reinterpret_cast<float2*>(P + 256) = make_float2(M * 0x1p43f, l);
         }
@@ -533,36 +638,44 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
 }
 
 // The splits' partials of query head h of batch row b, joined, and the gate:
-// one wave per (b, h, 64 dims), 32 splits' loads in flight at a time.
-#define KV4_MERGE_BATCH 32
+// one wave per (b, h, 64 dims), N splits' loads in flight at a time.
+struct Joined {
+    float m, l, o;
+};
+template <int N>
+QM_DEV void join(Joined& x, const float* P, int n, int d, int lane) {
+    const size_t step = 16 * KV4_PART_STRIDE;
+    for (int s0 = 0; s0 < n; s0 += N) {                     // uniform
+        float a[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = P[(size_t)min(s0 + j, n - 1) * step + d];
+        const float2 ml = *reinterpret_cast<const float2*>(P + (size_t)min(s0 + lane, n - 1) * step + 256);
+        const bool some = lane < N && s0 + lane < n && ml.y != 0.0f;     // a split of tokens
+        const float mb = fmaxf(x.m, max_xor32(max_xor16(row_max16(some ? ml.x : -INFINITY))));
+        const float c = x.m == mb ? 1.0f : __builtin_amdgcn_exp2f(x.m - mb);
+        const float f = !some ? 0.0f : ml.x == mb ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mb);
+        x.l = x.l * c + wave_sum64(some ? ml.y * f : 0.0f);
+        x.o *= c;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float fj = readlane_f32(f, j);
+            x.o = fj != 0.0f ? fmaf(a[j], fj, x.o) : x.o;
+        }
+        x.m = mb;
+    }
+}
 extern "C" __global__ __launch_bounds__(64) void qm_gqa_kv4_merge(GqaKv4Args A) {
     const int lane = threadIdx.x, d = 64 * (blockIdx.x & 3) + lane;
     const int h = (blockIdx.x >> 2) % QM_GQA_HEADS, b = blockIdx.x / (4 * QM_GQA_HEADS);
     const float gate = A.q_gate[((size_t)b * QM_GQA_HEADS + h) * (2 * QM_GQA_HD) + QM_GQA_HD + d];
-    const float* P = A.partial + ((size_t)(b * QM_GQA_KV_HEADS + (h >> 2)) * A.nsplit * 4 + (h & 3)) * KV4_PART_STRIDE;
-    const size_t step = 4 * KV4_PART_STRIDE;
-    const StepRow r = step_row(A, b);
-    const int n = (r.len + A.chunk - 1) / A.chunk;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int s0 = 0; s0 < n; s0 += KV4_MERGE_BATCH) {       // uniform
-        float a[KV4_MERGE_BATCH];
-#pragma unroll
-        for (int j = 0; j < KV4_MERGE_BATCH; ++j) a[j] = P[(size_t)min(s0 + j, n - 1) * step + d];
-        float2 ml = *reinterpret_cast<const float2*>(P + (size_t)min(s0 + lane, n - 1) * step + 256);
-        const bool some = lane < KV4_MERGE_BATCH && s0 + lane < n && ml.y != 0.0f;     // a split of tokens
-        const float mb = fmaxf(m, max_xor32(max_xor16(row_max16(some ? ml.x : -INFINITY))));
-        const float c = m == mb ? 1.0f : __builtin_amdgcn_exp2f(m - mb);
-        const float f = !some ? 0.0f : ml.x == mb ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mb);
-        l = l * c + wave_sum64(some ? ml.y * f : 0.0f);
-        o *= c;
-#pragma unroll
-        for (int j = 0; j < KV4_MERGE_BATCH; ++j) {
-            const float fj = readlane_f32(f, j);
-            o = fj != 0.0f ? fmaf(a[j], fj, o) : o;
-        }
-        m = mb;
-    }
-    float y = l != 0.0f ? (o * __builtin_amdgcn_rcpf(l)) * sigmoid_fast(gate) : 0.0f;
-    if (r.refused) y = __builtin_nanf("");
+    const bool off = A.result && A.result[0] != 0;          // nobody has dealt
+    const int2 mine = off ? make_int2(0, 0) : reinterpret_cast<const int2*>(A.splits)[b];
+    // split (first + s) and kv head h >> 2: workgroup 4 (first + s) + (h >> 2)
+    const float* P = A.partial + ((size_t)mine.x * 16 + h) * KV4_PART_STRIDE;
+    Joined x{-INFINITY, 0.0f, 0.0f};
+    if (mine.y <= 8) join<8>(x, P, mine.y, d, lane);
+    else join<32>(x, P, mine.y, d, lane);
+    float y = x.l != 0.0f ? (x.o * __builtin_amdgcn_rcpf(x.l)) * sigmoid_fast(gate) : 0.0f;
+    if (mine.y < 0) y = __builtin_nanf("");
     A.out[((size_t)b * QM_GQA_HEADS + h) * QM_GQA_HD + d] = y;
 }

@@ -122,8 +122,9 @@ struct GqaKv4Args {
     const float* rope_sin;
     const int32_t* result;   // null, or a resize's result
     float* out;              // [B][16][256]
-    float* partial;          // [B][4][nsplit][4 heads][260]: acc[256], m, l, pad
+    float* partial;          // [splits][4 kv heads][4 heads][260]: acc[256], m, l, pad
+    int32_t* splits;         // [B] {first, splits}: for the merge
     int32_t layer, batch, max_len;
-    int32_t chunk;           // tokens per split, a multiple of 128, at most QMK_KV4_MAX_SPLIT
-    int32_t nsplit;
+    int32_t cus;             // compute units of the device
+    int32_t single;          // a workgroup per batch row and head, no merge
 };

@@ -111,20 +111,19 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
     return Fault{};
 }
 
-// Tokens per split workgroup: a multiple of 128 (a round of its four waves),
-// at most QMK_KV4_MAX_SPLIT (its page ids are one a lane), and within that at
-// most 64 splits per sequence and head and about kSplitGroups workgroups.
-constexpr int64_t kSplitGroups = 2048;
-inline int64_t split_tokens(int64_t len, int32_t batch) {
-    int64_t want = (len + 63) / 64;
-    const int64_t fill = (len * batch * 4 + kSplitGroups - 1) / kSplitGroups;
-    if (fill > want) want = fill;
-    want = (want + 127) / 128 * 128;
-    return want < QMK_KV4_MAX_SPLIT ? want : QMK_KV4_MAX_SPLIT;
-}
-inline int64_t splits(int64_t len, int32_t batch) {
-    const int64_t t = split_tokens(len, batch);
-    return (len + t - 1) / t;
+// The decode's workgroups.  Rows of at most kSingleTokens take one workgroup
+// each per kv head and no merge.  Longer ones are dealt out by the kernel
+// (deal_chunk): splits of 128 n tokens, n such that one or two workgroups a CU
+// have about the same number, at most QMK_KV4_MAX_SPLIT.  max_splits bounds the
+// splits of all rows: below the cap they are two workgroups a CU over the four
+// kv heads, and one per row (and two for the rounding of their f32 sum), at
+// the cap ceil(len / QMK_KV4_MAX_SPLIT) per row.
+constexpr int64_t kSingleTokens = 128;
+inline int64_t max_splits(int64_t len, int64_t batch, int cus) {
+    const int64_t least = (len + 127) / 128 * batch, capped = (len + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT * batch;
+    int64_t n = cus / 2 + batch + 2;
+    if (capped > n) n = capped;
+    return least < n ? least : n;
 }
 
 // Workspace of each call, bytes.
@@ -133,21 +132,15 @@ inline size_t fork_ws(int32_t count, int32_t max_pages) {
     return 4 * (4 + static_cast<size_t>(count) * (1 + static_cast<size_t>(max_pages)));
 }
 inline size_t compact_ws(int32_t num_pages) { return 4 * (4 + 3 * static_cast<size_t>(num_pages)); }
-inline size_t decode_ws(int32_t batch, int64_t nsplit) { return static_cast<size_t>(batch) * 4 * nsplit * 4 * 260 * 4; }
+inline size_t partial_bytes(int64_t splits) { return static_cast<size_t>(splits) * 4 * 4 * 260 * 4; }
+inline size_t decode_ws(int64_t splits, int32_t batch) { return partial_bytes(splits) + static_cast<size_t>(batch) * 8; }
 
 // A bound of all of them for batches up to `batch` over lengths up to `len`,
 // a pool of no more pages than those need, forks and resizes of at most
-// `batch` rows.  Decode: below the cap a split holds at least len / 64 and
-// len batch 4 / kSplitGroups tokens; at the cap there are ceil(len / 4096).
-inline size_t reserve_ws(int32_t batch, int32_t len) {
+// `batch` rows.
+inline size_t reserve_ws(int32_t batch, int32_t len, int cus) {
     const int64_t pages = (static_cast<int64_t>(len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
-    const int64_t capped = (static_cast<int64_t>(len) + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT;
-    int64_t each = capped > 64 ? capped : 64;
-    if (pages < each) each = pages;
-    int64_t all = kSplitGroups / 4 + batch;
-    if (capped * batch > all) all = capped * batch;
-    if (each * batch < all) all = each * batch;
-    size_t ws = static_cast<size_t>(all) * 4 * 4 * 260 * 4;
+    size_t ws = decode_ws(max_splits(len, batch, cus), batch);
     const size_t lists = resize_ws(batch), forks = fork_ws(batch, static_cast<int32_t>(pages));
     const size_t pool = 4 * (4 + 3 * static_cast<size_t>(pages) * static_cast<size_t>(batch));
     if (lists > ws) ws = lists;

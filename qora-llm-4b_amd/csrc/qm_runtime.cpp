@@ -805,7 +805,7 @@ int32_t qm_reserve(qm_context* c, int32_t max_batch, int32_t max_kv_len, int32_t
             bn = std::min<int64_t>(B * per_seq, std::max<int64_t>(512 + B, B * ((L + 2047) / 2048)));
         }
         ws = std::max(ws, static_cast<size_t>(bn) * QM_GQA_KV_HEADS * 4 * 260 * sizeof(float));
-        ws = std::max(ws, qm_kv4::reserve_ws(max_batch, max_kv_len));
+        ws = std::max(ws, qm_kv4::reserve_ws(max_batch, max_kv_len, c->num_cu));
     }
     if (max_prefill_tokens > 0) {
         ws = std::max(ws, dn_prefill_layout(max_prefill_tokens).total);
@@ -1323,17 +1323,20 @@ int32_t qm_gqa_decode_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* c
         cache, layer, batch, slots, {q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, out}, rope_len, max_len, result);
     if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
     hipStream_t s = pick(c, stream);
-    const int64_t chunk = qm_kv4::split_tokens(max_len, batch), nsplit = qm_kv4::splits(max_len, batch);
-    const uint64_t grid = static_cast<uint64_t>(batch) * QM_GQA_KV_HEADS * nsplit;
-    if (grid > 0x7fffffffull || static_cast<uint64_t>(batch) * QM_GQA_HEADS * 4 > 0x7fffffffull)
+    const bool single = max_len <= qm_kv4::kSingleTokens;
+    const int64_t splits = single ? batch : qm_kv4::max_splits(max_len, batch, c->num_cu);
+    const int64_t merge = static_cast<int64_t>(batch) * QM_GQA_HEADS * 4;
+    if (splits * QM_GQA_KV_HEADS > 0x7fffffff || merge > 0x7fffffff)
         return fail(c, QM_ERR_INVALID_ARG, "qm_gqa_decode_kv4: grid too large");
-    int32_t st = ensure(c, s, nsplit > 1 ? qm_kv4::decode_ws(batch, nsplit) : 0);
+    int32_t st = ensure(c, s, single ? 0 : qm_kv4::decode_ws(splits, batch));
     if (st != QM_OK) return st;
     GqaKv4Args a{kv4_of(*cache), slots, q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, result, out,
-                 static_cast<float*>(c->ws), layer, batch, max_len, static_cast<int32_t>(chunk), static_cast<int32_t>(nsplit)};
-    st = launch(c, c->f_gqa_kv4_split, static_cast<uint32_t>(grid), 256, a, s, "qm_gqa_kv4_split");
-    if (st != QM_OK || nsplit == 1) return st;
-    return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(batch) * QM_GQA_HEADS * 4, 64, a, s, "qm_gqa_kv4_merge");
+                 static_cast<float*>(c->ws),
+                 reinterpret_cast<int32_t*>(static_cast<char*>(c->ws) + (single ? 0 : qm_kv4::partial_bytes(splits))), layer,
+                 batch, max_len, c->num_cu, single};
+    st = launch(c, c->f_gqa_kv4_split, static_cast<uint32_t>(splits * QM_GQA_KV_HEADS), 256, a, s, "qm_gqa_kv4_split");
+    if (st != QM_OK || single) return st;
+    return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(merge), 64, a, s, "qm_gqa_kv4_merge");
 }
 
 }  // extern "C"

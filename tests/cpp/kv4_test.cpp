@@ -2,8 +2,7 @@
 // line on stdin (host headers only):
 //   at t d                  -> K word, K nibble, V word, V nibble of a half page
 //   meta t group            -> f16 index of the scale and of the minimum
-//   split len batch         -> tokens per split, splits
-//   ws len batch            -> decode's workspace, the reserve that covers it
+//   splits len batch cus    -> bound of the decode's splits, its workspace, the reserve that covers it
 //   cache pages table lens refs layers num_pages rows max_pages
 //                           -> the cache that the following calls name
 //   resize count rows lens flags result
@@ -35,13 +34,11 @@ int main() {
         } else if (what == "meta" && std::cin >> i[0] >> i[1]) {
             std::cout << kv4_s_at(static_cast<int>(i[0]), static_cast<int>(i[1])) << " "
                       << kv4_lo_at(static_cast<int>(i[0]), static_cast<int>(i[1])) << "\n";
-        } else if (what == "split" && std::cin >> i[0] >> i[1]) {
-            std::cout << qm_kv4::split_tokens(i[0], static_cast<int32_t>(i[1])) << " "
-                      << qm_kv4::splits(i[0], static_cast<int32_t>(i[1])) << "\n";
-        } else if (what == "ws" && std::cin >> i[0] >> i[1]) {
-            const int32_t b = static_cast<int32_t>(i[1]);
-            std::cout << qm_kv4::decode_ws(b, qm_kv4::splits(i[0], b)) << " "
-                      << qm_kv4::reserve_ws(b, static_cast<int32_t>(i[0])) << "\n";
+        } else if (what == "splits" && std::cin >> i[0] >> i[1] >> i[2]) {
+            const int cus = static_cast<int>(i[2]);
+            const int64_t n = qm_kv4::max_splits(i[0], i[1], cus);
+            std::cout << n << " " << qm_kv4::decode_ws(n, static_cast<int32_t>(i[1])) << " "
+                      << qm_kv4::reserve_ws(static_cast<int32_t>(i[1]), static_cast<int32_t>(i[0]), cus) << "\n";
         } else if (what == "cache" && std::cin >> p[0] >> p[1] >> p[2] >> p[3] >> i[0] >> i[1] >> i[2] >> i[3]) {
             c = qm_kv4_cache{at<uint8_t>(p[0]), at<int32_t>(p[1]), at<int32_t>(p[2]), at<int32_t>(p[3]),
                              static_cast<int32_t>(i[0]), static_cast<int32_t>(i[1]), static_cast<int32_t>(i[2]),

@@ -64,7 +64,7 @@ def test_values_are_within_half_a_step(scale):
     assert (err <= np.maximum(s.astype(np.float64) / 2, 15 * 2.0 ** -25)).all()
 
 
-def test_values_of_odd_groups():
+def test_values_of_odd_cus():
     x = np.zeros((1, 256), np.float16)
     x[0, :64] = 3.5                                                           # one value: exact
     x[0, 64:128] = np.tile([-65504, 65504], 32)                               # the widest range
@@ -179,17 +179,41 @@ def test_entries_refuse_a_null_context():
     assert lib.qm_gqa_decode_kv4(None, None, None, 0, 1, *([None] * 8), 1, 1, None, None) == 3
 
 
-def test_splits_cover_the_length_in_whole_pages_and_fit_the_reserve():
-    sizes = [(n, b) for n in (1, 63, 64, 65, 4097, 20000, 32769, 131072, 2 ** 20, 2 ** 31 - 1) for b in (1, 2, 7, 19, 64, 200, 1024)]
-    got = [[int(x) for x in a.split()] for a in ask([f"split {n} {b}" for n, b in sizes] + [f"ws {n} {b}" for n, b in sizes])]
-    for (n, b), (tokens, splits), (ws, reserve) in zip(sizes, got, got[len(sizes):]):
-        assert tokens % 128 == 0 and tokens <= 4096 and (splits - 1) * tokens < n <= splits * tokens
-        assert tokens == 4096 or (splits <= 64 and b * splits <= 512 + b)
-        assert ws <= reserve, (n, b)
+def dealt(lens, cus):
+    """The kernel's rule (deal_chunk) on the rows' lengths: tokens per split, splits of all rows."""
+    count = lambda chunk: sum(-(-n // chunk) for n in lens)
+
+    def chunk_for(cus):
+        chunk = (int(min(np.float32(sum(lens)) * 4 / np.float32(cus), 4095)) + 128) // 128 * 128
+        for _ in range(4 if len(lens) <= 64 else 0):
+            if chunk >= 4096 or 4 * count(chunk) <= cus:
+                break
+            chunk += 128
+        return chunk
+
+    one, two = chunk_for(cus), chunk_for(2 * cus)
+    chunk = one if one == 128 or (10 * one <= 17 * two and one < 4096) else two
+    return chunk, count(chunk)
+
+
+def test_splits_fit_the_grid_and_the_reserve():
+    rng = np.random.default_rng(4)
+    cases = []
+    for most in (129, 500, 4097, 32769, 131072, 2 ** 20):
+        for batch in (1, 2, 7, 19, 64, 65, 300):
+            for cus in (4, 32, 256):
+                cases.append(([most] * batch, most, batch, cus))
+                cases.append((rng.integers(0, most + 1, batch).tolist(), most, batch, cus))
+                cases.append((np.minimum(most, rng.integers(1, 200, batch)).tolist(), most, batch, cus))
+    got = [[int(x) for x in a.split()] for a in ask([f"splits {m} {b} {g}" for _, m, b, g in cases])]
+    for (lens, most, batch, cus), (bound, ws, reserve) in zip(cases, got):
+        chunk, n = dealt(lens, cus)
+        assert chunk % 128 == 0 and 128 <= chunk <= 4096
+        assert n <= bound and ws <= reserve, (most, batch, cus)
     # a reserve for the largest covers the smaller
-    reserve = int(ask(["ws 32769 64"])[0].split()[1])
-    for n in (1, 64, 700, 4097, 32769):
-        assert all(int(a.split()[0]) <= reserve for a in ask([f"ws {n} {b}" for b in range(1, 65)]))
+    reserve = int(ask(["splits 32769 64 256"])[0].split()[2])
+    for n in (129, 700, 4097, 32769):
+        assert all(int(a.split()[1]) <= reserve for a in ask([f"splits {n} {b} 256" for b in range(1, 65)]))
 
 
 def test_rust_struct_matches_the_header():
