@@ -177,26 +177,43 @@ QM_DEV double wave_sum64_f64(double x) {
     return (readlane_f64(x, 0) + readlane_f64(x, 16)) + (readlane_f64(x, 32) + readlane_f64(x, 48));
 }
 
-// The new k row of a head as the f16 cache holds it: per-head RMSNorm
-// (1 + gamma, eps 1e-6) and RoPE in 64 bits, rounded to f32 and f16.  64 bits
-// because a code beside a border must not depend on the order of a sum.
-// Lane l has dims 4 l .. 4 l + 3.
-QM_DEV void new_k(const float4 x, uint2 gw, float4 c, float4 s, int lane, uint16_t (&out)[4]) {
-    const double v[4] = {x.x, x.y, x.z, x.w};
-    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+// A head's row, lane l with dims 4 l .. 4 l + 3: RMSNorm (1 + gamma, eps
+// 1e-6), and the rotation of dims 0..63 (gemv.rs:586-627).  Apart, so that the
+// norm is done by the time the RoPE rows arrive.
+QM_DEV void norm_head(float (&x)[4], uint2 gw) {
     const uint16_t g[4] = {(uint16_t)(gw.x & 0xffffu), (uint16_t)(gw.x >> 16), (uint16_t)(gw.y & 0xffffu), (uint16_t)(gw.y >> 16)};
-    const double mean = wave_sum64_f64((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3])) * (1.0 / QM_GQA_HD) + 1e-6;
+    const float ss = wave_sum64((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]));
+    const float inv = 1.0f / sqrtf(ss / (float)QM_GQA_HD + 1e-6f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (1.0f + f16_to_f32(g[i]));
+}
+QM_DEV void rotate_head(float (&x)[4], const float (&c)[4], const float (&s)[4], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p = dpp_f32<0x128>(x[i]);
+        x[i] = lane < 8 ? x[i] * c[i] - p * s[i] : lane < 16 ? x[i] * c[i] + p * s[i] : x[i];
+    }
+}
+// The new k row likewise, in 64 bits: a code beside a border must not depend
+// on the order of a sum.
+QM_DEV void norm_new_k(double (&x)[4], uint2 gw) {
+    const uint16_t g[4] = {(uint16_t)(gw.x & 0xffffu), (uint16_t)(gw.x >> 16), (uint16_t)(gw.y & 0xffffu), (uint16_t)(gw.y >> 16)};
+    const double mean = wave_sum64_f64((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) * (1.0 / QM_GQA_HD) + 1e-6;
     // v_rsq_f64 is good to about 2^-24; each step of Newton's squares the error
     double inv = __builtin_amdgcn_rsq(mean);
 #pragma unroll
     for (int i = 0; i < 2; ++i) inv = inv * __builtin_fma(-0.5 * mean * inv, inv, 1.5);
     if (!(mean < __builtin_inf())) inv = mean == mean ? 0.0 : mean;      // rsq's own 0 for an infinity, NaN for NaN
 #pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (1.0 + (double)f16_to_f32(g[i]));
+}
+// Its rotation, and the roundings to f32 and to the f16 cache's type.
+QM_DEV void rotate_new_k(uint16_t (&out)[4], const double (&x)[4], const float (&c)[4], const float (&s)[4], int lane) {
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const double y = v[i] * inv * (1.0 + (double)f16_to_f32(g[i]));
-        const double partner = dpp_f64<0x128>(y);
-        const double turned = lane < 8 ? y * cc[i] - partner * ss[i] : y * cc[i] + partner * ss[i];
-        out[i] = f64_to_f16_by_f32(lane < 16 ? turned : y);
+        const double p = dpp_f64<0x128>(x[i]);
+        const double turned = lane < 8 ? x[i] * c[i] - p * s[i] : x[i] * c[i] + p * s[i];
+        out[i] = f64_to_f16_by_f32(lane < 16 ? turned : x[i]);
     }
 }
 
@@ -374,19 +391,21 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
     float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     mx = max_xor32(max_xor16(mx));
     if (__ballot(mx > st.m + 0x1p-40f)) {                // uniform: 2^8
-        const float m = mx > st.m + 0x1p-40f ? mx : st.m;
-        const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f((st.m - m) * 0x1p43f);
+        const float m = mx > st.m + 0x1p-40f ? mx : st.m, was = st.m;
         st.m = m;
-        st.l *= f;
-        st.l16 *= f;
-        st.lo *= f;
-        const float f0 = readlane_f32(f, 0), f1 = readlane_f32(f, 1), f2 = readlane_f32(f, 2), f3 = readlane_f32(f, 3);
+        if (__ballot(was != -INFINITY)) {                // else nothing is summed yet
+            const float f = was == m ? 1.0f : __builtin_amdgcn_exp2f((was - m) * 0x1p43f);
+            st.l *= f;
+            st.l16 *= f;
+            st.lo *= f;
+            const float f0 = readlane_f32(f, 0), f1 = readlane_f32(f, 1), f2 = readlane_f32(f, 2), f3 = readlane_f32(f, 3);
 #pragma unroll
-        for (int m4 = 0; m4 < 16; ++m4) {
-            st.o[m4][0] *= f0;
-            st.o[m4][1] *= f1;
-            st.o[m4][2] *= f2;
-            st.o[m4][3] *= f3;
+            for (int m4 = 0; m4 < 16; ++m4) {
+                st.o[m4][0] *= f0;
+                st.o[m4][1] *= f1;
+                st.o[m4][2] *= f2;
+                st.o[m4][3] *= f3;
+            }
         }
     }
     const float bias = fmaf(-st.m, 0x1p43f, KV4_P_BIAS), bias16 = fmaf(-st.m, 0x1p43f, KV4_P_BIAS - 4.0f);
@@ -476,6 +495,8 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     const uint2 qn = *reinterpret_cast<const uint2*>(A.q_norm + 4 * lane);
     const float4 nx = ld4((w == 0 ? A.k_new : A.v_new) + ((size_t)b * QM_GQA_KV_HEADS + kvh) * QM_GQA_HD + 4 * lane);
     const uint2 kn = *reinterpret_cast<const uint2*>(A.k_norm + 4 * lane);
+    float4 gate = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (A.single) gate = kv4_gate(A, b, 4 * kvh + w, lane);
     const int page0 = t_begin / QMK_KV4_PAGE_TOKENS;
     int ids = -1;
     if (lane < chunk / QMK_KV4_PAGE_TOKENS && page0 + lane < A.c.max_pages)
@@ -491,7 +512,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     };
     // The compiler does not count the DMA below: what it loads has to be here
     // before that starts, or its waits would take the DMA's for its own.
-    asm volatile("" ::"v"(qx.x), "v"(qn.x), "v"(nx.x), "v"(kn.x), "v"(ids));
+    asm volatile("" ::"v"(qx.x), "v"(qn.x), "v"(nx.x), "v"(kn.x), "v"(gate.x), "v"(ids));
 
     // The RoPE rows of the new position (to LDS, a q row that this wave writes
     // later), then the wave's first two half pages.
@@ -510,33 +531,41 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
             ahead += KV4_DMA;
         }
     }
+    // the norms meanwhile
+    const bool appends = pos >= t_begin && pos < t_end;
+    float q[4] = {qx.x, qx.y, qx.z, qx.w};
+    norm_head(q, qn);
+    double k64[4] = {nx.x, nx.y, nx.z, nx.w};
+    if (appends && w == 0) norm_new_k(k64, kn);
     if (ahead == 2 * KV4_DMA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KV4_DMA) : "memory");
     else if (ahead == KV4_DMA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KV4_DMA) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const float4 rc = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rope) + 4 * (lane & 7));
-    const float4 rs = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rope) + 32 + 4 * (lane & 7));
+    float rc[4], rs[4];
+    lds4(reinterpret_cast<uint32_t*>(rc), reinterpret_cast<const uint8_t*>(rope) + 16 * (lane & 7));
+    lds4(reinterpret_cast<uint32_t*>(rs), reinterpret_cast<const uint8_t*>(rope) + 128 + 16 * (lane & 7));
 
-    // q of head 4 kvh + w: norm, RoPE, the softmax's scale, and the parts
-    const bool appends = pos >= t_begin && pos < t_end;
+    // q of head 4 kvh + w: RoPE, the softmax's scale, and the parts
     {
-        float4 x = norm_rope_head(qx, qn, rc, rs, lane);
+        rotate_head(q, rc, rs, lane);
         const float scale = 1.4426950408889634f / 16.0f;
-        x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
-        const float sum = row_sum16((x.x + x.y) + (x.z + x.w));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] *= scale;
+        const float sum = row_sum16((q[0] + q[1]) + (q[2] + q[3]));
         if (c == 0) sh.qsum[w][g] = sum * 0x1p-43f;
-        float y[4] = {x.x * 0x1p90f, x.y * 0x1p90f, x.z * 0x1p86f, x.w * 0x1p86f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] *= i < 2 ? 0x1p90f : 0x1p86f;
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
             *reinterpret_cast<uint2*>(&sh.q[4 * j + w][4 * lane]) =
-                make_uint2(pack_hi(__float_as_uint(y[0]), __float_as_uint(y[1])), pack_hi(__float_as_uint(y[2]), __float_as_uint(y[3])));
+                make_uint2(pack_hi(__float_as_uint(q[0]), __float_as_uint(q[1])), pack_hi(__float_as_uint(q[2]), __float_as_uint(q[3])));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] -= upper8(y[i]);
+            for (int i = 0; i < 4; ++i) q[i] -= upper8(q[i]);
         }
         if (w == 3) *reinterpret_cast<uint2*>(&sh.q[12][4 * lane]) = make_uint2(0, 0);
     }
     if (appends && w < 2) {                                // uniform per wave
         uint16_t x[4] = {f32_to_f16(nx.x), f32_to_f16(nx.y), f32_to_f16(nx.z), f32_to_f16(nx.w)};
-        if (w == 0) new_k(nx, kn, rc, rs, lane, x);
+        if (w == 0) rotate_new_k(x, k64, rc, rs, lane);
         const CodedRow q = code_row(x);
         if (w == 0) {
             uint32_t word = 0;
@@ -628,7 +657,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
             o.w = fmaf(a.w, f, o.w);
         }
         if (A.single) {
-            kv4_out(A, b, 4 * kvh + h, lane, o, l, kv4_gate(A, b, 4 * kvh + h, lane), r.refused);
+            kv4_out(A, b, 4 * kvh + h, lane, o, l, gate, r.refused);
         } else {
             float* P = A.partial + ((size_t)blockIdx.x * 4 + h) * KV4_PART_STRIDE;
             st4(P + 4 * lane, o);

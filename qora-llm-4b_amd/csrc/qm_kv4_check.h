@@ -111,14 +111,17 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
     return Fault{};
 }
 
-// The decode's workgroups.  Rows of at most kSingleTokens take one workgroup
-// each per kv head and no merge.  Longer ones are dealt out by the kernel
+// The decode's workgroups.  Short rows, and somewhat longer ones where there
+// are enough of them, take one workgroup each per kv head and no merge
+// (measured, one workgroup / dealt out, us: 1 row of 300 tokens 9.4 / 9.0, of
+// 500 10.8 / 9.1, 64 rows of 250 8.8 / 12.7, of 500 13.2 / 17.5; rows of one
+// step may differ, so not much longer).  Others are dealt out by the kernel
 // (deal_chunk): splits of 128 n tokens, n such that one or two workgroups a CU
 // have about the same number, at most QMK_KV4_MAX_SPLIT.  max_splits bounds the
 // splits of all rows: below the cap they are two workgroups a CU over the four
 // kv heads, and one per row (and two for the rounding of their f32 sum), at
 // the cap ceil(len / QMK_KV4_MAX_SPLIT) per row.
-constexpr int64_t kSingleTokens = 128;
+inline bool single(int64_t len, int64_t batch) { return len <= 256 || (len <= 512 && batch >= 16); }
 inline int64_t max_splits(int64_t len, int64_t batch, int cus) {
     const int64_t least = (len + 127) / 128 * batch, capped = (len + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT * batch;
     int64_t n = cus / 2 + batch + 2;

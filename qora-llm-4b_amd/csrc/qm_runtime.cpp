@@ -1323,7 +1323,7 @@ int32_t qm_gqa_decode_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* c
         cache, layer, batch, slots, {q_gate, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin, out}, rope_len, max_len, result);
     if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
     hipStream_t s = pick(c, stream);
-    const bool single = max_len <= qm_kv4::kSingleTokens;
+    const bool single = qm_kv4::single(max_len, batch);
     const int64_t splits = single ? batch : qm_kv4::max_splits(max_len, batch, c->num_cu);
     const int64_t merge = static_cast<int64_t>(batch) * QM_GQA_HEADS * 4;
     if (splits * QM_GQA_KV_HEADS > 0x7fffffff || merge > 0x7fffffff)
