@@ -4,49 +4,53 @@
 #include "qm_kv4_device.h"
 
 // ---- f16 rows <-> pages ---------------------------------------------------
-// A workgroup takes half a page (32 tokens) of one sequence and head.  A
-// token's row is 32 lanes x 8 dims, so a group of 64 dims is 8 lanes and a
-// lane's 8 codes are one K word; V words hold 8 tokens of one dim, so V's
-// codes turn in LDS.
+// A workgroup takes half a page (32 tokens) of one sequence and head, whose
+// 9216 bytes it puts together in LDS.  A token's row is 32 lanes x 8 dims, so
+// a group of 64 dims is 8 lanes, and a lane's 8 codes of a token are one K
+// word.  A V word holds 8 tokens of one dim: a lane takes 8 tokens and turns
+// their 8 x 8 codes in registers.
 #define KV4_ROWS_THREADS 256
 
 struct HalfAt {
-    bool some, whole;        // any / all of the half page's tokens taken
+    int t0;                  // token 0 of the half page
     int lo, hi;              // tokens of the half page taken: [lo, hi)
     int64_t src0;            // row of the f16 side of token 0
-    uint8_t* page;
 };
-QM_DEV HalfAt half_at(const Kv4RowsArgs& A, int b, int head, int tile) {
-    HalfAt h;
+// false: none taken.
+QM_DEV bool half_at(const Kv4RowsArgs& A, int b, int tile, HalfAt& h) {
     const int first = A.first ? A.first[b] : 0;
-    const int row = A.row + b;
-    const int t0 = ((first >> 5) + tile) << 5;
-    const int64_t end = min((int64_t)first + A.n, (int64_t)A.c.lens[row]);
-    h.src0 = (int64_t)t0 - first;
-    h.lo = max(0, first - t0);
-    h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, max(end - t0, (int64_t)0));
-    h.some = first >= 0 && h.lo < h.hi && (t0 >> 6) < A.c.max_pages;
-    h.whole = h.lo == 0 && h.hi == QMK_KV4_HALF_TOKENS;
-    h.page = nullptr;
-    if (h.some) {
-        const int id = A.c.table[(size_t)row * A.c.max_pages + (t0 >> 6)];
-        h.some = kv4_is_page(A.c, id);
-        if (h.some) h.page = kv4_half(A.c, A.layer, id, head, (t0 >> 5) & 1);
-    }
-    return h;
+    h.t0 = ((first >> 5) + tile) << 5;
+    const int64_t end = min((int64_t)first + A.n, (int64_t)A.c.lens[A.row + b]);
+    h.src0 = (int64_t)h.t0 - first;
+    h.lo = max(0, first - h.t0);
+    h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, max(end - h.t0, (int64_t)0));
+    return first >= 0 && h.lo < h.hi && (h.t0 >> 6) < A.c.max_pages;
+}
+// Its place in the pool; null: its table entry is no page.
+QM_DEV uint8_t* half_page(const Kv4RowsArgs& A, int b, int head, const HalfAt& h) {
+    const int id = A.c.table[(size_t)(A.row + b) * A.c.max_pages + (h.t0 >> 6)];
+    return kv4_is_page(A.c, id) ? kv4_half(A.c, A.layer, id, head, (h.t0 >> 5) & 1) : nullptr;
 }
 
 // Smallest / largest over the 8 lanes of a group.
+template <int CTRL>
+QM_DEV float dpp_of(float x) {       // update_dpp, unlike mov_dpp, is folded into its user
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
 QM_DEV float min_of8(float x) {
-    x = fminf(x, dpp_f32<0xB1>(x));
-    x = fminf(x, dpp_f32<0x4E>(x));
-    return fminf(x, dpp_f32<0x141>(x));
+    x = fminf(x, dpp_of<0xB1>(x));
+    x = fminf(x, dpp_of<0x4E>(x));
+    return fminf(x, dpp_of<0x141>(x));
 }
 QM_DEV float max_of8(float x) {
-    x = fmaxf(x, dpp_f32<0xB1>(x));
-    x = fmaxf(x, dpp_f32<0x4E>(x));
-    return fmaxf(x, dpp_f32<0x141>(x));
+    x = fmaxf(x, dpp_of<0xB1>(x));
+    x = fmaxf(x, dpp_of<0x4E>(x));
+    return fmaxf(x, dpp_of<0x141>(x));
 }
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+QM_DEV f16x2 f16_pair(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
 
 // Eight f16 values of a lane -> their codes in a word (element e as in
 // kv4_nibble), and the group's scale and minimum.
@@ -54,105 +58,128 @@ struct Coded {
     uint32_t word;
     uint16_t s, lo;
 };
-QM_DEV Coded code8(uint4 raw) {
+QM_DEV Coded code8(uint4 raw, int lane) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
-    uint32_t big = 0;
+    const f16x2 least = __builtin_elementwise_min(__builtin_elementwise_min(f16_pair(w[0]), f16_pair(w[1])),
+                                                  __builtin_elementwise_min(f16_pair(w[2]), f16_pair(w[3])));
+    const f16x2 most = __builtin_elementwise_max(__builtin_elementwise_max(f16_pair(w[0]), f16_pair(w[1])),
+                                                 __builtin_elementwise_max(f16_pair(w[2]), f16_pair(w[3])));
+    const float lo = min_of8(fminf((float)least[0], (float)least[1])), hi = max_of8(fmaxf((float)most[0], (float)most[1]));
+    // an infinity or a NaN in the group's eight lanes
+    u16x2 big = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xffffu));
-        x[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
-        big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-    }
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-    }
-    lo = min_of8(lo);
-    hi = max_of8(hi);
-    const bool bad = max_of8(big >= 0x7c00u ? 1.0f : 0.0f) > 0.0f;     // an infinity or a NaN
+    for (int i = 0; i < 4; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    const uint64_t lanes = __ballot(max(big[0], big[1]) >= 0x7c00u);
+    const bool bad = (lanes >> (lane & 56)) & 0xffu;
     Coded c;
     c.s = bad ? (uint16_t)0x7e00u : kv4_scale(lo, hi);
     c.lo = bad ? (uint16_t)0x7e00u : f32_to_f16(lo);
-    const float s = f16_to_f32(c.s), inv = s > 0.0f ? 1.0f / s : 0.0f;
-    c.word = 0;
+    // In f32, x - lo is off by 2^-20 s at most and the rest by less: a
+    // remainder clearly under half a step says that the code is right.  For
+    // the others (one value in some 3000), and where s is subnormal, 0 or NaN,
+    // kv4_code decides.
+    const float s = f16_to_f32(c.s), inv = __builtin_amdgcn_rcpf(s);
+    float q[8], worst = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c.word |= kv4_code(x[e], lo, s, inv) << (4 * kv4_nibble(e));
+    for (int e = 0; e < 8; ++e) {
+        const float d = fmaf((float)f16_pair(w[e >> 1])[e & 1], 1.0f, -lo);
+        q[e] = rintf(d * inv);
+        worst = fmaxf(worst, fabsf(fmaf(-q[e], s, d)));
+    }
+    // nibbles 0..3 are the even elements, 4..7 the odd ones; 16 bits of codes are whole numbers in f32
+    const float even = fmaf(fmaf(fmaf(q[6], 16.0f, q[4]), 16.0f, q[2]), 16.0f, q[0]);
+    const float odd = fmaf(fmaf(fmaf(q[7], 16.0f, q[5]), 16.0f, q[3]), 16.0f, q[1]);
+    c.word = (uint32_t)even | (uint32_t)odd << 16;
+    const float sure = s >= 0x1p-14f ? s * (0.5f - 0x1p-18f) : -1.0f;
+    if (!(worst < sure)) {
+#pragma clang loop unroll(disable)
+        for (int e = 0; e < 8; ++e) {                   // rolled: this is rare, and code to be fetched
+            const uint32_t we = (e < 4 ? (e < 2 ? w[0] : w[1]) : (e < 6 ? w[2] : w[3])) >> (16 * (e & 1));
+            const float x = f16_to_f32((uint16_t)we), d = x - lo;
+            const int shift = 4 * kv4_nibble(e);
+            if (fabsf(fmaf(-rintf(d * inv), s, d)) < sure) continue;
+            c.word = (c.word & ~(15u << shift)) | kv4_code(x, lo, s, inv) << shift;
+        }
+    }
     return c;
 }
 
+// 8 x 8 nibbles: nibble a of r[b] and nibble b of r[a] change places.
+QM_DEV void turn_nibbles(uint32_t (&r)[8]) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {                       // halves of rows a, a + 4
+        const uint32_t x = r[a], y = r[a + 4];
+        r[a] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+        r[a + 4] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                       // bytes of rows a, a + 2
+        const int a = (i & 1) + 4 * (i >> 1);
+        const uint32_t x = r[a], y = r[a + 2];
+        r[a] = __builtin_amdgcn_perm(y, x, 0x06020400u);
+        r[a + 2] = __builtin_amdgcn_perm(y, x, 0x07030501u);
+    }
+#pragma unroll
+    for (int a = 0; a < 8; a += 2) {                    // nibbles of rows a, a + 1
+        const uint32_t x = r[a], y = r[a + 1];
+        r[a] = (x & 0x0f0f0f0fu) | (y & 0x0f0f0f0fu) << 4;
+        r[a + 1] = ((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
+    }
+}
+
 extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
-    __shared__ __attribute__((aligned(16))) uint32_t kw[1024];          // K words, in the page's order
-    __shared__ __attribute__((aligned(16))) uint32_t vt[32][33];        // V words of token t, dims 8 i ..
-    __shared__ uint16_t meta[4][128];                                   // sK, loK, sV, loV
+    __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
     const int tid = threadIdx.x;
     const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
     const int head = bh & 3, b = bh >> 2;
-    const HalfAt h = half_at(A, b, head, tile);
-    if (!h.some) return;
-    const int i = tid & 31;                       // dims 8 i .. 8 i + 7
+    HalfAt h;
+    if (!half_at(A, b, tile, h)) return;                // uniform
+    const bool whole = h.lo == 0 && h.hi == QMK_KV4_HALF_TOKENS;
+    // Waves 0 and 1 have V, 2 and 3 K; a lane eight tokens 16 (e >> 2) + 4 g +
+    // (e & 3) of dims 8 i ..
+    const bool is_v = tid < 128;
+    const int i = tid & 31, g = (tid >> 5) & 3;
     const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
+    const uint16_t* from = is_v ? A.v : A.k;
+    uint4 raw[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int t = (tid >> 5) + 8 * r;
+    for (int e = 0; e < 8; ++e) {
+        const int t = min(max(16 * (e >> 2) + 4 * g + (e & 3), h.lo), h.hi - 1);     // any token for those left out
+        raw[e] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * i);
+    }
+    uint8_t* page = half_page(A, b, head, h);
+    if (!page) return;                                  // uniform
+    if (!whole) {                                       // uniform: the tokens left out stay
+        for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
+            reinterpret_cast<uint4*>(image)[j] = reinterpret_cast<const uint4*>(page)[j];
+        __syncthreads();
+    }
+    uint16_t* meta = reinterpret_cast<uint16_t*>(image) + QMK_KV4_META / 2 + (is_v ? 256 : 0);
+    uint32_t word[8], keep = 0;                         // in the order of the nibbles
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int t = 16 * (e >> 2) + 4 * g + (e & 3);
         const bool in = t >= h.lo && t < h.hi;
-        const size_t at = (base + (size_t)(in ? h.src0 + t : h.src0 + h.lo)) * 256 + 8 * i;
-        const Coded ck = code8(*reinterpret_cast<const uint4*>(A.k + at));
-        const Coded cv = code8(*reinterpret_cast<const uint4*>(A.v + at));
-        kw[kv4_k_word(t, 8 * i)] = ck.word;
-        vt[t][i] = cv.word;
-        if ((i & 7) == 0) {
-            meta[0][kv4_s_at(t, i >> 3)] = ck.s;
-            meta[1][kv4_lo_at(t, i >> 3)] = ck.lo;
-            meta[2][kv4_s_at(t, i >> 3)] = cv.s;
-            meta[3][kv4_lo_at(t, i >> 3)] = cv.lo;
+        const Coded c = code8(raw[e], tid & 63);
+        word[kv4_nibble(e)] = c.word;
+        keep |= in ? 0u : 15u << (4 * kv4_nibble(e));
+        if (!is_v && in) image[kv4_k_word(t, 8 * i)] = c.word;
+        if ((i & 7) == 0 && in) {
+            meta[kv4_s_at(t, i >> 3)] = c.s;
+            meta[128 + kv4_lo_at(t, i >> 3)] = c.lo;
+        }
+    }
+    if (is_v) {
+        turn_nibbles(word);                             // word n: the tokens of dim 8 i + (the element of nibble n)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint32_t* at = &image[kv4_v_word(4 * g, 8 * i + k)];
+            *at = whole ? word[kv4_nibble(k)] : (word[kv4_nibble(k)] & ~keep) | (*at & keep);
         }
     }
     __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(h.page);
-    {   // K: chunk tid is four words of one token
-        const int t = (tid >> 7) * 16 + (tid & 15);
-        if (t >= h.lo && t < h.hi) out[tid] = *reinterpret_cast<const uint4*>(&kw[4 * tid]);
-    }
-    {   // V: chunk tid is dims 64 group + 16 word + c of eight tokens
-        const int group = tid >> 6, g = (tid >> 4) & 3, c = tid & 15;
-        uint32_t w[4], keep = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int t = 16 * (e >> 2) + 4 * g + (e & 3);
-            if (t < h.lo || t >= h.hi) keep |= 15u << (4 * kv4_nibble(e));
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const int d = 64 * group + 16 * m + c;
-            w[m] = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int t = 16 * (e >> 2) + 4 * g + (e & 3);
-                w[m] |= ((vt[t][d >> 3] >> (4 * kv4_nibble(d & 7))) & 15u) << (4 * kv4_nibble(e));
-            }
-        }
-        uint4 old = make_uint4(0, 0, 0, 0);
-        if (keep && keep != 0xffffffffu) old = out[256 + tid];
-        if (keep != 0xffffffffu)
-            out[256 + tid] = make_uint4((w[0] & ~keep) | (old.x & keep), (w[1] & ~keep) | (old.y & keep),
-                                        (w[2] & ~keep) | (old.z & keep), (w[3] & ~keep) | (old.w & keep));
-    }
-    uint16_t* mo = reinterpret_cast<uint16_t*>(h.page + QMK_KV4_META);
-    if (h.whole) {
-        reinterpret_cast<uint32_t*>(mo)[tid] = reinterpret_cast<const uint32_t*>(&meta[0][0])[tid];
-    } else {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int j = tid + 256 * r, which = j >> 7, t = (j & 127) >> 2, group = j & 3;
-            if (t >= h.lo && t < h.hi) {
-                const int at = (which & 1) ? kv4_lo_at(t, group) : kv4_s_at(t, group);
-                mo[which * 128 + at] = meta[which][at];
-            }
-        }
-    }
+    for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
+        reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }
 
 QM_DEV float kv4_read(uint32_t word, int e, float s, float lo) {
@@ -164,10 +191,12 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
     const int tid = threadIdx.x;
     const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
     const int head = bh & 3, b = bh >> 2;
-    const HalfAt h = half_at(A, b, head, tile);
-    if (!h.some) return;
+    HalfAt h;
+    if (!half_at(A, b, tile, h)) return;                // uniform
+    const uint8_t* page = half_page(A, b, head, h);
+    if (!page) return;
     for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
-        reinterpret_cast<uint4*>(w)[j] = reinterpret_cast<const uint4*>(h.page)[j];
+        reinterpret_cast<uint4*>(w)[j] = reinterpret_cast<const uint4*>(page)[j];
     __syncthreads();
     const uint16_t* meta = reinterpret_cast<const uint16_t*>(&w[QMK_KV4_META / 4]);
     const int i = tid & 31, group = i >> 3;
