@@ -318,7 +318,7 @@ typedef struct {
     int32_t* lens_dev;         /* [rows] */
     int32_t* refs_dev;         /* [num_pages] */
     int32_t layers;
-    int32_t num_pages;
+    int32_t num_pages;         /* at most 4194303 */
     int32_t rows;              /* at most 65536 */
     int32_t max_pages;         /* pages of a row, at most 33554431 */
 } qm_kv4_cache;

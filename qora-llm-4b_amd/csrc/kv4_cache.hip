@@ -233,25 +233,28 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
 #define KV4_BLOCK_PAGES (64 * KV4_PLAN_THREADS)     // pages whose state one pass holds, 64 a thread
 #define KV4_WINDOW 4096                              // free pages handed out at a time
 
-// Exclusive sum over the workgroup's 1024 threads, and the total.
-QM_DEV uint64_t plan_scan(uint64_t x, uint64_t* sums, uint64_t& total) {
+// Inclusive sum over the wave's lanes: within the rows of 16, then the last
+// lane of a row into the next row, and of the lower half into the upper.
+template <int CTRL, int ROWS>
+QM_DEV uint32_t scan_step(uint32_t x) { return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
+QM_DEV uint32_t wave_scan(uint32_t x) {
+    x = scan_step<0x111, 0xF>(x);
+    x = scan_step<0x112, 0xF>(x);
+    x = scan_step<0x114, 0xF>(x);
+    x = scan_step<0x118, 0xF>(x);
+    x = scan_step<0x142, 0xA>(x);
+    return scan_step<0x143, 0xC>(x);
+}
+// Exclusive sum over the workgroup's 1024 threads, and the total.  `sums`
+// (one word a wave) must not be in use: calls in a row take different ones.
+QM_DEV uint32_t plan_scan(uint32_t x, uint32_t* sums, uint32_t& total) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    uint64_t incl = x;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t o = __shfl_up(incl, off);
-        if (lane >= off) incl += o;
-    }
-    __syncthreads();
+    const uint32_t incl = wave_scan(x);
     if (lane == 63) sums[w] = incl;
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int j = 0; j < KV4_PLAN_THREADS / 64; ++j) {
-        if (j < w) before += sums[j];
-        total += sums[j];
-    }
+    const uint32_t all = wave_scan(lane < KV4_PLAN_THREADS / 64 ? sums[lane] : 0u);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)all, 63);
+    const uint32_t before = w ? (uint32_t)__builtin_amdgcn_readlane((int)all, __builtin_amdgcn_readfirstlane(w) - 1) : 0u;
     return before + incl - x;
 }
 
@@ -261,21 +264,23 @@ QM_DEV uint64_t free_pages(const Kv4Cache& c, int64_t block) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint64_t mine = 0;
     const int64_t at = block + (int64_t)w * 4096;
-    for (int r0 = 0; r0 < 64; r0 += 16) {
+    for (int r0 = 0; r0 < 64; r0 += 32) {               // 32 loads in flight
         if (at + r0 * 64 >= c.num_pages) break;
-        int v[16];
+        int v[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 32; ++j) {
             const int64_t p = at + (r0 + j) * 64 + lane;
-            v[j] = p < c.num_pages ? c.refs[p] : 1;
+            v[j] = c.refs[min(p, (int64_t)c.num_pages - 1)];
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 32; ++j) {
             const uint64_t m = __ballot(v[j] == 0);
-            if (lane == r0 + j) mine = m;
+            mine = lane == r0 + j ? m : mine;
         }
     }
-    return mine;
+    // bits past the pool
+    const int64_t in = c.num_pages - (block + 64 * (int64_t)threadIdx.x);
+    return in >= 64 ? mine : in <= 0 ? 0ull : mine & ((1ull << in) - 1);
 }
 
 // 16-byte copy of a third of a page by a workgroup of 256.
@@ -300,43 +305,52 @@ QM_DEV void copy_part(const Kv4Cache& c, int layer, int src, int dst, int part) 
 // holder.  When every holder of such a page grows in this call, the first of
 // them keeps it.  Fresh pages are the lowest free ids before the call, in
 // list order.  Nothing is changed unless all of it can be.
+//
+// Bound by its chain of dependent loads (lengths, entry, count) and barriers;
+// the pool's counts are loaded first, beside them.
 extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4ResizeArgs A) {
-    __shared__ uint64_t sums[KV4_PLAN_THREADS / 64];
+    __shared__ uint32_t sums[2][KV4_PLAN_THREADS / 64];
     __shared__ uint32_t seen[QMK_KV4_MAX_ROWS / 32];
-    __shared__ int last[QMK_KV4_MAX_COUNT];
+    __shared__ __attribute__((aligned(16))) int last[QMK_KV4_MAX_COUNT];
     __shared__ uint32_t off[QMK_KV4_MAX_COUNT];
     __shared__ int row_of[QMK_KV4_MAX_COUNT], begin_of[QMK_KV4_MAX_COUNT];
     __shared__ int list[KV4_WINDOW];
     __shared__ uint32_t copies;
+    __shared__ unsigned long long lacking;
     const int tid = threadIdx.x;
     const Kv4Cache& c = A.c;
     for (int j = tid; j < (c.rows + 31) / 32; j += KV4_PLAN_THREADS) seen[j] = 0;
-    if (tid == 0) copies = 0;
+    if (tid == 0) {
+        copies = 0;
+        lacking = 0;
+    }
+    const bool mine = tid < A.count;
+    const int row = !mine ? -1 : A.list ? A.list[tid] : tid;
+    const bool in = mine && (uint32_t)row < (uint32_t)c.rows;
+    const int old = in ? c.lens[row] : 0;
+    const int change = mine ? A.lens[tid] : 0;
+    uint64_t mask = free_pages(c, 0);
     __syncthreads();
 
     // the list, checked
-    const bool mine = tid < A.count;
-    int row = -1, old = 0, want = 0, page = -1, held = 0;
-    bool bad = false, grow = false;
-    if (mine) {
-        row = A.list ? A.list[tid] : tid;
-        bad = (uint32_t)row >= (uint32_t)c.rows;
-        if (!bad) {
-            const uint32_t bit = 1u << (row & 31);
-            bad = (atomicOr(&seen[row >> 5], bit) & bit) != 0;
-            old = c.lens[row];
-            const int64_t to = (int64_t)A.lens[tid] + (A.add ? old : 0);
-            const int64_t most = (int64_t)c.max_pages * QMK_KV4_PAGE_TOKENS;
-            bad = bad || old < 0 || old > most || to < 0 || to > most;
-            want = bad ? 0 : (int)to;
-            grow = !bad && want > old;
-            if (grow && (old & (QMK_KV4_PAGE_TOKENS - 1))) {
-                page = c.table[(size_t)row * c.max_pages + old / QMK_KV4_PAGE_TOKENS];
-                if (kv4_is_page(c, page)) held = c.refs[page];
-                bad = held < 1;
-            }
+    int want = 0, page = -1, held = 0;
+    bool bad = mine && !in, grow = false;
+    if (in) {
+        const uint32_t bit = 1u << (row & 31);
+        bad = (atomicOr(&seen[row >> 5], bit) & bit) != 0;
+        const int64_t to = (int64_t)change + (A.add ? old : 0);
+        const int64_t most = (int64_t)c.max_pages * QMK_KV4_PAGE_TOKENS;
+        bad = bad || old < 0 || old > most || to < 0 || to > most;
+        want = bad ? 0 : (int)to;
+        grow = !bad && want > old;
+        if (grow && (old & (QMK_KV4_PAGE_TOKENS - 1))) {
+            page = c.table[(size_t)row * c.max_pages + old / QMK_KV4_PAGE_TOKENS];
+            if (kv4_is_page(c, page)) held = c.refs[page];
+            bad = held < 1;
         }
     }
+    last[tid] = page;
+    row_of[tid] = row;
     if (__syncthreads_or(bad)) {
         if (tid == 0) {
             A.result[0] = -1;
@@ -344,39 +358,41 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
         }
         return;
     }
-    last[tid] = page;
-    __syncthreads();
     bool copy = false;
-    if (page >= 0) {
-        int growing = 0;
-        bool first = true;
-        for (int j = 0; j < A.count; ++j) {
-            const bool same = last[j] == page;
-            growing += same;
-            first = first && !(same && j < tid);
+    if (held > 1) {                                     // a page of one holder is its own
+        int growing = 0, before = 0;
+        for (int j = 0; j < A.count; j += 4) {          // past the list: -1
+            const int4 o = *reinterpret_cast<const int4*>(&last[j]);
+            const int n = (o.x == page) + (o.y == page) + (o.z == page) + (o.w == page);
+            growing += n;
+            before += j + 4 <= tid ? n : (o.x == page && j < tid) + (o.y == page && j + 1 < tid) + (o.z == page && j + 2 < tid);
         }
-        copy = !(growing == held && first);
+        copy = !(growing == held && before == 0);
     }
     const int had = kv4_pages_of(old), pages = kv4_pages_of(want);
     const int begin = copy ? old / QMK_KV4_PAGE_TOKENS : had;
-    uint64_t need;
-    const uint64_t before = plan_scan(grow ? (uint64_t)(pages - begin) : 0, sums, need);
-    off[tid] = (uint32_t)min(before, (uint64_t)0xffffffffu);
-    row_of[tid] = row;
-    begin_of[tid] = copy ? ~begin : begin;             // the sign: its first fresh page is a copy
+    const int mine_need = grow ? pages - begin : 0;
+    uint32_t need;
+    off[tid] = plan_scan((uint32_t)min(mine_need, QMK_KV4_MAX_PAGES), sums[0], need);
+    begin_of[tid] = copy ? ~begin : begin;              // the sign: its first fresh page is a copy
 
     // enough free pages?
-    uint64_t mask = 0, ahead = 0, found = 0;
+    uint32_t ahead = 0, found = 0;
     int64_t block = 0;
     for (; block < c.num_pages && found < need; block += KV4_BLOCK_PAGES) {
-        mask = free_pages(c, block);
-        uint64_t total;
-        ahead = plan_scan((uint64_t)__popcll(mask), sums, total);
+        if (block) {
+            __syncthreads();
+            mask = free_pages(c, block);
+        }
+        uint32_t total;
+        ahead = plan_scan((uint32_t)__popcll(mask), sums[1], total);
         found += total;
     }
     if (found < need) {
+        if (mine_need > 0) atomicAdd(&lacking, (unsigned long long)mine_need);
+        __syncthreads();
         if (tid == 0) {
-            A.result[0] = (int)min(need - found, (uint64_t)0x7fffffff);
+            A.result[0] = (int)min(lacking - found, 0x7fffffffull);
             A.state[0] = 1;
         }
         return;
@@ -385,23 +401,25 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
     // hand them out, KV4_WINDOW at a time
     const bool kept = block <= KV4_BLOCK_PAGES;          // the first pass saw them all
     int32_t* job = A.state + 4;
-    uint64_t done = 0;
+    uint32_t done = 0;
     for (int64_t blk = 0; done < need; blk += KV4_BLOCK_PAGES) {
-        uint64_t total = found;
+        uint32_t total = found;
         if (!kept) {
+            __syncthreads();
             mask = free_pages(c, blk);
-            ahead = plan_scan((uint64_t)__popcll(mask), sums, total);
+            ahead = plan_scan((uint32_t)__popcll(mask), sums[1], total);
         }
-        const uint64_t take = min(total, need - done);
-        for (uint64_t w0 = 0; w0 < take; w0 += KV4_WINDOW) {
+        const uint32_t take = min(total, need - done);
+        for (uint32_t w0 = 0; w0 < take; w0 += KV4_WINDOW) {
+            if (w0) __syncthreads();
+            uint32_t k = ahead;
+            if (k < w0 + KV4_WINDOW && k < take)
+                for (uint64_t m = mask; m && k < min(w0 + KV4_WINDOW, take); m &= m - 1, ++k)
+                    if (k >= w0) list[k - w0] = (int)(blk + 64 * tid + __builtin_ctzll(m));
             __syncthreads();
-            uint64_t k = ahead;
-            for (uint64_t m = mask; m && k < w0 + KV4_WINDOW; m &= m - 1, ++k)
-                if (k >= w0) list[k - w0] = (int)(blk + 64 * tid + __builtin_ctzll(m));
-            __syncthreads();
-            const int n = (int)min((uint64_t)KV4_WINDOW, take - w0);
+            const int n = (int)min((uint32_t)KV4_WINDOW, take - w0);
             for (int j = tid; j < n; j += KV4_PLAN_THREADS) {
-                const uint32_t at = (uint32_t)(done + w0 + j);
+                const uint32_t at = done + w0 + j;
                 int lo = 0, hi = A.count;               // the last list row that begins at or before `at`
                 while (hi - lo > 1) {
                     const int mid = (lo + hi) >> 1;
@@ -410,13 +428,12 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
                 }
                 const int from = begin_of[lo], index = (from < 0 ? ~from : from) + (int)(at - off[lo]);
                 const int id = list[j];
-                int32_t* entry = c.table + (size_t)row_of[lo] * c.max_pages + index;
                 if (from < 0 && at == off[lo]) {
                     const uint32_t slot = atomicAdd(&copies, 1u);
                     job[2 * slot] = last[lo];
                     job[2 * slot + 1] = id;
                 }
-                *entry = id;
+                c.table[(size_t)row_of[lo] * c.max_pages + index] = id;
                 c.refs[id] = 1;
             }
         }
@@ -425,8 +442,7 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
     if (copy) atomicSub(&c.refs[page], 1);
     if (mine) {
         c.lens[row] = want;
-        job[2 * A.count + 2 * tid] = pages;
-        job[2 * A.count + 2 * tid + 1] = had;
+        *reinterpret_cast<int2*>(job + 2 * A.count + 2 * tid) = make_int2(pages, had);
     }
     __syncthreads();
     if (tid == 0) {
@@ -520,44 +536,45 @@ extern "C" __global__ __launch_bounds__(256) void qm_kv4_fork_rows(Kv4ForkArgs A
 // to the k-th free page below it.  First the plan (one workgroup), then the
 // moves.
 extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_compact(Kv4CompactArgs A) {
-    __shared__ uint64_t sums[KV4_PLAN_THREADS / 64];
+    __shared__ uint32_t sums[2][KV4_PLAN_THREADS / 64];
     const int tid = threadIdx.x;
     const Kv4Cache& c = A.c;
-    int64_t free = 0;
+    uint32_t free = 0;
     uint64_t mask = 0;
     for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
+        if (block) __syncthreads();
         mask = free_pages(c, block);
-        uint64_t total;
-        plan_scan((uint64_t)__popcll(mask), sums, total);
-        free += (int64_t)total;
+        uint32_t total;
+        plan_scan((uint32_t)__popcll(mask), sums[0], total);
+        free += total;
     }
-    const int64_t live = c.num_pages - free;
+    const int64_t live = c.num_pages - (int64_t)free;
     int32_t* movers = A.state + 4;
     int32_t* holes = movers + c.num_pages;
     int32_t* to = holes + c.num_pages;
-    uint64_t moves = 0, gaps = 0;
+    uint32_t moves = 0, gaps = 0;
     for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
-        if (c.num_pages > KV4_BLOCK_PAGES) mask = free_pages(c, block);
+        if (c.num_pages > KV4_BLOCK_PAGES) {
+            __syncthreads();
+            mask = free_pages(c, block);
+        }
         // bits of this thread's pages: in the pool, and below the bound
         const int64_t p0 = block + 64 * tid;
         const int in = (int)min(max(c.num_pages - p0, (int64_t)0), (int64_t)64);
         const int low = (int)min(max(live - p0, (int64_t)0), (int64_t)64);
         const uint64_t pool = in == 64 ? ~0ull : (1ull << in) - 1, below = low == 64 ? ~0ull : (1ull << low) - 1;
         const uint64_t hole = mask & below, move = ~mask & pool & ~below;
-        // both counts in one scan (at most 65536 each)
-        uint64_t total;
-        const uint64_t at = plan_scan((uint64_t)__popcll(hole) << 32 | (uint64_t)__popcll(move), sums, total);
-        uint64_t k = gaps + (at >> 32);
+        uint32_t h_all, m_all;
+        uint32_t k = gaps + plan_scan((uint32_t)__popcll(hole), sums[1], h_all);
         for (uint64_t m = hole; m; m &= m - 1) holes[k++] = (int)(p0 + __builtin_ctzll(m));
-        k = moves + (at & 0xffffffffu);
+        k = moves + plan_scan((uint32_t)__popcll(move), sums[0], m_all);
         for (uint64_t m = move; m; m &= m - 1) movers[k++] = (int)(p0 + __builtin_ctzll(m));
-        gaps += total >> 32;
-        moves += total & 0xffffffffu;
+        gaps += h_all;
+        moves += m_all;
     }
-    __syncthreads();
     for (int64_t p = live + tid; p < c.num_pages; p += KV4_PLAN_THREADS) to[p] = (int)p;
     __syncthreads();
-    for (uint64_t k = tid; k < moves; k += KV4_PLAN_THREADS) to[movers[k]] = holes[k];
+    for (uint32_t k = tid; k < moves; k += KV4_PLAN_THREADS) to[movers[k]] = holes[k];
     if (tid == 0) {
         A.state[0] = (int)live;
         A.state[1] = (int)moves;

@@ -30,6 +30,7 @@
 #define QMK_KV4_PAGE_BYTES (4 * QMK_KV4_HEAD_BYTES)
 #define QMK_KV4_V_WORDS 1024        // first word of the V codes
 #define QMK_KV4_META 8192           // first byte of the scales and minima
+#define QMK_KV4_MAX_PAGES 4194303   // pages of a pool (309 GB a layer): 1024 rows' needs are a uint32
 #define QMK_KV4_MAX_COUNT 1024      // rows of one resize or fork: one thread each
 #define QMK_KV4_MAX_ROWS 65536      // table rows: the LDS bitmap of those seen
 #define QMK_KV4_MAX_SPLIT 4096      // tokens of a decode workgroup: 64 pages

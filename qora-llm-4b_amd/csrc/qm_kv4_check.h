@@ -43,9 +43,9 @@ inline Fault check_cache(const char* who, const qm_kv4_cache* c) {
     if (c->layers <= 0 || c->num_pages <= 0 || c->rows <= 0 || c->max_pages <= 0)
         return fault(QM_ERR_INVALID_ARG, "%s: cache of %d layers, %d pages, %d rows of %d pages", who, c->layers,
                      c->num_pages, c->rows, c->max_pages);
-    if (c->rows > QMK_KV4_MAX_ROWS || c->max_pages > QMK_KV4_LEN_PAGES)
-        return fault(QM_ERR_SHAPE, "%s: %d rows (at most %d) of %d pages (at most %d)", who, c->rows, QMK_KV4_MAX_ROWS,
-                     c->max_pages, QMK_KV4_LEN_PAGES);
+    if (c->num_pages > QMK_KV4_MAX_PAGES || c->rows > QMK_KV4_MAX_ROWS || c->max_pages > QMK_KV4_LEN_PAGES)
+        return fault(QM_ERR_SHAPE, "%s: %d pages (at most %d), %d rows (at most %d) of %d pages (at most %d)", who,
+                     c->num_pages, QMK_KV4_MAX_PAGES, c->rows, QMK_KV4_MAX_ROWS, c->max_pages, QMK_KV4_LEN_PAGES);
     return Fault{};
 }
 

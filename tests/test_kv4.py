@@ -141,7 +141,7 @@ def test_refusals_of_caches():
                       ("4096 8193 8196 8200 8 100 16 32", 3), ("4096 8192 8196 8202 8 100 16 32", 3),
                       ("4096 8192 8196 8200 0 100 16 32", 3), ("4096 8192 8196 8200 8 -1 16 32", 3),
                       ("4096 8192 8196 8200 8 100 0 32", 3), ("4096 8192 8196 8200 8 100 16 0", 3),
-                      ("4096 8192 8196 8200 8 100 65537 32", 4), ("4096 8192 8196 8200 8 100 16 33554432", 4)]:
+                      ("4096 8192 8196 8200 8 100 65537 32", 4), ("4096 8192 8196 8200 8 4194304 16 32", 4), ("4096 8192 8196 8200 8 100 16 33554432", 4)]:
         got = ask([f"cache {bad}"] + calls)[1:]
         assert [a.split()[0] for a in got] == [str(code)] * 5, (bad, got)
         assert all(len(a.split()) > 1 for a in got)
