@@ -249,7 +249,6 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 #define KV4_WAVES 4
 #define KV4_Q_STRIDE (QM_GQA_HD + 8)   // bf16 of a q row in LDS: 16 rows 528 bytes apart fall into different banks
-#define KV4_P_BIAS 90.0f               // p and q carry 2^90: codes are bf16 subnormals
 
 // A wave's half pages come by LDS DMA, as they stand, into one of its two
 // buffers, the one after the next in flight; lane (g, c) = (lane >> 4,
@@ -274,6 +273,16 @@ QM_DEV bf16x8 codes_bf16(uint32_t w) {
     return __builtin_bit_cast(bf16x8, m);
 }
 
+// The same with the odd elements' codes from the other end, 15 - c (they are
+// the upper halves): one v_bitop3 each instead of the and.
+QM_DEV bf16x8 codes_bf16_turned(uint32_t w) {
+    const uint32_t v = w >> 8;
+    uint4 m = make_uint4((w & 0x000f000fu) ^ 0x000f0000u, (w & 0x00f000f0u) ^ 0x00f00000u, (v & 0x000f000fu) ^ 0x000f0000u,
+                         (v & 0x00f000f0u) ^ 0x00f00000u);
+    asm("" : "+v"(m.x), "+v"(m.y), "+v"(m.z), "+v"(m.w));
+    return __builtin_bit_cast(bf16x8, m);
+}
+
 // An f32 with the upper 8 bits of its significand: what a bf16 of its upper
 // half holds.
 QM_DEV float upper8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
@@ -283,10 +292,9 @@ QM_DEV half2_t halves(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
 // Per-wave softmax state and accumulators.  m: the maximum, in the scores'
 // units.  o[m]: dims 16 m + c; in lane group g = m >> 2, whose group of dims
 // that is, element e is head e's sum, in units of 2^-43; lo: the lane's share
-// of its head's and group's minimum terms, l of its head's sum (elements 2, 3,
-// 6, 7 apart), in units of 2^90.
+// of its head's and group's minimum terms, l of its head's sum.
 struct WaveKv4 {
-    float m, l, l16, lo;
+    float m, l, lo;
     floatx4 o[16];
 };
 
@@ -396,7 +404,6 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
         if (__ballot(was != -INFINITY)) {                // else nothing is summed yet
             const float f = was == m ? 1.0f : __builtin_amdgcn_exp2f((was - m) * 0x1p43f);
             st.l *= f;
-            st.l16 *= f;
             st.lo *= f;
             const float f0 = readlane_f32(f, 0), f1 = readlane_f32(f, 1), f2 = readlane_f32(f, 2), f3 = readlane_f32(f, 3);
 #pragma unroll
@@ -408,20 +415,20 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
             }
         }
     }
-    const float bias = fmaf(-st.m, 0x1p43f, KV4_P_BIAS), bias16 = fmaf(-st.m, 0x1p43f, KV4_P_BIAS - 4.0f);
+    const float bias = -st.m * 0x1p43f;
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], 0x1p43f, e & 2 ? bias16 : bias));
-    st.l += (p[0] + p[1]) + (p[4] + p[5]);
-    st.l16 += (p[2] + p[3]) + (p[6] + p[7]);
-    float lo1 = 0.0f, lo16 = 0.0f;
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], 0x1p43f, bias));
+    st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    // Every other token from the other end of its range, lo + s c = (lo + 15 s)
+    // - s (15 - c): both sums then hover about the result instead of growing
+    // with the tokens and cancelling at the end (at 32769 tokens of like weight
+    // that cost a factor 5 of the error).
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float w = (float)halves(lo[e >> 1])[e & 1];
-        if (e & 2) lo16 = fmaf(p[e], w, lo16);
-        else lo1 = fmaf(p[e], w, lo1);
+        const float from = (float)halves(lo[e >> 1])[e & 1];
+        st.lo = fmaf(p[e], e & 1 ? fmaf((float)__builtin_bit_cast(_Float16, sv[e]), 15.0f, from) : from, st.lo);
     }
-    st.lo += fmaf(lo16, 16.0f, lo1);
     // the three parts of p s: upper 8, middle 8 and lower 8 bits of its significand
     uint32_t part[3][4];
 #pragma unroll
@@ -429,7 +436,8 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
         float a[2], r[2], q[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            a[h] = fmaf(p[2 * i + h], (float)__builtin_bit_cast(_Float16, sv[2 * i + h]), 0.0f);
+            const float w = p[2 * i + h] * ((i & 1 ? 0x1p86f : 0x1p90f) * (h ? -1.0f : 1.0f));
+            a[h] = fmaf(w, (float)__builtin_bit_cast(_Float16, sv[2 * i + h]), 0.0f);
             r[h] = a[h] - upper8(a[h]);
             q[h] = r[h] - upper8(r[h]);
         }
@@ -444,7 +452,7 @@ QM_DEV void weigh(WaveKv4& st, float (&x)[8], const uint8_t* buf, int left, int 
     for (int j = 0; j < 4; ++j) {
         bf16x8 v[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) v[m] = codes_bf16(vw[4 * j + m]);
+        for (int m = 0; m < 4; ++m) v[m] = codes_bf16_turned(vw[4 * j + m]);
 #pragma unroll
         for (int n = 0; n < 3; ++n)
 #pragma unroll
@@ -591,7 +599,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
 
     WaveKv4 st;
     st.m = -INFINITY;
-    st.l = st.l16 = st.lo = 0.0f;
+    st.l = st.lo = 0.0f;
 #pragma unroll
     for (int m = 0; m < 16; ++m) st.o[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint16_t* qsrc = &sh.q[min(c, 12)][8 * g];
@@ -621,15 +629,15 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     // Lane group g has group g of the dims, for its four heads.  A head's
     // minimum term of that group stands in the lanes of column 4 g + head.
     {
-        const float l = sum_xor32(sum_xor16(fmaf(st.l16, 16.0f, st.l))), lo = sum_xor32(sum_xor16(st.lo));
+        const float l = sum_xor32(sum_xor16(st.l)), lo = sum_xor32(sum_xor16(st.lo));
         if (lane < 4) {
             sh.m[w][lane] = st.m;
-            sh.l[w][lane] = l * 0x1p-90f;
+            sh.l[w][lane] = l;
         }
         float* acc = reinterpret_cast<float*>(sh.ring[w]);          // the wave's own buffers, all read
 #pragma unroll
         for (int head = 0; head < 4; ++head) {
-            const float base = __shfl(lo, 4 * g + head) * 0x1p-90f;
+            const float base = __shfl(lo, 4 * g + head);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const float a = g & 1 ? st.o[4 + m][head] : st.o[m][head], d = g & 1 ? st.o[12 + m][head] : st.o[8 + m][head];
