@@ -19,12 +19,14 @@ struct HalfAt {
 // false: none taken.
 QM_DEV bool half_at(const Kv4RowsArgs& A, int b, int tile, HalfAt& h) {
     const int first = A.first ? A.first[b] : 0;
-    h.t0 = ((first >> 5) + tile) << 5;
     const int64_t end = min((int64_t)first + A.n, (int64_t)A.c.lens[A.row + b]);
-    h.src0 = (int64_t)h.t0 - first;
-    h.lo = max(0, first - h.t0);
-    h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, max(end - h.t0, (int64_t)0));
-    return first >= 0 && h.lo < h.hi && (h.t0 >> 6) < A.c.max_pages;
+    const int64_t t0 = ((int64_t)(first >> 5) + tile) << 5;
+    if (first < 0 || first >= end || t0 >= end || (t0 >> 6) >= A.c.max_pages) return false;
+    h.t0 = (int)t0;
+    h.src0 = t0 - first;
+    h.lo = (int)max((int64_t)0, -h.src0);
+    h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, end - t0);
+    return true;
 }
 // Its place in the pool; null: its table entry is no page.
 QM_DEV uint8_t* half_page(const Kv4RowsArgs& A, int b, int head, const HalfAt& h) {

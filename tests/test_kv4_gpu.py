@@ -128,6 +128,21 @@ def test_store_leaves_out_what_has_no_place(ctx):
     assert np.array_equal(got, np.where(there[:, None, :, None], want, np.uint16(0x1234)))
 
 
+def test_store_of_tokens_at_the_ends_of_int32(ctx):
+    """Positions near the ends of int32 (past every length, or negative) leave the pool as it was."""
+    ref = R.Cache(1, 6, 6, 1, seed=9)
+    assert ref.resize([0, 1, 2, 3, 4], [64] * 5) == 0
+    c = upload(ctx, ref)
+    k, v = kv_rows(np.random.default_rng(10), 6, 4, 70)
+    kd, vd = ctx.upload(k.view(np.uint16)), ctx.upload(v.view(np.uint16))
+    first = [2 ** 31 - 1, 2 ** 31 - 33, -2 ** 31, -1, 64, 0]
+    print("case: store, positions at the ends of int32", flush=True)
+    ctx.kv4_store(c, 0, 0, 6, ints(ctx, first), 70, kd, vd, 70)
+    assert_same(ctx, c, ref)
+    ctx.kv4_load(c, 0, 0, 6, ints(ctx, first), 70, kd, vd, 70)
+    assert np.array_equal(ctx.download(kd, k.shape, np.uint16), k.view(np.uint16))
+
+
 def test_store_values_at_the_edges_of_f16(ctx):
     """Equal values, the widest range, subnormals, signed zeros, infinities and NaN, group by group."""
     rng = np.random.default_rng(7)
@@ -394,13 +409,58 @@ def test_decode_more_rows_than_a_wave_looks_at(ctx):
     assert_same(ctx, s.c, s.ref)
 
 
+def test_decode_slots_of_long_rows(ctx):
+    """The same where the tokens are dealt to workgroups and joined: slots in any order, padded rows, repeats, rows longer
+    than max_len, empty ones."""
+    s = Step(ctx, [900, 0, 1400, 333, 2600, 64, 1, 1201, 700, 5], seed=83)
+    slots = [4, -1, 0, 4, 2, 10, 3, 0, 1, 8]
+    print(f"case: kv4 decode slots={slots} of long rows", flush=True)
+    got, want = s.run(ctx, 1400, slots=slots)
+    s.check(got, want)
+    assert np.isnan(got[[0, 3, 7]]).all() and (got[[1, 5, 8]] == 0).all()
+    assert_same(ctx, s.c, s.ref)
+
+
+def test_decode_dealt_to_more_rows_than_a_wave(ctx):
+    """150 batch rows, lengths up to 900, the tokens dealt in blocks of 64 rows; with slots, repeats in later blocks."""
+    rng = np.random.default_rng(84)
+    lens = rng.integers(0, 900, 150)
+    lens[[0, 63, 64, 149]], lens[[1, 127, 128]] = 900, 0
+    for slots in (None, list(rng.permutation(150)[:140]) + [-1, 150] + [0] * 8):
+        s = Step(ctx, lens.tolist(), seed=85, max_pages=15)
+        print(f"case: kv4 decode of 150 rows, slots={slots is not None}", flush=True)
+        got, want = s.run(ctx, 900, slots=slots)
+        s.check(got, want)
+        assert_same(ctx, s.c, s.ref)
+
+
+def test_decode_long_splits(ctx):
+    """Enough tokens that a split has its most, 4096: 64 rows of up to 9300 tokens, some checked."""
+    lens = [5000 + 70 * i for i in range(62)] + [4097, 3]
+    s = Step(ctx, lens, seed=86)
+    print("case: kv4 decode, the longest splits", flush=True)
+    cos, sin = M.rope_table(max(lens))
+    out = ctx.alloc(64 * 4096 * 4)
+    ctx.gqa_decode_kv4(s.c, 0, 64, None, *s.inputs(ctx), ctx.upload(cos), ctx.upload(sin), max(lens), max(lens), None, out)
+    got = ctx.download(out, (64, 16, 256), np.float32)
+    some = [0, 31, 61, 62, 63]
+    only = [i if i in some else -1 for i in range(64)]
+    want = s.ref.decode(0, only, 64, s.q_gate, s.k_new, s.v_new, s.q_norm, s.k_norm, cos, sin, max(lens))
+    s.check(got[some], want[some])
+
+
 def test_decode_entries_that_are_no_page(ctx):
     """Pages outside the pool are skipped, also where the new token would go, and a row of none is zero."""
-    s = Step(ctx, [300, 200, 130, 64], seed=79)
+    for lens in ([300, 200, 130, 64], [1300, 200, 130, 64]):
+        _no_page(ctx, lens)
+
+
+def _no_page(ctx, lens):
+    s = Step(ctx, lens, seed=79)
     s.ref.table[0, 1], s.ref.table[1, 3], s.ref.table[2], s.ref.table[3, 0] = 10 ** 6, -1, -1, 2 ** 31 - 1
     ctx.upload(s.ref.table, s.c.table)
     print("case: kv4 decode, entries that are no page", flush=True)
-    got, want = s.run(ctx, 300)
+    got, want = s.run(ctx, max(lens))
     s.check(got, want)
     assert (got[2:] == 0).all()
     assert_same(ctx, s.c, s.ref)
@@ -421,12 +481,17 @@ def test_decode_nan_in_a_group_reaches_its_heads_only(ctx):
 
 
 def test_decode_after_a_refused_resize_does_nothing(ctx):
-    s = Step(ctx, [100, 64], seed=81)
+    for lens in ([100, 64], [100, 1000]):
+        _after_refused(ctx, lens)
+
+
+def _after_refused(ctx, lens):
+    s = Step(ctx, lens, seed=81)
     for gate, runs in ((ints(ctx, [3]), False), (ints(ctx, [-1]), False), (ints(ctx, [0]), True)):
         print(f"case: kv4 decode gated, runs={runs}", flush=True)
         before = R.Cache.__new__(R.Cache)
         before.__dict__ = {k: v.copy() for k, v in s.ref.__dict__.items()}
-        got, want = s.run(ctx, 100, gate=gate)
+        got, want = s.run(ctx, max(lens), gate=gate)
         if runs:
             s.check(got, want)
             assert_same(ctx, s.c, s.ref)
