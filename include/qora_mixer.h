@@ -361,8 +361,9 @@ int32_t qm_kv4_compact(qm_context* ctx, qm_stream stream, const qm_kv4_cache* ca
  * layer from f16 rows k_dev, v_dev [batch][4][capacity][256] (rows 0 .. n - 1
  * of each head; the layout of qm_gqa_prefill's and qm_gqa_decode's caches).
  * first_dev int32 [batch], or NULL: 0.  Tokens at or past a row's length are
- * left out, as are sequences whose first is negative: grow the row with
- * qm_kv4_resize first. */
+ * left out, as are sequences whose first is negative (grow the row with
+ * qm_kv4_resize first), and, by _store, tokens of pages that other rows hold
+ * too. */
 int32_t qm_kv4_store(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
                      int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
                      const uint16_t* k_dev, const uint16_t* v_dev, int64_t capacity);
@@ -379,8 +380,9 @@ int32_t qm_kv4_load(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache
  * and v are written there in 4 bits, and attention reads lens tokens, the new
  * one as it is kept.  A batch row whose slot is outside the table (-1) or
  * whose length is 0 writes nothing and its output is 0.  One whose length is
- * over max_len, or whose slot an earlier batch row has, writes nothing and its
- * output is NaN.
+ * over max_len, whose slot an earlier batch row has, or whose last page other
+ * rows hold too (it was forked after it grew), writes nothing and its output
+ * is NaN.
  * max_len  upper bound of the lengths: at most rope_len (else
  *          QM_ERR_ROPE_RANGE) and QM_KV4_PAGE_TOKENS * max_pages
  *          (QM_ERR_CAPACITY)

@@ -40,7 +40,8 @@
 // A batch row of the step: its table row and the tokens to read there, the
 // last of them new (0: none, the output is zero).  A row that is refused (its
 // output is NaN) is longer than max_len, or steps a table row that an earlier
-// batch row has.
+// batch row has; or other rows hold its last page too, which the wave that
+// would write there finds.
 struct StepRow {
     int row, len;
     bool refused;
@@ -541,6 +542,12 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     }
     // the norms meanwhile
     const bool appends = pos >= t_begin && pos < t_end;
+    const int new_half = appends ? pos / QMK_KV4_HALF_TOKENS : -1;
+    int holders = 0;                                       // of the page to write to
+    if (new_half >= h0 && (new_half - h0) % KV4_WAVES == 0) {
+        const int id = __builtin_amdgcn_readlane(ids, (new_half >> 1) - page0);
+        if (kv4_is_page(A.c, id)) holders = A.c.refs[id];
+    }
     float q[4] = {qx.x, qx.y, qx.z, qx.w};
     norm_head(q, qn);
     double k64[4] = {nx.x, nx.y, nx.z, nx.w};
@@ -604,7 +611,6 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
     for (int m = 0; m < 16; ++m) st.o[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint16_t* qsrc = &sh.q[min(c, 12)][8 * g];
     const float qsum = sh.qsum[c & 3][c >> 2];
-    const int new_half = appends ? pos / QMK_KV4_HALF_TOKENS : -1;
     int i = 0;
     for (int h = h0; h < h_end; h += KV4_WAVES, i ^= 1) {
         // this round's half page is here when only the next one's DMA is out
@@ -612,7 +618,10 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         uint8_t* buf = sh.ring[w][i];
         if (there[0]) {
-            if (h == new_half) put_token(buf, half[0], sh, pos & (QMK_KV4_HALF_TOKENS - 1), lane);
+            if (h == new_half) {
+                if (holders > 1) st.l = __builtin_nanf("");
+                else put_token(buf, half[0], sh, pos & (QMK_KV4_HALF_TOKENS - 1), lane);
+            }
             float x[8];
             scores(x, buf, qsrc, qsum, lane);
             weigh(st, x, buf, t_end - h * QMK_KV4_HALF_TOKENS, lane);

@@ -28,10 +28,12 @@ QM_DEV bool half_at(const Kv4RowsArgs& A, int b, int tile, HalfAt& h) {
     h.hi = (int)min((int64_t)QMK_KV4_HALF_TOKENS, end - t0);
     return true;
 }
-// Its place in the pool; null: its table entry is no page.
-QM_DEV uint8_t* half_page(const Kv4RowsArgs& A, int b, int head, const HalfAt& h) {
-    const int id = A.c.table[(size_t)(A.row + b) * A.c.max_pages + (h.t0 >> 6)];
-    return kv4_is_page(A.c, id) ? kv4_half(A.c, A.layer, id, head, (h.t0 >> 5) & 1) : nullptr;
+// Its table entry, and its place in the pool if that is a page.
+QM_DEV int half_id(const Kv4RowsArgs& A, int b, const HalfAt& h) {
+    return A.c.table[(size_t)(A.row + b) * A.c.max_pages + (h.t0 >> 6)];
+}
+QM_DEV uint8_t* half_page(const Kv4RowsArgs& A, int id, int head, const HalfAt& h) {
+    return kv4_half(A.c, A.layer, id, head, (h.t0 >> 5) & 1);
 }
 
 // Smallest / largest over the 8 lanes of a group.
@@ -149,8 +151,10 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4R
         const int t = min(max(16 * (e >> 2) + 4 * g + (e & 3), h.lo), h.hi - 1);     // any token for those left out
         raw[e] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * i);
     }
-    uint8_t* page = half_page(A, b, head, h);
-    if (!page) return;                                  // uniform
+    const int id = half_id(A, b, h);
+    if (!kv4_is_page(A.c, id)) return;                  // uniform
+    const int holders = A.c.refs[id];                   // looked at before the page is written
+    uint8_t* page = half_page(A, id, head, h);
     if (!whole) {                                       // uniform: the tokens left out stay
         for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
             reinterpret_cast<uint4*>(image)[j] = reinterpret_cast<const uint4*>(page)[j];
@@ -180,6 +184,7 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4R
         }
     }
     __syncthreads();
+    if (holders > 1) return;
     for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
         reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }
@@ -195,8 +200,9 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
     const int head = bh & 3, b = bh >> 2;
     HalfAt h;
     if (!half_at(A, b, tile, h)) return;                // uniform
-    const uint8_t* page = half_page(A, b, head, h);
-    if (!page) return;
+    const int id = half_id(A, b, h);
+    if (!kv4_is_page(A.c, id)) return;
+    const uint8_t* page = half_page(A, id, head, h);
     for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
         reinterpret_cast<uint4*>(w)[j] = reinterpret_cast<const uint4*>(page)[j];
     __syncthreads();

@@ -177,6 +177,8 @@ class Cache:
                 t = f + i
                 if t >= self.lens[row + b] or not self.is_page(self.table[row + b, t // TOKENS]):
                     continue
+                if self.refs[self.table[row + b, t // TOKENS]] > 1:
+                    continue
                 page = self.pages[layer, self.table[row + b, t // TOKENS]]
                 for head in range(KV):
                     put(page, head, t % TOKENS, k[b, head, i], 0)
@@ -208,6 +210,9 @@ class Cache:
             if n <= 0:
                 continue
             pos = n - 1
+            if self.is_page(self.table[r, pos // TOKENS]) and self.refs[self.table[r, pos // TOKENS]] > 1:
+                out[b] = np.nan
+                continue
             if self.is_page(self.table[r, pos // TOKENS]):
                 page = self.pages[layer, self.table[r, pos // TOKENS]]
                 k = _turn(k_new[b], k_norm, cos[pos], sin[pos]).astype(np.float32).astype(np.float16)

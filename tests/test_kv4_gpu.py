@@ -449,6 +449,36 @@ def test_decode_long_splits(ctx):
     s.check(got[some], want[some])
 
 
+@pytest.mark.parametrize("n", [70, 1500])
+def test_decode_of_rows_forked_after_they_grew(ctx, n):
+    """Their last page is not one row's: neither writes there, both outputs are NaN; once they have grown again, both step."""
+    s = Step(ctx, [n, 5, 20], seed=87, spare=6, max_pages=R.pages_of(n + 1))
+    assert run_fork(ctx, s.c, [0], [2]) == s.ref.fork([0], [2]) == 0
+    print(f"case: kv4 decode of forked rows, n={n}", flush=True)
+    got, want = s.run(ctx, n)
+    s.check(got, want)
+    assert np.isnan(got[[0, 2]]).all() and np.isfinite(got[1]).all()
+    assert_same(ctx, s.c, s.ref)
+    assert run_resize(ctx, s.c, None, [1, 0, 1], True) == s.ref.resize(None, [1, 0, 1], True) == 0
+    got, want = s.run(ctx, n + 1)
+    s.check(got, want)
+    assert np.isfinite(got).all()
+    assert_same(ctx, s.c, s.ref)
+
+
+def test_store_leaves_shared_pages_alone(ctx):
+    ref = R.Cache(1, 9, 3, 3, seed=11)
+    c = upload(ctx, ref)
+    assert run_resize(ctx, c, [0], [150]) == ref.resize([0], [150]) == 0
+    assert run_fork(ctx, c, [0], [1]) == ref.fork([0], [1]) == 0
+    assert run_resize(ctx, c, [1], [160]) == ref.resize([1], [160]) == 0      # its third page is its own now
+    k, v = kv_rows(np.random.default_rng(12), 1, 4, 160)
+    print("case: store over shared pages", flush=True)
+    ctx.kv4_store(c, 0, 1, 1, None, 160, ctx.upload(k.view(np.uint16)), ctx.upload(v.view(np.uint16)), 160)
+    ref.store(0, 1, 1, None, 160, k, v)
+    assert_same(ctx, c, ref)
+
+
 def test_decode_entries_that_are_no_page(ctx):
     """Pages outside the pool are skipped, also where the new token would go, and a row of none is zero."""
     for lens in ([300, 200, 130, 64], [1300, 200, 130, 64]):
