@@ -7,9 +7,11 @@
 // A workgroup takes half a page (32 tokens) of one sequence and head, whose
 // 9216 bytes it puts together in LDS.  A token's row is 32 lanes x 8 dims, so
 // a group of 64 dims is 8 lanes, and a lane's 8 codes of a token are one K
-// word.  A V word holds 8 tokens of one dim: a lane takes 8 tokens and turns
-// their 8 x 8 codes in registers.
+// word.  A V word holds 8 tokens of one dim: two lanes with 4 tokens each turn
+// their 4 x 8 codes in registers and exchange halves (a lane with all 8 was as
+// fast on long prompts and took twice the chain on short ones).
 #define KV4_ROWS_THREADS 256
+#define KV4_STORE_THREADS 512
 
 struct HalfAt {
     int t0;                  // token 0 of the half page
@@ -108,30 +110,24 @@ QM_DEV Coded code8(uint4 raw, int lane) {
     return c;
 }
 
-// 8 x 8 nibbles: nibble a of r[b] and nibble b of r[a] change places.
-QM_DEV void turn_nibbles(uint32_t (&r)[8]) {
+// Four rows of eight nibbles, as rows 0, 1, 4, 5 of an 8 x 8 whose others are
+// zero, turned: word n has nibble n of them in its nibbles 0, 1, 4, 5.
+QM_DEV void turn_nibbles(uint32_t (&out)[8], uint32_t r0, uint32_t r1, uint32_t r4, uint32_t r5) {
+    // halves of rows a, a + 4
+    const uint32_t h[4] = {__builtin_amdgcn_perm(r4, r0, 0x05040100u), __builtin_amdgcn_perm(r5, r1, 0x05040100u),
+                           __builtin_amdgcn_perm(r4, r0, 0x07060302u), __builtin_amdgcn_perm(r5, r1, 0x07060302u)};
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {                       // halves of rows a, a + 4
-        const uint32_t x = r[a], y = r[a + 4];
-        r[a] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-        r[a + 4] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-    }
+    for (int i = 0; i < 2; ++i) {                       // words 4 i ..
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                       // bytes of rows a, a + 2
-        const int a = (i & 1) + 4 * (i >> 1);
-        const uint32_t x = r[a], y = r[a + 2];
-        r[a] = __builtin_amdgcn_perm(y, x, 0x06020400u);
-        r[a + 2] = __builtin_amdgcn_perm(y, x, 0x07030501u);
-    }
-#pragma unroll
-    for (int a = 0; a < 8; a += 2) {                    // nibbles of rows a, a + 1
-        const uint32_t x = r[a], y = r[a + 1];
-        r[a] = (x & 0x0f0f0f0fu) | (y & 0x0f0f0f0fu) << 4;
-        r[a + 1] = ((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
+        for (int j = 0; j < 2; ++j) {                   // bytes of rows a, a + 2, then nibbles of rows a, a + 1
+            const uint32_t x = (j ? h[2 * i] >> 8 : h[2 * i]) & 0x00ff00ffu, y = (j ? h[2 * i + 1] >> 8 : h[2 * i + 1]) & 0x00ff00ffu;
+            out[4 * i + 2 * j] = (x & 0x000f000fu) | (y & 0x000f000fu) << 4;
+            out[4 * i + 2 * j + 1] = (x >> 4 & 0x000f000fu) | (y & 0x00f000f0u);
+        }
     }
 }
 
-extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
     __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
     const int tid = threadIdx.x;
     const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
@@ -139,53 +135,61 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_store(Kv4R
     HalfAt h;
     if (!half_at(A, b, tile, h)) return;                // uniform
     const bool whole = h.lo == 0 && h.hi == QMK_KV4_HALF_TOKENS;
-    // Waves 0 and 1 have V, 2 and 3 K; a lane eight tokens 16 (e >> 2) + 4 g +
-    // (e & 3) of dims 8 i ..
-    const bool is_v = tid < 128;
-    const int i = tid & 31, g = (tid >> 5) & 3;
+    // Waves 0..3 have V, 4..7 K; a lane four tokens 16 u + 4 g + k of dims 8 i ..
+    const bool is_v = tid < 256;
+    const int i = tid & 31, u = (tid >> 5) & 1, g = (tid >> 6) & 3;
     const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
     const uint16_t* from = is_v ? A.v : A.k;
-    uint4 raw[8];
+    uint4 raw[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int t = min(max(16 * (e >> 2) + 4 * g + (e & 3), h.lo), h.hi - 1);     // any token for those left out
-        raw[e] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * i);
+    for (int k = 0; k < 4; ++k) {
+        const int t = min(max(16 * u + 4 * g + k, h.lo), h.hi - 1);      // any token for those left out
+        raw[k] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * i);
     }
     const int id = half_id(A, b, h);
     if (!kv4_is_page(A.c, id)) return;                  // uniform
     const int holders = A.c.refs[id];                   // looked at before the page is written
     uint8_t* page = half_page(A, id, head, h);
     if (!whole) {                                       // uniform: the tokens left out stay
-        for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
+        for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_STORE_THREADS)
             reinterpret_cast<uint4*>(image)[j] = reinterpret_cast<const uint4*>(page)[j];
         __syncthreads();
     }
     uint16_t* meta = reinterpret_cast<uint16_t*>(image) + QMK_KV4_META / 2 + (is_v ? 256 : 0);
-    uint32_t word[8], keep = 0;                         // in the order of the nibbles
+    uint32_t word[4], keep = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int t = 16 * (e >> 2) + 4 * g + (e & 3);
+    for (int k = 0; k < 4; ++k) {
+        const int t = 16 * u + 4 * g + k;
         const bool in = t >= h.lo && t < h.hi;
-        const Coded c = code8(raw[e], tid & 63);
-        word[kv4_nibble(e)] = c.word;
-        keep |= in ? 0u : 15u << (4 * kv4_nibble(e));
+        const Coded c = code8(raw[k], tid & 63);
+        word[k] = c.word;
+        keep |= in ? 0u : 15u << (4 * kv4_nibble(k));
         if (!is_v && in) image[kv4_k_word(t, 8 * i)] = c.word;
         if ((i & 7) == 0 && in) {
             meta[kv4_s_at(t, i >> 3)] = c.s;
             meta[128 + kv4_lo_at(t, i >> 3)] = c.lo;
         }
     }
-    if (is_v) {
-        turn_nibbles(word);                             // word n: the tokens of dim 8 i + (the element of nibble n)
+    if (is_v) {                                         // uniform per wave
+        // The run's tokens are elements 4 u + k of the words: nibbles 0, 4, 1, 5,
+        // and for u = 1 two further up.  Lane and lane + 32 have the two runs of
+        // the same dims; after the exchange the one has elements 0..3 of dims
+        // 8 i .. + 3 and the other's there, the other likewise dims 8 i + 4 ..
+        uint32_t out[8];                                // word n: dim 8 i + (the element of nibble n)
+        turn_nibbles(out, word[0], word[2], word[1], word[3]);
+        const auto kept = __builtin_amdgcn_permlane32_swap(keep, keep, false, false);
+        const uint32_t stay = kept[0] | kept[1] << 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            uint32_t* at = &image[kv4_v_word(4 * g, 8 * i + k)];
-            *at = whole ? word[kv4_nibble(k)] : (word[kv4_nibble(k)] & ~keep) | (*at & keep);
+        for (int k = 0; k < 4; ++k) {
+            const auto w = __builtin_amdgcn_permlane32_swap(out[kv4_nibble(k)], out[kv4_nibble(k + 4)], false, false);
+            const uint32_t both = w[0] | w[1] << 8;
+            uint32_t* at = &image[kv4_v_word(4 * g, 8 * i + k + 4 * u)];
+            *at = whole ? both : (both & ~stay) | (*at & stay);
         }
     }
     __syncthreads();
     if (holders > 1) return;
-    for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_ROWS_THREADS)
+    for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_STORE_THREADS)
         reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }
 

@@ -1233,7 +1233,7 @@ Kv4Cache kv4_of(const qm_kv4_cache& c) {
     return Kv4Cache{c.pages_dev, c.table_dev, c.lens_dev, c.refs_dev, c.layers, c.num_pages, c.rows, c.max_pages};
 }
 
-int32_t kv4_rows(qm_context* c, qm_stream stream, hipFunction_t f, const char* who, const qm_kv4_cache* cache,
+int32_t kv4_rows(qm_context* c, qm_stream stream, hipFunction_t f, uint32_t threads, const char* who, const qm_kv4_cache* cache,
                  int32_t layer, int32_t row, int32_t batch, const int32_t* first, int32_t n, uint16_t* k, uint16_t* v,
                  int64_t capacity) {
     const OnDevice on(c);
@@ -1245,7 +1245,7 @@ int32_t kv4_rows(qm_context* c, qm_stream stream, hipFunction_t f, const char* w
     const int64_t grid = halves * batch * QM_GQA_KV_HEADS;
     if (grid > 0x7fffffff) return fail(c, QM_ERR_INVALID_ARG, "%s: grid too large", who);
     Kv4RowsArgs a{kv4_of(*cache), first, k, v, capacity, layer, row, batch, n, static_cast<int32_t>(halves)};
-    return launch(c, f, static_cast<uint32_t>(grid), 256, a, pick(c, stream), who);
+    return launch(c, f, static_cast<uint32_t>(grid), threads, a, pick(c, stream), who);
 }
 }  // namespace
 
@@ -1255,14 +1255,14 @@ int32_t qm_kv4_store(qm_context* c, qm_stream stream, const qm_kv4_cache* cache,
                      int32_t batch, const int32_t* first, int32_t n, const uint16_t* k, const uint16_t* v,
                      int64_t capacity) {
     if (!c) return QM_ERR_INVALID_ARG;
-    return kv4_rows(c, stream, c->f_kv4_store, "qm_kv4_store", cache, layer, row, batch, first, n,
+    return kv4_rows(c, stream, c->f_kv4_store, 512, "qm_kv4_store", cache, layer, row, batch, first, n,
                     const_cast<uint16_t*>(k), const_cast<uint16_t*>(v), capacity);
 }
 
 int32_t qm_kv4_load(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t row,
                     int32_t batch, const int32_t* first, int32_t n, uint16_t* k, uint16_t* v, int64_t capacity) {
     if (!c) return QM_ERR_INVALID_ARG;
-    return kv4_rows(c, stream, c->f_kv4_load, "qm_kv4_load", cache, layer, row, batch, first, n, k, v, capacity);
+    return kv4_rows(c, stream, c->f_kv4_load, 256, "qm_kv4_load", cache, layer, row, batch, first, n, k, v, capacity);
 }
 
 int32_t qm_kv4_resize(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t count, const int32_t* rows,
