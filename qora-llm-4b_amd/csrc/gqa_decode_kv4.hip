@@ -97,20 +97,23 @@ QM_DEV int splits_of(int len, int chunk) {
 // an equal one, and a captured step whose max_len is the capacity as one whose
 // max_len is its length.  Every workgroup finds the same chunk: one workgroup
 // per CU, or two where that makes the chunk enough shorter, and not a few more
-// than that, which would be a round of their own; at most QMK_KV4_MAX_SPLIT
-// tokens.  Two workgroups on a CU take 1.7 times as long as one (a round of a
-// lone wave is bound by its own chain of vector and matrix instructions, of
-// two by the vector unit).  Measured, the step in us, one per CU / two: 1 x
-// 32769 tokens 17.5 / 19.2, 8 x 4097 15.6 / 18.0, 16 ragged rows of up to 7001
-// 20.8 / 19.8, 64 x 2049 34.4 / 34.6.
+// than that, which would be a round of their own.  Two workgroups on a CU take
+// 1.7 times as long as one (a round of a lone wave is bound by its own chain
+// of vector and matrix instructions, of two by the vector unit).  Measured,
+// the step in us, one per CU / two: 1 x 32769 tokens 17.5 / 19.2, 8 x 4097
+// 15.6 / 18.0, 16 ragged rows of up to 7001 20.8 / 19.8, 64 x 2049 34.4 /
+// 34.6.
+// Where that passes QMK_KV4_MAX_SPLIT tokens, so many full rounds of two
+// workgroups a CU that it does not (the longest chunk / this: 64 x 10001 169 /
+// 146, 3 x 200001 157 / 139); past QMK_KV4_ROUNDS rounds, where a partial one no longer
+// counts, the longest chunk.
 struct Deal {
     int chunk;
     int b, first;            // a batch row, and the splits before its own
     StepRow r;
 };
-QM_DEV int chunk_for(const GqaKv4Args& A, float total, int groups, int len) {
-    const float want = fminf(total * __builtin_amdgcn_rcpf((float)groups), (float)(QMK_KV4_MAX_SPLIT - 1));
-    int chunk = __builtin_amdgcn_readfirstlane(((int)want + 128) / 128 * 128);      // more than `want`
+QM_DEV int chunk_for(const GqaKv4Args& A, float want, int groups, int len) {
+    int chunk = __builtin_amdgcn_readfirstlane(((int)fminf(want, (float)(QMK_KV4_MAX_SPLIT - 1)) + 128) / 128 * 128);   // more than `want`
     if (A.batch <= 64)
         for (int tries = 0; tries < 4 && chunk < QMK_KV4_MAX_SPLIT; ++tries, chunk += 128)
             if (QM_GQA_KV_HEADS * __builtin_amdgcn_readlane(wave_scan(splits_of(len, chunk)), 63) <= groups) break;
@@ -119,10 +122,14 @@ QM_DEV int chunk_for(const GqaKv4Args& A, float total, int groups, int len) {
 QM_DEV int deal_chunk(const GqaKv4Args& A, const StepRow& mine, int lane) {
     float total = (float)mine.len;                         // the first 64 rows stay in the lanes
     for (int b0 = 64; b0 < A.batch; b0 += 64) total += (float)lane_row(A, b0 + lane).len;
-    total = wave_sum64(total) * QM_GQA_KV_HEADS;
-    const int one = chunk_for(A, total, A.cus, mine.len);
+    const float want = wave_sum64(total) * QM_GQA_KV_HEADS * __builtin_amdgcn_rcpf((float)A.cus);
+    int one = QMK_KV4_MAX_SPLIT;
+    if (want < (float)(QMK_KV4_MAX_SPLIT - 1)) one = chunk_for(A, want, A.cus, mine.len);
     if (one == 128) return one;
-    const int two = chunk_for(A, total, 2 * A.cus, mine.len);
+    // (2^-7: the f32 sum's error must not make a round more than the host counts)
+    const float rounds = fmaxf(ceilf(want * (0.5f / QMK_KV4_MAX_SPLIT) - 0x1p-7f), 1.0f);
+    if (rounds > (float)QMK_KV4_ROUNDS) return QMK_KV4_MAX_SPLIT;
+    const int two = chunk_for(A, want * 0.5f * __builtin_amdgcn_rcpf(rounds), 2 * A.cus * (int)rounds, mine.len);
     return 10 * one <= 17 * two && one < QMK_KV4_MAX_SPLIT ? one : two;
 }
 // The row of split k (all lanes agree), false past the last split; and, where

@@ -34,6 +34,7 @@
 #define QMK_KV4_MAX_COUNT 1024      // rows of one resize or fork: one thread each
 #define QMK_KV4_MAX_ROWS 65536      // table rows: the LDS bitmap of those seen
 #define QMK_KV4_MAX_SPLIT 4096      // tokens of a decode workgroup: 64 pages
+#define QMK_KV4_ROUNDS 64           // full rounds of decode workgroups that are dealt evenly
 #define QMK_KV4_LEN_PAGES 33554431  // pages of a row: its length is an int32
 
 #ifdef __HIPCC__

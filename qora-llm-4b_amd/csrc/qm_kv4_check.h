@@ -116,16 +116,18 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
 // (measured, one workgroup / dealt out, us: 1 row of 300 tokens 9.4 / 9.0, of
 // 500 10.8 / 9.1, 64 rows of 250 8.8 / 12.7, of 500 13.2 / 17.5; rows of one
 // step may differ, so not much longer).  Others are dealt out by the kernel
-// (deal_chunk): splits of 128 n tokens, n such that one or two workgroups a CU
-// have about the same number, at most QMK_KV4_MAX_SPLIT.  max_splits bounds the
-// splits of all rows: below the cap they are two workgroups a CU over the four
-// kv heads, and one per row (and two for the rounding of their f32 sum), at
-// the cap ceil(len / QMK_KV4_MAX_SPLIT) per row.
+// (deal_chunk): splits of 128 n tokens, at most QMK_KV4_MAX_SPLIT, n such that
+// one or two workgroups a CU, or some full rounds of two, have about the same
+// number.  max_splits bounds the splits of all rows: two workgroups a CU and
+// round over the four kv heads and one per row, and cus / 16 for the errors of
+// the f32 sum that the rounds are counted by (under 2^-7 of one); past
+// QMK_KV4_ROUNDS rounds ceil(len / QMK_KV4_MAX_SPLIT) per row.
 inline bool single(int64_t len, int64_t batch) { return len <= 256 || (len <= 512 && batch >= 16); }
 inline int64_t max_splits(int64_t len, int64_t batch, int cus) {
-    const int64_t least = (len + 127) / 128 * batch, capped = (len + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT * batch;
-    int64_t n = cus / 2 + batch + 2;
-    if (capped > n) n = capped;
+    const int64_t least = (len + 127) / 128 * batch, longest = (len + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT * batch;
+    const int64_t rounds = len * batch / (static_cast<int64_t>(QMK_KV4_MAX_SPLIT) * cus / 2) + 1;
+    int64_t n = cus / 2 * (rounds < QMK_KV4_ROUNDS ? rounds : QMK_KV4_ROUNDS) + batch + cus / 16 + 1;
+    if (rounds >= QMK_KV4_ROUNDS && longest > n) n = longest;
     return least < n ? least : n;
 }
 

@@ -183,23 +183,27 @@ def dealt(lens, cus):
     """The kernel's rule (deal_chunk) on the rows' lengths: tokens per split, splits of all rows."""
     count = lambda chunk: sum(-(-n // chunk) for n in lens)
 
-    def chunk_for(cus):
-        chunk = (int(min(np.float32(sum(lens)) * 4 / np.float32(cus), 4095)) + 128) // 128 * 128
+    def chunk_for(want, groups):
+        chunk = (int(min(want, 4095)) + 128) // 128 * 128
         for _ in range(4 if len(lens) <= 64 else 0):
-            if chunk >= 4096 or 4 * count(chunk) <= cus:
+            if chunk >= 4096 or 4 * count(chunk) <= groups:
                 break
             chunk += 128
         return chunk
 
-    one, two = chunk_for(cus), chunk_for(2 * cus)
-    chunk = one if one == 128 or (10 * one <= 17 * two and one < 4096) else two
+    want = np.float32(sum(lens)) * 4 / np.float32(cus)
+    rounds = max(int(np.ceil(want / 8192 - 2.0 ** -7)), 1)
+    if rounds > 64:
+        return 4096, count(4096)
+    one, two = chunk_for(want, cus), chunk_for(want / 2 / rounds, 2 * cus * rounds)
+    chunk = one if want < 4095 and 10 * one <= 17 * two and one < 4096 else two
     return chunk, count(chunk)
 
 
 def test_splits_fit_the_grid_and_the_reserve():
     rng = np.random.default_rng(4)
     cases = []
-    for most in (129, 500, 4097, 32769, 131072, 2 ** 20):
+    for most in (129, 500, 4097, 32769, 131072, 2 ** 20, 2 ** 31 - 1):
         for batch in (1, 2, 7, 19, 64, 65, 300):
             for cus in (4, 32, 256):
                 cases.append(([most] * batch, most, batch, cus))

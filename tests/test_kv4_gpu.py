@@ -276,7 +276,8 @@ class Step:
         rng = np.random.default_rng(seed)
         pages = [R.pages_of(n) for n in lens]
         rows, max_pages = rows or len(lens), max_pages or max(1, max(pages))
-        count = sum(pages) + spare
+        common = [0] + [max(0, min(share, n - 1, pages[0] - 1)) for n in pages[1:]]     # first pages, those of row 0
+        count = sum(pages) - sum(common) + spare
         self.ref = ref = R.Cache(layers, count, rows, max_pages, fill=False)
         # pages written in earnest, a few dozen and their copies, and garbage in the scales past each row's end
         some = np.zeros((min(count, 12), R.PAGE), np.uint8)
@@ -288,13 +289,11 @@ class Step:
         ids = rng.permutation(count).astype(np.int32)
         at = 0
         for r, n in enumerate(pages):
-            ref.table[r, :n] = ids[at:at + n]
-            at += n
+            own = n - common[r]
+            ref.table[r, :common[r]] = ref.table[0, :common[r]]
+            ref.table[r, common[r]:n] = ids[at:at + own]
+            at += own
             ref.lens[r] = lens[r]
-        for r in range(1, len(lens)):
-            own = min(share, pages[r] - 1, pages[0] - 1)
-            if own > 0:
-                ref.table[r, :own] = ref.table[0, :own]
         for r in range(len(lens)):
             np.add.at(ref.refs, ref.ids(r), 1)
         ref.pages[:] = some[rng.integers(0, len(some), (layers, count))]
@@ -447,6 +446,25 @@ def test_decode_long_splits(ctx):
     only = [i if i in some else -1 for i in range(64)]
     want = s.ref.decode(0, only, 64, s.q_gate, s.k_new, s.v_new, s.q_norm, s.k_norm, cos, sin, max(lens))
     s.check(got[some], want[some])
+
+
+@pytest.mark.parametrize("lens", [
+    [40000 - 7 * i for i in range(24)], [16000] * 60 + [3] * 9 + [1] + [12345] * 5, [200001] * 3, [70000] * 511 + [1]])
+def test_decode_of_more_tokens_than_one_round_of_splits(ctx, lens):
+    """So many tokens that the chip's workgroups take several rounds of splits (the last: more rounds than are dealt evenly),
+    by a common prompt; some rows checked."""
+    s = Step(ctx, lens, seed=87, share=10 ** 6)
+    b, most = len(lens), max(lens)
+    print(f"case: kv4 decode of {sum(lens)} tokens", flush=True)
+    cos, sin = M.rope_table(most)
+    out = ctx.upload(np.full((b, 16, 256), 7.0, np.float32))
+    ctx.gqa_decode_kv4(s.c, 0, b, None, *s.inputs(ctx), ctx.upload(cos), ctx.upload(sin), most, most, None, out)
+    got = ctx.download(out, (b, 16, 256), np.float32)
+    some = sorted({0, b // 2, b - 2, b - 1})
+    only = [i if i in some else -1 for i in range(b)]
+    want = s.ref.decode(0, only, b, s.q_gate, s.k_new, s.v_new, s.q_norm, s.k_norm, cos, sin, most)
+    s.check(got[some], want[some])
+    assert np.isfinite(got).all() and (np.abs(got).max((1, 2)) > 0).all()
 
 
 @pytest.mark.parametrize("n", [70, 1500])
