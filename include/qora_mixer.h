@@ -105,7 +105,9 @@ const char* qm_last_error(const qm_context* ctx);
 int32_t     qm_device_count(int32_t* count);
 /* Size the workspace for batches up to max_batch and KV lengths up to
  * max_kv_len (and DeltaNet and GQA prefill up to max_prefill_tokens) so
- * that later mixer calls do not allocate (e.g. under graph capture). */
+ * that later mixer calls do not allocate (e.g. under graph capture); calls on
+ * a 4-bit KV cache likewise, for lists of up to max_batch rows and a pool of
+ * no more pages than max_batch rows of max_kv_len tokens fill. */
 int32_t     qm_reserve(qm_context* ctx, int32_t max_batch, int32_t max_kv_len,
                        int32_t max_prefill_tokens);
 /* Launch-shape overrides for tests and tuning (0 = automatic).  Results do
