@@ -41,6 +41,7 @@
 #include "qm_kv4_device.h"
 #include "qm_kernel_args.h"
 
+#define KV4_JOIN 32           // splits that the merge loads at a time
 #define KV4_PART_STRIDE 260   // acc[256], m, l, pad[2]
 
 // A batch row of the step: its table row and the tokens to read there, the
@@ -108,11 +109,12 @@ QM_DEV int splits_of(int len, int chunk) {
 // of vector and matrix instructions, of two by the vector unit).  Measured,
 // the step in us, one per CU / two: 1 x 32769 tokens 17.5 / 19.2, 8 x 4097
 // 15.6 / 18.0, 16 ragged rows of up to 7001 20.8 / 19.8, 64 x 2049 34.4 /
-// 34.6.
+// 34.6.  One, too, where the merge would have more splits of two than it loads
+// at a time (1 x 16000 12.7 / 15.5, 4 ragged rows of up to 20000 20.3 / 22.1).
 // Where that passes QMK_KV4_MAX_SPLIT tokens, so many full rounds of two
 // workgroups a CU that it does not (the longest chunk / this: 64 x 10001 169 /
-// 146, 3 x 200001 157 / 139); past QMK_KV4_ROUNDS rounds, where a partial one no longer
-// counts, the longest chunk.
+// 146, 3 x 200001 157 / 139); past QMK_KV4_ROUNDS rounds, where a partial one
+// no longer counts, the longest chunk.
 struct Deal {
     int chunk;
     int b, first;            // a batch row, and the splits before its own
@@ -126,8 +128,12 @@ QM_DEV int chunk_for(const GqaKv4Args& A, float want, int groups, int len) {
     return chunk;
 }
 QM_DEV int deal_chunk(const GqaKv4Args& A, const StepRow& mine, int lane) {
-    float total = (float)mine.len;                         // the first 64 rows stay in the lanes
-    for (int b0 = 64; b0 < A.batch; b0 += 64) total += (float)lane_row(A, b0 + lane).len;
+    float total = (float)mine.len, longest = total;        // the first 64 rows stay in the lanes
+    for (int b0 = 64; b0 < A.batch; b0 += 64) {
+        const float len = (float)lane_row(A, b0 + lane).len;
+        total += len;
+        longest = fmaxf(longest, len);
+    }
     const float want = wave_sum64(total) * QM_GQA_KV_HEADS * __builtin_amdgcn_rcpf((float)A.cus);
     int one = QMK_KV4_MAX_SPLIT;
     if (want < (float)(QMK_KV4_MAX_SPLIT - 1)) one = chunk_for(A, want, A.cus, mine.len);
@@ -136,7 +142,8 @@ QM_DEV int deal_chunk(const GqaKv4Args& A, const StepRow& mine, int lane) {
     const float rounds = fmaxf(ceilf(want * (0.5f / QMK_KV4_MAX_SPLIT) - 0x1p-7f), 1.0f);
     if (rounds > (float)QMK_KV4_ROUNDS) return QMK_KV4_MAX_SPLIT;
     const int two = chunk_for(A, want * 0.5f * __builtin_amdgcn_rcpf(rounds), 2 * A.cus * (int)rounds, mine.len);
-    return 10 * one <= 17 * two && one < QMK_KV4_MAX_SPLIT ? one : two;
+    const bool many = __builtin_amdgcn_readfirstlane(max_xor32(max_xor16(row_max16(longest))) > (float)(KV4_JOIN * two));
+    return (10 * one <= 17 * two || many) && one < QMK_KV4_MAX_SPLIT ? one : two;
 }
 // The row of split k (all lanes agree), false past the last split; and, where
 // `note`, batch row k's splits to the merge: {first, splits}, -1 splits where
@@ -739,7 +746,7 @@ extern "C" __global__ __launch_bounds__(64) void qm_gqa_kv4_merge(GqaKv4Args A) 
     const float* P = A.partial + ((size_t)mine.x * 16 + h) * KV4_PART_STRIDE;
     Joined x{-INFINITY, 0.0f, 0.0f};
     if (mine.y <= 8) join<8>(x, P, mine.y, d, lane);
-    else join<32>(x, P, mine.y, d, lane);
+    else join<KV4_JOIN>(x, P, mine.y, d, lane);
     float y = x.l != 0.0f ? (x.o * __builtin_amdgcn_rcpf(x.l)) * sigmoid_fast(gate) : 0.0f;
     if (mine.y < 0) y = __builtin_nanf("");
     A.out[((size_t)b * QM_GQA_HEADS + h) * QM_GQA_HD + d] = y;

@@ -196,7 +196,8 @@ def dealt(lens, cus):
     if rounds > 64:
         return 4096, count(4096)
     one, two = chunk_for(want, cus), chunk_for(want / 2 / rounds, 2 * cus * rounds)
-    chunk = one if want < 4095 and 10 * one <= 17 * two and one < 4096 else two
+    few = one == 128 or 10 * one <= 17 * two or max(lens) > 32 * two
+    chunk = one if want < 4095 and few and one < 4096 else two
     return chunk, count(chunk)
 
 
