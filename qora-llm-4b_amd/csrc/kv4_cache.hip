@@ -245,7 +245,7 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
 
 // ---- the pages ------------------------------------------------------------
 #define KV4_PLAN_THREADS 1024
-#define KV4_BLOCK_PAGES (64 * KV4_PLAN_THREADS)     // pages whose state one pass holds, 64 a thread
+#define KV4_BLOCK_PAGES (64 * KV4_PLAN_THREADS)     // pages whose state one pass holds: up to 64 a thread
 #define KV4_WINDOW 4096                              // free pages handed out at a time
 
 // Inclusive sum over the wave's lanes: within the rows of 16, then the last
@@ -273,28 +273,49 @@ QM_DEV uint32_t plan_scan(uint32_t x, uint32_t* sums, uint32_t& total) {
     return before + incl - x;
 }
 
-// Bit j: page block + 64 tid + j is free (reference count 0).  Ids past the
-// pool are not free.
-QM_DEV uint64_t free_pages(const Kv4Cache& c, int64_t block) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// A pass's pages go to the threads 64 at a time, in order, spread over the
+// waves: lane l of wave w has the w * each + l-th 64 where l < each.  (With 64 a
+// lane from the first wave on, a pool of 4096 was one wave's: 10.1 us to plan a
+// compaction, now 5.7; 512 pages 3.8 to resize, now 3.0.)
+struct Share {
+    int each;
+    int64_t page0;           // the lane's first page; past the pool where it has none
+};
+QM_DEV Share share_of(const Kv4Cache& c, int64_t block) {
+    constexpr int WAVES = KV4_PLAN_THREADS / 64;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pages = (int)min(c.num_pages - block, (int64_t)KV4_BLOCK_PAGES);
+    Share s;
+    s.each = (pages + 64 * WAVES - 1) / (64 * WAVES);
+    s.page0 = lane < s.each ? block + 64 * (int64_t)(w * s.each + lane) : (int64_t)c.num_pages;
+    return s;
+}
+// Bit j: page page0 + j is free (reference count 0).  Ids past the pool are
+// not free.  N loads in flight.
+template <int N>
+QM_DEV uint64_t free_of(const Kv4Cache& c, int64_t at, int each) {
+    const int lane = threadIdx.x & 63;
     uint64_t mine = 0;
-    const int64_t at = block + (int64_t)w * 4096;
-    for (int r0 = 0; r0 < 64; r0 += 32) {               // 32 loads in flight
-        if (at + r0 * 64 >= c.num_pages) break;
-        int v[32];
+    for (int r0 = 0; r0 < each; r0 += N) {
+        int v[N];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             const int64_t p = at + (r0 + j) * 64 + lane;
             v[j] = c.refs[min(p, (int64_t)c.num_pages - 1)];
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < N; ++j) {
             const uint64_t m = __ballot(v[j] == 0);
             mine = lane == r0 + j ? m : mine;
         }
     }
-    // bits past the pool
-    const int64_t in = c.num_pages - (block + 64 * (int64_t)threadIdx.x);
+    return mine;
+}
+QM_DEV uint64_t free_pages(const Kv4Cache& c, int64_t block, Share& s) {
+    s = share_of(c, block);
+    const int64_t at = block + 64 * (int64_t)(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * s.each);
+    const uint64_t mine = s.each <= 4 ? free_of<4>(c, at, s.each) : free_of<32>(c, at, s.each);
+    const int64_t in = c.num_pages - s.page0;           // bits past the pool
     return in >= 64 ? mine : in <= 0 ? 0ull : mine & ((1ull << in) - 1);
 }
 
@@ -322,8 +343,8 @@ QM_DEV void copy_part(const Kv4Cache& c, int layer, int src, int dst, int part) 
 // list order.  Nothing is changed unless all of it can be.
 //
 // Bound by its chain of dependent loads (lengths, entry, count) and barriers;
-// the pool's counts are loaded first, beside them (1 row, a pool of 512: 3.8 us;
-// 64 rows, 32768: 5.9).
+// the pool's counts are loaded first, beside them (1 row, a pool of 512: 3.0 us;
+// 64 rows, 32768: 5.6).
 extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4ResizeArgs A) {
     __shared__ uint32_t sums[2][KV4_PLAN_THREADS / 64];
     __shared__ uint32_t seen[QMK_KV4_MAX_ROWS / 32];
@@ -345,7 +366,8 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
     const bool in = mine && (uint32_t)row < (uint32_t)c.rows;
     const int old = in ? c.lens[row] : 0;
     const int change = mine ? A.lens[tid] : 0;
-    uint64_t mask = free_pages(c, 0);
+    Share share;
+    uint64_t mask = free_pages(c, 0, share);
     __syncthreads();
 
     // the list, checked
@@ -398,7 +420,7 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
     for (; block < c.num_pages && found < need; block += KV4_BLOCK_PAGES) {
         if (block) {
             __syncthreads();
-            mask = free_pages(c, block);
+            mask = free_pages(c, block, share);
         }
         uint32_t total;
         ahead = plan_scan((uint32_t)__popcll(mask), sums[1], total);
@@ -422,7 +444,7 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
         uint32_t total = found;
         if (!kept) {
             __syncthreads();
-            mask = free_pages(c, blk);
+            mask = free_pages(c, blk, share);
             ahead = plan_scan((uint32_t)__popcll(mask), sums[1], total);
         }
         const uint32_t take = min(total, need - done);
@@ -431,7 +453,7 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_resize(Kv4
             uint32_t k = ahead;
             if (k < w0 + KV4_WINDOW && k < take)
                 for (uint64_t m = mask; m && k < min(w0 + KV4_WINDOW, take); m &= m - 1, ++k)
-                    if (k >= w0) list[k - w0] = (int)(blk + 64 * tid + __builtin_ctzll(m));
+                    if (k >= w0) list[k - w0] = (int)(share.page0 + __builtin_ctzll(m));
             __syncthreads();
             const int n = (int)min((uint32_t)KV4_WINDOW, take - w0);
             for (int j = tid; j < n; j += KV4_PLAN_THREADS) {
@@ -548,8 +570,19 @@ extern "C" __global__ __launch_bounds__(256) void qm_kv4_fork_rows(Kv4ForkArgs A
     if (tid == 0) c.lens[dst] = len;
 }
 
+// The pages p0 + (a set bit) of lane j, to list from `at` on, in order.
+QM_DEV void write_set(int32_t* list, uint64_t bits, uint32_t at, int64_t p0, int j) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, j);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), j);
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)at, j);
+    const int page = __builtin_amdgcn_readlane((int)p0, j);
+    const uint32_t before = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
+    if (((uint64_t)hi << 32 | lo) >> lane & 1) list[first + before] = page + lane;
+}
+
 // Live pages move down to [0, live): the k-th live page past that bound goes
-// to the k-th free page below it.  First the plan (one workgroup; 10 us for a
+// to the k-th free page below it.  First the plan (one workgroup; 5.7 us for a
 // pool of 4096), then the moves (8200 pages of 73,728 bytes: 257 us, 4.7 TB/s
 // read + written, the rate of a large copy).
 extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_compact(Kv4CompactArgs A) {
@@ -558,9 +591,10 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_compact(Kv
     const Kv4Cache& c = A.c;
     uint32_t free = 0;
     uint64_t mask = 0;
+    Share share;
     for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
         if (block) __syncthreads();
-        mask = free_pages(c, block);
+        mask = free_pages(c, block, share);
         uint32_t total;
         plan_scan((uint32_t)__popcll(mask), sums[0], total);
         free += total;
@@ -573,19 +607,21 @@ extern "C" __global__ __launch_bounds__(KV4_PLAN_THREADS) void qm_kv4_compact(Kv
     for (int64_t block = 0; block < c.num_pages; block += KV4_BLOCK_PAGES) {
         if (c.num_pages > KV4_BLOCK_PAGES) {
             __syncthreads();
-            mask = free_pages(c, block);
+            mask = free_pages(c, block, share);
         }
         // bits of this thread's pages: in the pool, and below the bound
-        const int64_t p0 = block + 64 * tid;
+        const int64_t p0 = share.page0;
         const int in = (int)min(max(c.num_pages - p0, (int64_t)0), (int64_t)64);
         const int low = (int)min(max(live - p0, (int64_t)0), (int64_t)64);
         const uint64_t pool = in == 64 ? ~0ull : (1ull << in) - 1, below = low == 64 ? ~0ull : (1ull << low) - 1;
         const uint64_t hole = mask & below, move = ~mask & pool & ~below;
         uint32_t h_all, m_all;
-        uint32_t k = gaps + plan_scan((uint32_t)__popcll(hole), sums[1], h_all);
-        for (uint64_t m = hole; m; m &= m - 1) holes[k++] = (int)(p0 + __builtin_ctzll(m));
-        k = moves + plan_scan((uint32_t)__popcll(move), sums[0], m_all);
-        for (uint64_t m = move; m; m &= m - 1) movers[k++] = (int)(p0 + __builtin_ctzll(m));
+        const uint32_t h_at = gaps + plan_scan((uint32_t)__popcll(hole), sums[1], h_all);
+        const uint32_t m_at = moves + plan_scan((uint32_t)__popcll(move), sums[0], m_all);
+        for (int j = 0; j < share.each; ++j) {          // the 64 pages of lane j by the wave
+            write_set(holes, hole, h_at, p0, j);
+            write_set(movers, move, m_at, p0, j);
+        }
         gaps += h_all;
         moves += m_all;
     }
