@@ -710,7 +710,10 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
 }
 
 // The splits' partials of query head h of batch row b, joined, and the gate:
-// one wave per (b, h, 64 dims), N splits' loads in flight at a time.
+// one wave per (b, h, 64 dims), N splits' loads in flight at a time.  A split
+// whose weight underflows to 0 counts all the same, so that a NaN in it
+// reaches the output as it does within a split; a split of no tokens has
+// zeros, and past the last one the last is read again with weight 0.
 struct Joined {
     float m, l, o;
 };
@@ -729,10 +732,7 @@ QM_DEV void join(Joined& x, const float* P, int n, int d, int lane) {
         x.l = x.l * c + wave_sum64(some ? ml.y * f : 0.0f);
         x.o *= c;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float fj = readlane_f32(f, j);
-            x.o = fj != 0.0f ? fmaf(a[j], fj, x.o) : x.o;
-        }
+        for (int j = 0; j < N; ++j) x.o = fmaf(a[j], readlane_f32(f, j), x.o);
         x.m = mb;
     }
 }

@@ -705,3 +705,28 @@ def test_calls_on_a_stream_of_the_callers(ctx):
         ctx.sync()
         ctx.stream = before
         ctx._check(ctx.lib.qm_stream_destroy(ctx.h, h))
+
+
+@pytest.mark.parametrize("n, late", [(900, False), (900, True), (1500, False), (5000, False), (5000, True)])
+def test_decode_nan_in_a_split_of_no_weight(ctx, n, late):
+    """A NaN group of V in a split whose scores are 300 below the others': its weight is 0, and 0 times NaN is NaN, in every
+    dealing of the tokens (8, 12 and 40 splits of 128 tokens).  Scores are relative to the query's own direction: k = -300 x
+    / |x| with |q| = 16 and q . k / 16."""
+    s = Step(ctx, [n], seed=110 + n)
+    x = np.zeros(256)
+    x[64:] = np.random.default_rng(n).standard_normal(192)         # past the rotary dims
+    s.q_gate[0, 8:12, :256] = x
+    s.q_norm[:] = 0
+    rows = np.tile((-300 * x / np.linalg.norm(x)).astype(np.float16), (64, 1))
+    page0 = (n - 1) // 128 * 2 - 2 if late else 0                  # the last split but one, or the first
+    for j in (page0, page0 + 1):
+        _put_all(s.ref.pages[0, s.ref.table[0, j]], 2, rows, 0)
+    meta = R._half(s.ref.pages[0, s.ref.table[0, page0 + 1]], 2, 40)[8192:].view(np.float16)
+    meta[256 + R.S_AT[8, 1]] = meta[256 + 128 + R.LO_AT[8, 1]] = np.nan
+    ctx.upload(s.ref.pages, s.c.pages)
+    print(f"case: kv4 decode n={n}, NaN in a split of no weight, late={late}", flush=True)
+    got, want = s.run(ctx, n)
+    bad = np.zeros_like(want, bool)
+    bad[0, 8:12, 64:128] = True
+    assert np.array_equal(np.isnan(want), bad)
+    s.check(got, want)
