@@ -336,8 +336,11 @@ typedef struct {
  * free from the next call on.
  * result_dev int32 [1]: 0; or, with nothing changed, the number of free
  * pages lacking, or -1 where a row is out of range or listed twice, a length
- * is negative or needs more than max_pages pages, or the table, lens and refs
- * contradict each other. */
+ * (lens' own too) is negative or needs more than max_pages pages, or the
+ * partly filled last page of a row that grows is none of the pool or by refs
+ * held by none.  Other contradictions of table, lens and refs, which only a
+ * writer other than the library makes, are not looked for; no access leaves
+ * the buffers for them. */
 enum { QM_KV4_LENS = 0, QM_KV4_ADD = 1 };
 int32_t qm_kv4_resize(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache,
                       int32_t count, const int32_t* rows_dev, const int32_t* lens_dev,
@@ -365,7 +368,7 @@ int32_t qm_kv4_compact(qm_context* ctx, qm_stream stream, const qm_kv4_cache* ca
  * first_dev int32 [batch], or NULL: 0.  Tokens at or past a row's length are
  * left out, as are sequences whose first is negative (grow the row with
  * qm_kv4_resize first), and, by _store, tokens of pages that other rows hold
- * too. */
+ * too, or that by refs no row holds. */
 int32_t qm_kv4_store(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
                      int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
                      const uint16_t* k_dev, const uint16_t* v_dev, int64_t capacity);
@@ -383,8 +386,8 @@ int32_t qm_kv4_load(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache
  * one as it is kept.  A batch row whose slot is outside the table (-1) or
  * whose length is 0 writes nothing and its output is 0.  One whose length is
  * over max_len, whose slot an earlier batch row has, or whose last page other
- * rows hold too (it was forked after it grew), writes nothing and its output
- * is NaN.
+ * rows hold too (it was forked after it grew) or by refs none, writes nothing
+ * and its output is NaN.
  * max_len  upper bound of the lengths: at most rope_len (else
  *          QM_ERR_ROPE_RANGE) and QM_KV4_PAGE_TOKENS * max_pages
  *          (QM_ERR_CAPACITY)

@@ -47,8 +47,8 @@
 // A batch row of the step: its table row and the tokens to read there, the
 // last of them new (0: none, the output is zero).  A row that is refused (its
 // output is NaN) is longer than max_len, or steps a table row that an earlier
-// batch row has; or other rows hold its last page too, which the wave that
-// would write there finds.
+// batch row has; or its last page is not its alone (other rows hold it too, or
+// by its count none), which the wave that would write there finds.
 struct StepRow {
     int row, len;
     bool refused;
@@ -645,7 +645,7 @@ extern "C" __global__ __launch_bounds__(64 * KV4_WAVES, 2) void qm_gqa_kv4_split
         uint8_t* buf = sh.ring[w][i];
         if (there[0]) {
             if (h == new_half) {
-                if (holders > 1) st.l = __builtin_nanf("");
+                if (holders != 1) st.l = __builtin_nanf("");
                 else put_token(buf, half[0], sh, pos & (QMK_KV4_HALF_TOKENS - 1), lane);
             }
             float x[8];

@@ -191,7 +191,7 @@ extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4
         }
     }
     __syncthreads();
-    if (holders > 1) return;
+    if (holders != 1) return;                           // not the row's alone
     for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_STORE_THREADS)
         reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }

@@ -730,3 +730,32 @@ def test_decode_nan_in_a_split_of_no_weight(ctx, n, late):
     bad[0, 8:12, 64:128] = True
     assert np.array_equal(np.isnan(want), bad)
     s.check(got, want)
+
+
+@pytest.mark.parametrize("count", [0, -1])
+def test_pages_that_no_row_holds_are_not_written(ctx, count):
+    """Where the counts say that nobody holds a row's page (the next resize may hand it to another row), a store leaves its
+    tokens out, and a step over it writes nothing and gives NaN; the other rows are as ever."""
+    ref = R.Cache(1, 9, 3, 3, seed=13)
+    assert ref.resize([0, 1], [150, 70]) == 0
+    ref.refs[ref.table[0, 1]] = count
+    c = upload(ctx, ref)
+    k, v = kv_rows(np.random.default_rng(14), 2, 4, 150)
+    print(f"case: store to a page of count {count}", flush=True)
+    ctx.kv4_store(c, 0, 0, 2, None, 150, ctx.upload(k.view(np.uint16)), ctx.upload(v.view(np.uint16)), 150)
+    before = ref.pages[0, ref.table[0, 1]].copy()
+    ref.store(0, 0, 2, None, 150, k, v)
+    ref.pages[0, ref.table[0, 1]] = before
+    assert_same(ctx, c, ref)
+    for n in (70, 1500):
+        s = Step(ctx, [n, 5], seed=88, max_pages=R.pages_of(n))
+        page = s.ref.table[0, (n - 1) // 64]
+        s.ref.refs[page] = count
+        ctx.upload(s.ref.refs, s.c.refs)
+        before = s.ref.pages[:, page].copy()
+        print(f"case: kv4 decode into a page of count {count}, n={n}", flush=True)
+        got, want = s.run(ctx, n)
+        want[0] = np.nan
+        s.ref.pages[:, page] = before
+        s.check(got, want)
+        assert_same(ctx, s.c, s.ref)
