@@ -106,8 +106,10 @@ int32_t     qm_device_count(int32_t* count);
 /* Size the workspace for batches up to max_batch and KV lengths up to
  * max_kv_len (and DeltaNet and GQA prefill up to max_prefill_tokens) so
  * that later mixer calls do not allocate (e.g. under graph capture); calls on
- * a 4-bit KV cache likewise, for lists of up to max_batch rows and a pool of
- * no more pages than max_batch rows of max_kv_len tokens fill. */
+ * a 4-bit KV cache likewise, for lists of up to max_batch rows, a table of up
+ * to ceil(max_kv_len / QM_KV4_PAGE_TOKENS) pages a row (max_pages; a fork of a
+ * wider one may need more) and a pool of no more pages than max_batch such
+ * rows have. */
 int32_t     qm_reserve(qm_context* ctx, int32_t max_batch, int32_t max_kv_len,
                        int32_t max_prefill_tokens);
 /* Launch-shape overrides for tests and tuning (0 = automatic).  Results do

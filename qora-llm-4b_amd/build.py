@@ -116,6 +116,13 @@ def build_kv4_test() -> None:
           str(ROOT / "tests" / "cpp" / "kv4_test.cpp"), "-o", str(LIB / "kv4_test")])
 
 
+def build_kv4_reserve_test() -> None:
+    """tests/cpp/kv4_reserve_test.cpp: the 4-bit KV cache's workspaces against the reserve
+    (g++ only, no device code; test infrastructure)."""
+    _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-I", str(ROOT / "include"), "-I", str(CSRC),
+          str(ROOT / "tests" / "cpp" / "kv4_reserve_test.cpp"), "-o", str(LIB / "kv4_reserve_test")])
+
+
 if __name__ == "__main__":
     build()
     if "--no-oracle" not in sys.argv:
@@ -125,4 +132,5 @@ if __name__ == "__main__":
         build_plan_test()
         build_dispatch_test()
         build_kv4_test()
+        build_kv4_reserve_test()
     print("built:", ", ".join(sorted(p.name for p in LIB.iterdir())))

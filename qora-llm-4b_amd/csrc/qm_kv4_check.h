@@ -141,8 +141,8 @@ inline size_t partial_bytes(int64_t splits) { return static_cast<size_t>(splits)
 inline size_t decode_ws(int64_t splits, int32_t batch) { return partial_bytes(splits) + static_cast<size_t>(batch) * 8; }
 
 // A bound of all of them for batches up to `batch` over lengths up to `len`,
-// a pool of no more pages than those need, forks and resizes of at most
-// `batch` rows.
+// a table of no more pages a row than those need, a pool of no more than
+// `batch` such rows have, forks and resizes of at most `batch` rows.
 inline size_t reserve_ws(int32_t batch, int32_t len, int cus) {
     const int64_t pages = (static_cast<int64_t>(len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
     size_t ws = decode_ws(max_splits(len, batch, cus), batch);

@@ -223,3 +223,24 @@ def test_splits_fit_the_grid_and_the_reserve():
 
 def test_rust_struct_matches_the_header():
     assert ffi._c_struct_fields("qm_kv4_cache") == ffi._r_struct_fields("qm_kv4_cache")
+
+
+def test_a_reserve_covers_every_call_within_its_limits():
+    """Resize, fork, compaction and step at the limits that qm_reserve names, and at smaller ones."""
+    exe = PKG / "lib" / "kv4_reserve_test"
+    assert exe.exists(), "build with qora-llm-4b_amd/build.py"
+
+    def sizes(cases):
+        r = subprocess.run([str(exe)], input="\n".join(f"{b} {n} {g}" for b, n, g in cases) + "\n", capture_output=True,
+                           text=True, timeout=60)
+        assert r.returncode == 0, r.stderr
+        return [[int(x) for x in a.split()] for a in r.stdout.splitlines()]
+
+    batches, lens = (1, 2, 19, 64, 300, 1024, 3000), (1, 64, 65, 256, 4097, 32769, 1048576)
+    cases = [(b, n, g) for b in batches for n in lens for g in (4, 256)]
+    got = sizes(cases)
+    assert len(got) == len(cases)
+    for case, (*calls, reserve) in zip(cases, got):
+        assert max(calls) <= reserve, (case, calls, reserve)
+    most = got[cases.index((300, 32769, 256))][-1]
+    assert all(max(calls) <= most for (b, n, g), (*calls, _) in zip(cases, got) if b <= 300 and n <= 32769 and g == 256)

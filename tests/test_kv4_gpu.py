@@ -759,3 +759,46 @@ def test_pages_that_no_row_holds_are_not_written(ctx, count):
         s.ref.pages[:, page] = before
         s.check(got, want)
         assert_same(ctx, s.c, s.ref)
+
+
+def test_forks_and_compactions_in_a_graph_after_a_reserve():
+    """All of the cache's calls captured on a new context that was reserved for exactly its table, replayed with eager work
+    between: table, lengths, counts and contents are the numpy form's after every replay."""
+    with M.Context(0) as c:
+        ref = R.Cache(2, 40, 8, 5, fill=False)
+        assert ref.resize(None, [300, 64, 130, 5, 1, 0, 0, 0]) == 0
+        d = upload(c, ref)
+        src, dst, sent = [0, 2, 2], [5, 6, 2], [257, 40, 0]
+        rows, lens, first, res = ints(c, [2, 5, 0]), ints(c, sent), ints(c, [3, 1]), ints(c, [-7, -7, -7])
+        srcs, dsts = ints(c, src), ints(c, dst)
+        k, v = kv_rows(np.random.default_rng(16), 2, 4, 70)
+        kd, vd, kb, vb = (c.upload(x.view(np.uint16)) for x in (k, v, k, v))
+        c.reserve(8, 5 * 64)
+        c.sync()
+        c.graph_begin()
+        c.kv4_fork(d, 3, srcs, dsts, res)
+        c.kv4_resize(d, 3, rows, lens, res.ptr + 4)
+        c.kv4_store(d, 1, 2, 2, first, 70, kd, vd, 70)
+        c.kv4_compact(d, res.ptr + 8)
+        c.kv4_load(d, 1, 2, 2, first, 70, kb, vb, 70)
+        g = c.graph_end()
+        for rep in range(4):
+            sent = [257 - 50 * rep, 40 + 64 * rep, 0 if rep != 2 else 320]
+            c.upload(np.asarray(sent, np.int32), lens)
+            c.sync()
+            print(f"case: kv4 calls in a graph, replay {rep}", flush=True)
+            g.launch()
+            c.sync()
+            want = [ref.fork(src, dst), ref.resize([2, 5, 0], sent)]
+            ref.store(1, 2, 2, [3, 1], 70, k, v)
+            want.append(ref.compact())
+            assert c.download(res, (3,), np.int32).tolist() == want and want[:2] == [0, 0]
+            assert_same(c, d, ref)
+            back = c.download(vb, v.shape, np.float16)
+            for b, (row, first_of, n) in enumerate([(2, 3, min(70, sent[0] - 3)), (3, 1, 4)]):
+                for head in range(4):
+                    held = ref.rows64(1, row, head, 1)[0][first_of:first_of + n].astype(np.float32).astype(np.float16)
+                    assert np.array_equal(back[b, head, :n], held, equal_nan=True)
+            assert run_fork(c, d, [1], [7]) == ref.fork([1], [7]) == 0           # between the replays
+            assert run_resize(c, d, [7], [0]) == ref.resize([7], [0]) == 0
+        g.close()
