@@ -196,8 +196,14 @@ extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4
         reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }
 
-QM_DEV float kv4_read(uint32_t word, int e, float s, float lo) {
-    return __builtin_fmaf((float)((word >> (4 * kv4_nibble(e))) & 15u), s, lo);
+// lo + s q of the code in bits `shift` .., rounded to f32 and then to f16.  In
+// one step (v_fma_mixlo_f16, which the compiler takes otherwise) it would be
+// one rounding, which differs where the f32 sum is halfway between two f16
+// values.
+QM_DEV uint32_t kv4_read(uint32_t word, int shift, float s, float lo) {
+    float x = __builtin_fmaf((float)((word >> shift) & 15u), s, lo);
+    asm("" : "+v"(x));
+    return f32_to_f16(x);
 }
 
 extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4RowsArgs A) {
@@ -228,14 +234,9 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
         uint32_t ko[4], vo[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            ko[p] = (uint32_t)f32_to_f16(kv4_read(kw, 2 * p, sk, lk)) | (uint32_t)f32_to_f16(kv4_read(kw, 2 * p + 1, sk, lk)) << 16;
-            uint32_t o = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t q = (w[kv4_v_word(t, 8 * i + 2 * p + e)] >> shift) & 15u;
-                o |= (uint32_t)f32_to_f16(__builtin_fmaf((float)q, sv, lv)) << (16 * e);
-            }
-            vo[p] = o;
+            ko[p] = kv4_read(kw, 4 * kv4_nibble(2 * p), sk, lk) | kv4_read(kw, 4 * kv4_nibble(2 * p + 1), sk, lk) << 16;
+            const int d = 8 * i + 2 * p;
+            vo[p] = kv4_read(w[kv4_v_word(t, d)], shift, sv, lv) | kv4_read(w[kv4_v_word(t, d + 1)], shift, sv, lv) << 16;
         }
         const size_t at = (base + (size_t)(h.src0 + t)) * 256 + 8 * i;
         *reinterpret_cast<uint4*>(A.k + at) = make_uint4(ko[0], ko[1], ko[2], ko[3]);

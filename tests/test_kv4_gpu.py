@@ -802,3 +802,24 @@ def test_forks_and_compactions_in_a_graph_after_a_reserve():
             assert run_fork(c, d, [1], [7]) == ref.fork([1], [7]) == 0           # between the replays
             assert run_resize(c, d, [7], [0]) == ref.resize([7], [0]) == 0
         g.close()
+
+
+def test_load_rounds_the_sum_to_f32_first(ctx):
+    """Minima far below the scale, and values lo + s q beside a tie of f16: the sum is rounded to f32, which is the tie, and
+    then to f16."""
+    rng = np.random.default_rng(17)
+    x = rng.uniform(0, 1, (1, 4, 64, 256)) * 2.0 ** rng.integers(6, 14, (1, 4, 64, 1))
+    x[..., ::64] = 2.0 ** -24 * rng.integers(1, 9, (1, 4, 64, 4))
+    x = x.astype(np.float16)
+    exact = R.value(*R.quantise(x))
+    want = exact.astype(np.float32).astype(np.float16)
+    assert (want != exact.astype(np.float16)).sum() > 1000
+    ref = R.Cache(1, 1, 1, 1, fill=False)
+    assert ref.resize([0], [64]) == 0
+    c = upload(ctx, ref)
+    d, kb, vb = ctx.upload(x.view(np.uint16)), ctx.alloc(x.nbytes), ctx.alloc(x.nbytes)
+    print("case: load, sums beside a tie", flush=True)
+    ctx.kv4_store(c, 0, 0, 1, None, 64, d, d, 64)
+    ctx.kv4_load(c, 0, 0, 1, None, 64, kb, vb, 64)
+    for buf in (kb, vb):
+        assert np.array_equal(ctx.download(buf, x.shape, np.float16), want)
