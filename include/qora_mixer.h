@@ -299,8 +299,10 @@ int32_t qm_gqa_prefill(qm_context* ctx, qm_stream stream, int32_t seq_len,
  *   lo = min x,  s = f16(f32((max x - min x) / 15)),
  *   q = clamp(round((x - lo) / s), 0, 15), ties to even (0 where s = 0),
  * and stand for lo + s q: within s / 2 of x (within 15 2^-25 where that is
- * more, s being subnormal or 0).  A group with an infinity or a NaN reads
- * back as NaN.
+ * more, s being subnormal or 0).  With s rounded up, lo + 15 s may lie a
+ * little past f16's largest value, 65504: the step takes it as it is, and
+ * qm_kv4_load gives infinity from 65520 on, as any rounding to f16 does.  A
+ * group with an infinity or a NaN reads back as NaN.
  *
  * Pages.  A page holds QM_KV4_PAGE_TOKENS tokens of the four kv heads' K and
  * V of one layer, QM_KV4_PAGE_BYTES; what stands where in it is the library's
@@ -375,8 +377,9 @@ int32_t qm_kv4_store(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cach
                      int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
                      const uint16_t* k_dev, const uint16_t* v_dev, int64_t capacity);
 
-/* The other way: f16(lo + s q), the sum rounded to f32 first.  f16 rows of
- * tokens left out stay as they were. */
+/* The other way: f16(lo + s q), the sum rounded to f32 first (infinity from
+ * 65520 on, which a group that reaches to f16's largest values can come to).
+ * f16 rows of tokens left out stay as they were. */
 int32_t qm_kv4_load(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
                     int32_t row, int32_t batch, const int32_t* first_dev, int32_t n,
                     uint16_t* k_dev, uint16_t* v_dev, int64_t capacity);

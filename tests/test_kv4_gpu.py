@@ -823,3 +823,21 @@ def test_load_rounds_the_sum_to_f32_first(ctx):
     ctx.kv4_load(c, 0, 0, 1, None, 64, kb, vb, 64)
     for buf in (kb, vb):
         assert np.array_equal(ctx.download(buf, x.shape, np.float16), want)
+
+
+def test_values_a_little_past_f16(ctx):
+    """Groups that reach to 65504 stand for values of up to 65536: infinity where they are loaded as f16, finite in a step (of
+    one token, whose output is its v times the gate)."""
+    s = Step(ctx, [1], seed=113)
+    s.v_new[0, :, ::2], s.v_new[0, :, 1::2] = 65504, -65504
+    s.v_new[0, 1, ::2], s.v_new[0, 1, 1::2] = 65504, 0
+    print("case: values past f16", flush=True)
+    got, want = s.run(ctx, 1)
+    assert np.isfinite(got).all()
+    s.check(got / 65536, want / 65536)
+    kb, vb = (ctx.alloc(4 * 256 * 2) for _ in range(2))
+    ctx.kv4_load(s.c, 0, 0, 1, None, 1, kb, vb, 1)
+    held = np.stack([s.ref.rows64(0, 0, head, 1)[0] for head in range(4)])
+    assert held.max() == 65536 and held[1].max() == 65520
+    with np.errstate(over="ignore"):
+        assert np.array_equal(ctx.download(vb, (4, 1, 256), np.float16), held.astype(np.float32).astype(np.float16))
