@@ -841,3 +841,100 @@ def test_values_a_little_past_f16(ctx):
     assert held.max() == 65536 and held[1].max() == 65520
     with np.errstate(over="ignore"):
         assert np.array_equal(ctx.download(vb, (4, 1, 256), np.float16), held.astype(np.float32).astype(np.float16))
+
+
+# ---- where the forms meet: one workgroup a head, or dealt and joined -------------------------
+@pytest.mark.parametrize("n", [255, 256, 257, 384, 511, 512, 513])
+def test_decode_lengths_around_the_forms_border(ctx, n):
+    """One row: up to 256 tokens by one workgroup a head."""
+    s = Step(ctx, [n], seed=120 + n)
+    print(f"case: kv4 decode n={n}", flush=True)
+    got, want = s.run(ctx, n)
+    s.check(got, want)
+    assert_same(ctx, s.c, s.ref)
+
+
+@pytest.mark.parametrize("rows", [15, 16, 17])
+@pytest.mark.parametrize("most", [256, 257, 512, 513])
+def test_decode_batches_around_the_forms_border(ctx, rows, most):
+    """Ragged batches: up to 512 tokens a row by one workgroup a head from 16 rows on."""
+    lens = np.random.default_rng(rows * most).integers(0, most + 1, rows)
+    lens[[0, 3, 7]] = most, 0, 1
+    s = Step(ctx, lens.tolist(), seed=121)
+    print(f"case: kv4 decode of {rows} rows of up to {most}", flush=True)
+    got, want = s.run(ctx, most)
+    s.check(got, want)
+    assert (got[lens == 0] == 0).all()
+    assert_same(ctx, s.c, s.ref)
+
+
+@pytest.mark.parametrize("lens", [[500, 1], [700, 1], [5001, 1]])
+def test_decode_nan_in_a_group_of_long_rows(ctx, lens):
+    """An infinity in the new k (kv head 1) and a NaN in the new v (head 2, dims 64 ..) of a row of many splits: NaN in its
+    outputs there, none elsewhere, and none in the other row."""
+    s = Step(ctx, lens, seed=122)
+    s.k_new[0, 1, 200] = np.inf
+    s.v_new[0, 2, 70] = np.nan
+    s.v_new[1, 3, 0] = 1e6                        # beyond f16: an infinity there
+    print(f"case: kv4 decode, NaN in groups, lens={lens}", flush=True)
+    got, want = s.run(ctx, lens[0])
+    bad = np.zeros_like(got, bool)
+    bad[0, 4:8], bad[0, 8:12, 64:128], bad[1, 12:, :64] = True, True, True
+    assert np.array_equal(np.isnan(got), bad)
+    fine = np.where(np.isnan(want), 0, want), np.where(bad, 0, got)
+    s.check(fine[1], fine[0])
+
+
+# ---- beside the f16 cache's step ------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 40, 256, 257, 1500, 5000])
+def test_step_agrees_with_the_f16_caches_step_and_the_oracle(ctx, n):
+    """qm_gqa_decode over f16 rows and qm_gqa_decode_kv4 over the same rows in pages: rows of multiples of 1/8 with the whole
+    range in every group, which 4 bits hold exactly, and a new token whose k is 0 (gamma = -1) and whose v is such a row.
+    The f16 step's own bar (its weights enter the products in 16 bits) is 1e-3.  The oracle sums in f32: a score's 256
+    products with A = sum |q k| / 16 of about 6 are off by 2^-24 * 16 * 6, the output's n terms of at most 1 by 2^-24 sqrt(n);
+    six deviations of both are under 6e-5 up to n = 5000.  With another gamma the new k rows agree within half a step of the
+    codes, a step of f16 for the f32 norm, and the roundings of the row read back."""
+    from conftest import load_oracle, load_workloads
+    O, W = load_oracle(), load_workloads()
+    rng = np.random.default_rng(130 + n)
+
+    def grid(*lead):
+        x = rng.integers(0, 16, (*lead, 256)) * 0.125 - 1
+        x[..., ::64], x[..., 1::64] = -1, 0.875
+        return x.astype(np.float16)
+
+    k, v = grid(1, 4, n), grid(1, 4, n)
+    w = {x: rng.standard_normal((1, *shape), dtype=np.float32) for x, shape in (("q_gate", (16, 512)), ("k_new", (4, 256)))}
+    w["v_new"] = grid(1, 4).astype(np.float32)
+    q_norm = (0.1 * rng.standard_normal(256)).astype(np.float16)
+    cos, sin = M.rope_table(n)
+    rc, rs, qn = ctx.upload(cos), ctx.upload(sin), ctx.upload(q_norm)
+    q_gate, k_new, v_new = (ctx.upload(w[x]) for x in ("q_gate", "k_new", "v_new"))
+    kf, vf = ctx.upload(k.view(np.uint16)), ctx.upload(v.view(np.uint16))
+    c = M.Kv4Cache(ctx, 1, R.pages_of(n) + 2, 1, R.pages_of(n))
+    assert run_resize(ctx, c, None, [n]) == 0
+    ctx.kv4_store(c, 0, 0, 1, None, n, kf, vf, n)
+    a, b = ctx.alloc(4096 * 4), ctx.alloc(4096 * 4)
+    for gamma in (np.full(256, -1, np.float16), (0.1 * rng.standard_normal(256)).astype(np.float16)):
+        kn = ctx.upload(gamma)
+        print(f"case: both steps, n={n}", flush=True)
+        ctx.gqa_decode(1, q_gate, k_new, v_new, qn, kn, rc, rs, n, None, n - 1, kf, vf, n, a)
+        ctx.gqa_decode_kv4(c, 0, 1, None, q_gate, k_new, v_new, qn, kn, rc, rs, n, n, None, b)
+        kb, vb = (ctx.alloc(4 * 256 * 2) for _ in range(2))
+        ctx.kv4_load(c, 0, 0, 1, ints(ctx, [n - 1]), 1, kb, vb, 1)
+        kb, vb = (ctx.download(x, (4, 256), np.float16).astype(np.float64) for x in (kb, vb))
+        k16 = ctx.download(kf, (4, n, 256), np.float16)[:, n - 1].astype(np.float64)
+        assert np.array_equal(vb, w["v_new"][0])
+        step = np.repeat(np.ptp(k16.reshape(4, 4, 64), axis=-1) / 15, 64, axis=-1).reshape(4, 256)
+        near = step * (0.5 + 2.0 ** -9) + 2.0 ** -10 * (np.abs(k16) + 16 * step)
+        assert (np.abs(kb - k16) <= near).all()
+        if gamma[0] != -1:
+            continue
+        assert not kb.any()
+        f16, kv4 = (ctx.download(x, (16, 256), np.float32) for x in (a, b))
+        K, V = (np.ascontiguousarray(np.transpose(x[0].astype(np.float32), (1, 0, 2))) for x in (k, v))
+        want = O.attn_decode_step(O.config(), w["q_gate"].ravel(), w["k_new"].ravel(), w["v_new"].ravel(), q_norm.view(np.uint16),
+                                  gamma.view(np.uint16), cos, sin, K, V, n - 1, round_kv_f16=True, nthreads=8).reshape(16, 256)
+        print(f"f16 step {np.abs(kv4 - f16).max():.2e} oracle {np.abs(kv4 - want).max():.2e}", flush=True)
+        assert np.abs(kv4 - f16).max() <= 1e-3
+        assert np.abs(kv4 - want).max() <= 6e-5
