@@ -745,6 +745,9 @@ extern "C" __global__ __launch_bounds__(64) void qm_gqa_kv4_merge(GqaKv4Args A) 
     // split (first + s) and kv head h >> 2: workgroup 4 (first + s) + (h >> 2)
     const float* P = A.partial + ((size_t)mine.x * 16 + h) * KV4_PART_STRIDE;
     Joined x{-INFINITY, 0.0f, 0.0f};
+    // Few splits: few loads, and few past the last one (the step, 8 / 32 loads
+    // at a time, us: 900 tokens, 8 splits, 9.05 / 9.33, 4097 tokens, 33 splits,
+    // 10.81 / 10.19, 16000 tokens 13.25 / 11.65).
     if (mine.y <= 8) join<8>(x, P, mine.y, d, lane);
     else join<KV4_JOIN>(x, P, mine.y, d, lane);
     float y = x.l != 0.0f ? (x.o * __builtin_amdgcn_rcpf(x.l)) * sigmoid_fast(gate) : 0.0f;

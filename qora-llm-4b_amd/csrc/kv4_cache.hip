@@ -292,7 +292,12 @@ QM_DEV Share share_of(const Kv4Cache& c, int64_t block) {
     return s;
 }
 // Bit j: page page0 + j is free (reference count 0).  Ids past the pool are
-// not free.  N loads in flight.
+// not free.  N loads in flight, of 64 counts each whether the pool has them or
+// not: few where there is little to load, many where the loads take the time
+// (4 / 32, us, 16 rows grown and shrunk again: a pool of 512 14.3 / 19.5, 8192
+// 15.2 / 19.6, 16384 16.7 / 19.6, 32768 19.6 / 19.7, 262144 57.4 / 54.9,
+// 2097152 283 / 226; compacted with nothing to move: 16384 10.2 / 11.4, 32768
+// 15.1 / 14.7).
 template <int N>
 QM_DEV uint64_t free_of(const Kv4Cache& c, int64_t at, int each) {
     const int lane = threadIdx.x & 63;
@@ -315,7 +320,7 @@ QM_DEV uint64_t free_of(const Kv4Cache& c, int64_t at, int each) {
 QM_DEV uint64_t free_pages(const Kv4Cache& c, int64_t block, Share& s) {
     s = share_of(c, block);
     const int64_t at = block + 64 * (int64_t)(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * s.each);
-    const uint64_t mine = s.each <= 4 ? free_of<4>(c, at, s.each) : free_of<32>(c, at, s.each);
+    const uint64_t mine = s.each <= 16 ? free_of<4>(c, at, s.each) : free_of<32>(c, at, s.each);
     const int64_t in = c.num_pages - s.page0;           // bits past the pool
     return in >= 64 ? mine : in <= 0 ? 0ull : mine & ((1ull << in) - 1);
 }
