@@ -75,18 +75,6 @@ QM_DEV bool repeated(const GqaKv4Args& A, int b, int row, int lane) {
         }
     return found;
 }
-// Inclusive sum over the wave's lanes: within the rows of 16, then the last
-// lane of a row into the next row, and of the lower half into the upper.
-template <int CTRL, int ROWS>
-QM_DEV int scan_step(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
-QM_DEV int wave_scan(int x) {
-    x = scan_step<0x111, 0xF>(x);
-    x = scan_step<0x112, 0xF>(x);
-    x = scan_step<0x114, 0xF>(x);
-    x = scan_step<0x118, 0xF>(x);
-    x = scan_step<0x142, 0xA>(x);
-    return scan_step<0x143, 0xC>(x);
-}
 // ceil(len / chunk), chunk a multiple of 128: the f32 quotient is off by two at
 // most, and put right.
 QM_DEV int splits_of(int len, int chunk) {
@@ -124,7 +112,7 @@ QM_DEV int chunk_for(const GqaKv4Args& A, float want, int groups, int len) {
     int chunk = __builtin_amdgcn_readfirstlane(((int)fminf(want, (float)(QMK_KV4_MAX_SPLIT - 1)) + 128) / 128 * 128);   // more than `want`
     if (A.batch <= 64)
         for (int tries = 0; tries < 4 && chunk < QMK_KV4_MAX_SPLIT; ++tries, chunk += 128)
-            if (QM_GQA_KV_HEADS * __builtin_amdgcn_readlane(wave_scan(splits_of(len, chunk)), 63) <= groups) break;
+            if (QM_GQA_KV_HEADS * __builtin_amdgcn_readlane((int)wave_scan((uint32_t)splits_of(len, chunk)), 63) <= groups) break;
     return chunk;
 }
 QM_DEV int deal_chunk(const GqaKv4Args& A, const StepRow& mine, int lane) {
@@ -156,7 +144,7 @@ QM_DEV bool deal_split(const GqaKv4Args& A, Deal& d, int k, bool note, int lane)
     int first = 0;
     for (int b0 = 0; b0 < A.batch; b0 += 64) {             // uniform
         if (b0) mine = lane_row(A, b0 + lane);
-        const int n = splits_of(mine.len, d.chunk), incl = wave_scan(n), all = __builtin_amdgcn_readlane(incl, 63);
+        const int n = splits_of(mine.len, d.chunk), incl = (int)wave_scan((uint32_t)n), all = __builtin_amdgcn_readlane(incl, 63);
         if (!found && k < first + all) {
             const int at = __popcll(__ballot(first + incl <= k));
             found = true;

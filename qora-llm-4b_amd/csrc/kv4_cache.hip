@@ -249,18 +249,6 @@ extern "C" __global__ __launch_bounds__(KV4_ROWS_THREADS) void qm_kv4_load(Kv4Ro
 #define KV4_BLOCK_PAGES (64 * KV4_PLAN_THREADS)     // pages whose state one pass holds: up to 64 a thread
 #define KV4_WINDOW 4096                              // free pages handed out at a time
 
-// Inclusive sum over the wave's lanes: within the rows of 16, then the last
-// lane of a row into the next row, and of the lower half into the upper.
-template <int CTRL, int ROWS>
-QM_DEV uint32_t scan_step(uint32_t x) { return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
-QM_DEV uint32_t wave_scan(uint32_t x) {
-    x = scan_step<0x111, 0xF>(x);
-    x = scan_step<0x112, 0xF>(x);
-    x = scan_step<0x114, 0xF>(x);
-    x = scan_step<0x118, 0xF>(x);
-    x = scan_step<0x142, 0xA>(x);
-    return scan_step<0x143, 0xC>(x);
-}
 // Exclusive sum over the workgroup's 1024 threads, and the total.  `sums`
 // (one word a wave) must not be in use: calls in a row take different ones.
 QM_DEV uint32_t plan_scan(uint32_t x, uint32_t* sums, uint32_t& total) {

@@ -39,3 +39,16 @@ QM_DEV uint32_t kv4_code(float x, float lo, float s, float inv) {
     q = min(max(q, 0), 15);
     return s > 0.0f ? (uint32_t)q : 0u;     // s = 0, NaN
 }
+
+// Inclusive sum over the wave's lanes: within the rows of 16, then the last
+// lane of a row into the next row, and of the lower half into the upper.
+template <int CTRL, int ROWS>
+QM_DEV uint32_t scan_step(uint32_t x) { return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
+QM_DEV uint32_t wave_scan(uint32_t x) {
+    x = scan_step<0x111, 0xF>(x);
+    x = scan_step<0x112, 0xF>(x);
+    x = scan_step<0x114, 0xF>(x);
+    x = scan_step<0x118, 0xF>(x);
+    x = scan_step<0x142, 0xA>(x);
+    return scan_step<0x143, 0xC>(x);
+}
