@@ -113,16 +113,18 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
 
 // The decode's workgroups.  Short rows, and somewhat longer ones where there
 // are enough of them, take one workgroup each per kv head and no merge
-// (measured, one workgroup / dealt out, us: 1 row of 300 tokens 9.4 / 9.0, of
-// 500 10.8 / 9.1, 64 rows of 250 8.8 / 12.7, of 500 13.2 / 17.5; rows of one
-// step may differ, so not much longer).  Others are dealt out by the kernel
+// (measured, one workgroup / dealt out, us: 1 row of 250 tokens 8.1 / 9.1, of
+// 257 9.5 / 9.1, of 500 10.8 / 9.1; 16 rows of 400 11.1 / 9.5, of 512 11.0 /
+// 10.0; 24 rows of 400 11.2 / 11.2, of 512 11.1 / 11.7; 32 rows of 512 11.1 /
+// 12.7; 64 rows of 250 8.6 / 12.8, of 500 13.0 / 17.7; rows of one step may
+// differ, so not much longer).  Others are dealt out by the kernel
 // (deal_chunk): splits of 128 n tokens, at most QMK_KV4_MAX_SPLIT, n such that
 // one or two workgroups a CU, or some full rounds of two, have about the same
 // number.  max_splits bounds the splits of all rows: two workgroups a CU and
 // round over the four kv heads and one per row, and cus / 16 for the errors of
 // the f32 sum that the rounds are counted by (under 2^-7 of one); past
 // QMK_KV4_ROUNDS rounds ceil(len / QMK_KV4_MAX_SPLIT) per row.
-inline bool single(int64_t len, int64_t batch) { return len <= 256 || (len <= 512 && batch >= 16); }
+inline bool single(int64_t len, int64_t batch) { return len <= 256 || (len <= 512 && batch >= 24); }
 inline int64_t max_splits(int64_t len, int64_t batch, int cus) {
     const int64_t least = (len + 127) / 128 * batch, longest = (len + QMK_KV4_MAX_SPLIT - 1) / QMK_KV4_MAX_SPLIT * batch;
     const int64_t rounds = len * batch / (static_cast<int64_t>(QMK_KV4_MAX_SPLIT) * cus / 2) + 1;

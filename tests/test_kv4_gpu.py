@@ -854,10 +854,10 @@ def test_decode_lengths_around_the_forms_border(ctx, n):
     assert_same(ctx, s.c, s.ref)
 
 
-@pytest.mark.parametrize("rows", [15, 16, 17])
+@pytest.mark.parametrize("rows", [15, 16, 17, 23, 24, 25])
 @pytest.mark.parametrize("most", [256, 257, 512, 513])
 def test_decode_batches_around_the_forms_border(ctx, rows, most):
-    """Ragged batches: up to 512 tokens a row by one workgroup a head from 16 rows on."""
+    """Ragged batches: up to 512 tokens a row by one workgroup a head from 24 rows on."""
     lens = np.random.default_rng(rows * most).integers(0, most + 1, rows)
     lens[[0, 3, 7]] = most, 0, 1
     s = Step(ctx, lens.tolist(), seed=121)
