@@ -14,8 +14,10 @@
 //   A code c in bits 0..3 (4..7) of a half is the bf16 subnormal c 2^-133
 //   (16 c 2^-133): masks alone make operands of a word (5 instructions for 8
 //   codes).  The other operand carries 2^90 (2^86 for the elements of bits
-//   4..7), which keeps products normal: for p down to 2^-216, q up to 2^37.
-//   Products are in units of 2^-43.
+//   4..7), so products are in units of 2^-43: p s c of 2^-83 and more is a
+//   normal f32, with all three parts from 2^-67 on.  What is lost below is
+//   nothing beside K and V, multiples of 2^-24 or 0, and beside the largest
+//   weight of a row, 2^-8 at least.  q may be up to 2^37.
 //   That operand is f32 and enters as three bf16 parts, 24 bits, exactly.
 //   QK: A = 16 tokens' codes, B = q (column 4 part + head: 12 of the 16
 //   columns that the instruction has anyway).  Lane (g, c) ends with tokens
@@ -25,19 +27,23 @@
 //   one group only), B = the codes of 16 dims, an instruction per part; of the
 //   result the rows of the dims' own group count.  With the parts as rows each
 //   lane would weigh all four groups: a third of the instructions, but 144
-//   vector instructions a round to make the operands instead of 52, and the
-//   vector unit is what the kernel waits for.
+//   vector instructions a round to make the operands instead of 52 (19 ragged
+//   rows 29.5 us instead of 27.7 when it was changed, 64 x 32769 the same).
 //   The minimum terms are the lanes' own: the lane of column 4 j + head adds
 //   group j's.
 // Softmax in base 2; a running maximum is raised only where a score passes it
 // by 2^8, so the accumulators are seldom rescaled.
 //
-// What bounds it.  64 x 32769 tokens: the HBM stream (434 us, 2.42 GB at 5.6
-// TB/s; a copy of the kernel that only loads takes 419).  Batches of some
-// thousand tokens a row: the vector unit, with 375 vector and 64 matrix
-// instructions a wave and round (19 ragged rows of up to 7001, 57k tokens: 18
-// us).  Few tokens: the chain of dependent loads, lengths to table to pages, and
-// the launches (1 token 6.2 us; 4097 7.1 and 3.1 for the merge).
+// What bounds it.  64 x 32769 tokens: the HBM stream (2.42 GB; the least of 24
+// launches 430 us, 5.6 TB/s, their median 480 to 490; a copy of the kernel that
+// only loads takes 419 at least).  Batches of some thousand tokens a row: the
+// loads and what comes before the first of them (lengths, the deal, table,
+// page), not the arithmetic: 19 ragged rows of up to 7001, 57k tokens, take 19
+// us and a copy that only loads 4 less.  While its CUs work there, the vector
+// unit is busy half of the time (375 instructions a wave and round; 39% of all
+// lie outside the rounds) and the matrix unit a fifth (64).  Few tokens: the
+// chain of dependent loads and the launches (1 token 6.4 us; 4097 7.3 and 2.5
+// for the merge).
 #include "qm_kv4_device.h"
 #include "qm_kernel_args.h"
 
@@ -93,16 +99,14 @@ QM_DEV int splits_of(int len, int chunk) {
 // max_len is its length.  Every workgroup finds the same chunk: one workgroup
 // per CU, or two where that makes the chunk enough shorter, and not a few more
 // than that, which would be a round of their own.  Two workgroups on a CU take
-// 1.7 times as long as one (a round of a lone wave is bound by its own chain
-// of vector and matrix instructions, of two by the vector unit).  Measured,
-// the step in us, one per CU / two: 1 x 32769 tokens 17.5 / 19.2, 8 x 4097
-// 15.6 / 18.0, 16 ragged rows of up to 7001 20.8 / 19.8, 64 x 2049 34.4 /
-// 34.6.  One, too, where the merge would have more splits of two than it loads
-// at a time (1 x 16000 12.7 / 15.5, 4 ragged rows of up to 20000 20.3 / 22.1).
-// Where that passes QMK_KV4_MAX_SPLIT tokens, so many full rounds of two
-// workgroups a CU that it does not (the longest chunk / this: 64 x 10001 169 /
-// 146, 3 x 200001 157 / 139); past QMK_KV4_ROUNDS rounds, where a partial one
-// no longer counts, the longest chunk.
+// 1.7 times as long as one.  Measured, the step in us, one per CU / two: 1 x
+// 32769 tokens 16.7 / 18.3, 8 x 4097 15.8 / 17.9, 16 ragged rows of up to 7001
+// 20.6 / 21.1, 64 x 2049 35.1 / 33.3.  One, too, where the merge would have
+// more splits of two than it loads at a time (1 x 16000 11.4 / 13.7, 4 rows of
+// 20000 and less 17.9 / 19.7).  Where that passes QMK_KV4_MAX_SPLIT tokens, so
+// many full rounds of two workgroups a CU that it does not (the longest chunk /
+// this: 64 x 10001 166 / 145, 3 x 200001 157 / 139); past QMK_KV4_ROUNDS rounds,
+// where a partial one no longer counts, the longest chunk.
 struct Deal {
     int chunk;
     int b, first;            // a batch row, and the splits before its own

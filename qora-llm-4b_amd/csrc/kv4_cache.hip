@@ -10,9 +10,11 @@
 // word.  A V word holds 8 tokens of one dim: two lanes with 4 tokens each turn
 // their 4 x 8 codes in registers and exchange halves (a lane with all 8 was as
 // fast on long prompts and took twice the chain on short ones: 45 tokens 10.4 us
-// against 7.8).  Long ones are bound by HBM (4 x 32701 tokens, 687 MB: stored in
-// 160 to 186 us, loaded in 114), short ones by the chain of length, table entry
-// and page.
+// against 7.8).  Long loads are bound by HBM (4 x 32701 tokens, 687 MB: 113 us
+// at least, 117 the median), long stores of the same bytes by the vector unit
+// (157, 185): 645 instructions a wave keep it busy 85% of the time, 96% of that
+// in which the CUs work.  Short ones are bound by the chain of length, table
+// entry and page.
 #define KV4_ROWS_THREADS 256
 #define KV4_STORE_THREADS 512
 
@@ -85,7 +87,8 @@ QM_DEV Coded code8(uint4 raw, int lane) {
     c.lo = bad ? (uint16_t)0x7e00u : f32_to_f16(lo);
     // In f32, x - lo is off by 2^-20 s at most and the rest by less: a
     // remainder clearly under half a step says that the code is right.  For
-    // the others (one value in some 3000), and where s is subnormal, 0 or NaN,
+    // the others (one value in some 4000 of normal ones: one in 500 of these
+    // words, and more than a third of the waves), and where s is subnormal, 0 or NaN,
     // kv4_code decides.
     const float s = f16_to_f32(c.s), inv = __builtin_amdgcn_rcpf(s);
     float q[8], worst = 0.0f;
@@ -102,7 +105,7 @@ QM_DEV Coded code8(uint4 raw, int lane) {
     const float sure = s >= 0x1p-14f ? s * (0.5f - 0x1p-18f) : -1.0f;
     if (!(worst < sure)) {
 #pragma clang loop unroll(disable)
-        for (int e = 0; e < 8; ++e) {                   // rolled: this is rare, and code to be fetched
+        for (int e = 0; e < 8; ++e) {                   // rolled: code to be fetched, and few lanes come here
             const uint32_t we = (e < 4 ? (e < 2 ? w[0] : w[1]) : (e < 6 ? w[2] : w[3])) >> (16 * (e & 1));
             const float x = f16_to_f32((uint16_t)we), d = x - lo;
             const int shift = 4 * kv4_nibble(e);
