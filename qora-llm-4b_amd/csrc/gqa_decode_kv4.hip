@@ -16,8 +16,8 @@
 //   codes).  The other operand carries 2^90 (2^86 for the elements of bits
 //   4..7), so products are in units of 2^-43: p s c of 2^-83 and more is a
 //   normal f32, with all three parts from 2^-67 on.  What is lost below is
-//   nothing beside K and V, multiples of 2^-24 or 0, and beside the largest
-//   weight of a row, 2^-8 at least.  q may be up to 2^37.
+//   nothing beside K and V, multiples of 2^-24 or 0, and beside a row's largest
+//   weight, 1 to 2^8.  q may be up to 2^37.
 //   That operand is f32 and enters as three bf16 parts, 24 bits, exactly.
 //   QK: A = 16 tokens' codes, B = q (column 4 part + head: 12 of the 16
 //   columns that the instruction has anyway).  Lane (g, c) ends with tokens

@@ -88,8 +88,8 @@ QM_DEV Coded code8(uint4 raw, int lane) {
     // In f32, x - lo is off by 2^-20 s at most and the rest by less: a
     // remainder clearly under half a step says that the code is right.  For
     // the others (one value in some 4000 of normal ones: one in 500 of these
-    // words, and more than a third of the waves), and where s is subnormal, 0 or NaN,
-    // kv4_code decides.
+    // words, and more than a third of the waves), and where s is subnormal, 0
+    // or NaN, kv4_code decides.
     const float s = f16_to_f32(c.s), inv = __builtin_amdgcn_rcpf(s);
     float q[8], worst = 0.0f;
 #pragma unroll
