@@ -5,14 +5,16 @@
  * MI355X (gfx950) with hand-written HIP kernels loaded from code objects:
  *   - Gated DeltaNet: recurrent decode step and chunked prefill;
  *   - full-attention GQA: decode step over an f16 KV cache and causal
- *     prefill that writes that cache; the decode step also over a paged
- *     4-bit KV cache, with what keeps its pages.
+ *     prefill that writes that cache; the decode step, and chunks of new
+ *     tokens of several rows, also over a paged 4-bit KV cache, with what
+ *     keeps its pages.
  * Each mixer entry replaces the middle of one reference layer-forward
  * (cited per entry).  Around the mixer the library also exports the
  * neighbouring steps of a decode or prefill layer, each a separate entry
  * the caller may use or not: the Q4 projections (GEMV for decode with the
  * RMSNorm, residual, SiLU gate/up and DeltaNet conv fused; an MFMA GEMM for
- * prefill), lm_head and the embedding lookup, and next-token sampling.
+ * prefill), lm_head and the embedding lookup, next-token sampling, and beam
+ * search's selection with the reordering of the recurrent states.
  * F16 projections stay with the caller.
  *
  * Conventions
@@ -108,8 +110,8 @@ int32_t     qm_device_count(int32_t* count);
  * that later mixer calls do not allocate (e.g. under graph capture); calls on
  * a 4-bit KV cache likewise, for lists of up to max_batch rows, a table of up
  * to ceil(max_kv_len / QM_KV4_PAGE_TOKENS) pages a row (max_pages; a fork of a
- * wider one may need more) and a pool of no more pages than max_batch such
- * rows have. */
+ * wider one may need more), a pool of no more pages than max_batch such
+ * rows have, and qm_gqa_chunk_kv4 of up to max_prefill_tokens tokens. */
 int32_t     qm_reserve(qm_context* ctx, int32_t max_batch, int32_t max_kv_len,
                        int32_t max_prefill_tokens);
 /* Launch-shape overrides for tests and tuning (0 = automatic).  Results do
@@ -406,6 +408,60 @@ int32_t qm_gqa_decode_kv4(qm_context* ctx, qm_stream stream, const qm_kv4_cache*
                           const float* rope_cos_dev, const float* rope_sin_dev, int32_t rope_len,
                           int32_t max_len, const int32_t* result_dev, float* out_dev);
 
+/* New tokens of several rows at once: parts of prompts, whole prompts, drafted
+ * tokens.  Batch row b's new tokens are rows begins_dev[b] .. begins_dev[b + 1]
+ * - 1 of packed tensors of `tokens` rows, and the last ones of table row
+ * slots_dev[b] (NULL: b), which qm_kv4_resize has grown by them: the i-th of n
+ * stands at position lens - n + i.  begins_dev int32 [batch + 1] ascends from
+ * 0 or more to `tokens` at most (at most 1048576); a batch row whose range is
+ * none is passed over.  Nothing of it reaches the host, so a captured call
+ * replays as rows and lists change.
+ *
+ * qm_kv4_append writes their keys and values into a layer's pages: k RMSNorm'd
+ * (1 + gamma, eps 1e-6) and rotated, in 64 bits, rounded to f32 and f16 as
+ * qm_gqa_decode_kv4's new row is, v rounded to f16, both in 4 bits.  Nothing is
+ * written of a batch row whose slot is outside the table or an earlier batch
+ * row's, or that has more new tokens than its length or a length over max_len;
+ * nor to pages that other rows hold too, or by refs none, or that are none of
+ * the pool.
+ * dtype        of k_dev and v_dev: QM_F32 or QM_BF16 [tokens][4][256]
+ * k_norm_dev   f16 [256]
+ * rope_cos_dev, rope_sin_dev f32 [rope_len][32]
+ * max_len      upper bound of the lengths: at most rope_len (else
+ *              QM_ERR_ROPE_RANGE) and QM_KV4_PAGE_TOKENS * max_pages
+ *              (QM_ERR_CAPACITY)
+ * result_dev   NULL, or a resize's result: where it is not 0 (the rows did not
+ *              grow) nothing is written */
+int32_t qm_kv4_append(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
+                      int32_t batch, const int32_t* slots_dev, const int32_t* begins_dev,
+                      int32_t tokens, int32_t dtype, const void* k_dev, const void* v_dev,
+                      const uint16_t* k_norm_dev, const float* rope_cos_dev,
+                      const float* rope_sin_dev, int32_t rope_len, int32_t max_len,
+                      const int32_t* result_dev);
+
+/* And attends over a layer's pages, for the same tokens once they are written:
+ * softmax(q K^T / 16) V of a token at position pos over the cached tokens
+ * 0 .. pos of its row, q RMSNorm'd and rotated, kv head h / 4, times
+ * sigmoid(gate): qm_gqa_prefill's attention, behind any context.  K and V are
+ * what the pages stand for, in f16 (f16's largest value where that is past it);
+ * q and the softmax's weights enter the products in f16, sums are f32, as in
+ * qm_gqa_prefill.  A token that stands in a group of NaN does so for the
+ * queries that see it only.
+ * q_gate_dev   bf16 [tokens][16][512]; q_norm_dev f16 [256]
+ * out_dev      bf16 [tokens][16][256]; rows of no batch row stay as they were
+ * max_new      upper bound of a row's new tokens
+ * A batch row whose slot is outside the table (-1) or whose length is 0 gives
+ * outputs of 0, as does every one where result_dev is not NULL and not 0; one
+ * with more new tokens than max_new or than its length, or with a length over
+ * max_len, gives NaN.  Table entries that are no page of the pool are passed
+ * over, and a token that sees none gives 0.  Two batch rows may have one slot. */
+int32_t qm_gqa_chunk_kv4(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cache, int32_t layer,
+                         int32_t batch, const int32_t* slots_dev, const int32_t* begins_dev,
+                         int32_t tokens, int32_t max_new, const uint16_t* q_gate_dev,
+                         const uint16_t* q_norm_dev, const float* rope_cos_dev,
+                         const float* rope_sin_dev, int32_t rope_len, int32_t max_len,
+                         const int32_t* result_dev, uint16_t* out_dev);
+
 /* ---- Q4 projections --------------------------------------------------- */
 /* A Q4Weight (gemv.rs:29-34, written by quantize_q4, convert.rs:437-467)
  * maps k inputs to n outputs, n a multiple of 32 (the reference stores
@@ -588,6 +644,61 @@ int32_t qm_sample(qm_context* ctx, qm_stream stream, int32_t vocab, float* logit
                   const int32_t* generated_dev, int32_t n_generated,
                   const qm_sample_params* params, uint64_t* rng_state_dev,
                   int32_t* token_out_dev, int32_t* top_ids_dev, float* top_probs_dev);
+
+/* ---- beam search --------------------------------------------------------- */
+/* No counterpart in the reference, which follows one sequence.  A step of a
+ * search with `beams` sequences for each of `groups` requests: logits of every
+ * sequence, qm_beam_select, then the chosen sequences' states in the places of
+ * their own: qm_kv4_fork for the paged cache's rows, qm_state_fork for the
+ * recurrent states, with parents_dev as the sources. */
+
+/* The `take` best continuations of each request, best first.  Continuation t
+ * of a sequence is worth its score + logits[t] - log(sum exp logits), the
+ * summed log-probability, compared in 64 bits (the log-sum is good to about
+ * 2^-23); of equal ones the lower sequence and then the lower token is first.
+ * A sequence at its end (done not 0) has one continuation: end_id, worth its
+ * score.  One whose score is not finite takes no part, nor one whose logits
+ * hold a NaN or +infinity or nothing but -infinity; a logit of -infinity is no
+ * continuation.
+ * beams, take  1 .. 64 (take 2 * beams leaves as many where half of them end)
+ * vocab        at most 262144 (QM_ERR_SHAPE)
+ * logits_dev   f32 [groups * beams][vocab], not changed
+ * scores_dev   f32 [groups * beams]
+ * done_dev     int32 [groups * beams], or NULL: none is at its end
+ * end_id       the token that ends a sequence, or -1 (without done_dev)
+ * parents_dev  int32 [groups][take]: the row it continues, of groups * beams
+ * tokens_dev   int32 [groups][take]
+ * scores_out_dev  f32 [groups][take]: its worth
+ * done_out_dev NULL, or int32 [groups][take]: whether it is at its end
+ * Where there are fewer, the rest have parent -1, token -1, score -infinity
+ * and done 0.  With take = beams the scores and flags may be written where
+ * they were read.  Pointers need 4-byte alignment.  Uses 16 bytes of the
+ * context's workspace per row and 1024 logits (reserved by qm_reserve for
+ * groups * beams up to max_batch). */
+int32_t qm_beam_select(qm_context* ctx, qm_stream stream, int32_t groups, int32_t beams,
+                       int32_t take, int32_t vocab, const float* logits_dev,
+                       const float* scores_dev, const int32_t* done_dev, int32_t end_id,
+                       int32_t* parents_dev, int32_t* tokens_dev, float* scores_out_dev,
+                       int32_t* done_out_dev);
+
+/* Rows of recurrent states (DeltaNet's states and conv buffers, of any layers)
+ * become copies of others in place: row dst_dev[i] of every buffer becomes its
+ * row src_dev[i] as it was before the call (i < count, at most 1024; dst_dev
+ * NULL: row i; the destinations all different, a row may be both source and
+ * destination), as qm_kv4_fork does for the rows of a cache.  Rows that become
+ * themselves are not touched.  buffers: host array of `n_buffers` (at most 64)
+ * descriptions of [rows] rows each, at most 65536; no two may overlap.
+ * result_dev int32 [1]: 0, or -1 with nothing changed where a row is out of
+ * range or a destination listed twice.  Lists and result need 4-byte
+ * alignment. */
+typedef struct {
+    void* rows_dev;            /* 16-byte aligned */
+    int64_t row_bytes;         /* a multiple of 16 */
+    int64_t stride_bytes;      /* from row to row: a multiple of 16 */
+} qm_state_rows;
+int32_t qm_state_fork(qm_context* ctx, qm_stream stream, int32_t n_buffers,
+                      const qm_state_rows* buffers, int32_t rows, int32_t count,
+                      const int32_t* src_dev, const int32_t* dst_dev, int32_t* result_dev);
 
 #ifdef __cplusplus
 }

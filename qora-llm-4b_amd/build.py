@@ -33,7 +33,7 @@ HIPCC_FLAGS = [
 ]
 
 KERNELS = ["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample",
-           "kv4_cache", "gqa_decode_kv4"]
+           "kv4_cache", "gqa_decode_kv4", "gqa_chunk_kv4", "beam_select", "state_fork"]
 
 
 def _run(cmd: list[str]) -> None:

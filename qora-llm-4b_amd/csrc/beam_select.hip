@@ -1,0 +1,234 @@
+// beam_select.hip -- beam search's selection for gfx950: the best continuations
+// of each request's sequences, over sequences and vocabulary.
+//
+// A sequence's continuation by token t is worth score + x_t - log sum exp x.
+// Within a row the logits' order is the values', so the selection needs the
+// whole row's largest logits and its sum only:
+//   qm_beam_slices  a wave per 1024 logits: their largest, its token, the sum
+//                   of exp(x - largest).  The one pass over the logits.
+//   qm_beam_draw    a workgroup per request: the rows' log-sums, the `take`
+//                   best slices by their largest logits' values, and the best
+//                   of those slices' logits.  No other slice can hold a chosen
+//                   one: `take` continuations are before all of its.
+// Values are compared in 64 bits (the log-sum is f64 of f32 sums: off by some
+// 2^-24), ties to the lower row and then the lower token.
+#include "qm_device.h"
+#include "qm_beam.h"
+
+// Rows that take part and are read: a finite score, not at their end.
+QM_DEV bool beam_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+QM_DEV bool beam_live(const BeamArgs& A, int row) { return beam_finite(A.scores[row]) && !(A.done && A.done[row]); }
+
+extern "C" __global__ __launch_bounds__(256) void qm_beam_slices(BeamArgs A) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = (int)(at / A.ns), slice = (int)(at - (int64_t)row * A.ns);
+    if (row >= A.groups * A.beams || !beam_live(A, row)) return;      // uniform per wave
+    const int t0 = slice * QMK_BEAM_SLICE + lane;
+    const float* x = A.logits + (size_t)row * A.vocab;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = x[min(t0 + 64 * i, A.vocab - 1)];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (t0 + 64 * i >= A.vocab) v[i] = -INFINITY;
+        top = fmaxf(top, v[i]);
+    }
+    top = max_xor32(max_xor16(row_max16(top)));
+    // the lowest token that has it
+    int token = A.vocab;
+#pragma unroll
+    for (int i = 15; i >= 0; --i) {
+        const uint64_t have = __ballot(v[i] == top);
+        if (have) token = t0 - lane + 64 * i + __builtin_ctzll(have);
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;                                      // NaN where a logit is, or an infinity
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += exp_fast(v[i] - base);
+    sum = wave_sum64(sum);
+    if (lane == 0) A.slices[at] = BeamSlice{top, sum, token, 0};
+}
+
+// ---- the request's choice ------------------------------------------------------
+// A continuation's key: larger is better.  value: the f64's bits in order, 0:
+// none; index: row of the request * vocab + token.
+struct BeamKey {
+    uint64_t value;
+    uint32_t index;
+};
+QM_DEV bool before(const BeamKey& a, const BeamKey& b) { return a.value != b.value ? a.value > b.value : a.index < b.index; }
+QM_DEV uint64_t ordered(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);          // no -0
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+QM_DEV double unordered(uint64_t u) { return __builtin_bit_cast(double, u >> 63 ? u & ~(1ull << 63) : ~u); }
+
+#define BEAM_THREADS 1024
+#define BEAM_LIST 128              // keys that are sorted by counting
+struct BeamLds {
+    double base[QMK_BEAM_MAX];     // score - log-sum of a row, or an ended one's score; not finite: takes no part
+    int32_t ended[QMK_BEAM_MAX];
+    int32_t hist[256];
+    BeamKey list[BEAM_LIST], sorted[QMK_BEAM_MAX];
+    BeamKey leaders[QMK_BEAM_MAX];
+    int32_t n, digit, above, inside;
+};
+
+// Digit d of a key, from the top: eight of the value, then four of the index
+// (from the other end: the lower is before).
+QM_DEV int key_digit(const BeamKey& k, int d) {
+    return d < 8 ? (int)(k.value >> (56 - 8 * d)) & 255 : (int)(~k.index >> (24 - 8 * (d - 8))) & 255;
+}
+// Whether the digits before d are those of `prefix` (0), or larger (1), or smaller (-1).
+QM_DEV int key_against(const BeamKey& k, const BeamKey& prefix, int d) {
+    const int vb = min(d, 8) * 8;
+    const uint64_t kv = vb ? k.value >> (64 - vb) : 0, pv = vb ? prefix.value >> (64 - vb) : 0;
+    if (kv != pv) return kv > pv ? 1 : -1;
+    if (d <= 8) return 0;
+    const int ib = (d - 8) * 8;
+    const uint32_t ki = ~k.index >> (32 - ib), pi = ~prefix.index >> (32 - ib);
+    return ki == pi ? 0 : ki > pi ? 1 : -1;
+}
+
+// The best `take` of keys key(0 .. n - 1), in order, into `out`; their number.
+// A radix select narrows them, from the top digit on, until BEAM_LIST are left
+// that may be among them (keys differ, so in the end there are).
+template <class F>
+QM_DEV int beam_best(BeamLds& sh, int n, int take, BeamKey* out, F key) {
+    const int tid = threadIdx.x;
+    BeamKey prefix{0, ~0u};
+    int digits = 0, above = 0;
+    for (;;) {
+        // those at or above the prefix
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += BEAM_THREADS) {
+            const BeamKey k = key(i);
+            if (k.value == 0 || key_against(k, prefix, digits) < 0) continue;
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < BEAM_LIST) sh.list[at] = k;
+        }
+        __syncthreads();
+        if (sh.n <= BEAM_LIST || digits == 12) break;      // uniform
+        for (int i = tid; i < 256; i += BEAM_THREADS) sh.hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += BEAM_THREADS) {
+            const BeamKey k = key(i);
+            if (k.value != 0 && key_against(k, prefix, digits) == 0) atomicAdd(&sh.hist[key_digit(k, digits)], 1);
+        }
+        __syncthreads();
+        // the digit at which `take` are reached: a wave, lane l with bins 255 - 4 l ..
+        if (tid < 64) {
+            int bin[4], mine = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mine += bin[j] = sh.hist[255 - 4 * tid - j];
+            int incl = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int y = __shfl_up(incl, d);
+                incl += tid >= d ? y : 0;
+            }
+            const uint64_t reach = __ballot(above + incl >= take);
+            // there are more than BEAM_LIST >= take at or above the prefix
+            if (reach && tid == __builtin_ctzll(reach)) {
+                int a = above + incl - mine, j = 0;
+#pragma unroll
+                for (; j < 3; ++j) {
+                    if (a + bin[j] >= take) break;
+                    a += bin[j];
+                }
+                sh.digit = 255 - 4 * tid - j;
+                sh.above = a;
+            }
+        }
+        __syncthreads();
+        above = sh.above;
+        if (digits < 8) prefix.value |= (uint64_t)sh.digit << (56 - 8 * digits);
+        else prefix.index = ~(~prefix.index | (uint32_t)sh.digit << (24 - 8 * (digits - 8)));
+        ++digits;
+    }
+    const int found = min(sh.n, BEAM_LIST);
+    if (tid < found) {
+        const BeamKey k = sh.list[tid];
+        int rank = 0;
+        for (int i = 0; i < found; ++i) rank += before(sh.list[i], k);
+        if (rank < take) out[rank] = k;
+    }
+    __syncthreads();
+    return min(found, take);
+}
+
+extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs A) {
+    __shared__ BeamLds sh;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row0 = blockIdx.x * A.beams;
+    for (int b = w; b < A.beams; b += BEAM_THREADS / 64) {             // uniform per wave
+        const float score = A.scores[row0 + b];
+        const bool ended = A.done && A.done[row0 + b] != 0;
+        double base = __builtin_nan("");
+        if (beam_finite(score) && ended) {
+            base = score;
+        } else if (beam_finite(score)) {
+            const BeamSlice* s = A.slices + (size_t)(row0 + b) * A.ns;
+            float top = -INFINITY;
+            for (int i = lane; i < A.ns; i += 64) top = fmaxf(top, s[i].top);
+            top = max_xor32(max_xor16(row_max16(top)));
+            double sum = 0.0;
+            for (int i = lane; i < A.ns; i += 64) {
+                const BeamSlice x = s[i];
+                if (x.sum != 0.0f) sum += (double)x.sum * exp((double)(x.top == -INFINITY ? 0.0f : x.top) - (double)top);
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+            base = (double)score - ((double)top + log(sum));           // NaN, infinite: takes no part
+        }
+        if (lane == 0) {
+            sh.base[b] = base;
+            sh.ended[b] = ended;
+        }
+    }
+    __syncthreads();
+    auto value = [&](int b, float x) {
+        const double v = sh.base[b] + (double)x;
+        return __builtin_isfinite(v) ? ordered(v) : 0ull;
+    };
+    // the best slices, by their best tokens; a row at its end has one continuation
+    const int leaders = beam_best(sh, A.beams * A.ns, A.take, sh.leaders, [&](int i) {
+        const int b = i / A.ns, j = i - b * A.ns;
+        if (sh.ended[b]) return BeamKey{j == 0 ? value(b, 0.0f) : 0ull, (uint32_t)(b * A.vocab + A.end_id)};
+        if (!__builtin_isfinite(sh.base[b])) return BeamKey{0ull, 0u};
+        const BeamSlice s = A.slices[(size_t)(row0 + b) * A.ns + j];
+        return BeamKey{value(b, s.top), (uint32_t)(b * A.vocab + s.token)};
+    });
+    // and the best of those slices' tokens: where the slices are `take`, none is worth less than the last one's best
+    const uint64_t least = leaders == A.take ? sh.leaders[leaders - 1].value : 0ull;
+    const int found = beam_best(sh, leaders * QMK_BEAM_SLICE, A.take, sh.sorted, [&](int i) {
+        const BeamKey lead = sh.leaders[i / QMK_BEAM_SLICE];
+        const int b = lead.index / A.vocab, at = i % QMK_BEAM_SLICE;
+        if (sh.ended[b]) return BeamKey{at == 0 ? lead.value : 0ull, lead.index};
+        const int t = (int)(lead.index - b * A.vocab) / QMK_BEAM_SLICE * QMK_BEAM_SLICE + at;
+        if (t >= A.vocab) return BeamKey{0ull, 0u};
+        const uint64_t v = value(b, A.logits[(size_t)(row0 + b) * A.vocab + t]);
+        return BeamKey{v >= least ? v : 0ull, (uint32_t)(b * A.vocab + t)};
+    });
+    if (tid < A.take) {
+        const size_t to = (size_t)blockIdx.x * A.take + tid;
+        int parent = -1, token = -1, over = 0;
+        float score = -INFINITY;
+        if (tid < found) {
+            const BeamKey k = sh.sorted[tid];
+            const int b = k.index / A.vocab;
+            parent = row0 + b;
+            token = (int)(k.index - b * A.vocab);
+            score = (float)unordered(k.value);
+            over = sh.ended[b] || token == A.end_id;
+        }
+        // (its scores and flags may stand where its choice goes: all are read)
+        A.parents[to] = parent;
+        A.tokens[to] = token;
+        A.out_scores[to] = score;
+        if (A.out_done) A.out_done[to] = over;
+    }
+}

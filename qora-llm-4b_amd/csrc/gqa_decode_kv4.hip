@@ -169,13 +169,6 @@ QM_DEV bool deal_split(const GqaKv4Args& A, Deal& d, int k, bool note, int lane)
     return found;
 }
 
-template <int CTRL>
-QM_DEV double dpp_f64(double x) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 QM_DEV double readlane_f64(double x, int lane) {
     const uint64_t u = __builtin_bit_cast(uint64_t, x);
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
@@ -212,11 +205,7 @@ QM_DEV void rotate_head(float (&x)[4], const float (&c)[4], const float (&s)[4],
 QM_DEV void norm_new_k(double (&x)[4], uint2 gw) {
     const uint16_t g[4] = {(uint16_t)(gw.x & 0xffffu), (uint16_t)(gw.x >> 16), (uint16_t)(gw.y & 0xffffu), (uint16_t)(gw.y >> 16)};
     const double mean = wave_sum64_f64((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) * (1.0 / QM_GQA_HD) + 1e-6;
-    // v_rsq_f64 is good to about 2^-24; each step of Newton's squares the error
-    double inv = __builtin_amdgcn_rsq(mean);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) inv = inv * __builtin_fma(-0.5 * mean * inv, inv, 1.5);
-    if (!(mean < __builtin_inf())) inv = mean == mean ? 0.0 : mean;      // rsq's own 0 for an infinity, NaN for NaN
+    const double inv = inverse_root_f64(mean);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (1.0 + (double)f16_to_f32(g[i]));
 }

@@ -2,6 +2,7 @@
 // into the pages and back, and the pages themselves: growing, shrinking and
 // freeing rows, forking them, and moving the live pages together.
 #include "qm_kv4_device.h"
+#include "qm_kernel_args.h"
 
 // ---- f16 rows <-> pages ---------------------------------------------------
 // A workgroup takes half a page (32 tokens) of one sequence and head, whose
@@ -133,50 +134,38 @@ QM_DEV void turn_nibbles(uint32_t (&out)[8], uint32_t r0, uint32_t r1, uint32_t 
     }
 }
 
-extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
-    __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
-    const int tid = threadIdx.x;
-    const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
-    const int head = bh & 3, b = bh >> 2;
-    HalfAt h;
-    if (!half_at(A, b, tile, h)) return;                // uniform
-    const bool whole = h.lo == 0 && h.hi == QMK_KV4_HALF_TOKENS;
-    // Waves 0..3 have V, 4..7 K; a lane four tokens 16 u + 4 g + k of dims 8 i ..
-    const bool is_v = tid < 256;
-    const int i = tid & 31, u = (tid >> 5) & 1, g = (tid >> 6) & 3;
-    const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
-    const uint16_t* from = is_v ? A.v : A.k;
-    uint4 raw[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int t = min(max(16 * u + 4 * g + k, h.lo), h.hi - 1);      // any token for those left out
-        raw[k] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * i);
-    }
-    const int id = half_id(A, b, h);
-    if (!kv4_is_page(A.c, id)) return;                  // uniform
-    const int holders = A.c.refs[id];                   // looked at before the page is written
-    uint8_t* page = half_page(A, id, head, h);
+// A half page, put together in LDS: tokens lo .. hi - 1 are `raw`, the others
+// as they stand.  Waves 0..3 have V, 4..7 K; a lane four tokens 16 u + 4 g + k
+// of dims 8 i ..  `holders`: of the page; only a row's own is written to.
+struct HalfLane {
+    bool is_v;
+    int i, u, g;
+};
+QM_DEV HalfLane half_lane(int tid) { return HalfLane{tid < 256, tid & 31, (tid >> 5) & 1, (tid >> 6) & 3}; }
+QM_DEV void write_half(uint32_t* image, uint8_t* page, const uint4 (&raw)[4], int lo, int hi, int holders, int tid) {
+    const bool whole = lo == 0 && hi == QMK_KV4_HALF_TOKENS;
+    const HalfLane at = half_lane(tid);
     if (!whole) {                                       // uniform: the tokens left out stay
         for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_STORE_THREADS)
             reinterpret_cast<uint4*>(image)[j] = reinterpret_cast<const uint4*>(page)[j];
         __syncthreads();
     }
-    uint16_t* meta = reinterpret_cast<uint16_t*>(image) + QMK_KV4_META / 2 + (is_v ? 256 : 0);
+    uint16_t* meta = reinterpret_cast<uint16_t*>(image) + QMK_KV4_META / 2 + (at.is_v ? 256 : 0);
     uint32_t word[4], keep = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const int t = 16 * u + 4 * g + k;
-        const bool in = t >= h.lo && t < h.hi;
+        const int t = 16 * at.u + 4 * at.g + k;
+        const bool in = t >= lo && t < hi;
         const Coded c = code8(raw[k], tid & 63);
         word[k] = c.word;
         keep |= in ? 0u : 15u << (4 * kv4_nibble(k));
-        if (!is_v && in) image[kv4_k_word(t, 8 * i)] = c.word;
-        if ((i & 7) == 0 && in) {
-            meta[kv4_s_at(t, i >> 3)] = c.s;
-            meta[128 + kv4_lo_at(t, i >> 3)] = c.lo;
+        if (!at.is_v && in) image[kv4_k_word(t, 8 * at.i)] = c.word;
+        if ((at.i & 7) == 0 && in) {
+            meta[kv4_s_at(t, at.i >> 3)] = c.s;
+            meta[128 + kv4_lo_at(t, at.i >> 3)] = c.lo;
         }
     }
-    if (is_v) {                                         // uniform per wave
+    if (at.is_v) {                                      // uniform per wave
         // The run's tokens are elements 4 u + k of the words: nibbles 0, 4, 1, 5,
         // and for u = 1 two further up.  Lane and lane + 32 have the two runs of
         // the same dims; after the exchange the one has elements 0..3 of dims
@@ -189,8 +178,8 @@ extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4
         for (int k = 0; k < 4; ++k) {
             const auto w = __builtin_amdgcn_permlane32_swap(out[kv4_nibble(k)], out[kv4_nibble(k + 4)], false, false);
             const uint32_t both = w[0] | w[1] << 8;
-            uint32_t* at = &image[kv4_v_word(4 * g, 8 * i + k + 4 * u)];
-            *at = whole ? both : (both & ~stay) | (*at & stay);
+            uint32_t* to = &image[kv4_v_word(4 * at.g, 8 * at.i + k + 4 * at.u)];
+            *to = whole ? both : (both & ~stay) | (*to & stay);
         }
     }
     __syncthreads();
@@ -198,6 +187,183 @@ extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4
     for (int j = tid; j < QMK_KV4_HALF_BYTES / 16; j += KV4_STORE_THREADS)
         reinterpret_cast<uint4*>(page)[j] = reinterpret_cast<const uint4*>(image)[j];
 }
+
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4RowsArgs A) {
+    __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
+    const int tid = threadIdx.x;
+    const int tile = blockIdx.x % A.halves, bh = blockIdx.x / A.halves;
+    const int head = bh & 3, b = bh >> 2;
+    HalfAt h;
+    if (!half_at(A, b, tile, h)) return;                // uniform
+    const HalfLane at = half_lane(tid);
+    const size_t base = ((size_t)b * 4 + head) * (size_t)A.cap;
+    const uint16_t* from = at.is_v ? A.v : A.k;
+    uint4 raw[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int t = min(max(16 * at.u + 4 * at.g + k, h.lo), h.hi - 1);      // any token for those left out
+        raw[k] = *reinterpret_cast<const uint4*>(from + (base + (size_t)(h.src0 + t)) * 256 + 8 * at.i);
+    }
+    const int id = half_id(A, b, h);
+    if (!kv4_is_page(A.c, id)) return;                  // uniform
+    const int holders = A.c.refs[id];                   // looked at before the page is written
+    write_half(image, half_page(A, id, head, h), raw, h.lo, h.hi, holders, tid);
+}
+
+// ---- new tokens of ragged rows into the pages --------------------------------
+// K's RMSNorm (1 + gamma, eps 1e-6; gemv.rs:586-597) and RoPE (:604-627) in 64
+// bits, rounded to f32 and to f16 as the decode step's new row is, so that a
+// code beside a border does not depend on the order of a sum.  A token's row is
+// half a wave (32 lanes x 8 dims).  A workgroup takes half a page of one batch
+// row and head, as a store does; the half pages that the rows touch are dealt
+// in list order.
+struct AppendAt {
+    int row, first, len, begin;          // table row, its first new token's position, length, packed row
+    int t0;                              // token 0 of the half page
+};
+QM_DEV bool append_at(const Kv4AppendArgs& A, int index, int lane, AppendAt& at) {
+    int before = 0;
+    for (int b0 = 0; b0 < A.batch; b0 += 64) {          // uniform
+        const int b = b0 + lane;
+        int row = -1, len = 0, n = 0, begin = 0;
+        if (b < A.batch) {
+            begin = A.begins[b];
+            const int end = A.begins[b + 1];
+            row = A.slots ? A.slots[b] : b;
+            if (begin >= 0 && end > begin && end <= A.tokens && (uint32_t)row < (uint32_t)A.c.rows) {
+                len = A.c.lens[row];
+                n = end - begin;
+            }
+        }
+        const bool some = n > 0 && n <= len && len <= A.max_len;
+        const int halves = some ? ((len - 1) >> 5) - ((len - n) >> 5) + 1 : 0;
+        const int incl = (int)wave_scan((uint32_t)halves), all = __builtin_amdgcn_readlane(incl, 63);
+        if (index < before + all) {
+            const int from = __popcll(__ballot(before + incl <= index));
+            at.row = __builtin_amdgcn_readlane(row, from);
+            at.len = __builtin_amdgcn_readlane(len, from);
+            at.first = at.len - __builtin_amdgcn_readlane(n, from);
+            at.begin = __builtin_amdgcn_readlane(begin, from);
+            at.t0 = ((at.first >> 5) + index - before - __builtin_amdgcn_readlane(incl - halves, from)) << 5;
+            if (A.slots)                                // a table row that an earlier batch row has: left out
+                for (int j0 = 0; j0 < b0 + from; j0 += 64) {
+                    const int j = j0 + lane;
+                    if (__ballot(j < b0 + from && A.slots[min(j, b0 + from - 1)] == at.row)) return false;
+                }
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
+
+QM_DEV double xor16_sum_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+// The value four lanes on (lanes 0..3 of a row of 16) or back (4..7).
+QM_DEV uint32_t partner4(uint32_t x) {
+    const int on = __builtin_amdgcn_update_dpp(0, (int)x, 0x104, 0xF, 0x1, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(on, (int)x, 0x114, 0xF, 0x2, false);
+}
+QM_DEV double partner4(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)partner4((uint32_t)(u >> 32)) << 32 | partner4((uint32_t)u));
+}
+
+// Dims 8 i .. of a token's row, as f32.
+struct Row8 {
+    float x[8];
+};
+QM_DEV Row8 row8(const uint16_t* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    Row8 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        r.x[2 * e] = bf16_to_f32((uint16_t)(w[e] & 0xffffu));
+        r.x[2 * e + 1] = bf16_to_f32((uint16_t)(w[e] >> 16));
+    }
+    return r;
+}
+QM_DEV Row8 row8(const float* p) {
+    const float4 a = ld4(p), b = ld4(p + 4);
+    return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+QM_DEV uint4 pack8(const uint16_t (&h)[8]) {
+    return make_uint4((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16,
+                      (uint32_t)h[4] | (uint32_t)h[5] << 16, (uint32_t)h[6] | (uint32_t)h[7] << 16);
+}
+
+template <class T>
+QM_DEV void kv4_append(const Kv4AppendArgs& A) {
+    __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
+    const int tid = threadIdx.x, head = blockIdx.x & 3;
+    if (A.result && A.result[0] != 0) return;           // uniform, as are the returns below
+    AppendAt h;
+    if (!append_at(A, blockIdx.x >> 2, tid & 63, h)) return;
+    const int lo = max(0, h.first - h.t0), hi = min(QMK_KV4_HALF_TOKENS, h.len - h.t0);
+    if ((h.t0 >> 6) >= A.c.max_pages) return;
+    const int id = A.c.table[(size_t)h.row * A.c.max_pages + (h.t0 >> 6)];
+    const HalfLane at = half_lane(tid);
+    const T* from = reinterpret_cast<const T*>(at.is_v ? A.v : A.k);
+    Row8 x[4];
+    float cs[4][8], sn[4][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int t = min(max(16 * at.u + 4 * at.g + k, lo), hi - 1);          // any new token for the others
+        x[k] = row8(from + ((size_t)(h.begin + (h.t0 - h.first) + t) * 4 + head) * 256 + 8 * at.i);
+        if (!at.is_v) {                                 // uniform per wave
+            const size_t r = (size_t)(h.t0 + t) * (QM_GQA_ROT / 2) + 8 * (at.i & 3);
+            const Row8 c = row8(A.rope_cos + r), s = row8(A.rope_sin + r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) cs[k][e] = c.x[e], sn[k][e] = s.x[e];
+        }
+    }
+    if (!kv4_is_page(A.c, id)) return;
+    const int holders = A.c.refs[id];
+    uint4 raw[4];
+    if (at.is_v) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint16_t out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = f32_to_f16(x[k].x[e]);
+            raw[k] = pack8(out);
+        }
+    } else {
+        const uint4 gw = *reinterpret_cast<const uint4*>(A.k_norm + 8 * at.i);
+        const uint32_t g[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            double y[8], ss = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] = (double)x[k].x[e];
+                ss = __builtin_fma(y[e], y[e], ss);
+            }
+            ss += dpp_f64<0xB1>(ss);
+            ss += dpp_f64<0x4E>(ss);
+            ss += dpp_f64<0x141>(ss);
+            ss += dpp_f64<0x140>(ss);
+            const double inv = inverse_root_f64(xor16_sum_f64(ss) * (1.0 / QM_GQA_HD) + 1e-6);
+            uint16_t out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] = y[e] * inv * (1.0 + (double)f16_to_f32((uint16_t)(g[e >> 1] >> (16 * (e & 1)))));
+                const double p = partner4(y[e]);        // 32 dims on or back
+                const double turned = at.i < 4 ? y[e] * cs[k][e] - p * sn[k][e] : y[e] * cs[k][e] + p * sn[k][e];
+                out[e] = f64_to_f16_by_f32(at.i < 8 ? turned : y[e]);
+            }
+            raw[k] = pack8(out);
+        }
+    }
+    write_half(image, kv4_half(A.c, A.layer, id, head, (h.t0 >> 5) & 1), raw, lo, hi, holders, tid);
+}
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_append_f32(Kv4AppendArgs A) { kv4_append<float>(A); }
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_append_bf16(Kv4AppendArgs A) { kv4_append<uint16_t>(A); }
 
 // lo + s q of the code in bits `shift` .., rounded to f32 and then to f16.  In
 // one step (v_fma_mixlo_f16, which the compiler takes otherwise) it would be

@@ -36,6 +36,9 @@
 #define QMK_KV4_MAX_SPLIT 4096      // tokens of a decode workgroup: 64 pages
 #define QMK_KV4_ROUNDS 64           // full rounds of decode workgroups that are dealt evenly
 #define QMK_KV4_LEN_PAGES 33554431  // pages of a row: its length is an int32
+#define QMK_CHUNK_TOKENS 64         // new tokens of a row block of the chunk attention
+#define QMK_CHUNK_MAX_TOKENS (1 << 20)     // new tokens of a call
+#define QMK_CHUNK_PARTIAL 66048     // f32 of a row block's partial: 16 x (16 dim groups x 256, m[16], l[16])
 
 #ifdef __HIPCC__
 #define QMK_HD __host__ __device__ inline
@@ -129,4 +132,35 @@ struct GqaKv4Args {
     int32_t layer, batch, max_len;
     int32_t cus;             // compute units of the device
     int32_t single;          // a workgroup per batch row and head, no merge
+};
+
+// New tokens of ragged rows: batch row b's are rows begins[b] .. begins[b + 1]
+// of packed tensors, and the last ones of its table row's length.
+struct Kv4AppendArgs {
+    Kv4Cache c;
+    const int32_t* slots;    // [batch] or null: row b
+    const int32_t* begins;   // [batch + 1]
+    const void* k;           // [tokens][4][256] f32 or bf16
+    const void* v;
+    const uint16_t* k_norm;  // [256] f16
+    const float* rope_cos;   // [rope_len][32]
+    const float* rope_sin;
+    const int32_t* result;   // null, or a resize's result
+    int32_t layer, batch, tokens, max_len;
+};
+
+// Attention of such tokens.
+struct GqaChunkArgs {
+    Kv4Cache c;
+    const int32_t* slots;
+    const int32_t* begins;
+    const uint16_t* q_gate;  // bf16 [tokens][16][512]
+    const uint16_t* q_norm;
+    const float* rope_cos;
+    const float* rope_sin;
+    const int32_t* result;
+    uint16_t* out;           // bf16 [tokens][16][256]
+    float* partial;          // [groups][4 kv heads][2][QMK_CHUNK_PARTIAL]
+    int32_t layer, batch, tokens, max_new, max_len;
+    int32_t groups;          // workgroups per kv head
 };

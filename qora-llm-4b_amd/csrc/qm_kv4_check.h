@@ -111,6 +111,59 @@ inline Fault check_decode(const qm_kv4_cache* c, int32_t layer, int32_t batch, c
     return Fault{};
 }
 
+// What append and chunk attention have in common: the batch's lists and bounds.
+inline Fault check_ragged(const char* who, const qm_kv4_cache* c, int32_t layer, int32_t batch, const int32_t* slots,
+                          const int32_t* begins, int32_t tokens, std::initializer_list<const void*> data,
+                          int32_t rope_len, int32_t max_len, const int32_t* result) {
+    Fault f = check_cache(who, c);
+    if (f.code != QM_OK) return f;
+    if (layer < 0 || layer >= c->layers) return fault(QM_ERR_INVALID_ARG, "%s: layer %d of %d", who, layer, c->layers);
+    if (batch <= 0 || batch > QMK_KV4_MAX_ROWS || (!slots && batch > c->rows))
+        return fault(QM_ERR_INVALID_ARG, "%s: batch %d of a cache of %d rows", who, batch, c->rows);
+    if (tokens <= 0 || tokens > QMK_CHUNK_MAX_TOKENS)
+        return fault(QM_ERR_INVALID_ARG, "%s: %d tokens (1 .. %d)", who, tokens, QMK_CHUNK_MAX_TOKENS);
+    if (!begins) return fault(QM_ERR_INVALID_ARG, "%s: null begins", who);
+    for (const void* p : data)
+        if (!p) return fault(QM_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (off_grid(16, data) || off_grid(4, {slots, begins, result}))
+        return fault(QM_ERR_INVALID_ARG, "%s: device pointers must be 16-byte aligned (slots, begins and result 4-byte)", who);
+    if (max_len <= 0) return fault(QM_ERR_INVALID_ARG, "%s: max_len %d", who, max_len);
+    if (max_len > rope_len) return fault(QM_ERR_ROPE_RANGE, "length %d beyond RoPE table of %d rows", max_len, rope_len);
+    if (max_len > static_cast<int64_t>(c->max_pages) * QMK_KV4_PAGE_TOKENS)
+        return fault(QM_ERR_CAPACITY, "length %d beyond the %d pages of a row", max_len, c->max_pages);
+    return Fault{};
+}
+inline Fault check_append(const qm_kv4_cache* c, int32_t layer, int32_t batch, const int32_t* slots, const int32_t* begins,
+                          int32_t tokens, int32_t dtype, std::initializer_list<const void*> data, int32_t rope_len,
+                          int32_t max_len, const int32_t* result) {
+    if (dtype != QM_F32 && dtype != QM_BF16)
+        return fault(QM_ERR_INVALID_ARG, "qm_kv4_append: dtype %d (QM_F32 or QM_BF16)", dtype);
+    return check_ragged("qm_kv4_append", c, layer, batch, slots, begins, tokens, data, rope_len, max_len, result);
+}
+inline Fault check_chunk(const qm_kv4_cache* c, int32_t layer, int32_t batch, const int32_t* slots, const int32_t* begins,
+                         int32_t tokens, int32_t max_new, std::initializer_list<const void*> data, int32_t rope_len,
+                         int32_t max_len, const int32_t* result) {
+    if (max_new <= 0) return fault(QM_ERR_INVALID_ARG, "qm_gqa_chunk_kv4: max_new %d", max_new);
+    return check_ragged("qm_gqa_chunk_kv4", c, layer, batch, slots, begins, tokens, data, rope_len, max_len, result);
+}
+
+// Half pages that `tokens` new tokens of `batch` rows touch at most: n of a row
+// floor((n + 30) / 32) + 1.
+inline int64_t append_halves(int32_t tokens, int32_t batch) {
+    return (static_cast<int64_t>(tokens) + 30ll * batch) / QMK_KV4_HALF_TOKENS + batch;
+}
+// Row blocks of the chunk attention, and its workgroups per kv head: one a CU,
+// or fewer where the blocks' pages are fewer.
+inline int64_t chunk_blocks(int32_t tokens, int32_t batch) {
+    return (static_cast<int64_t>(tokens) + (QMK_CHUNK_TOKENS - 1ll) * batch) / QMK_CHUNK_TOKENS;
+}
+inline int64_t chunk_groups(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
+    const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
+    const int64_t units = chunk_blocks(tokens, batch) * tiles, most = cus / 4 > 0 ? cus / 4 : 1;
+    return units < most ? units : most;
+}
+inline size_t chunk_ws(int64_t groups) { return static_cast<size_t>(groups) * 4 * 2 * QMK_CHUNK_PARTIAL * 4; }
+
 // The decode's workgroups.  Short rows, and somewhat longer ones where there
 // are enough of them, take one workgroup each per kv head and no merge
 // (measured, one workgroup / dealt out, us: 1 row of 250 tokens 8.1 / 9.1, of

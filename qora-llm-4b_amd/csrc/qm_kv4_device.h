@@ -18,6 +18,23 @@ QM_DEV uint16_t f64_to_f16_by_f32(double x) {
     return f32_to_f16(f);
 }
 
+template <int CTRL>
+QM_DEV double dpp_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// 1 / sqrt(x): v_rsq_f64 is good to about 2^-24; each step of Newton's squares
+// the error.
+QM_DEV double inverse_root_f64(double x) {
+    double inv = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) inv = inv * __builtin_fma(-0.5 * x * inv, inv, 1.5);
+    if (!(x < __builtin_inf())) inv = x == x ? 0.0 : x;      // rsq's own 0 for an infinity, NaN for NaN
+    return inv;
+}
+
 // The scale of a group, f16 bits: the quotient in 64 bits, so that it is the
 // same whoever computes it, then f32, then f16.
 QM_DEV uint16_t kv4_scale(float lo, float hi) {

@@ -11,6 +11,7 @@
 #include "qora_mixer.h"
 #include "qm_kernel_args.h"
 #include "qm_gqa_plan.h"
+#include "qm_beam_check.h"
 #include "qm_kv4_check.h"
 #include "qm_noalloc.h"
 #include "qm_q4_tiles.h"
@@ -69,6 +70,10 @@ struct qm_context {
     hipFunction_t f_kv4_fork = nullptr, f_kv4_fork_rows = nullptr;
     hipFunction_t f_kv4_compact = nullptr, f_kv4_compact_pages = nullptr;
     hipFunction_t f_gqa_kv4_split = nullptr, f_gqa_kv4_merge = nullptr;
+    hipFunction_t f_kv4_append[2] = {};      // k and v f32, bf16
+    hipFunction_t f_gqa_chunk = nullptr, f_gqa_chunk_merge = nullptr;
+    hipFunction_t f_beam_slices = nullptr, f_beam_draw = nullptr;
+    hipFunction_t f_state_fork[3] = {};      // up to 8 rows, up to 32, more
     int lm_head_hidden = 0;              // the hidden size lm_head_wg_per_cu was computed for
     int lm_head_wg_per_cu = 1;
     int dnp_chunk_threads = 0;     // the DeltaNet prefill chunk kernel's workgroup size (its launch bounds)
@@ -336,8 +341,9 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     std::string dir = code_object_dir ? code_object_dir : library_dir();
     const char* files[] = {"qm_dn_decode.hsaco", "qm_gqa_decode.hsaco", "qm_util.hsaco",
                            "qm_dn_prefill.hsaco", "qm_gqa_prefill.hsaco", "qm_q4_proj.hsaco",
-                           "qm_q4_vocab.hsaco", "qm_sample.hsaco", "qm_kv4_cache.hsaco", "qm_gqa_decode_kv4.hsaco"};
-    constexpr int kModules = 10;
+                           "qm_q4_vocab.hsaco", "qm_sample.hsaco", "qm_kv4_cache.hsaco", "qm_gqa_decode_kv4.hsaco",
+                           "qm_gqa_chunk_kv4.hsaco", "qm_beam_select.hsaco", "qm_state_fork.hsaco"};
+    constexpr int kModules = 13;
     hipModule_t mods[kModules] = {};
     for (int i = 0; i < kModules; ++i) {
         std::string path = dir + "/" + files[i];
@@ -401,6 +407,15 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_compact_pages", &c->f_kv4_compact_pages);
     if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_split", &c->f_gqa_kv4_split);
     if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_merge", &c->f_gqa_kv4_merge);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_append_f32", &c->f_kv4_append[0]);
+    if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_append_bf16", &c->f_kv4_append[1]);
+    if (st == QM_OK) st = load_function(c, mods[10], "qm_gqa_chunk_kv4", &c->f_gqa_chunk);
+    if (st == QM_OK) st = load_function(c, mods[10], "qm_gqa_chunk_merge", &c->f_gqa_chunk_merge);
+    if (st == QM_OK) st = load_function(c, mods[11], "qm_beam_slices", &c->f_beam_slices);
+    if (st == QM_OK) st = load_function(c, mods[11], "qm_beam_draw", &c->f_beam_draw);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_8", &c->f_state_fork[0]);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_32", &c->f_state_fork[1]);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_many", &c->f_state_fork[2]);
     if (st == QM_OK &&
         (hipFuncGetAttribute(&c->q4_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gemv) != hipSuccess ||
          hipFuncGetAttribute(&c->q4_gu_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gate_up) !=
@@ -812,7 +827,10 @@ int32_t qm_reserve(qm_context* c, int32_t max_batch, int32_t max_kv_len, int32_t
         const size_t s_pad = (static_cast<size_t>(max_prefill_tokens) + 63) / 64 * 64;
         ws = std::max(ws, gqa_prefill_kvf_bytes(s_pad) + 256);
     }
+    if (max_kv_len > 0 && max_prefill_tokens > 0)
+        ws = std::max(ws, qm_kv4::chunk_ws(qm_kv4::chunk_groups(max_prefill_tokens, max_batch, max_kv_len, c->num_cu)));
     ws = std::max(ws, kSampleWsBytes);
+    ws = std::max(ws, qm_beam::select_ws(max_batch, QMK_BEAM_VOCAB));
     return ensure(c, c->stream, ws, true);
 }
 
@@ -1337,6 +1355,79 @@ int32_t qm_gqa_decode_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* c
     st = launch(c, c->f_gqa_kv4_split, static_cast<uint32_t>(splits * QM_GQA_KV_HEADS), 256, a, s, "qm_gqa_kv4_split");
     if (st != QM_OK || single) return st;
     return launch(c, c->f_gqa_kv4_merge, static_cast<uint32_t>(merge), 64, a, s, "qm_gqa_kv4_merge");
+}
+
+int32_t qm_kv4_append(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t batch,
+                      const int32_t* slots, const int32_t* begins, int32_t tokens, int32_t dtype, const void* k,
+                      const void* v, const uint16_t* k_norm, const float* rope_cos, const float* rope_sin,
+                      int32_t rope_len, int32_t max_len, const int32_t* result) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_append(cache, layer, batch, slots, begins, tokens, dtype,
+                                                   {k, v, k_norm, rope_cos, rope_sin}, rope_len, max_len, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    const int64_t grid = qm_kv4::append_halves(tokens, batch) * QM_GQA_KV_HEADS;
+    Kv4AppendArgs a{kv4_of(*cache), slots, begins, k, v, k_norm, rope_cos, rope_sin, result, layer, batch, tokens, max_len};
+    return launch(c, c->f_kv4_append[dtype == QM_BF16], static_cast<uint32_t>(grid), 512, a, pick(c, stream), "qm_kv4_append");
+}
+
+int32_t qm_gqa_chunk_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* cache, int32_t layer, int32_t batch,
+                         const int32_t* slots, const int32_t* begins, int32_t tokens, int32_t max_new,
+                         const uint16_t* q_gate, const uint16_t* q_norm, const float* rope_cos, const float* rope_sin,
+                         int32_t rope_len, int32_t max_len, const int32_t* result, uint16_t* out) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_kv4::check_chunk(cache, layer, batch, slots, begins, tokens, max_new,
+                                                  {q_gate, q_norm, rope_cos, rope_sin, out}, rope_len, max_len, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    const int64_t groups = qm_kv4::chunk_groups(tokens, batch, max_len, c->num_cu);
+    const int64_t merge = qm_kv4::chunk_blocks(tokens, batch) * QM_GQA_KV_HEADS * 64;
+    int32_t st = ensure(c, s, groups > 1 ? qm_kv4::chunk_ws(groups) : 0);
+    if (st != QM_OK) return st;
+    GqaChunkArgs a{kv4_of(*cache), slots, begins, q_gate, q_norm, rope_cos, rope_sin, result, out, static_cast<float*>(c->ws),
+                   layer, batch, tokens, max_new, max_len, static_cast<int32_t>(groups)};
+    st = launch(c, c->f_gqa_chunk, static_cast<uint32_t>(groups * QM_GQA_KV_HEADS), 512, a, s, "qm_gqa_chunk_kv4");
+    if (st != QM_OK || groups == 1) return st;
+    return launch(c, c->f_gqa_chunk_merge, static_cast<uint32_t>(merge), 64, a, s, "qm_gqa_chunk_merge");
+}
+
+// ---- beam search -------------------------------------------------------------------
+int32_t qm_beam_select(qm_context* c, qm_stream stream, int32_t groups, int32_t beams, int32_t take, int32_t vocab,
+                       const float* logits, const float* scores, const int32_t* done, int32_t end_id, int32_t* parents,
+                       int32_t* tokens, float* scores_out, int32_t* done_out) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_beam::check_select(groups, beams, take, vocab, logits, scores, done, end_id, parents, tokens,
+                                                    scores_out, done_out);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    hipStream_t s = pick(c, stream);
+    const int64_t rows = static_cast<int64_t>(groups) * beams;
+    int32_t st = ensure(c, s, qm_beam::select_ws(rows, vocab));
+    if (st != QM_OK) return st;
+    BeamArgs a{logits, scores, done, parents, tokens, scores_out, done_out, static_cast<BeamSlice*>(c->ws), groups, beams,
+               take, vocab, end_id, qm_beam::slices(vocab)};
+    st = launch(c, c->f_beam_slices, static_cast<uint32_t>((rows * a.ns + 3) / 4), 256, a, s, "qm_beam_slices");
+    if (st != QM_OK) return st;
+    return launch(c, c->f_beam_draw, static_cast<uint32_t>(groups), 1024, a, s, "qm_beam_draw");
+}
+
+int32_t qm_state_fork(qm_context* c, qm_stream stream, int32_t n_buffers, const qm_state_rows* buffers, int32_t rows,
+                      int32_t count, const int32_t* src, const int32_t* dst, int32_t* result) {
+    if (!c) return QM_ERR_INVALID_ARG;
+    const OnDevice on(c);
+    const qm_kv4::Fault bad = qm_beam::check_fork(n_buffers, buffers, rows, count, src, dst, result);
+    if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
+    StateForkArgs a{};
+    a.src = src, a.dst = dst, a.result = result;
+    a.rows = rows, a.count = count, a.buffers = n_buffers, a.column = qm_beam::fork_column(count);
+    for (int32_t i = 0; i < n_buffers; ++i) {
+        a.buffer[i] = StateBuffer{static_cast<uint8_t*>(buffers[i].rows_dev), buffers[i].row_bytes, buffers[i].stride_bytes};
+        a.first[i + 1] = a.first[i] + (buffers[i].row_bytes + a.column - 1) / a.column;
+    }
+    const int64_t grid = std::min<int64_t>(a.first[n_buffers], 8 * c->num_cu);
+    return launch(c, c->f_state_fork[count <= 8 ? 0 : count <= 32 ? 1 : 2], static_cast<uint32_t>(grid), 256, a,
+                  pick(c, stream), "qm_state_fork");
 }
 
 }  // extern "C"

@@ -61,6 +61,10 @@ class QmKv4Cache(C.Structure):
                 ("rows", C.c_int32), ("max_pages", C.c_int32)]
 
 
+class QmStateRows(C.Structure):
+    _fields_ = [("rows_dev", C.c_void_p), ("row_bytes", C.c_int64), ("stride_bytes", C.c_int64)]
+
+
 class QmConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "num_qk_heads", "num_v_heads", "dn_head_dim", "conv_kernel",
@@ -116,6 +120,10 @@ _SIGNATURES = {
     "qm_kv4_store": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _I32, _P, _I32, _P, _P, _I64],
     "qm_kv4_load": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _I32, _P, _I32, _P, _P, _I64],
     "qm_gqa_decode_kv4": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P],
+    "qm_kv4_append": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _P],
+    "qm_gqa_chunk_kv4": [_P, _P, C.POINTER(QmKv4Cache), _I32, _I32, _P, _P, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _P, _P],
+    "qm_beam_select": [_P, _P, _I32, _I32, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P],
+    "qm_state_fork": [_P, _P, _I32, C.POINTER(QmStateRows), _I32, _I32, _P, _P, _P],
     "qm_q4_repack": [_P, _P, _I32, _I32, _P, _P, _P, _P],
     "qm_q4_gemv": [_P, _P, _I32, _I32, _P, _P, _P, _P],
     "qm_q4_gemv_multi": [_P, _P, _I32, _P, _P, _I32, _P],
@@ -382,6 +390,21 @@ class Context:
             self.h, self.stream, C.byref(cache.c), layer, batch, _addr(slots), _addr(q_gate), _addr(k_new), _addr(v_new),
             _addr(q_norm), _addr(k_norm), _addr(rope_cos), _addr(rope_sin), rope_len, max_len, _addr(result), _addr(out)))
 
+    def kv4_append(self, cache, layer, batch, slots, begins, tokens, k, v, k_norm, rope_cos, rope_sin, rope_len, max_len,
+                   result, dtype=QM_F32):
+        """k (normed, rotated) and v [tokens][4][256] of batch row b's new tokens begins[b] .. begins[b + 1] - 1 into the
+        pages of table row slots[b] (None: b), the last tokens of its length."""
+        self._check(self.lib.qm_kv4_append(
+            self.h, self.stream, C.byref(cache.c), layer, batch, _addr(slots), _addr(begins), tokens, dtype, _addr(k), _addr(v),
+            _addr(k_norm), _addr(rope_cos), _addr(rope_sin), rope_len, max_len, _addr(result)))
+
+    def gqa_chunk_kv4(self, cache, layer, batch, slots, begins, tokens, max_new, q_gate, q_norm, rope_cos, rope_sin,
+                      rope_len, max_len, result, out):
+        """Attention of such tokens (bf16 [tokens][16][512]) over their rows' pages into out, bf16 [tokens][16][256]."""
+        self._check(self.lib.qm_gqa_chunk_kv4(
+            self.h, self.stream, C.byref(cache.c), layer, batch, _addr(slots), _addr(begins), tokens, max_new, _addr(q_gate),
+            _addr(q_norm), _addr(rope_cos), _addr(rope_sin), rope_len, max_len, _addr(result), _addr(out)))
+
     def gqa_prefill(self, seq_len, q_gate, k, v, q_norm, k_norm, rope_cos, rope_sin, rope_len,
                     k_cache, v_cache, cap, out):
         self._check(self.lib.qm_gqa_prefill(
@@ -456,6 +479,21 @@ class Context:
         self._check(self.lib.qm_sample(self.h, self.stream, vocab, _addr(logits), _addr(generated), n_generated,
                                        C.byref(p), _addr(rng_state), _addr(token_out), _addr(top_ids),
                                        _addr(top_probs)))
+
+    def beam_select(self, groups, beams, take, vocab, logits, scores, done, end_id, parents, tokens, scores_out,
+                    done_out=None):
+        """The take best continuations of each request's beams sequences by scores + log-softmax(logits): parent rows,
+        tokens, summed scores and whether they are at their end ([groups][take] each)."""
+        self._check(self.lib.qm_beam_select(
+            self.h, self.stream, groups, beams, take, vocab, _addr(logits), _addr(scores), _addr(done), end_id, _addr(parents),
+            _addr(tokens), _addr(scores_out), _addr(done_out)))
+
+    def state_fork(self, buffers, rows, count, src, dst, result):
+        """Row dst[i] (None: i) of every buffer becomes its row src[i] as it was; buffers: [(address, row bytes, bytes from
+        row to row), ...], host values; src, dst int32 [count]; result int32 [1]: 0 or -1."""
+        arr = (QmStateRows * len(buffers))(*[QmStateRows(_addr(b[0]), b[1], b[2]) for b in buffers])
+        self._check(self.lib.qm_state_fork(self.h, self.stream, len(buffers), arr, rows, count, _addr(src), _addr(dst),
+                                           _addr(result)))
 
 
 class Event:

@@ -11,7 +11,7 @@ use std::path::{Path, PathBuf};
 use std::process::Command;
 
 const KERNELS: &[&str] = &["dn_decode", "gqa_decode", "util", "dn_prefill", "gqa_prefill", "q4_proj", "q4_vocab", "sample",
-                         "kv4_cache", "gqa_decode_kv4"];
+                         "kv4_cache", "gqa_decode_kv4", "gqa_chunk_kv4", "beam_select", "state_fork"];
 
 // hipcc flags of every device compile: gfx950 only; no packed-fp32 VALU ops;
 // MFMA results in arch VGPRs.

@@ -114,6 +114,15 @@ pub mod raw {
         pub max_pages: i32,
     }
 
+    /// Rows of recurrent states in one buffer.
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct qm_state_rows {
+        pub rows_dev: *mut c_void,
+        pub row_bytes: i64,
+        pub stride_bytes: i64,
+    }
+
     #[link(name = "qora_mixer")]
     extern "C" {
         // ---- context
@@ -202,6 +211,26 @@ pub mod raw {
                                  v_new_dev: *const f32, q_norm_dev: *const u16, k_norm_dev: *const u16,
                                  rope_cos_dev: *const f32, rope_sin_dev: *const f32, rope_len: i32, max_len: i32,
                                  result_dev: *const i32, out_dev: *mut f32) -> i32;
+
+        pub fn qm_kv4_append(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, layer: i32,
+                             batch: i32, slots_dev: *const i32, begins_dev: *const i32, tokens: i32, dtype: i32,
+                             k_dev: *const c_void, v_dev: *const c_void, k_norm_dev: *const u16,
+                             rope_cos_dev: *const f32, rope_sin_dev: *const f32, rope_len: i32, max_len: i32,
+                             result_dev: *const i32) -> i32;
+        pub fn qm_gqa_chunk_kv4(ctx: *mut qm_context, stream: qm_stream, cache: *const qm_kv4_cache, layer: i32,
+                                batch: i32, slots_dev: *const i32, begins_dev: *const i32, tokens: i32, max_new: i32,
+                                q_gate_dev: *const u16, q_norm_dev: *const u16, rope_cos_dev: *const f32,
+                                rope_sin_dev: *const f32, rope_len: i32, max_len: i32, result_dev: *const i32,
+                                out_dev: *mut u16) -> i32;
+
+        // ---- beam search
+        pub fn qm_beam_select(ctx: *mut qm_context, stream: qm_stream, groups: i32, beams: i32, take: i32, vocab: i32,
+                              logits_dev: *const f32, scores_dev: *const f32, done_dev: *const i32, end_id: i32,
+                              parents_dev: *mut i32, tokens_dev: *mut i32, scores_out_dev: *mut f32,
+                              done_out_dev: *mut i32) -> i32;
+        pub fn qm_state_fork(ctx: *mut qm_context, stream: qm_stream, n_buffers: i32, buffers: *const qm_state_rows,
+                             rows: i32, count: i32, src_dev: *const i32, dst_dev: *const i32,
+                             result_dev: *mut i32) -> i32;
 
         // ---- Q4 projections
         pub fn qm_q4_repack(ctx: *mut qm_context, stream: qm_stream, k: i32, n: i32, packed_dev: *const u8,

@@ -1,0 +1,389 @@
+"""GPU: chunks of new tokens over the paged 4-bit KV cache against numpy in 64 bits (tests/chunk_reference.py).
+
+What is appended has to be the reference's, byte for byte.  Attention's outputs are bf16: off by half a step,
+2^-8 of themselves, beside the bound that chunk_reference.attend derives for what is rounded before.  Over all
+outputs the roundings are independent: that of a bf16 is 2^-8 / sqrt(3) = 2.3e-3 of the value at most in the
+2-norm, those of q, K, V and p to f16 together at most sqrt(6) 2^-11 / sqrt(3) times |score| (about 2) = 1.4e-3; the bar is 3e-3.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import chunk_reference as CR
+import kv4_reference as R
+from conftest import load_mixer
+from test_kv4_gpu import assert_same, ints, result, run_fork, run_resize, upload
+
+pytestmark = pytest.mark.gpu
+
+M = load_mixer()
+FILL = 0x4141
+
+
+def rope(n):
+    return M.rope_table(max(n, 8))
+
+
+def cache_of(lens, layers=2, spare=3, seed=0, room=0):
+    """A numpy cache whose rows have these lengths, in scattered pages of values, its unused tokens random bytes."""
+    most = max(1, R.pages_of(max(lens) + room))
+    pages = sum(R.pages_of(n) for n in lens) + spare
+    ref = R.Cache(layers, pages, len(lens), most, seed=seed)
+    assert ref.resize(None, list(lens)) == 0
+    perm = np.random.default_rng(seed + 1).permutation(pages)
+    ref.table = np.where(ref.table >= 0, perm[np.maximum(ref.table, 0)], -1).astype(np.int32)
+    refs = np.zeros_like(ref.refs)
+    refs[perm] = ref.refs
+    ref.refs = refs
+    rng = np.random.default_rng(seed + 2)
+    for r, n in enumerate(lens):
+        for j in range(R.pages_of(n)):
+            fill_page(ref.pages[:, ref.table[r, j]], min(R.TOKENS, n - j * R.TOKENS), rng)
+    return ref
+
+
+def fill_page(pages, n, rng):
+    """The first n tokens of a page of every layer: scales and minima of ordinary values beside the random codes."""
+    for layer in range(pages.shape[0]):
+        for half in range(8):
+            meta = pages[layer, half * R.HALF_BYTES + 8192:(half + 1) * R.HALF_BYTES].view(np.float16)
+            for t in range(32):
+                if 32 * (half % 2) + t >= n:
+                    continue
+                for is_v in (0, 1):
+                    s = rng.uniform(0.1, 0.3, 4).astype(np.float16)
+                    meta[256 * is_v + R.S_AT[t]] = s
+                    meta[256 * is_v + 128 + R.LO_AT[t]] = (-7.5 * s.astype(np.float64) * rng.uniform(0.8, 1.2, 4)).astype(np.float16)
+
+
+def queries(rng, tokens):
+    q = CR.bf16(rng.standard_normal((tokens, 16, 512)))
+    return q, (0.1 * rng.standard_normal(256)).astype(np.float16)
+
+
+def begins_of(news, start=0):
+    return np.concatenate([[start], start + np.cumsum(news)]).astype(np.int32)
+
+
+def run_chunk(ctx, ref, news, slots=None, layer=1, max_new=None, max_len=None, res=None, tokens=None, begins=None, seed=3, c=None):
+    """The call on the device and in numpy: outputs have to agree, rows of nobody to stay.  The bf16 outputs."""
+    begins = begins_of(news) if begins is None else np.asarray(begins, np.int32)
+    tokens = int(begins.max()) if tokens is None else tokens
+    batch = len(begins) - 1
+    max_new = max_new or max(1, int(np.diff(begins).max()))
+    max_len = max_len or max(1, int(ref.lens.max()))
+    q, gamma = queries(np.random.default_rng(seed), tokens)
+    cos, sin = rope(max_len)
+    c = upload(ctx, ref) if c is None else c
+    out = ctx.upload(np.full((tokens, 16, 256), FILL, np.uint16))
+    print(f"case: chunk lens={ref.lens[:8]} begins={begins[:9]} slots={slots} max_new={max_new} max_len={max_len}", flush=True)
+    ctx.gqa_chunk_kv4(c, layer, batch, None if slots is None else ints(ctx, slots), ints(ctx, begins), tokens, max_new,
+                      ctx.upload(q), ctx.upload(gamma.view(np.uint16)), ctx.upload(cos), ctx.upload(sin), len(cos), max_len,
+                      None if res is None else ints(ctx, [res]), out)
+    got = ctx.download(out, (tokens, 16, 256), np.uint16)
+    want, bound, touched = CR.attend(ref, layer, batch, slots, begins, tokens, max_new, CR.bf16_value(q), gamma, cos, sin, max_len)
+    if res:
+        want[touched] = 0
+    assert (got[~touched] == FILL).all()
+    assert_near(CR.bf16_value(got[touched]), want[touched], bound[touched])
+    return got
+
+
+def assert_near(got, want, bound):
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    got, want, bound = got[fine].astype(np.float64), want[fine], bound[fine]
+    if not want.size:
+        return
+    off = np.abs(got - want)
+    room = bound + 2.0 ** -8 * (np.abs(want) + bound)
+    assert (off <= room).all(), (off - room).max()
+    assert np.linalg.norm(off) <= 3e-3 * np.linalg.norm(want)
+
+
+# ---- appending -------------------------------------------------------------------------------
+def run_append(ctx, ref, news, slots=None, layer=1, dtype="f32", max_len=None, res=None, begins=None, tokens=None, seed=5, k=None, v=None):
+    begins = begins_of(news) if begins is None else np.asarray(begins, np.int32)
+    tokens = int(begins.max()) if tokens is None else tokens
+    max_len = max_len or max(1, int(ref.lens.max()))
+    rng = np.random.default_rng(seed)
+    k = rng.standard_normal((tokens, 4, 256)) * (1 + np.abs(rng.standard_normal(256))) if k is None else k
+    v = 0.7 * rng.standard_normal((tokens, 4, 256)) if v is None else v
+    gamma = (0.1 * rng.standard_normal(256)).astype(np.float16)
+    cos, sin = rope(max_len)
+    with np.errstate(over="ignore"):
+        k, v = (CR.bf16(x) if dtype == "bf16" else x.astype(np.float32) for x in (k, v))
+    c = upload(ctx, ref)
+    print(f"case: append {dtype} lens={ref.lens[:8]} begins={begins[:9]} slots={slots}", flush=True)
+    ctx.kv4_append(c, layer, len(begins) - 1, None if slots is None else ints(ctx, slots), ints(ctx, begins), tokens, ctx.upload(k),
+                   ctx.upload(v), ctx.upload(gamma.view(np.uint16)), ctx.upload(cos), ctx.upload(sin), len(cos), max_len,
+                   None if res is None else ints(ctx, [res]), dtype=M.QM_BF16 if dtype == "bf16" else M.QM_F32)
+    if not res:
+        values = [CR.bf16_value(x) if dtype == "bf16" else x for x in (k, v)]
+        CR.append(ref, layer, len(begins) - 1, slots, begins, tokens, *values, gamma, cos, sin, max_len)
+    assert_same(ctx, c, ref)
+    return c, k, v, gamma
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens, news", [
+    ([1], [1]), ([31], [31]), ([32], [1]), ([33], [2]), ([64], [64]), ([65], [1]), ([97], [34]), ([130], [66]), ([100, 40, 7], [33, 40, 1]),
+    ([64, 1, 200, 65], [2, 1, 37, 64])])
+def test_append(ctx, lens, news, dtype):
+    """Every byte of the pool is the reference's: the new tokens', and the others of their words and pages."""
+    run_append(ctx, cache_of(lens, seed=len(lens) + sum(news)), news, dtype=dtype)
+
+
+def test_append_slots_and_rows_without_tokens(ctx):
+    """Slots out of order; a batch row of no tokens, one outside the table, one that an earlier batch row has."""
+    ref = cache_of([40, 70, 130, 9, 64], seed=8)
+    run_append(ctx, ref, [5, 0, 7, 20, 3, 2], slots=[3, 1, 9, 2, 0, 2])
+
+
+def test_append_of_more_rows_than_a_wave(ctx):
+    rng = np.random.default_rng(9)
+    lens = rng.integers(1, 80, 150).tolist()
+    news = [int(rng.integers(0, n + 1)) for n in lens]
+    run_append(ctx, cache_of(lens, layers=1, seed=9), news, layer=0, slots=rng.permutation(150))
+
+
+def test_append_refused_rows_and_lists(ctx):
+    """More new tokens than the length, a length over max_len, ranges that are none: passed over; the others written."""
+    ref = cache_of([10, 90, 20, 30], seed=10)
+    run_append(ctx, ref, [11, 3, 5, 6], max_len=64)
+    ref = cache_of([10, 90, 20, 30], seed=11)
+    run_append(ctx, ref, None, begins=[-1, 4, 4, 9, 200], tokens=12)
+
+
+def test_append_after_a_refused_resize_writes_nothing(ctx):
+    run_append(ctx, cache_of([10, 90], seed=12), [4, 9], res=3)
+
+
+def test_append_leaves_pages_of_others_alone(ctx):
+    """Pages that two rows hold, that by refs none does, and entries that are no page."""
+    ref = cache_of([200, 128, 190, 70], seed=13)
+    ref.table[1, 0] = ref.table[0, 1]
+    ref.refs[ref.table[0, 1]] = 2
+    ref.refs[ref.table[2, 1]] = 0
+    ref.table[3, 0] = len(ref.refs)
+    run_append(ctx, ref, [150, 100, 160, 70])
+
+
+def test_append_of_infinities_and_nan(ctx):
+    """A group with one reads back as NaN, the others as ever; the norm of a row with one is NaN or 0 as the formula's."""
+    rng = np.random.default_rng(14)
+    k, v = rng.standard_normal((2, 40, 4, 256))
+    v[3, 1, 70], v[9, 2, 5], v[11, 0, 255] = np.nan, np.inf, 1e30
+    k[5, 2, 100] = np.nan
+    ref = cache_of([70], seed=14)
+    run_append(ctx, ref, [40], k=k, v=v)
+
+
+@pytest.mark.parametrize("n", [1, 64, 65, 300])
+def test_append_is_what_the_decode_step_appends(ctx, n):
+    ref = cache_of([n], seed=15)
+    c, k, v, gamma = run_append(ctx, ref, [1], layer=1)
+    cos, sin = rope(n)
+    d = upload(ctx, ref)
+    ctx.memset(d.pages, 0, d.pages.nbytes)
+    ctx.copy(d.pages, c.pages, c.pages.nbytes)
+    q = np.random.default_rng(1).standard_normal((1, 16, 512)).astype(np.float32)
+    out = ctx.alloc(16 * 256 * 4)
+    ctx.gqa_decode_kv4(d, 1, 1, None, ctx.upload(q), ctx.upload(k), ctx.upload(v), ctx.upload(gamma.view(np.uint16)),
+                       ctx.upload(gamma.view(np.uint16)), ctx.upload(cos), ctx.upload(sin), len(cos), n, None, out)
+    assert_same(ctx, d, ref)
+
+
+# ---- attention ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("n, new", [
+    (1, 1), (2, 1), (31, 2), (32, 32), (33, 1), (63, 63), (64, 1), (64, 64), (65, 1), (65, 65), (66, 3), (96, 4), (127, 5), (128, 8), (129, 16),
+    (130, 17), (200, 31), (200, 33), (257, 100), (320, 256), (500, 129), (700, 1), (1000, 4)])
+def test_chunk_lengths(ctx, n, new):
+    run_chunk(ctx, cache_of([n], seed=n), [new])
+
+
+@pytest.mark.parametrize("lens, news", [
+    ([5, 70, 130], [5, 1, 64]), ([300, 1, 64, 65], [1, 1, 1, 1]), ([64, 200, 90, 33, 257], [3, 130, 90, 0, 16]), ([900, 40], [2, 40])])
+def test_chunk_batches(ctx, lens, news):
+    run_chunk(ctx, cache_of(lens, seed=sum(lens)), news)
+
+
+def test_chunk_slots(ctx):
+    """Slots out of order, outside the table, of an empty row, one slot twice; rows of nobody stay as they were."""
+    ref = cache_of([100, 0, 64, 150, 10], seed=21)
+    run_chunk(ctx, ref, None, slots=[3, -1, 1, 3, 0, 7], begins=[2, 22, 25, 30, 95, 100, 103], tokens=110)
+
+
+def test_chunk_refused_rows(ctx):
+    """More new tokens than max_new or than the length, a length over max_len: NaN; ranges that are none: nothing."""
+    ref = cache_of([10, 90, 20, 30, 60], seed=22)
+    run_chunk(ctx, ref, [11, 3, 20, 6, 70], max_len=64, max_new=19)
+    run_chunk(ctx, ref, None, begins=[-1, 4, 4, 9, 200, 3], tokens=12, max_new=9)
+    run_chunk(ctx, ref, [10, 4, 5, 6, 7], res=2)
+    run_chunk(ctx, ref, [10, 4, 5, 6, 7], res=-1)
+
+
+def test_chunk_of_more_rows_than_a_wave(ctx):
+    rng = np.random.default_rng(23)
+    lens = rng.integers(1, 90, 140).tolist()
+    news = [int(rng.integers(0, n + 1)) for n in lens]
+    run_chunk(ctx, cache_of(lens, layers=1, seed=23), news, layer=0, slots=rng.permutation(140))
+
+
+@pytest.mark.parametrize("n, new", [(6001, 70), (9000, 3), (5000, 300), (20011, 1), (20011, 64)])
+def test_chunk_of_long_rows(ctx, n, new):
+    """Row blocks whose pages fall to several workgroups."""
+    run_chunk(ctx, cache_of([n], layers=1, seed=n), [new], layer=0)
+
+
+def test_chunk_ragged_and_long(ctx):
+    run_chunk(ctx, cache_of([3000, 10, 700, 4097, 1], layers=1, seed=25), [65, 10, 300, 2, 1], layer=0, slots=[0, 1, 2, 3, 4])
+
+
+def test_chunk_over_shared_pages(ctx):
+    """Rows forked from one prompt, grown apart."""
+    ref = cache_of([150, 0, 0], seed=26, spare=12, room=100)
+    assert ref.fork([0, 0], [1, 2]) == 0 and ref.resize([0, 1, 2], [155, 190, 161]) == 0
+    rng = np.random.default_rng(27)
+    for r in range(3):
+        for j in range(2, R.pages_of(int(ref.lens[r]))):
+            fill_page(ref.pages[:, ref.table[r, j]], 64, rng)
+    run_chunk(ctx, ref, [5, 40, 11])
+
+
+def test_chunk_entries_that_are_no_page(ctx):
+    """Tokens in them are not seen; a query that sees no others gives 0."""
+    ref = cache_of([200, 70, 64], seed=28)
+    ref.table[0, 1], ref.table[1, 0], ref.table[2, 0] = len(ref.refs), -3, -1
+    run_chunk(ctx, ref, [100, 70, 64])
+
+
+@pytest.mark.parametrize("at", [0, 37, 63, 64, 90, 127, 128, 139])
+@pytest.mark.parametrize("is_v", [0, 1])
+def test_chunk_nan_reaches_those_that_see_it(ctx, at, is_v):
+    """A token's NaN group: queries before it are as without it, heads of the other kv heads too; V's only in its dims."""
+    ref = cache_of([140], seed=29)
+    half = ref.pages[1, ref.table[0, at // 64]][R.HEAD_BYTES * 2 + at % 64 // 32 * R.HALF_BYTES:][:R.HALF_BYTES]
+    meta = half[8192:].view(np.float16)
+    meta[256 * is_v + R.S_AT[at % 32, 1]] = meta[256 * is_v + 128 + R.LO_AT[at % 32, 1]] = np.nan
+    got = CR.bf16_value(run_chunk(ctx, ref, [100]))
+    first = max(0, at - 40)
+    assert not np.isnan(got[:first]).any() and np.isnan(got[first:, 8:12, 64:128]).all()
+
+
+def test_chunk_values_at_the_edges_of_f16(ctx):
+    """Groups that reach to f16's largest values stay finite: what passes 65504 is 65504."""
+    ref = cache_of([100], seed=30)
+    meta = ref.pages[1, ref.table[0, 0]][R.HEAD_BYTES:][:R.HALF_BYTES][8192:].view(np.float16)
+    meta[256 + R.S_AT[7]], meta[256 + 128 + R.LO_AT[7]] = np.float16(8736), np.float16(-65504)       # lo + 15 s = 65536
+    meta[256 + R.S_AT[9]], meta[256 + 128 + R.LO_AT[9]] = np.float16(6e-8), np.float16(1e-7)
+    run_chunk(ctx, ref, [60])
+
+
+@pytest.mark.parametrize("n", [1, 40, 257, 1500])
+def test_one_token_is_the_decode_steps(ctx, n):
+    """The step appends and attends in f32; the call over what it appended gives the same, rounded."""
+    ref = cache_of([n], seed=31)
+    rng = np.random.default_rng(32)
+    q, gamma = queries(rng, 1)
+    k, v = rng.standard_normal((2, 1, 4, 256)).astype(np.float32)
+    cos, sin = rope(n)
+    c = upload(ctx, ref)
+    out = ctx.alloc(16 * 256 * 4)
+    norm, qf = ctx.upload(gamma.view(np.uint16)), ctx.upload(CR.bf16_value(q))
+    rc, rs = ctx.upload(cos), ctx.upload(sin)
+    ctx.gqa_decode_kv4(c, 1, 1, None, qf, ctx.upload(k), ctx.upload(v), norm, norm, rc, rs, len(cos), n, None, out)
+    want = ctx.download(out, (1, 16, 256), np.float32)
+    CR.append(ref, 1, 1, None, [0, 1], 1, k, v, gamma, cos, sin, n)
+    assert_same(ctx, c, ref)
+    out16 = ctx.alloc(16 * 256 * 2)
+    ctx.gqa_chunk_kv4(c, 1, 1, None, ints(ctx, [0, 1]), 1, 1, ctx.upload(q), norm, rc, rs, len(cos), n, None, out16)
+    _, bound, _ = CR.attend(ref, 1, 1, None, [0, 1], 1, 1, CR.bf16_value(q), gamma, cos, sin, n)
+    assert_near(CR.bf16_value(ctx.download(out16, (1, 16, 256), np.uint16)), want.astype(np.float64), bound + 2e-5 * np.abs(want).max())
+
+
+# ---- together, captured, elsewhere ------------------------------------------------------------
+def test_prompts_in_parts_in_a_graph(ctx):
+    """Grow, append, attend, captured once and replayed as the rows' lists change; every replay as the eager call."""
+    rng = np.random.default_rng(40)
+    rows, tokens = 3, 96
+    ref = R.Cache(1, 40, rows, 8, seed=41)
+    steps = [([40, 0, 7], None), ([1, 64, 31], [2, 0, 1]), ([30, 30, 36], None), ([0, 0, 90], None), ([1, 1, 1], [1, 2, 0])]
+    cos, sin = rope(512)
+    gamma = (0.1 * rng.standard_normal(256)).astype(np.float16)
+    own = M.Context(0)
+    own.reserve(rows, 512, tokens)
+    c = upload(own, ref)
+    bufs = {key: own.alloc(size) for key, size in (("q", tokens * 16384), ("k", tokens * 2048), ("v", tokens * 2048),
+                                                    ("out", tokens * 8192), ("begins", 16), ("slots", 16), ("add", 16), ("res", 16))}
+    norm, rc, rs = own.upload(gamma.view(np.uint16)), own.upload(cos), own.upload(sin)
+
+    def enqueue():
+        own.kv4_resize(c, rows, bufs["slots"], bufs["add"], bufs["res"], M.QM_KV4_ADD)
+        own.kv4_append(c, 0, rows, bufs["slots"], bufs["begins"], tokens, bufs["k"], bufs["v"], norm, rc, rs, 512, 512, bufs["res"],
+                       dtype=M.QM_BF16)
+        own.gqa_chunk_kv4(c, 0, rows, bufs["slots"], bufs["begins"], tokens, tokens, bufs["q"], norm, rc, rs, 512, 512, bufs["res"],
+                          bufs["out"])
+
+    own.graph_begin()
+    enqueue()
+    graph = own.graph_end()
+    for i, (news, slots) in enumerate(steps):
+        slots = slots or list(range(rows))
+        begins = begins_of(news)
+        q = CR.bf16(rng.standard_normal((tokens, 16, 512)))
+        k, v = (CR.bf16(rng.standard_normal((tokens, 4, 256))) for _ in range(2))
+        for key, arr in (("q", q), ("k", k), ("v", v), ("begins", begins), ("slots", np.asarray(slots, np.int32)),
+                         ("add", np.asarray(news, np.int32)), ("out", np.full((tokens, 16, 256), FILL, np.uint16))):
+            own.upload(arr, bufs[key])
+        print(f"case: graph step {i}", flush=True)
+        if i == 2:
+            enqueue()                                                   # eager in between
+        else:
+            graph.launch()
+        assert result(own, bufs["res"]) == ref.resize(slots, news, add=True) == 0
+        CR.append(ref, 0, rows, slots, begins, tokens, CR.bf16_value(k), CR.bf16_value(v), gamma, cos, sin, 512)
+        assert_same(own, c, ref)
+        want, bound, touched = CR.attend(ref, 0, rows, slots, begins, tokens, tokens, CR.bf16_value(q), gamma, cos, sin, 512)
+        got = own.download(bufs["out"], (tokens, 16, 256), np.uint16)
+        assert (got[~touched] == FILL).all()
+        assert_near(CR.bf16_value(got[touched]), want[touched], bound[touched])
+    graph.close()
+    own.close()
+
+
+def test_a_chunk_that_would_grow_the_workspace_under_capture_is_refused():
+    own = M.Context(0)
+    ref = cache_of([3000], layers=1, seed=42)
+    c = upload(own, ref)
+    z = own.alloc(70 * 16384)
+    begins = ints(own, [0, 70])
+    own.graph_begin()
+    with pytest.raises(M.MixerError) as e:
+        own.gqa_chunk_kv4(c, 0, 1, None, begins, 70, 70, z, z, z, z, 3000, 3000, None, z)
+    assert e.value.code == 9
+    own.graph_end().close()
+    own.close()
+
+
+def test_chunk_on_a_stream_of_the_callers(ctx):
+    import ctypes
+    s = ctypes.c_void_p(0)
+    ctx._check(ctx.lib.qm_stream_create(ctx.h, ctypes.byref(s)))
+    before, ctx.stream = ctx.stream, s.value
+    try:
+        ref = cache_of([333], seed=43)
+        run_append(ctx, ref, [90], dtype="bf16")
+        run_chunk(ctx, ref, [90])
+    finally:
+        ctx.sync()
+        ctx.stream = before
+        ctx._check(ctx.lib.qm_stream_destroy(ctx.h, s))
+
+
+def test_a_chunk_twice_gives_the_same_bits(ctx):
+    ref = cache_of([2500, 80], layers=1, seed=44)
+    a = run_chunk(ctx, ref, [130, 80], layer=0)
+    b = run_chunk(ctx, ref, [130, 80], layer=0)
+    assert np.array_equal(a, b)
