@@ -443,9 +443,9 @@ int32_t qm_kv4_append(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cac
  * softmax(q K^T / 16) V of a token at position pos over the cached tokens
  * 0 .. pos of its row, q RMSNorm'd and rotated, kv head h / 4, times
  * sigmoid(gate): qm_gqa_prefill's attention, behind any context.  K and V are
- * what the pages stand for, in f16 (f16's largest value where that is past it);
- * q and the softmax's weights enter the products in f16, sums are f32, as in
- * qm_gqa_prefill.  A token that stands in a group of NaN does so for the
+ * what the pages stand for, in f16 (a scale whose rounding takes its group past
+ * f16's largest value counts as the next lower one); q and the softmax's
+ * weights enter the products in f16, sums are f32, as in qm_gqa_prefill.  A token that stands in a group of NaN does so for the
  * queries that see it only.
  * q_gate_dev   bf16 [tokens][16][512]; q_norm_dev f16 [256]
  * out_dev      bf16 [tokens][16][256]; rows of no batch row stay as they were

@@ -32,7 +32,6 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 #define CHUNK_WAVES 8
 #define CHUNK_COLS 2                   // operand columns (of 16 rows) a wave
-#define CHUNK_MIN_TILES 4              // pages of a row block that are worth a workgroup
 // A row's reference maximum moves only where a score passes it by this (log2
 // units): p <= 2^8 is exact enough in f16, and outputs are seldom rescaled.
 #define CHUNK_SLACK 8.0f
@@ -40,8 +39,8 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 // ---- how the work is dealt --------------------------------------------------
 // A batch row of the call.  A row that has no tokens to read (its slot is
 // outside the table, or empty) or is refused (longer than max_len, more new
-// tokens than max_new or than its length) takes one unit a block, in which its
-// outputs, 0 or NaN, are written.
+// tokens than max_new or than its length) takes one page's units a block, in
+// which its outputs, 0 or NaN, are written.
 enum { CHUNK_RUN = 0, CHUNK_NONE = 1, CHUNK_REFUSED = 2 };
 struct ChunkRow {
     int row, len, n, begin, kind;
@@ -49,11 +48,10 @@ struct ChunkRow {
 QM_DEV ChunkRow chunk_row(const GqaChunkArgs& A, int b) {
     ChunkRow r{0, 0, 0, 0, CHUNK_NONE};
     if (b >= A.batch) return r;
-    const int begin = A.begins[b], end = A.begins[b + 1];
+    const int begin = A.begins[b], end = A.begins[b + 1], row = A.slots ? A.slots[b] : b;
     if (begin < 0 || end < begin || end > A.tokens) return r;
     r.begin = begin;
     r.n = end - begin;
-    const int row = A.slots ? A.slots[b] : b;
     if ((A.result && A.result[0] != 0) || (uint32_t)row >= (uint32_t)A.c.rows) return r;
     r.row = row;
     r.len = A.c.lens[row];
@@ -61,94 +59,141 @@ QM_DEV ChunkRow chunk_row(const GqaChunkArgs& A, int b) {
     r.kind = r.len > A.max_len || r.n > A.max_new || r.n > r.len ? CHUNK_REFUSED : CHUNK_RUN;
     return r;
 }
-QM_DEV int chunk_blocks(const ChunkRow& r) { return (r.n + QMK_CHUNK_TOKENS - 1) / QMK_CHUNK_TOKENS; }
-// Pages that block j reads, and that the blocks before it do: a block but the
-// row's last one ends 64 j + 63 tokens after the row's first new one.
-QM_DEV int chunk_tiles(const ChunkRow& r, int j) {
-    if (r.kind != CHUNK_RUN) return 1;
-    return (r.len - r.n + min(r.n, QMK_CHUNK_TOKENS * (j + 1)) - 1) / QMK_KV4_PAGE_TOKENS + 1;
-}
-QM_DEV uint64_t chunk_before(const ChunkRow& r, int j) {
-    if (r.kind != CHUNK_RUN) return j;
-    const uint64_t first = (r.len - r.n + 63) / QMK_KV4_PAGE_TOKENS + 1;
-    return j * first + (uint64_t)j * (j - 1) / 2;
-}
-QM_DEV uint64_t chunk_units(const ChunkRow& r) {
-    const int nb = chunk_blocks(r);
-    return nb ? chunk_before(r, nb - 1) + chunk_tiles(r, nb - 1) : 0;
-}
-QM_DEV uint64_t shfl64(uint64_t x, int lane) {
-    const uint32_t lo = __shfl((int)(uint32_t)x, lane), hi = __shfl((int)(uint32_t)(x >> 32), lane);
-    return (uint64_t)hi << 32 | lo;
-}
-QM_DEV uint64_t scan64(uint64_t x, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t y = shfl64(x, lane - d);
-        x += lane >= d ? y : 0;
-    }
-    return x;
-}
-QM_DEV uint64_t uniform64(uint64_t x) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32 |
-           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
-}
-QM_DEV ChunkRow uniform_row(const ChunkRow& r, int lane) {
-    return ChunkRow{__builtin_amdgcn_readlane(r.row, lane), __builtin_amdgcn_readlane(r.len, lane),
-                    __builtin_amdgcn_readlane(r.n, lane), __builtin_amdgcn_readlane(r.begin, lane),
-                    __builtin_amdgcn_readlane(r.kind, lane)};
-}
 
-// A row block: its row, number, pages, and the units before it.
-struct ChunkItem {
-    ChunkRow r;
-    int block, tiles;
-    uint64_t first;
-};
-// All units of a kv head, and (all lanes agree) units a workgroup.
-QM_DEV uint64_t chunk_total(const GqaChunkArgs& A, int lane) {
-    uint64_t all = 0;
-    for (int b0 = 0; b0 < A.batch; b0 += 64) all += chunk_units(chunk_row(A, b0 + lane));      // uniform
-    return uniform64(shfl64(scan64(all, lane), 63));
-}
-QM_DEV uint64_t chunk_share(uint64_t total, int groups) {
-    const uint64_t each = (total + groups - 1) / groups;
-    return each < CHUNK_MIN_TILES ? CHUNK_MIN_TILES : each;
-}
-// The row block that unit u falls into (u < total), or block number `at` of
-// all row blocks where `by_block`; false: there is none.
-template <bool BY_BLOCK>
-QM_DEV bool chunk_find(const GqaChunkArgs& A, uint64_t u, int lane, ChunkItem& it) {
-    uint64_t units = 0, keys = 0;
-    for (int b0 = 0; b0 < A.batch; b0 += 64) {             // uniform
-        const ChunkRow mine = chunk_row(A, b0 + lane);
-        const uint64_t n = chunk_units(mine), incl = scan64(n, lane);
-        const uint64_t kn = BY_BLOCK ? (uint64_t)chunk_blocks(mine) : n, kincl = BY_BLOCK ? scan64(kn, lane) : incl;
-        const uint64_t all = uniform64(shfl64(kincl, 63));
-        if (u < keys + all) {
-            const int at = __popcll(__ballot(keys + kincl <= u));
-            it.r = uniform_row(mine, at);
-            const uint64_t rest = u - keys - uniform64(shfl64(kincl - kn, at));
-            int j = (int)rest;
-            if (!BY_BLOCK) {                               // the last block that begins at or before `rest`
-                int lo = 0, hi = chunk_blocks(it.r) - 1;
-                while (lo < hi) {
-                    const int mid = lo + (hi - lo + 1) / 2;
-                    if (chunk_before(it.r, mid) <= rest) lo = mid;
-                    else hi = mid - 1;
-                }
-                j = lo;
-            }
-            it.block = j;
-            it.tiles = chunk_tiles(it.r, j);
-            it.first = units + uniform64(shfl64(incl - n, at)) + chunk_before(it.r, j);
-            return true;
-        }
-        units += uniform64(shfl64(incl, 63));
-        keys += all;
+// NF: operand columns of a row block of few tokens (4 NF tokens of four heads).
+template <int NF>
+struct Deal {
+    static constexpr int kFew = 4 * NF;
+    const GqaChunkArgs& A;
+    const int lane;
+    double total;                      // units of a kv head
+    double each;                       // of a workgroup
+    ChunkRow mine;                     // batch row `lane`, if there are no more than 64
+    double incl, units;
+
+    QM_DEV static bool few(const ChunkRow& r) { return r.n <= QMK_CHUNK_FEW; }
+    QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
+    QM_DEV static int blocks(const ChunkRow& r) { return (r.n + tokens(r) - 1) / tokens(r); }
+    QM_DEV static int weight(const ChunkRow& r) { return few(r) ? 1 : QMK_CHUNK_WEIGHT; }
+    // Pages that block j reads, and that the blocks before it do.
+    QM_DEV static int tiles(const ChunkRow& r, int j) {
+        if (r.kind != CHUNK_RUN) return 1;
+        return (r.len - r.n + min(r.n, tokens(r) * (j + 1)) - 1) / QMK_KV4_PAGE_TOKENS + 1;
     }
-    return false;
-}
+    QM_DEV static double before(const ChunkRow& r, int j) {
+        if (r.kind != CHUNK_RUN) return j;
+        if (!few(r)) {                 // block j, but the row's last, ends 64 j + 63 tokens after the first new one
+            const double first = (r.len - r.n + 63) / QMK_KV4_PAGE_TOKENS + 1;
+            return j * first + (double)j * (j - 1) * 0.5;
+        }
+        int sum = 0;
+        for (int i = 0; i < j; ++i) sum += tiles(r, i);    // a few blocks of at most 2^25 pages
+        return sum;
+    }
+    QM_DEV static double row_units(const ChunkRow& r) {
+        const int nb = blocks(r);
+        return nb ? weight(r) * (before(r, nb - 1) + tiles(r, nb - 1)) : 0.0;
+    }
+    template <int CTRL, int ROWS>
+    QM_DEV static double step(double x) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+        return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    }
+    // Inclusive sum over the lanes, of whole numbers below 2^53.
+    QM_DEV static double scan(double x) {
+        x = step<0x111, 0xF>(x);
+        x = step<0x112, 0xF>(x);
+        x = step<0x114, 0xF>(x);
+        x = step<0x118, 0xF>(x);
+        x = step<0x142, 0xA>(x);
+        return step<0x143, 0xC>(x);
+    }
+    QM_DEV static double lane_of(double x, int lane) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+        return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    }
+    QM_DEV static ChunkRow lane_of(const ChunkRow& r, int lane) {
+        return ChunkRow{__builtin_amdgcn_readlane(r.row, lane), __builtin_amdgcn_readlane(r.len, lane),
+                        __builtin_amdgcn_readlane(r.n, lane), __builtin_amdgcn_readlane(r.begin, lane),
+                        __builtin_amdgcn_readlane(r.kind, lane)};
+    }
+
+    QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), total(0.0) {
+        for (int b0 = 0; b0 < A.batch; b0 += 64) {         // uniform
+            mine = chunk_row(A, b0 + lane);
+            units = row_units(mine);
+            incl = scan(units);
+            total += lane_of(incl, 63);
+        }
+        each = fmax(ceil(total / A.groups), (double)QMK_CHUNK_MIN_UNITS);
+    }
+
+    // A row block: its row, number among the row's, pages, the units before it,
+    // and its number among the blocks of few tokens, or of many.
+    struct Item {
+        ChunkRow r;
+        int block, tiles, number;
+        double first;
+    };
+    // The row block that unit u (< total) falls into.
+    QM_DEV Item find(double u, bool numbered) const {
+        Item it;
+        double past = 0.0;
+        int number[2] = {0, 0};
+        ChunkRow r = mine;
+        double n = units, in = incl;
+        for (int b0 = 0;; b0 += 64) {                      // uniform
+            if (A.batch > 64) {
+                r = chunk_row(A, b0 + lane);
+                n = row_units(r);
+                in = scan(n);
+            }
+            const double all = lane_of(in, 63);
+            const bool here = u < past + all;
+            const int at = here ? __popcll(__ballot(past + in <= u)) : 64;
+            if (numbered) {
+                const int nb = lane < at ? blocks(r) : 0;
+                const bool f = few(r);
+                number[0] += __builtin_amdgcn_readlane((int)wave_scan(f ? 0u : (uint32_t)nb), 63);
+                number[1] += __builtin_amdgcn_readlane((int)wave_scan(f ? (uint32_t)nb : 0u), 63);
+            }
+            if (here || b0 + 64 >= A.batch) {              // (u < total: here)
+                it.r = lane_of(r, at);
+                it.first = past + lane_of(in - n, at);
+                break;
+            }
+            past += all;
+        }
+        // the last block that begins at or before u
+        const int w = weight(it.r);
+        const double rest = u - it.first;
+        int lo = 0, hi = blocks(it.r) - 1;
+        while (lo < hi) {
+            const int mid = lo + (hi - lo + 1) / 2;
+            if (before(it.r, mid) * w <= rest) lo = mid;
+            else hi = mid - 1;
+        }
+        it.block = __builtin_amdgcn_readfirstlane(lo);
+        it.tiles = __builtin_amdgcn_readfirstlane(tiles(it.r, it.block));
+        it.first = lane_of(it.first + before(it.r, it.block) * w, 0);
+        it.number = number[few(it.r)] + it.block;
+        return it;
+    }
+    // Where workgroup i begins: a multiple of `each`, but whole pages, and none
+    // inside a block of few pages.
+    QM_DEV double begin(int i) const {
+        const double u = each * i;
+        if (u >= total) return total;
+        const Item it = find(u, false);
+        const int w = weight(it.r);
+        int t = (int)((u - it.first) / w);
+        if (it.tiles <= QMK_CHUNK_WHOLE) t = 2 * (u - it.first) < (double)it.tiles * w ? 0 : it.tiles;
+        return it.first + (double)t * w;
+    }
+};
 
 // ---- a tile -------------------------------------------------------------------
 // LDS: two buffers of f16 operands, block entry l the 16 bytes that lane
@@ -201,47 +246,78 @@ QM_DEV half8 chunk_values(uint32_t word, const half2_t (&s)[4], const half2_t (&
     return out;
 }
 
-// The same where a group may be NaN, or its largest values past f16's: those
-// are f16's largest, and NaN is `nan`.
-QM_DEV half8 chunk_values_odd(uint32_t word, const half2_t (&s)[4], const half2_t (&lo)[4], _Float16 nan) {
-    half8 x = chunk_values(word, s, lo);
+// V of the half page's tokens from `left` on is 0, whatever stands there.
+QM_DEV void chunk_cut(half2_t (&s)[4], half2_t (&lo)[4], int left, int g) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float y = (float)x[e];
-        x[e] = y != y ? nan : (_Float16)fminf(fmaxf(y, -65504.0f), 65504.0f);
-    }
-    return x;
+    for (int e = 0; e < 8; ++e)
+        if (chunk_token(e >> 2, g, e & 3) >= left) s[e >> 1][e & 1] = lo[e >> 1][e & 1] = (_Float16)0.0f;
 }
-// Whether a group's largest value, lo + 15 s, is finite (lo is where s is).
-QM_DEV bool chunk_odd(half2_t s, half2_t lo) {
-    const half2_t fifteen = {(_Float16)15.0f, (_Float16)15.0f};
-    const uint32_t top = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(fifteen, s, lo));
-    return (top & 0x7c00u) == 0x7c00u || (top & 0x7c000000u) == 0x7c000000u;
+
+// Whether some of a half page's scales or minima (at `meta`) are NaN, or so
+// large that its values may not be finite (2^10 and 2^14: lo + 15 s is under
+// 2^15).
+QM_DEV bool chunk_odd(const uint8_t* meta, int lane) {
+    const uint32_t* m = reinterpret_cast<const uint32_t*>(meta) + lane;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = m[64 * i] & 0x7c007c00u, most = i & 1 ? 0x7400u : 0x6400u;
+        odd = odd || (x & 0xffffu) >= most || x >= most << 16;
+    }
+    return __any(odd);
+}
+// Puts such a half page right, in LDS.  A scale that takes the group past
+// f16's largest value becomes the next lower one.  V that is NaN becomes 0, and
+// its tokens (a bit each) are returned, a word per group: the rows that see
+// them are given the NaN beside the product, as a weight of 0 times it would
+// give it to the others too.
+QM_DEV uintx4 chunk_mend(uint8_t* meta, int lane) {
+    uintx4 nan = {0, 0, 0, 0};
+#pragma unroll
+    for (int is_v = 0; is_v < 2; ++is_v)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int t = 16 * k + (lane >> 2), group = lane & 3;
+            uint16_t* s = reinterpret_cast<uint16_t*>(meta + 512 * is_v) + kv4_s_at(t, group);
+            uint16_t* lo = reinterpret_cast<uint16_t*>(meta + 512 * is_v + 256) + kv4_lo_at(t, group);
+            const float fs = f16_to_f32(*s), fl = f16_to_f32(*lo), top = fmaf(15.0f, fs, fl);
+            const bool bad = top != top;
+            if (top >= 65520.0f) *s = *s - 1;
+            if (bad && is_v) *s = *lo = 0;
+            const uint64_t lanes = __ballot(bad && is_v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) nan[q] |= (uint32_t)(lanes >> (4 * j + q) & 1) << (16 * k + j);
+        }
+    asm volatile("" ::: "memory");                         // read again as other types
+    return nan;
 }
 
 // The wave's part of a tile of which `left` tokens are the row's (64 and more:
-// all), from its codes into buffer `buf`.  V of the others is 0, and V that is
-// NaN too, which the rows that see it are given beside the product: a weight
-// of 0 times it would give it to the others.
+// all; V of the others is 0), from its codes into buffer `buf`.
 QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
     const uint8_t* raw = sh.raw[w][0];
-    const uint8_t* meta = sh.raw[w][2];
+    uint8_t* meta = sh.raw[w][2];
     const int half = w >> 2, i = w & 3, c = lane & 15, g = lane >> 4;
     const int run = i >> 1, dims = i & 1;
+    uint32_t nan = 0;
+    if (chunk_odd(meta, lane)) {
+        const uintx4 all = chunk_mend(meta, lane);
+        nan = i < 2 ? (i == 0 ? all[0] : all[1]) : i == 2 ? all[2] : all[3];
+    }
+    if (lane == 0) sh.nan[buf][half][i] = nan;
     {
         const uintx4 k = *reinterpret_cast<const uintx4*>(raw + 16 * lane);
         const half2_t s = as_half2(*reinterpret_cast<const uint32_t*>(meta + 2 * kv4_s_at(16 * run + c, 2 * dims)));
         const half2_t lo = {*reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims)),
                             *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims + 1))};
-        const bool odd = __any(chunk_odd(s, lo));
         uint8_t* to = sh.tile[buf] + (8 * (2 * half + run) + 4 * dims) * 1024 + 16 * lane;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const half2_t s2 = {s[m >> 1], s[m >> 1]}, l2 = {lo[m >> 1], lo[m >> 1]};
             const half2_t ss[4] = {s2, s2, s2, s2}, ll[4] = {l2, l2, l2, l2};
-            half8 x = chunk_values(k[m], ss, ll);
-            if (odd) x = chunk_values_odd(k[m], ss, ll, (_Float16)__builtin_nanf(""));
-            *reinterpret_cast<half8*>(to + 1024 * m) = x;
+            *reinterpret_cast<half8*>(to + 1024 * m) = chunk_values(k[m], ss, ll);
         }
     }
     {
@@ -253,32 +329,10 @@ QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
             s[e >> 1][e & 1] = *reinterpret_cast<const _Float16*>(meta + 512 + 2 * (g * 32 + (e >> 2) * 16 + (e & 3) * 4 + i));
 #pragma unroll
         for (int n = 0; n < 4; ++n) lo[n] = as_half2(lo4[n]);
-        if (left < QMK_KV4_PAGE_TOKENS) {                  // uniform
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (32 * half + chunk_token(e >> 2, g, e & 3) >= left) s[e >> 1][e & 1] = lo[e >> 1][e & 1] = (_Float16)0.0f;
-        }
-        bool odd = false;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) odd = odd || chunk_odd(s[n], lo[n]);
-        odd = __any(odd);
-        uint32_t nan = 0;
-        if (odd) {                                         // uniform
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint64_t lanes = __ballot(s[e >> 1][e & 1] != s[e >> 1][e & 1]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) nan |= (uint32_t)(lanes >> (16 * q) & 1) << chunk_token(e >> 2, q, e & 3);
-            }
-        }
-        if (lane == 0) sh.nan[buf][half][i] = nan;
+        if (left < QMK_KV4_PAGE_TOKENS) chunk_cut(s, lo, left - 32 * half, g);      // uniform
         uint8_t* to = sh.tile[buf] + 32768 + (8 * i + half) * 1024 + 16 * lane;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            half8 x = chunk_values(v[m], s, lo);
-            if (odd) x = chunk_values_odd(v[m], s, lo, (_Float16)0.0f);
-            *reinterpret_cast<half8*>(to + 2048 * m) = x;
-        }
+        for (int m = 0; m < 4; ++m) *reinterpret_cast<half8*>(to + 2048 * m) = chunk_values(v[m], s, lo);
     }
 }
 
@@ -305,62 +359,98 @@ QM_DEV void unpack8(uint4 v, float (&x)[8]) {
     }
 }
 
-// The rows' queries: RMSNorm (1 + gamma, eps 1e-6) and RoPE straight into the
-// operand; a row's sum of squares is over the four lanes c + 16 g, and the
-// pairs (i, i + 32) of a rotation are in one lane.
-QM_DEV void chunk_query(const GqaChunkArgs& A, ChunkWave& st, const ChunkItem& it, int head, int w, int lane) {
-    const int c = lane & 15, g = lane >> 4;
+// A column's query, token i of row r: RMSNorm (1 + gamma, eps 1e-6) and RoPE
+// straight into the operand; a row's sum of squares is over the four lanes
+// c + 16 g, and the pairs (i, i + 32) of a rotation are in one lane.
+QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[8], const ChunkRow& r, int i, int head, int g) {
+    const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + 8 * g;
+    const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 8 * g;
+    uint4 u[8], gq[8];
 #pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f) {
-        const int i = QMK_CHUNK_TOKENS * it.block + 16 * CHUNK_COLS * (w >> 2) + 16 * f + c;
-        const int have = min(i, it.r.n - 1);               // rows past the last: any row, never written
-        st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
-        const uint16_t* row = A.q_gate + ((size_t)(it.r.begin + have) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + 8 * g;
-        const size_t at = (size_t)(it.r.len - it.r.n + have) * (QM_GQA_ROT / 2) + 8 * g;
-        uint4 u[8], gq[8];
+    for (int s = 0; s < 8; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 32 * s);
 #pragma unroll
-        for (int s = 0; s < 8; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 32 * s);
+    for (int s = 0; s < 8; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 32 * s + 8 * g);
+    const float4 c0 = ld4(A.rope_cos + at), c1 = ld4(A.rope_cos + at + 4), s0 = ld4(A.rope_sin + at), s1 = ld4(A.rope_sin + at + 4);
+    float ss = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 32 * s + 8 * g);
-        const float4 c0 = ld4(A.rope_cos + at), c1 = ld4(A.rope_cos + at + 4), s0 = ld4(A.rope_sin + at), s1 = ld4(A.rope_sin + at + 4);
-        float ss = 0.0f;
+    for (int s = 0; s < 8; ++s) {
+        float x[8];
+        unpack8(u[s], x);
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            float x[8];
-            unpack8(u[s], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        }
-        ss = sum_xor32(sum_xor16(ss));
-        // the softmax's scale in base 2 as well, so that the scores come out of the product in log2 units
-        const float inv = (1.4426950408889634f / 16.0f) / sqrtf(ss / (float)QM_GQA_HD + 1e-6f);
-        auto normed = [&](int s, float (&x)[8]) {
-            unpack8(u[s], x);
-            const uint32_t gv[4] = {gq[s].x, gq[s].y, gq[s].z, gq[s].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[2 * e] = x[2 * e] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] & 0xffffu)));
-                x[2 * e + 1] = x[2 * e + 1] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] >> 16)));
-            }
-        };
-        float x1[8], x2[8];
-        normed(0, x1);
-        normed(1, x2);
-        const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            st.q[f][0][e] = (_Float16)(x1[e] * cs[e] - x2[e] * sn[e]);
-            st.q[f][1][e] = (_Float16)(x2[e] * cs[e] + x1[e] * sn[e]);
-        }
-#pragma unroll
-        for (int s = 2; s < 8; ++s) {
-            float x[8];
-            normed(s, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) st.q[f][s][e] = (_Float16)x[e];
-        }
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
     }
+    ss = sum_xor32(sum_xor16(ss));
+    // the softmax's scale in base 2 as well, so that the scores come out of the product in log2 units
+    const float inv = (1.4426950408889634f / 16.0f) / sqrtf(ss / (float)QM_GQA_HD + 1e-6f);
+    auto normed = [&](int s, float (&x)[8]) {
+        unpack8(u[s], x);
+        const uint32_t gv[4] = {gq[s].x, gq[s].y, gq[s].z, gq[s].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = x[2 * e] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] & 0xffffu)));
+            x[2 * e + 1] = x[2 * e + 1] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] >> 16)));
+        }
+    };
+    float x1[8], x2[8];
+    normed(0, x1);
+    normed(1, x2);
+    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        q[0][e] = (_Float16)(x1[e] * cs[e] - x2[e] * sn[e]);
+        q[1][e] = (_Float16)(x2[e] * cs[e] + x1[e] * sn[e]);
+    }
+#pragma unroll
+    for (int s = 2; s < 8; ++s) {
+        float x[8];
+        normed(s, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)x[e];
+    }
+}
+
+// The weights of a half page's scores (runs 0, 1), and what a new maximum does
+// to the row's sums.
+QM_DEV half8 chunk_weights(floatx4 (&x)[2], floatx4 (&o)[16], float& m, float& l, int pos, int k0, bool edge, int g) {
+    if (edge) {                                            // uniform: some row does not see all of it
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[r][e] = k0 + chunk_token(r, g, e) > pos ? -INFINITY : x[r][e];
+    }
+    float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    mx = max_xor32(max_xor16(mx));
+    const float was = m;
+    m = mx > was + CHUNK_SLACK ? mx : was;                 // from -inf: any score
+    if (__any(m != was)) {
+        // sums beside a maximum of -inf are those of NaN scores
+        const float corr = was == m ? 1.0f : __builtin_amdgcn_exp2f(was - m);
+        l *= corr;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) o[dt] *= corr;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;          // a row that sees nothing yet: weights of 0
+    half8 p;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const _Float16 w = (_Float16)__builtin_amdgcn_exp2f(x[r][e] - base);
+            p[4 * r + e] = w;
+            l += (float)w;                                 // of what is multiplied
+        }
+    return p;
+}
+// Values that are NaN, for a row that sees their tokens; nan[group]: the half
+// page's tokens.
+QM_DEV void chunk_nan(floatx4 (&o)[16], uintx4 nan, int pos, int k0) {
+    const int seen = pos - k0;                             // the last of them that the row sees
+    const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
+    const float bad = __builtin_nanf("");
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt)
+        if (nan[dt >> 2] & mask) o[dt] = floatx4{bad, bad, bad, bad};
 }
 
 // Half a tile (32 tokens from k0 on) at a time, so that outputs, queries and
@@ -384,35 +474,7 @@ QM_DEV void chunk_half(ChunkWave& st, const ChunkLds& sh, int buf, int h, int k0
         }
     half8 p[CHUNK_COLS];
 #pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f) {
-        if (edge) {                                        // uniform: some row does not see all of it
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[f][r][e] = k0 + chunk_token(r, g, e) > st.pos[f] ? -INFINITY : x[f][r][e];
-        }
-        float mx = fmaxf(fmaxf(fmaxf(x[f][0][0], x[f][0][1]), fmaxf(x[f][0][2], x[f][0][3])),
-                         fmaxf(fmaxf(x[f][1][0], x[f][1][1]), fmaxf(x[f][1][2], x[f][1][3])));
-        mx = max_xor32(max_xor16(mx));
-        const float was = st.m[f], m = mx > was + CHUNK_SLACK ? mx : was;      // from -inf: any score
-        if (__any(m != was)) {
-            // sums beside a maximum of -inf are those of NaN scores
-            const float corr = was == m ? 1.0f : __builtin_amdgcn_exp2f(was - m);
-            st.m[f] = m;
-            st.l[f] *= corr;
-#pragma unroll
-            for (int dt = 0; dt < 16; ++dt) st.o[f][dt] *= corr;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;      // a row that sees nothing yet: weights of 0
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const _Float16 w = (_Float16)__builtin_amdgcn_exp2f(x[f][r][e] - base);
-                p[f][4 * r + e] = w;
-                st.l[f] += (float)w;                       // of what is multiplied
-            }
-    }
+    for (int f = 0; f < CHUNK_COLS; ++f) p[f] = chunk_weights(x[f], st.o[f], st.m[f], st.l[f], st.pos[f], k0, edge, g);
 #pragma unroll
     for (int dt = 0; dt < 16; ++dt) {
         const half8 a = *reinterpret_cast<const half8*>(V + 2048 * dt);
@@ -422,13 +484,7 @@ QM_DEV void chunk_half(ChunkWave& st, const ChunkLds& sh, int buf, int h, int k0
     const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][h]);
     if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
 #pragma unroll
-        for (int f = 0; f < CHUNK_COLS; ++f) {
-            const int seen = st.pos[f] - k0;               // the last token of the half that the row sees
-            const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
-#pragma unroll
-            for (int dt = 0; dt < 16; ++dt)
-                if (nan[dt >> 2] & mask) st.o[f][dt] = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        }
+        for (int f = 0; f < CHUNK_COLS; ++f) chunk_nan(st.o[f], nan, st.pos[f], k0);
     }
 }
 QM_DEV void chunk_tile(ChunkWave& st, const ChunkLds& sh, int buf, int k0, int first_pos, int lane) {
@@ -447,104 +503,336 @@ QM_DEV void chunk_out(uint16_t* to, floatx4 o, float inv, uint2 gate) {
 }
 QM_DEV float chunk_inverse(float l) { return l != 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f; }      // 0: nothing to see
 
-extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_kv4(GqaChunkArgs A) {
-    __shared__ ChunkLds sh;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2, head = 4 * kvh + (w & 3);
-    const uint64_t total = chunk_total(A, lane), each = chunk_share(total, A.groups);
-    const uint64_t end = min(total, each * (index + 1));
-    for (uint64_t u = each * index; u < end;) {            // uniform, as all of it
-        ChunkItem it;
-        if (!chunk_find<false>(A, u, lane, it)) return;    // never: u < total
-        const int ta = (int)(u - it.first), tb = (int)min((uint64_t)it.tiles, end - it.first);
-        u += tb - ta;
-        const int i0 = QMK_CHUNK_TOKENS * it.block + 16 * CHUNK_COLS * (w >> 2);      // the wave's first row
-        if (it.r.kind != CHUNK_RUN) {
-            const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;
-            for (int i = i0; i < min(i0 + 16 * CHUNK_COLS, it.r.n); ++i)
-                *reinterpret_cast<uint2*>(A.out + ((size_t)(it.r.begin + i) * QM_GQA_HEADS + head) * QM_GQA_HD + 4 * lane) = make_uint2(fill, fill);
-            continue;
-        }
-        const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
-        auto page = [&](int t) { return t < tb ? __builtin_amdgcn_readfirstlane(table[t]) : -1; };
-        int now = page(ta), next = page(ta + 1), after = page(ta + 2);
-        if (kv4_is_page(A.c, now)) chunk_fetch(A, sh, now, kvh, w, lane);
-        ChunkWave st;
-        chunk_query(A, st, it, head, w, lane);
+// ---- few tokens ------------------------------------------------------------------
+// A row of up to QMK_CHUNK_FEW new tokens: blocks of 4 NF of them, an operand
+// column 4 tokens of the four heads.  Every wave has all columns and every
+// eighth half page, whose codes come by LDS DMA, two ahead, and become operands
+// in its registers; the waves' sums are joined at the end.
+struct FewLds {
+    __attribute__((aligned(1024))) uint8_t ring[CHUNK_WAVES][2][QMK_KV4_HALF_BYTES];      // later o: [dim group][lane][4] f32
+    float m[CHUNK_WAVES][16], l[CHUNK_WAVES][16];
+};
+template <int NF>
+struct FewWave {
+    half8 q[NF][8];
+    floatx4 o[NF][16];
+    float m[NF], l[NF];
+    int pos[NF];
+};
+#define FEW_DMA (QMK_KV4_HALF_BYTES / 1024)
+QM_DEV void few_fetch(const uint8_t* half, uint32_t buf, int lane) {
 #pragma unroll
-        for (int f = 0; f < CHUNK_COLS; ++f) {
-            st.m[f] = -INFINITY;
-            st.l[f] = 0.0f;
+    for (int i = 0; i < FEW_DMA; ++i) dma16_off(half + 1024 * i, 16 * lane, buf + 1024 * i);
+}
+// `left` tokens of the half page are the row's.
+template <int NF>
+QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, int k0, int left, bool edge, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    uint8_t* meta = buf + QMK_KV4_META;
+    uintx4 nan = {0, 0, 0, 0};
+    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
+    floatx4 x[NF][2];
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) st.o[f][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (kv4_is_page(A.c, now)) chunk_expand(sh, ta & 1, it.r.len - QMK_KV4_PAGE_TOKENS * ta, w, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int first_pos = it.r.len - it.r.n + i0;
-        for (int t = ta; t < tb; ++t) {
-            // Half of the waves make the next tile's operands before their
-            // products and half after them, so that a SIMD has one of each.
-            auto prepare = [&] {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                if (kv4_is_page(A.c, next)) chunk_expand(sh, (t + 1) & 1, it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), w, lane);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the codes are read
-                if (kv4_is_page(A.c, after)) chunk_fetch(A, sh, after, kvh, w, lane);
-            };
-            if (w < CHUNK_WAVES / 2) prepare();
-            if (kv4_is_page(A.c, now) && i0 < it.r.n) chunk_tile(st, sh, t & 1, QMK_KV4_PAGE_TOKENS * t, first_pos, lane);
-            if (w >= CHUNK_WAVES / 2) prepare();
-            now = next;
-            next = after;
-            after = page(t + 3);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        const bool whole = tb - ta == it.tiles;
-        float* part = A.partial + (size_t)(2 * blockIdx.x + (ta == 0)) * QMK_CHUNK_PARTIAL + (size_t)w * CHUNK_COLS * (QMK_CHUNK_PARTIAL / 16);
+    for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int f = 0; f < CHUNK_COLS; ++f) {
-            const float l = sum_xor32(sum_xor16(st.l[f]));
-            const int i = i0 + 16 * f + c;
-            if (whole) {
-                const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
-                const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * g;
-                uint2 x[16];
+        for (int r = 0; r < 2; ++r) x[f][r] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int dt = 0; dt < 16; ++dt) x[dt] = *reinterpret_cast<const uint2*>(gate + 16 * dt);
-                if (i < it.r.n) {
+    for (int r = 0; r < 2; ++r) {
+        const uint2 s4 = *reinterpret_cast<const uint2*>(meta + 2 * kv4_s_at(16 * r + c, 0));
+        const half2_t s01 = as_half2(s4.x), s23 = as_half2(s4.y);
+        _Float16 lo[4];
 #pragma unroll
-                    for (int dt = 0; dt < 16; ++dt) chunk_out(A.out + at * QM_GQA_HD + 16 * dt + 4 * g, st.o[f][dt], chunk_inverse(l), x[dt]);
-                }
-            } else {
+        for (int j = 0; j < 4; ++j) lo[j] = *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * r + c, j));
 #pragma unroll
-                for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(part + 256 * dt + 4 * lane) = st.o[f][dt];
-                if (lane < 16) {
-                    part[4096 + lane] = st.m[f];
-                    part[4112 + lane] = l;
-                }
-                part += QMK_CHUNK_PARTIAL / 16;
+        for (int d = 0; d < 2; ++d) {
+            const uintx4 k = *reinterpret_cast<const uintx4*>(buf + 1024 * (2 * r + d) + 16 * lane);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int j = 2 * d + (m >> 1);            // the words' group
+                const _Float16 sj = j < 2 ? s01[j & 1] : s23[j & 1];
+                const half2_t s2 = {sj, sj}, l2 = {lo[j], lo[j]};
+                const half2_t ss[4] = {s2, s2, s2, s2}, ll[4] = {l2, l2, l2, l2};
+                const half8 a = chunk_values(k[m], ss, ll);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) x[f][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.q[f][4 * d + m], x[f][r], 0, 0, 0);
             }
+        }
+    }
+    half8 p[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) p[f] = chunk_weights(x[f], st.o[f], st.m[f], st.l[f], st.pos[f], k0, edge, g);
+    // scales of the lane's eight tokens, all groups: [token][group]
+    uintx4 sv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sv[i] = *reinterpret_cast<const uintx4*>(meta + 512 + 64 * g + 16 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uintx4 v = *reinterpret_cast<const uintx4*>(buf + 4 * QMK_KV4_V_WORDS + 1024 * j + 16 * lane);
+        const uintx4 lo4 = *reinterpret_cast<const uintx4*>(meta + 768 + (4 * j + g) * 16);
+        half2_t s[4], lo[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {                      // tokens 2 n, 2 n + 1: dwords 4 n + j / 2 and two on
+            s[n] = as_half2(__builtin_amdgcn_perm(sv[n][2 + (j >> 1)], sv[n][j >> 1], j & 1 ? 0x07060302u : 0x05040100u));
+            lo[n] = as_half2(lo4[n]);
+        }
+        if (left < QMK_KV4_HALF_TOKENS) chunk_cut(s, lo, left, g);      // uniform
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const half8 a = chunk_values(v[m], s, lo);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) st.o[f][4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[f], st.o[f][4 * j + m], 0, 0, 0);
+        }
+    }
+    if (nan[0] | nan[1] | nan[2] | nan[3]) {               // uniform
+#pragma unroll
+        for (int f = 0; f < NF; ++f) chunk_nan(st.o[f], nan, st.pos[f], k0);
+    }
+}
+
+template <int NF>
+QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
+    const int c = lane & 15, g = lane >> 4, head = 4 * kvh + (c & 3);
+    const int i0 = 4 * NF * it.block, first_pos = it.r.len - it.r.n + i0;
+    const int end = it.r.len - it.r.n + min(it.r.n, i0 + 4 * NF);             // past the block's last token
+    const int h0 = 2 * ta + w, h_end = min(2 * tb, (end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
+    // page ids of the wave's rounds, one a lane, 64 rounds at a time
+    const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
+    auto load_ids = [&](int round) {
+        const int t = ta + (w >> 1) + 4 * (round + lane);
+        return t < tb ? table[t] : -1;
+    };
+    int ids = load_ids(0);
+    const uint32_t ring = lds_addr(sh.ring[w]);
+    auto fetch = [&](int round, int h) {                   // the half page of that round, if there is one
+        if (h >= h_end) return false;
+        const int id = __builtin_amdgcn_readlane(ids, round & 63);
+        if (!kv4_is_page(A.c, id)) return false;
+        few_fetch(kv4_half(A.c, A.layer, id, kvh, h & 1), ring + QMK_KV4_HALF_BYTES * (round & 1), lane);
+        return true;
+    };
+    FewWave<NF> st;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int i = i0 + 4 * f + (c >> 2);
+        st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
+    }
+    bool now = fetch(0, h0);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) chunk_query(A, st.q[f], it.r, min(i0 + 4 * f + (c >> 2), it.r.n - 1), head, g);
+    bool next = fetch(1, h0 + CHUNK_WAVES);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        st.m[f] = -INFINITY;
+        st.l[f] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) st.o[f][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int round = 0;
+    for (int h = h0; h < h_end; h += CHUNK_WAVES, ++round) {
+        if (next) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FEW_DMA) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        uint8_t* buf = sh.ring[w][round & 1];
+        if (now) {
+            const int k0 = QMK_KV4_HALF_TOKENS * h;
+            const bool edge = k0 + QMK_KV4_HALF_TOKENS - 1 > first_pos;
+            few_half<NF>(st, buf, k0, it.r.len - k0, edge, lane);
+        }
+        if (((round + 2) & 63) == 0) ids = load_ids(round + 2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the buffer's reads are done
+        now = next;
+        next = fetch(round + 2, h + 2 * CHUNK_WAVES);
+    }
+    // The waves' sums: dim groups 2 w, 2 w + 1 of all columns are this wave's to join.
+    const bool whole = tb - ta == it.tiles;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const float l = sum_xor32(sum_xor16(st.l[f]));
+        if (lane < 16) {
+            sh.m[w][lane] = st.m[f];
+            sh.l[w][lane] = l;
+        }
+        float* mine = reinterpret_cast<float*>(sh.ring[w][0]) + 4 * lane;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt) = st.o[f][dt];
+        const int i = i0 + 4 * f + (c >> 2);
+        const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
+        uint2 gate[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 16 * (2 * w + j) + 4 * g);
+        __syncthreads();
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, sh.m[k][c]);
+        floatx4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int k = 0; k < CHUNK_WAVES; ++k) {
+            const float e = sh.m[k][c] == M ? 1.0f : __builtin_amdgcn_exp2f(sh.m[k][c] - M);
+            L = fmaf(sh.l[k][c], e, L);
+            const float* a = reinterpret_cast<const float*>(sh.ring[k][0]) + 4 * lane + 512 * w;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const floatx4*>(a + 256 * j) * e;
+        }
+        if (!whole) {
+            float* to = part + f * QMK_CHUNK_COLUMN;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<floatx4*>(to + 256 * (2 * w + j) + 4 * lane) = o[j];
+            if (w == 0 && lane < 16) {
+                to[4096 + lane] = M;
+                to[4112 + lane] = L;
+            }
+        } else if (i < it.r.n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                chunk_out(A.out + at * QM_GQA_HD + 16 * (2 * w + j) + 4 * g, o[j], chunk_inverse(L), gate[j]);
+        }
+        __syncthreads();                                   // before the next column's, or the next block's pages
+    }
+}
+
+// ---- many tokens ------------------------------------------------------------------
+template <int NF>
+QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
+    const int c = lane & 15, g = lane >> 4, head = 4 * kvh + (w & 3);
+    const int i0 = QMK_CHUNK_TOKENS * it.block + 16 * CHUNK_COLS * (w >> 2);      // the wave's first row
+    const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
+    auto page = [&](int t) { return t < tb ? __builtin_amdgcn_readfirstlane(table[t]) : -1; };
+    int now = page(ta), next = page(ta + 1), after = page(ta + 2);
+    if (kv4_is_page(A.c, now)) chunk_fetch(A, sh, now, kvh, w, lane);
+    ChunkWave st;
+#pragma unroll
+    for (int f = 0; f < CHUNK_COLS; ++f) {
+        const int i = i0 + 16 * f + c;                     // rows past the last: any row, never written
+        st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
+        chunk_query(A, st.q[f], it.r, min(i, it.r.n - 1), head, g);
+        st.m[f] = -INFINITY;
+        st.l[f] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) st.o[f][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // the row's tokens in tile t are len - 64 t
+    if (kv4_is_page(A.c, now)) chunk_expand(sh, ta & 1, it.r.len - QMK_KV4_PAGE_TOKENS * ta, w, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int first_pos = it.r.len - it.r.n + i0;
+    for (int t = ta; t < tb; ++t) {
+        // Half of the waves make the next tile's operands before their
+        // products and half after them, so that a SIMD has one of each.
+        auto prepare = [&] {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (kv4_is_page(A.c, next)) chunk_expand(sh, (t + 1) & 1, it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), w, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the codes are read
+            if (kv4_is_page(A.c, after)) chunk_fetch(A, sh, after, kvh, w, lane);
+        };
+        if (w < CHUNK_WAVES / 2) prepare();
+        if (kv4_is_page(A.c, now) && i0 < it.r.n) chunk_tile(st, sh, t & 1, QMK_KV4_PAGE_TOKENS * t, first_pos, lane);
+        if (w >= CHUNK_WAVES / 2) prepare();
+        now = next;
+        next = after;
+        after = page(t + 3);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    const bool whole = tb - ta == it.tiles;
+    part += w * CHUNK_COLS * QMK_CHUNK_COLUMN;
+#pragma unroll
+    for (int f = 0; f < CHUNK_COLS; ++f) {
+        const float l = sum_xor32(sum_xor16(st.l[f]));
+        const int i = i0 + 16 * f + c;
+        if (whole) {
+            const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
+            const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * g;
+            uint2 x[16];
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt) x[dt] = *reinterpret_cast<const uint2*>(gate + 16 * dt);
+            if (i < it.r.n) {
+#pragma unroll
+                for (int dt = 0; dt < 16; ++dt) chunk_out(A.out + at * QM_GQA_HD + 16 * dt + 4 * g, st.o[f][dt], chunk_inverse(l), x[dt]);
+            }
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(part + 256 * dt + 4 * lane) = st.o[f][dt];
+            if (lane < 16) {
+                part[4096 + lane] = st.m[f];
+                part[4112 + lane] = l;
+            }
+            part += QMK_CHUNK_COLUMN;
         }
     }
 }
 
+// MANY: rows of more than QMK_CHUNK_FEW tokens as well (max_new says whether
+// there can be any).
+template <int NF, bool MANY>
+QM_DEV void chunk_attention(const GqaChunkArgs& A) {
+    constexpr int kColumns = MANY ? CHUNK_WAVES * CHUNK_COLS : NF;
+    constexpr size_t kBytes = MANY && sizeof(ChunkLds) > sizeof(FewLds) ? sizeof(ChunkLds) : sizeof(FewLds);
+    __shared__ __attribute__((aligned(1024))) uint8_t sm[kBytes];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2;
+    const Deal<NF> deal(A, lane);
+    if (blockIdx.x == 0 && w == 0) {                       // for the merge
+        int many = 0, few = 0;
+        for (int b = lane; b < A.batch; b += 64) {
+            const ChunkRow r = chunk_row(A, b);
+            (Deal<NF>::few(r) ? few : many) += Deal<NF>::blocks(r);
+        }
+        many = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)many), 63);
+        few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
+        if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
+    }
+    const double end = deal.begin(index + 1);
+    for (double u = deal.begin(index); u < end;) {         // uniform, as all of it
+        const typename Deal<NF>::Item it = deal.find(u, true);
+        const int weight = Deal<NF>::weight(it.r);
+        const bool few = Deal<NF>::few(it.r);
+        const int ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
+        const int tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
+        u = it.first + (double)tb * weight;
+        if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few)) {
+            ChunkRecord r{index, index, it.r.begin, it.r.n, it.block, {0, 0, 0}};
+            if (tb < it.tiles) r.to = (int)((it.first + (double)it.tiles * weight - 1.0) / deal.each);
+            A.records[(few ? A.many : 0) + it.number] = r;
+        }
+        if (it.r.kind != CHUNK_RUN) {
+            const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;
+            const int i0 = Deal<NF>::tokens(it.r) * it.block, count = min(Deal<NF>::tokens(it.r), it.r.n - i0);
+            uint16_t* out = A.out + (size_t)(it.r.begin + i0) * QM_GQA_HEADS * QM_GQA_HD + (size_t)4 * kvh * QM_GQA_HD + 4 * lane;
+            for (int j = w; j < 4 * count; j += CHUNK_WAVES)
+                *reinterpret_cast<uint2*>(out + ((size_t)(j >> 2) * QM_GQA_HEADS + (j & 3)) * QM_GQA_HD) = make_uint2(fill, fill);
+            continue;
+        }
+        // a workgroup's first block may have begun before it, its last end after it
+        float* part = A.partial + (size_t)(2 * blockIdx.x + (ta == 0)) * kColumns * QMK_CHUNK_COLUMN;
+        if (MANY && !few) many_item<NF>(A, *reinterpret_cast<ChunkLds*>(sm), it, ta, tb, kvh, part, w, lane);
+        else few_item<NF>(A, *reinterpret_cast<FewLds*>(sm), it, ta, tb, kvh, part, w, lane);
+    }
+}
+extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_4(GqaChunkArgs A) { chunk_attention<1, false>(A); }
+extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_32(GqaChunkArgs A) { chunk_attention<2, false>(A); }
+extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_many(GqaChunkArgs A) { chunk_attention<2, true>(A); }
+
 // The partial sums of a row block that several workgroups share, joined: a
-// wave per (kv head, operand column of a wave, four of the 16 dim groups).
+// workgroup per (row block, kv head, operand column), a wave four of the 16 dim
+// groups.
 #define CHUNK_JOIN 8                   // partials loaded at a time
-extern "C" __global__ __launch_bounds__(64) void qm_gqa_chunk_merge(GqaChunkArgs A) {
-    const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-    const int dt0 = 4 * (blockIdx.x & 3), col = (blockIdx.x >> 2) & 15, kvh = (blockIdx.x >> 6) & 3;
-    ChunkItem it;
-    if (!chunk_find<true>(A, blockIdx.x >> 8, lane, it)) return;
-    const uint64_t each = chunk_share(chunk_total(A, lane), A.groups);
-    const uint64_t from = it.first / each, to = (it.first + it.tiles - 1) / each;
-    if (from == to) return;                                // one workgroup had it
-    const int w = col / CHUNK_COLS, head = 4 * kvh + (w & 3);
-    const int i = QMK_CHUNK_TOKENS * it.block + 16 * CHUNK_COLS * (w >> 2) + 16 * (col % CHUNK_COLS) + c;
-    const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
+template <int NF, bool MANY>
+QM_DEV void chunk_merge(const GqaChunkArgs& A) {
+    constexpr int kColumns = MANY ? CHUNK_WAVES * CHUNK_COLS : NF;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, dt0 = 4 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = MANY ? A.many * 4 * CHUNK_WAVES * CHUNK_COLS : 0;        // workgroups for blocks of many tokens
+    const bool few = (int)blockIdx.x >= first;
+    const int k = few ? blockIdx.x - first : blockIdx.x, columns = few ? NF : CHUNK_WAVES * CHUNK_COLS;
+    const int col = k % columns, kvh = (k / columns) & 3, number = k / (4 * columns);
+    const int count = A.counts[few];
+    const ChunkRecord rec = A.records[(few ? A.many : 0) + number];
+    if (number >= count || rec.from == rec.to) return;     // uniform
+    const int w = col / CHUNK_COLS;
+    const int head = 4 * kvh + (few ? c & 3 : w & 3);
+    const int i = few ? 4 * NF * rec.block + 4 * col + (c >> 2)
+                      : QMK_CHUNK_TOKENS * rec.block + 16 * CHUNK_COLS * (w >> 2) + 16 * (col % CHUNK_COLS) + c;
+    const size_t at = (size_t)(rec.begin + min(i, rec.n - 1)) * QM_GQA_HEADS + head;
     const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 16 * dt0 + 4 * g;
     uint2 x[4];
 #pragma unroll
@@ -553,39 +841,41 @@ extern "C" __global__ __launch_bounds__(64) void qm_gqa_chunk_merge(GqaChunkArgs
     floatx4 o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint64_t s0 = from; s0 <= to; s0 += CHUNK_JOIN) {
+    for (int s0 = rec.from; s0 <= rec.to; s0 += CHUNK_JOIN) {
         floatx4 a[CHUNK_JOIN][4];
         float pm[CHUNK_JOIN], pl[CHUNK_JOIN];
 #pragma unroll
-        for (int k = 0; k < CHUNK_JOIN; ++k) {             // past the last: the last again, with weight 0
-            const uint64_t wg = min(s0 + k, to);
-            const float* part = A.partial + (size_t)(2 * (4 * wg + kvh) + (each * wg <= it.first)) * QMK_CHUNK_PARTIAL +
-                                (size_t)col * (QMK_CHUNK_PARTIAL / 16);
+        for (int n = 0; n < CHUNK_JOIN; ++n) {             // past the last: the last again, with weight 0
+            const int wg = min(s0 + n, rec.to);
+            const float* part = A.partial + ((size_t)(2 * (4 * wg + kvh) + (wg == rec.from)) * kColumns + col) * QMK_CHUNK_COLUMN;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (dt0 + j) + 4 * lane);
-            pm[k] = part[4096 + c];
-            pl[k] = part[4112 + c];
+            for (int j = 0; j < 4; ++j) a[n][j] = *reinterpret_cast<const floatx4*>(part + 256 * (dt0 + j) + 4 * lane);
+            pm[n] = part[4096 + c];
+            pl[n] = part[4112 + c];
         }
         float top = m;
 #pragma unroll
-        for (int k = 0; k < CHUNK_JOIN; ++k) top = fmaxf(top, pm[k]);
+        for (int n = 0; n < CHUNK_JOIN; ++n) top = fmaxf(top, pm[n]);
         const float corr = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         l *= corr;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] *= corr;
 #pragma unroll
-        for (int k = 0; k < CHUNK_JOIN; ++k) {
-            if (s0 + k > to) break;                        // uniform
+        for (int n = 0; n < CHUNK_JOIN; ++n) {
+            if (s0 + n > rec.to) break;                    // uniform
             // a partial of no weight counts all the same: a NaN in it reaches the output
-            const float f = pm[k] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - top);
-            l = fmaf(pl[k], f, l);
+            const float f = pm[n] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[n] - top);
+            l = fmaf(pl[n], f, l);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += a[k][j] * f;
+            for (int j = 0; j < 4; ++j) o[j] += a[n][j] * f;
         }
         m = top;
     }
-    if (i < it.r.n) {
+    if (i < rec.n) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) chunk_out(A.out + at * QM_GQA_HD + 16 * (dt0 + j) + 4 * g, o[j], chunk_inverse(l), x[j]);
     }
 }
+extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_4(GqaChunkArgs A) { chunk_merge<1, false>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_32(GqaChunkArgs A) { chunk_merge<2, false>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_many(GqaChunkArgs A) { chunk_merge<2, true>(A); }

@@ -36,9 +36,13 @@
 #define QMK_KV4_MAX_SPLIT 4096      // tokens of a decode workgroup: 64 pages
 #define QMK_KV4_ROUNDS 64           // full rounds of decode workgroups that are dealt evenly
 #define QMK_KV4_LEN_PAGES 33554431  // pages of a row: its length is an int32
-#define QMK_CHUNK_TOKENS 64         // new tokens of a row block of the chunk attention
 #define QMK_CHUNK_MAX_TOKENS (1 << 20)     // new tokens of a call
-#define QMK_CHUNK_PARTIAL 66048     // f32 of a row block's partial: 16 x (16 dim groups x 256, m[16], l[16])
+#define QMK_CHUNK_FEW 32            // a row of up to so many is attended in blocks of few tokens
+#define QMK_CHUNK_TOKENS 64         // others in blocks of so many
+#define QMK_CHUNK_WEIGHT 10         // what a page costs a block of many tokens, against one of few
+#define QMK_CHUNK_MIN_UNITS 4       // pages of a block of few tokens that are worth a workgroup
+#define QMK_CHUNK_WHOLE 8           // a row block of so many pages falls to one
+#define QMK_CHUNK_COLUMN 4128       // f32 of an operand column's partial: 16 dim groups x 256, m[16], l[16]
 
 #ifdef __HIPCC__
 #define QMK_HD __host__ __device__ inline
@@ -149,7 +153,12 @@ struct Kv4AppendArgs {
     int32_t layer, batch, tokens, max_len;
 };
 
-// Attention of such tokens.
+// Attention of such tokens.  A row block's partial sums, where several
+// workgroups (from .. to) had its pages, and whose they are.
+struct ChunkRecord {
+    int32_t from, to;        // the same: one had them all
+    int32_t begin, n, block, pad[3];
+};
 struct GqaChunkArgs {
     Kv4Cache c;
     const int32_t* slots;
@@ -160,7 +169,10 @@ struct GqaChunkArgs {
     const float* rope_sin;
     const int32_t* result;
     uint16_t* out;           // bf16 [tokens][16][256]
-    float* partial;          // [groups][4 kv heads][2][QMK_CHUNK_PARTIAL]
+    float* partial;          // [groups][4 kv heads][2][columns][QMK_CHUNK_COLUMN]
+    int32_t* counts;         // [2]: row blocks of many and of few tokens
+    ChunkRecord* records;    // [most of many][most of few]
     int32_t layer, batch, tokens, max_new, max_len;
     int32_t groups;          // workgroups per kv head
+    int32_t many;            // the most row blocks of many tokens that there can be
 };

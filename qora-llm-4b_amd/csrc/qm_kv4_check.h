@@ -152,17 +152,50 @@ inline Fault check_chunk(const qm_kv4_cache* c, int32_t layer, int32_t batch, co
 inline int64_t append_halves(int32_t tokens, int32_t batch) {
     return (static_cast<int64_t>(tokens) + 30ll * batch) / QMK_KV4_HALF_TOKENS + batch;
 }
-// Row blocks of the chunk attention, and its workgroups per kv head: one a CU,
-// or fewer where the blocks' pages are fewer.
-inline int64_t chunk_blocks(int32_t tokens, int32_t batch) {
-    return (static_cast<int64_t>(tokens) + (QMK_CHUNK_TOKENS - 1ll) * batch) / QMK_CHUNK_TOKENS;
-}
-inline int64_t chunk_groups(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
+// The chunk attention's shape: operand columns of a block of few tokens (4 new
+// tokens each), whether rows can have more than few, the most row blocks of
+// both kinds, workgroups per kv head (one a CU, or fewer where the blocks'
+// pages are fewer) and whether blocks may be split over them.
+struct Chunk {
+    int32_t columns;
+    bool many, split;
+    int64_t most_many, most_few, groups;
+};
+inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus) {
+    Chunk c{};
+    c.columns = max_new <= 4 ? 1 : 2;
+    c.many = max_new > QMK_CHUNK_FEW;
+    // a row of n: ceil(n / tokens of a block) <= n / that + 1, and many is FEW + 1 at least
+    const int64_t t = tokens, b = batch, block = 4 * c.columns, with_many = t / (QMK_CHUNK_FEW + 1);
+    c.most_many = c.many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
+    c.most_few = t / block + b < b * (QMK_CHUNK_FEW / block) ? t / block + b : b * (QMK_CHUNK_FEW / block);
     const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
-    const int64_t units = chunk_blocks(tokens, batch) * tiles, most = cus / 4 > 0 ? cus / 4 : 1;
-    return units < most ? units : most;
+    c.split = tiles > QMK_CHUNK_WHOLE;
+    // rows that are refused for their new tokens are written in blocks of many
+    const int64_t blocks = c.most_few + t / QMK_CHUNK_TOKENS + with_many;
+    const int64_t most = cus / 4 > 0 ? cus / 4 : 1;
+    const int64_t parts = c.split ? (tiles * QMK_CHUNK_WEIGHT + QMK_CHUNK_MIN_UNITS - 1) / QMK_CHUNK_MIN_UNITS : 1;
+    c.groups = blocks >= most || blocks * parts >= most ? most : blocks * parts;
+    if (c.groups < 1) c.groups = 1;
+    c.split = c.split && c.groups > 1;
+    return c;
 }
-inline size_t chunk_ws(int64_t groups) { return static_cast<size_t>(groups) * 4 * 2 * QMK_CHUNK_PARTIAL * 4; }
+inline size_t chunk_partial_bytes(const Chunk& c) {
+    const int64_t columns = c.many ? 16 : c.columns;
+    return c.split ? static_cast<size_t>(c.groups) * 4 * 2 * columns * QMK_CHUNK_COLUMN * 4 : 0;
+}
+inline size_t chunk_ws(const Chunk& c) {
+    return chunk_partial_bytes(c) + 16 + static_cast<size_t>(c.most_many + c.most_few) * sizeof(ChunkRecord);
+}
+// A bound of it for up to so many tokens and rows, whatever max_new is.
+inline size_t chunk_reserve_ws(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
+    size_t ws = 0;
+    for (int32_t max_new : {4, QMK_CHUNK_FEW, QMK_CHUNK_FEW + 1}) {
+        const size_t one = chunk_ws(chunk_shape(tokens, batch, max_new, max_len, cus));
+        if (one > ws) ws = one;
+    }
+    return ws;
+}
 
 // The decode's workgroups.  Short rows, and somewhat longer ones where there
 // are enough of them, take one workgroup each per kv head and no merge

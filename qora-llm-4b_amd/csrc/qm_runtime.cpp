@@ -71,7 +71,7 @@ struct qm_context {
     hipFunction_t f_kv4_compact = nullptr, f_kv4_compact_pages = nullptr;
     hipFunction_t f_gqa_kv4_split = nullptr, f_gqa_kv4_merge = nullptr;
     hipFunction_t f_kv4_append[2] = {};      // k and v f32, bf16
-    hipFunction_t f_gqa_chunk = nullptr, f_gqa_chunk_merge = nullptr;
+    hipFunction_t f_gqa_chunk[3] = {}, f_gqa_chunk_merge[3] = {};      // rows of up to 4 new tokens, up to 32, more
     hipFunction_t f_beam_slices = nullptr, f_beam_draw = nullptr;
     hipFunction_t f_state_fork[3] = {};      // up to 8 rows, up to 32, more
     int lm_head_hidden = 0;              // the hidden size lm_head_wg_per_cu was computed for
@@ -409,8 +409,12 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     if (st == QM_OK) st = load_function(c, mods[9], "qm_gqa_kv4_merge", &c->f_gqa_kv4_merge);
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_append_f32", &c->f_kv4_append[0]);
     if (st == QM_OK) st = load_function(c, mods[8], "qm_kv4_append_bf16", &c->f_kv4_append[1]);
-    if (st == QM_OK) st = load_function(c, mods[10], "qm_gqa_chunk_kv4", &c->f_gqa_chunk);
-    if (st == QM_OK) st = load_function(c, mods[10], "qm_gqa_chunk_merge", &c->f_gqa_chunk_merge);
+    const char* chunk_names[3] = {"4", "32", "many"};
+    for (int i = 0; i < 3; ++i) {
+        if (st == QM_OK) st = load_function(c, mods[10], (std::string("qm_gqa_chunk_") + chunk_names[i]).c_str(), &c->f_gqa_chunk[i]);
+        if (st == QM_OK)
+            st = load_function(c, mods[10], (std::string("qm_gqa_chunk_merge_") + chunk_names[i]).c_str(), &c->f_gqa_chunk_merge[i]);
+    }
     if (st == QM_OK) st = load_function(c, mods[11], "qm_beam_slices", &c->f_beam_slices);
     if (st == QM_OK) st = load_function(c, mods[11], "qm_beam_draw", &c->f_beam_draw);
     if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_8", &c->f_state_fork[0]);
@@ -828,7 +832,7 @@ int32_t qm_reserve(qm_context* c, int32_t max_batch, int32_t max_kv_len, int32_t
         ws = std::max(ws, gqa_prefill_kvf_bytes(s_pad) + 256);
     }
     if (max_kv_len > 0 && max_prefill_tokens > 0)
-        ws = std::max(ws, qm_kv4::chunk_ws(qm_kv4::chunk_groups(max_prefill_tokens, max_batch, max_kv_len, c->num_cu)));
+        ws = std::max(ws, qm_kv4::chunk_reserve_ws(max_prefill_tokens, max_batch, max_kv_len, c->num_cu));
     ws = std::max(ws, kSampleWsBytes);
     ws = std::max(ws, qm_beam::select_ws(max_batch, QMK_BEAM_VOCAB));
     return ensure(c, c->stream, ws, true);
@@ -1381,15 +1385,19 @@ int32_t qm_gqa_chunk_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* ca
                                                   {q_gate, q_norm, rope_cos, rope_sin, out}, rope_len, max_len, result);
     if (bad.code != QM_OK) return fail(c, bad.code, "%s", bad.text);
     hipStream_t s = pick(c, stream);
-    const int64_t groups = qm_kv4::chunk_groups(tokens, batch, max_len, c->num_cu);
-    const int64_t merge = qm_kv4::chunk_blocks(tokens, batch) * QM_GQA_KV_HEADS * 64;
-    int32_t st = ensure(c, s, groups > 1 ? qm_kv4::chunk_ws(groups) : 0);
+    const qm_kv4::Chunk shape = qm_kv4::chunk_shape(tokens, batch, max_new, max_len, c->num_cu);
+    int32_t st = ensure(c, s, qm_kv4::chunk_ws(shape));
     if (st != QM_OK) return st;
-    GqaChunkArgs a{kv4_of(*cache), slots, begins, q_gate, q_norm, rope_cos, rope_sin, result, out, static_cast<float*>(c->ws),
-                   layer, batch, tokens, max_new, max_len, static_cast<int32_t>(groups)};
-    st = launch(c, c->f_gqa_chunk, static_cast<uint32_t>(groups * QM_GQA_KV_HEADS), 512, a, s, "qm_gqa_chunk_kv4");
-    if (st != QM_OK || groups == 1) return st;
-    return launch(c, c->f_gqa_chunk_merge, static_cast<uint32_t>(merge), 64, a, s, "qm_gqa_chunk_merge");
+    char* ws = static_cast<char*>(c->ws);
+    char* records = ws + qm_kv4::chunk_partial_bytes(shape);
+    GqaChunkArgs a{kv4_of(*cache), slots, begins, q_gate, q_norm, rope_cos, rope_sin, result, out, reinterpret_cast<float*>(ws),
+                   reinterpret_cast<int32_t*>(records), reinterpret_cast<ChunkRecord*>(records + 16), layer, batch, tokens, max_new,
+                   max_len, static_cast<int32_t>(shape.groups), static_cast<int32_t>(shape.most_many)};
+    const int form = shape.many ? 2 : shape.columns - 1;
+    st = launch(c, c->f_gqa_chunk[form], static_cast<uint32_t>(shape.groups * QM_GQA_KV_HEADS), 512, a, s, "qm_gqa_chunk");
+    if (st != QM_OK || !shape.split) return st;
+    const int64_t merge = (shape.most_many * 16 + shape.most_few * shape.columns) * QM_GQA_KV_HEADS;
+    return launch(c, c->f_gqa_chunk_merge[form], static_cast<uint32_t>(merge), 256, a, s, "qm_gqa_chunk_merge");
 }
 
 // ---- beam search -------------------------------------------------------------------

@@ -56,6 +56,25 @@ def append(ref: R.Cache, layer, batch, slots, begins, tokens, k, v, k_norm, cos,
                 R.put(ref.pages[layer, p], head, t % R.TOKENS, vh[i, head], 1)
 
 
+def kept(ref: R.Cache, layer, r, head, is_v):
+    """rows64 as attention takes it: a scale that takes its group past f16's largest value is the next lower one."""
+    n = int(ref.lens[r])
+    out, there = np.zeros((R.pages_of(n) * R.TOKENS, R.HD)), np.zeros(R.pages_of(n) * R.TOKENS, bool)
+    for j in range(R.pages_of(n)):
+        if not ref.is_page(ref.table[r, j]):
+            continue
+        page = ref.pages[layer, ref.table[r, j]].copy()
+        for half in range(2):
+            meta = R._half(page, head, half * R.HALF)[8192:].view(np.float16)
+            s, lo = meta[256 * is_v + R.S_AT], meta[256 * is_v + 128 + R.LO_AT]
+            with np.errstate(invalid="ignore"):
+                over = lo.astype(np.float64) + 15 * s.astype(np.float64) >= 65520
+            meta[256 * is_v + R.S_AT] = np.where(over, np.nextafter(s, np.float16(0)), s)
+        out[j * R.TOKENS:(j + 1) * R.TOKENS] = R.get(page, head, is_v)
+        there[j * R.TOKENS:(j + 1) * R.TOKENS] = True
+    return out[:n], there[:n]
+
+
 def attend(ref: R.Cache, layer, batch, slots, begins, tokens, max_new, q_gate, q_norm, cos, sin, max_len):
     """q_gate values [tokens, 16, 512] -> out f64 [tokens, 16, 256] (untouched rows: 7), the bound of each output's
     error before it is rounded, and which rows were touched.
@@ -84,8 +103,8 @@ def attend(ref: R.Cache, layer, batch, slots, begins, tokens, max_new, q_gate, q
         gate = 1 / (1 + np.exp(-q_gate[lo:hi, :, 256:].astype(np.float64)))
         pos = length - n + np.arange(n)
         for g in range(R.KV):
-            K, there = ref.rows64(layer, r, g, 0)
-            V, _ = ref.rows64(layer, r, g, 1)
+            K, there = kept(ref, layer, r, g, 0)
+            V, _ = kept(ref, layer, r, g, 1)
             sees = there & (np.arange(length) <= pos[:, None])
             for h in range(4 * g, 4 * g + 4):
                 s = np.where(sees, q[:, h] @ np.nan_to_num(K).T, -np.inf)

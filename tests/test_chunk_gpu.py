@@ -273,7 +273,7 @@ def test_chunk_nan_reaches_those_that_see_it(ctx, at, is_v):
 
 
 def test_chunk_values_at_the_edges_of_f16(ctx):
-    """Groups that reach to f16's largest values stay finite: what passes 65504 is 65504."""
+    """Groups that reach to f16's largest values stay finite: a scale that would take them past it is a step less."""
     ref = cache_of([100], seed=30)
     meta = ref.pages[1, ref.table[0, 0]][R.HEAD_BYTES:][:R.HALF_BYTES][8192:].view(np.float16)
     meta[256 + R.S_AT[7]], meta[256 + 128 + R.LO_AT[7]] = np.float16(8736), np.float16(-65504)       # lo + 15 s = 65536
