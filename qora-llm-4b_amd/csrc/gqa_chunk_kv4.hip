@@ -10,14 +10,13 @@
 // the operands are f16, all sums f32.
 //
 // A workgroup (8 waves) owns a row block of 64 new tokens of the four query
-// heads of a kv head: wave w has head w & 3 and 32 tokens, two operand columns
-// of 16, so that every K and V operand read from LDS feeds two matrix
-// instructions.  Both products run transposed, S^T = K Q^T and O^T = V^T P^T,
-// so that a lane's scores, its running maximum and its outputs are all of one
-// row, and the scores of two runs of 16 tokens are, as they stand, the eight
-// keys that a word of V codes holds.  A page of the kv head (64 tokens) is a
-// tile: its codes come by LDS DMA, each wave makes f16 operands of an eighth of
-// them, and the tile before it is multiplied meanwhile.
+// heads of a kv head: wave w has head w & 3 and 32 tokens, the columns of a
+// 32 x 32 x 16 matrix instruction.  Both products run transposed, S^T = K Q^T
+// and O^T = V^T P^T, so that a lane's scores, its running maximum and its
+// outputs are all of one row, and its scores are, as they stand, the eight keys
+// that a word of V codes holds.  A page of the kv head (64 tokens) is a tile:
+// its codes come by LDS DMA, each wave makes f16 operands of an eighth of them,
+// and the tile before it is multiplied meanwhile.
 //
 // The pages of all row blocks of a kv head are dealt to the workgroups in equal
 // runs; where a block's pages fall to several, they leave partial sums and
@@ -31,9 +30,8 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 #define CHUNK_WAVES 8
-#define CHUNK_COLS 2                   // operand columns (of 16 rows) a wave
-// A row's reference maximum moves only where a score passes it by this (log2
-// units): p <= 2^8 is exact enough in f16, and outputs are seldom rescaled.
+// A row's reference moves only where a score passes it by this (log2 units):
+// weights up to 2^8 are exact enough in f16, and outputs are seldom rescaled.
 #define CHUNK_SLACK 8.0f
 
 // ---- how the work is dealt --------------------------------------------------
@@ -196,10 +194,11 @@ struct Deal {
 };
 
 // ---- a tile -------------------------------------------------------------------
-// LDS: two buffers of f16 operands, block entry l the 16 bytes that lane
-// l = (c, g) = (l & 15, l >> 4) reads for a product:
-//   K block (kk, s) at 8 kk + s:      token 16 kk + c, dims 32 s + 8 g .. + 7
-//   V block (dt, h) at 32 + 2 dt + h: dim 16 dt + c, tokens 32 h + 16 (e >> 2) + 4 g + (e & 3), e < 8
+// LDS: two buffers of f16 operands, block entry l the 16 bytes that lane l
+// reads for a product:
+//   K block h, s (16 h + s):             dims 16 s + 8 (l >> 5) .. + 7 of token many_token(l & 31) of half page h
+//   V block h, dt, k (32 + 16 h + 2 dt + k): dim 32 dt + (l & 31), tokens 16 (e >> 2) + 4 (2 k + (l >> 5)) + (e & 3),
+//                                        e < 8, of half page h
 // and a wave's own part of the next tile's codes, with its half page's scales
 // and minima.  Wave w has half page w >> 2 and pieces i = w & 3: K's run i >> 1,
 // dims 128 (i & 1) .., and V's group i.
@@ -208,6 +207,7 @@ struct ChunkLds {
     __attribute__((aligned(1024))) uint8_t tile[2][CHUNK_TILE];
     __attribute__((aligned(1024))) uint8_t raw[CHUNK_WAVES][3][1024];
     __attribute__((aligned(16))) uint32_t nan[2][2][4];      // [buffer][half][group]: tokens whose V is NaN there
+    __attribute__((aligned(16))) uint32_t odd[CHUNK_WAVES][4];
 };
 
 QM_DEV uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
@@ -223,19 +223,29 @@ QM_DEV void chunk_fetch(const GqaChunkArgs& A, ChunkLds& sh, int id, int head, i
 // Token of score e of run r in lane group g.
 QM_DEV int chunk_token(int r, int g, int e) { return 16 * r + 4 * g + e; }
 
+// The lane, recomputed from: addresses that depend on it alone would be held
+// in registers across a loop that has none to spare.
+QM_DEV int chunk_lane(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 QM_DEV half2_t as_half2(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
 // The eight values of a word, s and lo in pairs of elements 2 i, 2 i + 1: a
 // code c in the low bits of 1024 (16 c in bits 4..7) is 1024 + c exactly, so
 // c is one exact packed step away and the value one rounding more.
 QM_DEV half8 chunk_values(uint32_t word, const half2_t (&s)[4], const half2_t (&lo)[4]) {
+    // in registers, opaque: the masking and the exponent are one instruction then
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, one = 0x64006400u;
+    asm("" : "+s"(low), "+s"(high), "+v"(one));
     const uint32_t v = word >> 8;
     const half2_t k1024 = {(_Float16)1024.0f, (_Float16)1024.0f}, k64 = {(_Float16)64.0f, (_Float16)64.0f},
                   sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     half2_t c[4];
-    c[0] = as_half2((word & 0x000f000fu) | 0x64006400u) - k1024;
-    c[1] = __builtin_elementwise_fma(as_half2((word & 0x00f000f0u) | 0x64006400u), sixteenth, -k64);
-    c[2] = as_half2((v & 0x000f000fu) | 0x64006400u) - k1024;
-    c[3] = __builtin_elementwise_fma(as_half2((v & 0x00f000f0u) | 0x64006400u), sixteenth, -k64);
+    c[0] = as_half2((word & low) | one) - k1024;
+    c[1] = __builtin_elementwise_fma(as_half2((word & high) | one), sixteenth, -k64);
+    c[2] = as_half2((v & low) | one) - k1024;
+    c[3] = __builtin_elementwise_fma(as_half2((v & high) | one), sixteenth, -k64);
     half8 out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -268,11 +278,11 @@ QM_DEV bool chunk_odd(const uint8_t* meta, int lane) {
 }
 // Puts such a half page right, in LDS.  A scale that takes the group past
 // f16's largest value becomes the next lower one.  V that is NaN becomes 0, and
-// its tokens (a bit each) are returned, a word per group: the rows that see
-// them are given the NaN beside the product, as a weight of 0 times it would
-// give it to the others too.
-QM_DEV uintx4 chunk_mend(uint8_t* meta, int lane) {
-    uintx4 nan = {0, 0, 0, 0};
+// its tokens (a bit each, a word per group) are noted in nan[4]: the rows that
+// see them are given the NaN beside the product, as a weight of 0 times it
+// would give it to the others too.
+QM_DEV void chunk_mend(uint8_t* meta, uint32_t* nan, int lane) {
+    if (lane < 4) nan[lane] = 0;
 #pragma unroll
     for (int is_v = 0; is_v < 2; ++is_v)
 #pragma unroll
@@ -280,18 +290,14 @@ QM_DEV uintx4 chunk_mend(uint8_t* meta, int lane) {
             const int t = 16 * k + (lane >> 2), group = lane & 3;
             uint16_t* s = reinterpret_cast<uint16_t*>(meta + 512 * is_v) + kv4_s_at(t, group);
             uint16_t* lo = reinterpret_cast<uint16_t*>(meta + 512 * is_v + 256) + kv4_lo_at(t, group);
-            const float fs = f16_to_f32(*s), fl = f16_to_f32(*lo), top = fmaf(15.0f, fs, fl);
-            const bool bad = top != top;
+            const float top = fmaf(15.0f, f16_to_f32(*s), f16_to_f32(*lo));
             if (top >= 65520.0f) *s = *s - 1;
-            if (bad && is_v) *s = *lo = 0;
-            const uint64_t lanes = __ballot(bad && is_v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) nan[q] |= (uint32_t)(lanes >> (4 * j + q) & 1) << (16 * k + j);
+            if (is_v && top != top) {
+                *s = *lo = 0;
+                atomicOr(nan + group, 1u << t);
+            }
         }
-    asm volatile("" ::: "memory");                         // read again as other types
-    return nan;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read again as other types
 }
 
 // The wave's part of a tile of which `left` tokens are the row's (64 and more:
@@ -303,8 +309,8 @@ QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
     const int run = i >> 1, dims = i & 1;
     uint32_t nan = 0;
     if (chunk_odd(meta, lane)) {
-        const uintx4 all = chunk_mend(meta, lane);
-        nan = i < 2 ? (i == 0 ? all[0] : all[1]) : i == 2 ? all[2] : all[3];
+        chunk_mend(meta, sh.odd[w], lane);
+        nan = sh.odd[w][i];
     }
     if (lane == 0) sh.nan[buf][half][i] = nan;
     {
@@ -312,12 +318,14 @@ QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
         const half2_t s = as_half2(*reinterpret_cast<const uint32_t*>(meta + 2 * kv4_s_at(16 * run + c, 2 * dims)));
         const half2_t lo = {*reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims)),
                             *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims + 1))};
-        uint8_t* to = sh.tile[buf] + (8 * (2 * half + run) + 4 * dims) * 1024 + 16 * lane;
+        // dims 128 dims + 32 m + 8 g .. of token 16 run + c: block 2 (4 dims + m) + (g >> 1), entry of its row and g & 1
+        const int row = 16 * (c >> 3) + 8 * run + (c & 7);
+        uint8_t* to = sh.tile[buf] + (16 * half + 8 * dims + (g >> 1)) * 1024 + 16 * (row + 32 * (g & 1));
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const half2_t s2 = {s[m >> 1], s[m >> 1]}, l2 = {lo[m >> 1], lo[m >> 1]};
             const half2_t ss[4] = {s2, s2, s2, s2}, ll[4] = {l2, l2, l2, l2};
-            *reinterpret_cast<half8*>(to + 1024 * m) = chunk_values(k[m], ss, ll);
+            *reinterpret_cast<half8*>(to + 2048 * m) = chunk_values(k[m], ss, ll);
         }
     }
     {
@@ -330,21 +338,49 @@ QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) lo[n] = as_half2(lo4[n]);
         if (left < QMK_KV4_PAGE_TOKENS) chunk_cut(s, lo, left - 32 * half, g);      // uniform
-        uint8_t* to = sh.tile[buf] + 32768 + (8 * i + half) * 1024 + 16 * lane;
+        // dim 64 i + 16 m + c, tokens of g: block of dims 32 (2 i + (m >> 1)) .. and g >> 1
+        uint8_t* to = sh.tile[buf] + 32768 + (16 * half + 4 * i + (g >> 1)) * 1024 + 16 * (c + 32 * (g & 1));
 #pragma unroll
-        for (int m = 0; m < 4; ++m) *reinterpret_cast<half8*>(to + 2048 * m) = chunk_values(v[m], s, lo);
+        for (int m = 0; m < 4; ++m) *reinterpret_cast<half8*>(to + 2048 * (m >> 1) + 256 * (m & 1)) = chunk_values(v[m], s, lo);
     }
 }
 
 // ---- a wave's rows ---------------------------------------------------------------
-// Column f, lane (c, g): row c.  o[f][dt]: dims 16 dt + 4 g + e of it; l: the
-// lane's share of its sum.
-struct ChunkWave {
-    half8 q[CHUNK_COLS][8];            // dims 32 s + 8 g + e
-    floatx4 o[CHUNK_COLS][16];
-    float m[CHUNK_COLS], l[CHUNK_COLS];
-    int pos[CHUNK_COLS];               // -1: no row
+// A row's softmax: the reference m (-inf: none yet), from which its scores are
+// counted (0 before there is one), and as an integer the score at which a new
+// one is due.  A float's bits are in its order where it is positive, and
+// negative where it is.  l: the lane's share of the sum.
+struct ChunkSum {
+    float m, l;
+    int due;
 };
+QM_DEV ChunkSum chunk_sum() { return ChunkSum{-INFINITY, 0.0f, (int)0x80000000}; }
+QM_DEV float chunk_base(const ChunkSum& s) { return s.m == -INFINITY ? 0.0f : s.m; }
+
+// A new reference, where a row's largest score (of all its lanes) wants one;
+// returned: what its scores drop by, and the factor of its sums.
+QM_DEV float chunk_raise(ChunkSum& s, float mx, float& corr) {
+    const bool first = s.m == -INFINITY;                   // sums there may be only of NaN scores
+    const float up = first ? (mx == -INFINITY ? 0.0f : mx) : mx >= CHUNK_SLACK ? mx : 0.0f;
+    corr = first ? 1.0f : __builtin_amdgcn_exp2f(-up);
+    s.m = first ? mx : s.m + up;
+    s.due = s.m == -INFINITY ? (int)0x80000000 : __float_as_int(CHUNK_SLACK);
+    s.l *= corr;
+    return up;
+}
+// Two weights, in a word, and their sum.
+QM_DEV uint32_t chunk_pair(ChunkSum& s, float a, float b) {
+    typedef float float2_t __attribute__((ext_vector_type(2)));
+    const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+    const half2_t h = __builtin_convertvector((float2_t){__builtin_amdgcn_exp2f(a), __builtin_amdgcn_exp2f(b)}, half2_t);
+    s.l = __builtin_amdgcn_fdot2(h, ones, s.l, false);     // of what is multiplied
+    return __builtin_bit_cast(uint32_t, h);
+}
+// Whether a row at pos sees one of the half page's tokens (from k0 on) in the mask.
+QM_DEV bool chunk_sees(uint32_t mask, int pos, int k0) {
+    const int seen = pos - k0;                             // the last of them that it sees
+    return seen >= 0 && (mask & (seen >= 31 ? ~0u : (2u << seen) - 1)) != 0;
+}
 
 QM_DEV float4 bf16x4(uint2 u) {
     return make_float4(bf16_to_f32((uint16_t)(u.x & 0xffffu)), bf16_to_f32((uint16_t)(u.x >> 16)),
@@ -359,27 +395,37 @@ QM_DEV void unpack8(uint4 v, float (&x)[8]) {
     }
 }
 
-// A column's query, token i of row r: RMSNorm (1 + gamma, eps 1e-6) and RoPE
-// straight into the operand; a row's sum of squares is over the four lanes
-// c + 16 g, and the pairs (i, i + 32) of a rotation are in one lane.
-QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[8], const ChunkRow& r, int i, int head, int g) {
+// A row's query, token i of batch row r: RMSNorm (1 + gamma, eps 1e-6) and RoPE
+// straight into the operand, in which lane group g of N has dims
+// 8 N s + 8 g .. + 7 (N 4: 16 rows, lane c + 16 g; N 2: 32 rows, c + 32 g).  A
+// row's sum of squares is over its lanes, and the pairs (i, i + 32) of a
+// rotation are in one.
+template <int N>
+QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[32 / N], const ChunkRow& r, int i, int head, int g) {
+    constexpr int kSteps = 32 / N, kTurned = 4 / N;        // operands of 32 dims
     const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + 8 * g;
     const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 8 * g;
-    uint4 u[8], gq[8];
+    uint4 u[kSteps], gq[kSteps];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 32 * s);
+    for (int s = 0; s < kSteps; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 8 * N * s);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 32 * s + 8 * g);
-    const float4 c0 = ld4(A.rope_cos + at), c1 = ld4(A.rope_cos + at + 4), s0 = ld4(A.rope_sin + at), s1 = ld4(A.rope_sin + at + 4);
+    for (int s = 0; s < kSteps; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 8 * N * s + 8 * g);
+    float4 cs[2 * kTurned], sn[2 * kTurned];
+#pragma unroll
+    for (int j = 0; j < 2 * kTurned; ++j) {
+        cs[j] = ld4(A.rope_cos + at + 8 * N * (j >> 1) + 4 * (j & 1));
+        sn[j] = ld4(A.rope_sin + at + 8 * N * (j >> 1) + 4 * (j & 1));
+    }
     float ss = 0.0f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < kSteps; ++s) {
         float x[8];
         unpack8(u[s], x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
     }
-    ss = sum_xor32(sum_xor16(ss));
+    if (N == 4) ss = sum_xor16(ss);
+    ss = sum_xor32(ss);
     // the softmax's scale in base 2 as well, so that the scores come out of the product in log2 units
     const float inv = (1.4426950408889634f / 16.0f) / sqrtf(ss / (float)QM_GQA_HD + 1e-6f);
     auto normed = [&](int s, float (&x)[8]) {
@@ -391,18 +437,22 @@ QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[8], const ChunkRow& r,
             x[2 * e + 1] = x[2 * e + 1] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] >> 16)));
         }
     };
-    float x1[8], x2[8];
-    normed(0, x1);
-    normed(1, x2);
-    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        q[0][e] = (_Float16)(x1[e] * cs[e] - x2[e] * sn[e]);
-        q[1][e] = (_Float16)(x2[e] * cs[e] + x1[e] * sn[e]);
+    for (int s = 0; s < kTurned; ++s) {
+        float x1[8], x2[8];
+        normed(s, x1);
+        normed(s + kTurned, x2);
+        const float4 c0 = cs[2 * s], c1 = cs[2 * s + 1], s0 = sn[2 * s], s1 = sn[2 * s + 1];
+        const float c8[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        const float s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q[s][e] = (_Float16)(x1[e] * c8[e] - x2[e] * s8[e]);
+            q[s + kTurned][e] = (_Float16)(x2[e] * c8[e] + x1[e] * s8[e]);
+        }
     }
 #pragma unroll
-    for (int s = 2; s < 8; ++s) {
+    for (int s = 2 * kTurned; s < kSteps; ++s) {
         float x[8];
         normed(s, x);
 #pragma unroll
@@ -410,87 +460,31 @@ QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[8], const ChunkRow& r,
     }
 }
 
-// The weights of a half page's scores (runs 0, 1), and what a new maximum does
-// to the row's sums.
-QM_DEV half8 chunk_weights(floatx4 (&x)[2], floatx4 (&o)[16], float& m, float& l, int pos, int k0, bool edge, int g) {
+// The weights of a half page's scores (runs 0, 1 of 16 tokens), which come
+// counted from the reference: the products' sums begin at its negative.
+QM_DEV half8 few_weights(floatx4 (&x)[2], floatx4 (&o)[16], ChunkSum& s, int pos, int k0, bool edge, int g) {
     if (edge) {                                            // uniform: some row does not see all of it
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[r][e] = k0 + chunk_token(r, g, e) > pos ? -INFINITY : x[r][e];
+        for (int i = 0; i < 8; ++i)
+            x[i >> 2][i & 3] = k0 + chunk_token(i >> 2, g, i & 3) > pos ? -INFINITY : x[i >> 2][i & 3];
     }
-    float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    mx = max_xor32(max_xor16(mx));
-    const float was = m;
-    m = mx > was + CHUNK_SLACK ? mx : was;                 // from -inf: any score
-    if (__any(m != was)) {
-        // sums beside a maximum of -inf are those of NaN scores
-        const float corr = was == m ? 1.0f : __builtin_amdgcn_exp2f(was - m);
-        l *= corr;
+    int top = __float_as_int(x[0][0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = max(top, __float_as_int(x[i >> 2][i & 3]));
+    if (__any(top >= s.due)) {                             // seldom after the first
+        float mx = -INFINITY, corr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i >> 2][i & 3]);
+        const float up = chunk_raise(s, max_xor32(max_xor16(mx)), corr);
 #pragma unroll
         for (int dt = 0; dt < 16; ++dt) o[dt] *= corr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i >> 2][i & 3] -= up;
     }
-    const float base = m == -INFINITY ? 0.0f : m;          // a row that sees nothing yet: weights of 0
-    half8 p;
+    uintx4 p;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const _Float16 w = (_Float16)__builtin_amdgcn_exp2f(x[r][e] - base);
-            p[4 * r + e] = w;
-            l += (float)w;                                 // of what is multiplied
-        }
-    return p;
-}
-// Values that are NaN, for a row that sees their tokens; nan[group]: the half
-// page's tokens.
-QM_DEV void chunk_nan(floatx4 (&o)[16], uintx4 nan, int pos, int k0) {
-    const int seen = pos - k0;                             // the last of them that the row sees
-    const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
-    const float bad = __builtin_nanf("");
-#pragma unroll
-    for (int dt = 0; dt < 16; ++dt)
-        if (nan[dt >> 2] & mask) o[dt] = floatx4{bad, bad, bad, bad};
-}
-
-// Half a tile (32 tokens from k0 on) at a time, so that outputs, queries and
-// operands fit a wave's 256 registers.
-QM_DEV void chunk_half(ChunkWave& st, const ChunkLds& sh, int buf, int h, int k0, bool edge, int lane) {
-    const uint8_t* K = sh.tile[buf] + 16 * lane + 16384 * h;
-    const uint8_t* V = sh.tile[buf] + 16 * lane + 32768 + 1024 * h;
-    const int g = lane >> 4;
-    floatx4 x[CHUNK_COLS][2];
-#pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) x[f][r] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const half8 a = *reinterpret_cast<const half8*>(K + (8 * r + s) * 1024);
-#pragma unroll
-            for (int f = 0; f < CHUNK_COLS; ++f) x[f][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.q[f][s], x[f][r], 0, 0, 0);
-        }
-    half8 p[CHUNK_COLS];
-#pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f) p[f] = chunk_weights(x[f], st.o[f], st.m[f], st.l[f], st.pos[f], k0, edge, g);
-#pragma unroll
-    for (int dt = 0; dt < 16; ++dt) {
-        const half8 a = *reinterpret_cast<const half8*>(V + 2048 * dt);
-#pragma unroll
-        for (int f = 0; f < CHUNK_COLS; ++f) st.o[f][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[f], st.o[f][dt], 0, 0, 0);
-    }
-    const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][h]);
-    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
-#pragma unroll
-        for (int f = 0; f < CHUNK_COLS; ++f) chunk_nan(st.o[f], nan, st.pos[f], k0);
-    }
-}
-QM_DEV void chunk_tile(ChunkWave& st, const ChunkLds& sh, int buf, int k0, int first_pos, int lane) {
-    const bool edge = k0 + QMK_KV4_PAGE_TOKENS - 1 > first_pos;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) chunk_half(st, sh, buf, h, k0 + QMK_KV4_HALF_TOKENS * h, edge, lane);
+    for (int i = 0; i < 4; ++i) p[i] = chunk_pair(s, x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1]);
+    return __builtin_bit_cast(half8, p);
 }
 
 // Four outputs, gated.
@@ -511,12 +505,13 @@ QM_DEV float chunk_inverse(float l) { return l != 0.0f ? __builtin_amdgcn_rcpf(l
 struct FewLds {
     __attribute__((aligned(1024))) uint8_t ring[CHUNK_WAVES][2][QMK_KV4_HALF_BYTES];      // later o: [dim group][lane][4] f32
     float m[CHUNK_WAVES][16], l[CHUNK_WAVES][16];
+    __attribute__((aligned(16))) uint32_t odd[CHUNK_WAVES][4];
 };
 template <int NF>
 struct FewWave {
     half8 q[NF][8];
     floatx4 o[NF][16];
-    float m[NF], l[NF];
+    ChunkSum sum[NF];
     int pos[NF];
 };
 #define FEW_DMA (QMK_KV4_HALF_BYTES / 1024)
@@ -526,16 +521,17 @@ QM_DEV void few_fetch(const uint8_t* half, uint32_t buf, int lane) {
 }
 // `left` tokens of the half page are the row's.
 template <int NF>
-QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, int k0, int left, bool edge, int lane) {
+QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, uint32_t* odd, int k0, int left, bool edge, int lane) {
     const int c = lane & 15, g = lane >> 4;
     uint8_t* meta = buf + QMK_KV4_META;
-    uintx4 nan = {0, 0, 0, 0};
-    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
+    const bool mended = chunk_odd(meta, lane);
+    if (mended) chunk_mend(meta, odd, lane);
     floatx4 x[NF][2];
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) x[f][r] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int f = 0; f < NF; ++f) {
+        const float base = -chunk_base(st.sum[f]);
+        x[f][0] = x[f][1] = floatx4{base, base, base, base};
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const uint2 s4 = *reinterpret_cast<const uint2*>(meta + 2 * kv4_s_at(16 * r + c, 0));
@@ -560,7 +556,7 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, int k0, int left, bool edge,
     }
     half8 p[NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) p[f] = chunk_weights(x[f], st.o[f], st.m[f], st.l[f], st.pos[f], k0, edge, g);
+    for (int f = 0; f < NF; ++f) p[f] = few_weights(x[f], st.o[f], st.sum[f], st.pos[f], k0, edge, g);
     // scales of the lane's eight tokens, all groups: [token][group]
     uintx4 sv[4];
 #pragma unroll
@@ -583,9 +579,16 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, int k0, int left, bool edge,
             for (int f = 0; f < NF; ++f) st.o[f][4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[f], st.o[f][4 * j + m], 0, 0, 0);
         }
     }
-    if (nan[0] | nan[1] | nan[2] | nan[3]) {               // uniform
+    if (mended) {
+        const uintx4 nan = *reinterpret_cast<const uintx4*>(odd);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) chunk_nan(st.o[f], nan, st.pos[f], k0);
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float add = chunk_sees(nan[j], st.pos[f], k0) ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) st.o[f][4 * j + m] += add;
+            }
     }
 }
 
@@ -618,12 +621,11 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
     }
     bool now = fetch(0, h0);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) chunk_query(A, st.q[f], it.r, min(i0 + 4 * f + (c >> 2), it.r.n - 1), head, g);
+    for (int f = 0; f < NF; ++f) chunk_query<4>(A, st.q[f], it.r, min(i0 + 4 * f + (c >> 2), it.r.n - 1), head, g);
     bool next = fetch(1, h0 + CHUNK_WAVES);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-        st.m[f] = -INFINITY;
-        st.l[f] = 0.0f;
+        st.sum[f] = chunk_sum();
 #pragma unroll
         for (int dt = 0; dt < 16; ++dt) st.o[f][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -635,7 +637,7 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
         if (now) {
             const int k0 = QMK_KV4_HALF_TOKENS * h;
             const bool edge = k0 + QMK_KV4_HALF_TOKENS - 1 > first_pos;
-            few_half<NF>(st, buf, k0, it.r.len - k0, edge, lane);
+            few_half<NF>(st, buf, sh.odd[w], k0, it.r.len - k0, edge, lane);
         }
         if (((round + 2) & 63) == 0) ids = load_ids(round + 2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the buffer's reads are done
@@ -646,9 +648,9 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
     const bool whole = tb - ta == it.tiles;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-        const float l = sum_xor32(sum_xor16(st.l[f]));
+        const float l = sum_xor32(sum_xor16(st.sum[f].l));
         if (lane < 16) {
-            sh.m[w][lane] = st.m[f];
+            sh.m[w][lane] = st.sum[f].m;
             sh.l[w][lane] = l;
         }
         float* mine = reinterpret_cast<float*>(sh.ring[w][0]) + 4 * lane;
@@ -691,25 +693,100 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
 }
 
 // ---- many tokens ------------------------------------------------------------------
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+// Lane (c, h) = (l & 31, l >> 5) has row c: o[dt][i] is dim
+// 32 dt + 8 (i >> 2) + 4 h + (i & 3) of it.
+struct ManyWave {
+    half8 q[16];                       // dims 16 s + 8 h + e
+    floatx16 o[8];
+    ChunkSum sum;
+    int pos;                           // -1: no row
+};
+// Token (of a half page) of score i: what stands at rows 8 (i >> 2) + 4 h +
+// (i & 3) of the product.  Scores 8 k .. 8 k + 7 are those of a V operand.
+QM_DEV int many_token(int i, int h) { return 16 * ((i >> 2) & 1) + 8 * (i >> 3) + 4 * h + (i & 3); }
+
+// A product's 16 operand reads, CHUNK_AHEAD ahead of their use, so that LDS's
+// latency passes under the matrix instructions before.  The order is pinned:
+// the compiler's own had none ahead, where registers are short.
+#define CHUNK_AHEAD 3
+template <class Read, class Use>
+QM_DEV void many_product(Read read, Use use) {
+    half8 a[CHUNK_AHEAD + 1];
+#pragma unroll
+    for (int i = 0; i < CHUNK_AHEAD; ++i) a[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (i + CHUNK_AHEAD < 16) a[(i + CHUNK_AHEAD) % (CHUNK_AHEAD + 1)] = read(i + CHUNK_AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, a[i % (CHUNK_AHEAD + 1)]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Half a tile, the 32 tokens from k0 on.
+QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k0, bool edge, int lane) {
+    const uint8_t* K = sh.tile[buf] + 16 * lane + 16384 * half;
+    const uint8_t* V = K + 32768;
+    const int h = lane >> 5;
+    const float base = -chunk_base(st.sum);                // scores are counted from the reference
+    floatx16 x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = base;
+    many_product([&](int s) { return *reinterpret_cast<const half8*>(K + 1024 * s); },
+                 [&](int s, half8 a) { x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, st.q[s], x, 0, 0, 0); });
+    if (edge) {                                            // uniform: some row does not see all of it
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = k0 + many_token(i, h) > st.pos ? -INFINITY : x[i];
+    }
+    int top = __float_as_int(x[0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = max(top, __float_as_int(x[i]));
+    if (__any(top >= st.sum.due)) {                        // seldom after the first
+        float mx = -INFINITY, corr;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
+        const float up = chunk_raise(st.sum, max_xor32(mx), corr);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) st.o[dt] *= corr;
+        x -= up;
+    }
+    half8 p[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        uintx4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = chunk_pair(st.sum, x[8 * k + 2 * i], x[8 * k + 2 * i + 1]);
+        p[k] = __builtin_bit_cast(half8, w);
+    }
+    many_product([&](int i) { return *reinterpret_cast<const half8*>(V + 1024 * i); },
+                 [&](int i, half8 a) { st.o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[i & 1], st.o[i >> 1], 0, 0, 0); });
+    const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][half]);
+    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) st.o[dt] += chunk_sees(nan[dt >> 1], st.pos, k0) ? __builtin_nanf("") : 0.0f;
+    }
+}
+
+QM_DEV floatx4 many_four(const ManyWave& st, int j) {
+    const int i = 4 * (j & 3);
+    return floatx4{st.o[j >> 2][i], st.o[j >> 2][i + 1], st.o[j >> 2][i + 2], st.o[j >> 2][i + 3]};
+}
+
 template <int NF>
 QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
-    const int c = lane & 15, g = lane >> 4, head = 4 * kvh + (w & 3);
-    const int i0 = QMK_CHUNK_TOKENS * it.block + 16 * CHUNK_COLS * (w >> 2);      // the wave's first row
+    const int c = lane & 31, h = lane >> 5, head = 4 * kvh + (w & 3);
+    const int i0 = QMK_CHUNK_TOKENS * it.block + 32 * (w >> 2), i = i0 + c;      // the wave's first row, the lane's
     const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
     auto page = [&](int t) { return t < tb ? __builtin_amdgcn_readfirstlane(table[t]) : -1; };
     int now = page(ta), next = page(ta + 1), after = page(ta + 2);
     if (kv4_is_page(A.c, now)) chunk_fetch(A, sh, now, kvh, w, lane);
-    ChunkWave st;
+    ManyWave st;
+    st.pos = i < it.r.n ? it.r.len - it.r.n + i : -1;      // rows past the last: any row, never written
+    chunk_query<2>(A, st.q, it.r, min(i, it.r.n - 1), head, h);
+    st.sum = chunk_sum();
 #pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f) {
-        const int i = i0 + 16 * f + c;                     // rows past the last: any row, never written
-        st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
-        chunk_query(A, st.q[f], it.r, min(i, it.r.n - 1), head, g);
-        st.m[f] = -INFINITY;
-        st.l[f] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt) st.o[f][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int dt = 0; dt < 8; ++dt) st.o[dt] = floatx16{};
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // the row's tokens in tile t are len - 64 t
     if (kv4_is_page(A.c, now)) chunk_expand(sh, ta & 1, it.r.len - QMK_KV4_PAGE_TOKENS * ta, w, lane);
@@ -722,43 +799,42 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
         // products and half after them, so that a SIMD has one of each.
         auto prepare = [&] {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (kv4_is_page(A.c, next)) chunk_expand(sh, (t + 1) & 1, it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), w, lane);
+            if (kv4_is_page(A.c, next)) chunk_expand(sh, (t + 1) & 1, it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), w, chunk_lane(lane));
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the codes are read
-            if (kv4_is_page(A.c, after)) chunk_fetch(A, sh, after, kvh, w, lane);
+            if (kv4_is_page(A.c, after)) chunk_fetch(A, sh, after, kvh, w, chunk_lane(lane));
         };
         if (w < CHUNK_WAVES / 2) prepare();
-        if (kv4_is_page(A.c, now) && i0 < it.r.n) chunk_tile(st, sh, t & 1, QMK_KV4_PAGE_TOKENS * t, first_pos, lane);
+        if (kv4_is_page(A.c, now) && i0 < it.r.n) {
+            const int k0 = QMK_KV4_PAGE_TOKENS * t;
+            const bool edge = k0 + QMK_KV4_PAGE_TOKENS - 1 > first_pos;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) many_half(st, sh, t & 1, half, k0 + QMK_KV4_HALF_TOKENS * half, edge, chunk_lane(lane));
+        }
         if (w >= CHUNK_WAVES / 2) prepare();
         now = next;
         next = after;
         after = page(t + 3);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
-    const bool whole = tb - ta == it.tiles;
-    part += w * CHUNK_COLS * QMK_CHUNK_COLUMN;
+    const float l = sum_xor32(st.sum.l);
+    if (tb - ta == it.tiles) {
+        const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
+        const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * h;
+        uint2 x[32];
 #pragma unroll
-    for (int f = 0; f < CHUNK_COLS; ++f) {
-        const float l = sum_xor32(sum_xor16(st.l[f]));
-        const int i = i0 + 16 * f + c;
-        if (whole) {
-            const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
-            const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * g;
-            uint2 x[16];
+        for (int j = 0; j < 32; ++j) x[j] = *reinterpret_cast<const uint2*>(gate + 8 * j);
+        if (i < it.r.n) {
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) x[dt] = *reinterpret_cast<const uint2*>(gate + 16 * dt);
-            if (i < it.r.n) {
-#pragma unroll
-                for (int dt = 0; dt < 16; ++dt) chunk_out(A.out + at * QM_GQA_HD + 16 * dt + 4 * g, st.o[f][dt], chunk_inverse(l), x[dt]);
-            }
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(part + 256 * dt + 4 * lane) = st.o[f][dt];
-            if (lane < 16) {
-                part[4096 + lane] = st.m[f];
-                part[4112 + lane] = l;
-            }
-            part += QMK_CHUNK_COLUMN;
+            for (int j = 0; j < 32; ++j) chunk_out(A.out + at * QM_GQA_HD + 8 * j + 4 * h, many_four(st, j), chunk_inverse(l), x[j]);
         }
+        return;
+    }
+    part += w * 2 * QMK_CHUNK_COLUMN;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) *reinterpret_cast<floatx4*>(part + 256 * j + 4 * lane) = many_four(st, j);
+    if (lane < 32) {
+        part[8192 + lane] = st.sum.m;
+        part[8224 + lane] = l;
     }
 }
 
@@ -766,7 +842,7 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
 // there can be any).
 template <int NF, bool MANY>
 QM_DEV void chunk_attention(const GqaChunkArgs& A) {
-    constexpr int kColumns = MANY ? CHUNK_WAVES * CHUNK_COLS : NF;
+    constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;
     constexpr size_t kBytes = MANY && sizeof(ChunkLds) > sizeof(FewLds) ? sizeof(ChunkLds) : sizeof(FewLds);
     __shared__ __attribute__((aligned(1024))) uint8_t sm[kBytes];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -814,66 +890,75 @@ extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_3
 extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_many(GqaChunkArgs A) { chunk_attention<2, true>(A); }
 
 // The partial sums of a row block that several workgroups share, joined: a
-// workgroup per (row block, kv head, operand column), a wave four of the 16 dim
-// groups.
-#define CHUNK_JOIN 8                   // partials loaded at a time
+// workgroup per (row block, kv head, operand column or wave's rows, eight quads
+// of dims), a wave two of them.  N partials' loads are in flight at a time.
+struct Joined {
+    float m, l;
+    floatx4 o[2];
+};
+template <int N>
+QM_DEV void chunk_join(Joined& x, const float* first, const float* others, int n, size_t stride, int quad, int sums, int rows, int lane) {
+    const int c = lane & (rows - 1);
+    for (int s0 = 0; s0 < n; s0 += N) {                    // uniform
+        floatx4 a[N][2];
+        float pm[N], pl[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {                      // past the last: the last again, with weight 0
+            const int i = min(s0 + k, n - 1);
+            const float* part = i == 0 ? first : others + i * stride;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (quad + j) + 4 * lane);
+            pm[k] = part[sums + c];
+            pl[k] = part[sums + rows + c];
+        }
+        float top = x.m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k]);
+        const float corr = x.m == top ? 1.0f : __builtin_amdgcn_exp2f(x.m - top);
+        x.l *= corr;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x.o[j] *= corr;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            // a partial of no weight counts all the same: a NaN in it reaches the output (the last again has no other)
+            const float f = s0 + k >= n ? 0.0f : pm[k] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - top);
+            x.l = fmaf(pl[k], f, x.l);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x.o[j] += a[k][j] * f;
+        }
+        x.m = top;
+    }
+}
 template <int NF, bool MANY>
 QM_DEV void chunk_merge(const GqaChunkArgs& A) {
-    constexpr int kColumns = MANY ? CHUNK_WAVES * CHUNK_COLS : NF;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, dt0 = 4 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = MANY ? A.many * 4 * CHUNK_WAVES * CHUNK_COLS : 0;        // workgroups for blocks of many tokens
-    const bool few = (int)blockIdx.x >= first;
-    const int k = few ? blockIdx.x - first : blockIdx.x, columns = few ? NF : CHUNK_WAVES * CHUNK_COLS;
-    const int col = k % columns, kvh = (k / columns) & 3, number = k / (4 * columns);
+    constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;  // of a workgroup's partial
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int before = MANY ? A.many * 4 * CHUNK_WAVES * 4 : 0;       // workgroups for blocks of many tokens
+    const bool few = (int)blockIdx.x >= before;
+    const int k = few ? blockIdx.x - before : blockIdx.x, units = few ? NF : CHUNK_WAVES, parts = few ? 2 : 4;
+    const int quad = 8 * (k % parts) + 2 * wave, unit = k / parts % units, kvh = k / (parts * units) & 3, number = k / (4 * parts * units);
     const int count = A.counts[few];
     const ChunkRecord rec = A.records[(few ? A.many : 0) + number];
     if (number >= count || rec.from == rec.to) return;     // uniform
-    const int w = col / CHUNK_COLS;
-    const int head = 4 * kvh + (few ? c & 3 : w & 3);
-    const int i = few ? 4 * NF * rec.block + 4 * col + (c >> 2)
-                      : QMK_CHUNK_TOKENS * rec.block + 16 * CHUNK_COLS * (w >> 2) + 16 * (col % CHUNK_COLS) + c;
+    // row of the block, and first dim, of the lane's quads
+    const int rows = few ? 16 : 32, c = lane & (rows - 1), g = lane / rows;
+    const int head = 4 * kvh + (few ? c & 3 : unit & 3);
+    const int i = few ? 4 * NF * rec.block + 4 * unit + (c >> 2) : QMK_CHUNK_TOKENS * rec.block + 32 * (unit >> 2) + c;
+    const int d0 = (few ? 16 : 8) * quad + 4 * g, step = few ? 16 : 8;
     const size_t at = (size_t)(rec.begin + min(i, rec.n - 1)) * QM_GQA_HEADS + head;
-    const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 16 * dt0 + 4 * g;
-    uint2 x[4];
+    uint2 gate[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(gate + 16 * j);
-    float m = -INFINITY, l = 0.0f;
-    floatx4 o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = rec.from; s0 <= rec.to; s0 += CHUNK_JOIN) {
-        floatx4 a[CHUNK_JOIN][4];
-        float pm[CHUNK_JOIN], pl[CHUNK_JOIN];
-#pragma unroll
-        for (int n = 0; n < CHUNK_JOIN; ++n) {             // past the last: the last again, with weight 0
-            const int wg = min(s0 + n, rec.to);
-            const float* part = A.partial + ((size_t)(2 * (4 * wg + kvh) + (wg == rec.from)) * kColumns + col) * QMK_CHUNK_COLUMN;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a[n][j] = *reinterpret_cast<const floatx4*>(part + 256 * (dt0 + j) + 4 * lane);
-            pm[n] = part[4096 + c];
-            pl[n] = part[4112 + c];
-        }
-        float top = m;
-#pragma unroll
-        for (int n = 0; n < CHUNK_JOIN; ++n) top = fmaxf(top, pm[n]);
-        const float corr = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        l *= corr;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] *= corr;
-#pragma unroll
-        for (int n = 0; n < CHUNK_JOIN; ++n) {
-            if (s0 + n > rec.to) break;                    // uniform
-            // a partial of no weight counts all the same: a NaN in it reaches the output
-            const float f = pm[n] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[n] - top);
-            l = fmaf(pl[n], f, l);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += a[n][j] * f;
-        }
-        m = top;
-    }
+    for (int j = 0; j < 2; ++j) gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + d0 + j * step);
+    Joined x{-INFINITY, 0.0f, {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}};
+    // the first workgroup's part ends its run, the others' begin theirs
+    const size_t slot = (size_t)kColumns * QMK_CHUNK_COLUMN;
+    const float* base = A.partial + (size_t)(2 * (4 * rec.from + kvh)) * slot + (size_t)(few ? 1 : 2) * unit * QMK_CHUNK_COLUMN;
+    const int n = rec.to - rec.from + 1;
+    if (n <= 4) chunk_join<4>(x, base + slot, base, n, 8 * slot, quad, few ? 4096 : 8192, rows, lane);
+    else chunk_join<16>(x, base + slot, base, n, 8 * slot, quad, few ? 4096 : 8192, rows, lane);
     if (i < rec.n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) chunk_out(A.out + at * QM_GQA_HD + 16 * (dt0 + j) + 4 * g, o[j], chunk_inverse(l), x[j]);
+        for (int j = 0; j < 2; ++j) chunk_out(A.out + at * QM_GQA_HD + d0 + j * step, x.o[j], chunk_inverse(x.l), gate[j]);
     }
 }
 extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_4(GqaChunkArgs A) { chunk_merge<1, false>(A); }
