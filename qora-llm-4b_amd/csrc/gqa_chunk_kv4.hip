@@ -64,9 +64,14 @@ struct Deal {
     static constexpr int kFew = 4 * NF;
     const GqaChunkArgs& A;
     const int lane;
-    double total;                      // units of a kv head
-    double each;                       // of a workgroup
     ChunkRow mine;                     // batch row `lane`, if there are no more than 64
+    // No more row blocks than workgroups: a workgroup has a piece of one, and
+    // each block of the lane's row is cut into `cuts` of at most `piece` units.
+    bool pieces;
+    double piece;
+    int cuts;
+    // Otherwise equal runs of `each` of the `total` units of a kv head.
+    double total, each;
     double incl, units;
 
     QM_DEV static bool few(const ChunkRow& r) { return r.n <= QMK_CHUNK_FEW; }
@@ -119,9 +124,31 @@ struct Deal {
                         __builtin_amdgcn_readlane(r.kind, lane)};
     }
 
-    QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), total(0.0) {
+    QM_DEV static int cuts_of(double cost, double piece) { return (int)ceil(cost / piece); }
+
+    QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), pieces(false), piece(0.0), cuts(0), total(0.0), each(0.0), incl(0.0), units(0.0) {
+        mine = chunk_row(A, lane);
+        if (A.batch <= 64) {
+            const int nb = blocks(mine);
+            const uint32_t all = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)min(nb, 1 << 20)), 63);
+            if (all <= (uint32_t)A.groups) {
+                // the smallest piece with which they are no more than the
+                // workgroups, from an equal share on, in steps of an eighth
+                pieces = true;
+                const double most = nb ? (double)weight(mine) * tiles(mine, nb - 1) : 0.0;
+                const double least = few(mine) ? QMK_CHUNK_FEW_PIECE : QMK_CHUNK_MANY_PIECE * QMK_CHUNK_WEIGHT;
+                const bool cut = tiles(mine, max(nb - 1, 0)) > QMK_CHUNK_WHOLE || !few(mine);
+                piece = lane_of(scan(nb * most), 63) / A.groups;
+                for (;;) {
+                    cuts = !nb ? 0 : cut ? cuts_of(most, fmax(piece, least)) : 1;
+                    if (__builtin_amdgcn_readlane((int)wave_scan((uint32_t)(nb * cuts)), 63) <= A.groups) break;
+                    piece = fmax(piece, 1.0) * 1.125;
+                }
+                return;
+            }
+        }
         for (int b0 = 0; b0 < A.batch; b0 += 64) {         // uniform
-            mine = chunk_row(A, b0 + lane);
+            if (A.batch > 64) mine = chunk_row(A, b0 + lane);
             units = row_units(mine);
             incl = scan(units);
             total += lane_of(incl, 63);
@@ -179,6 +206,24 @@ struct Deal {
         it.first = lane_of(it.first + before(it.r, it.block) * w, 0);
         it.number = number[few(it.r)] + it.block;
         return it;
+    }
+    // Piece i: its row block, and which of its pages; false: there is none.
+    QM_DEV bool find_piece(int i, Item& it, int& ta, int& tb, int& n) const {
+        const int nb = blocks(mine), all = nb * cuts, in = (int)wave_scan((uint32_t)all);
+        if (i >= __builtin_amdgcn_readlane(in, 63)) return false;
+        const int at = __popcll(__ballot(in <= i));
+        it.r = lane_of(mine, at);
+        const int k = __builtin_amdgcn_readlane(cuts, at), rest = i - __builtin_amdgcn_readlane(in - all, at);
+        it.block = __builtin_amdgcn_readfirstlane((int)((uint32_t)rest / (uint32_t)k));
+        it.tiles = __builtin_amdgcn_readfirstlane(tiles(it.r, it.block));
+        it.first = 0.0;
+        const uint32_t same = lane < at && few(mine) == few(it.r) ? (uint32_t)nb : 0u;
+        it.number = __builtin_amdgcn_readlane((int)wave_scan(same), 63) + it.block;
+        const int q = rest - it.block * k;
+        n = min(k, it.tiles);                              // shorter blocks of the row are cut less finely
+        ta = (int)((int64_t)it.tiles * q / n);
+        tb = (int)((int64_t)it.tiles * (q + 1) / n);
+        return q < n;
     }
     // Where workgroup i begins: a multiple of `each`, but whole pages, and none
     // inside a block of few pages.
@@ -858,19 +903,26 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
         if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
     }
-    const double end = deal.begin(index + 1);
-    for (double u = deal.begin(index); u < end;) {         // uniform, as all of it
-        const typename Deal<NF>::Item it = deal.find(u, true);
-        const int weight = Deal<NF>::weight(it.r);
-        const bool few = Deal<NF>::few(it.r);
-        const int ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
-        const int tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
-        u = it.first + (double)tb * weight;
-        if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few)) {
-            ChunkRecord r{index, index, it.r.begin, it.r.n, it.block, {0, 0, 0}};
-            if (tb < it.tiles) r.to = (int)((it.first + (double)it.tiles * weight - 1.0) / deal.each);
-            A.records[(few ? A.many : 0) + it.number] = r;
+    const double end = deal.pieces ? 0.0 : deal.begin(index + 1);
+    for (double u = deal.pieces ? -1.0 : deal.begin(index); u < end;) {      // uniform, as all of it
+        typename Deal<NF>::Item it;
+        int ta, tb, last;                                  // the block's last workgroup
+        if (deal.pieces) {
+            int n;
+            if (!deal.find_piece(index, it, ta, tb, n)) return;
+            last = index + n - 1;
+            u = end;
+        } else {
+            it = deal.find(u, true);
+            const int weight = Deal<NF>::weight(it.r);
+            ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
+            tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
+            last = tb == it.tiles ? index : (int)((it.first + (double)it.tiles * weight - 1.0) / deal.each);
+            u = it.first + (double)tb * weight;
         }
+        const bool few = Deal<NF>::few(it.r);
+        if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few))
+            A.records[(few ? A.many : 0) + it.number] = ChunkRecord{index, last, it.r.begin, it.r.n, it.block, {0, 0, 0}};
         if (it.r.kind != CHUNK_RUN) {
             const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;
             const int i0 = Deal<NF>::tokens(it.r) * it.block, count = min(Deal<NF>::tokens(it.r), it.r.n - i0);

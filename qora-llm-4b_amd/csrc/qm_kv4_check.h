@@ -170,11 +170,11 @@ inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t
     c.most_many = c.many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
     c.most_few = t / block + b < b * (QMK_CHUNK_FEW / block) ? t / block + b : b * (QMK_CHUNK_FEW / block);
     const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
-    c.split = tiles > QMK_CHUNK_WHOLE;
+    c.split = c.many || tiles > QMK_CHUNK_WHOLE;
     // rows that are refused for their new tokens are written in blocks of many
     const int64_t blocks = c.most_few + t / QMK_CHUNK_TOKENS + with_many;
     const int64_t most = cus / 4 > 0 ? cus / 4 : 1;
-    const int64_t parts = c.split ? (tiles * QMK_CHUNK_WEIGHT + QMK_CHUNK_MIN_UNITS - 1) / QMK_CHUNK_MIN_UNITS : 1;
+    const int64_t parts = c.split ? tiles : 1;
     c.groups = blocks >= most || blocks * parts >= most ? most : blocks * parts;
     if (c.groups < 1) c.groups = 1;
     c.split = c.split && c.groups > 1;
