@@ -221,8 +221,9 @@ struct Deal {
         it.number = __builtin_amdgcn_readlane((int)wave_scan(same), 63) + it.block;
         const int q = rest - it.block * k;
         n = min(k, it.tiles);                              // shorter blocks of the row are cut less finely
-        ta = (int)((int64_t)it.tiles * q / n);
-        tb = (int)((int64_t)it.tiles * (q + 1) / n);
+        // (at most 2^25 pages and QMK_CHUNK_MAX_GROUPS pieces)
+        ta = __builtin_amdgcn_readfirstlane((int)((uint32_t)it.tiles * (uint32_t)q / (uint32_t)n));
+        tb = __builtin_amdgcn_readfirstlane((int)((uint32_t)it.tiles * (uint32_t)(q + 1) / (uint32_t)n));
         return q < n;
     }
     // Where workgroup i begins: a multiple of `each`, but whole pages, and none
@@ -238,6 +239,16 @@ struct Deal {
     }
 };
 
+// Groups whose V is NaN, of the half page's tokens: bit 4 t + group.
+struct ChunkNan {
+    uint64_t low, high;
+};
+// Whether a row at pos sees one of them, of the half page's from k0 on.
+QM_DEV bool chunk_sees(const ChunkNan& nan, int group, int pos, int k0) {
+    const int n = min(max(pos - k0 + 1, 0), QMK_KV4_HALF_TOKENS);            // tokens that it sees
+    const uint64_t low = n >= 16 ? ~0ull : (1ull << (4 * n)) - 1, high = n >= 32 ? ~0ull : n <= 16 ? 0ull : (1ull << (4 * n - 64)) - 1;
+    return ((nan.low & low) | (nan.high & high)) & 0x1111111111111111ull << group;
+}
 // ---- a tile -------------------------------------------------------------------
 // LDS: two buffers of f16 operands, block entry l the 16 bytes that lane l
 // reads for a product:
@@ -251,8 +262,7 @@ struct Deal {
 struct ChunkLds {
     __attribute__((aligned(1024))) uint8_t tile[2][CHUNK_TILE];
     __attribute__((aligned(1024))) uint8_t raw[CHUNK_WAVES][3][1024];
-    __attribute__((aligned(16))) uint32_t nan[2][2][4];      // [buffer][half][group]: tokens whose V is NaN there
-    __attribute__((aligned(16))) uint32_t odd[CHUNK_WAVES][4];
+    ChunkNan nan[2][2];                // [buffer][half]
 };
 
 QM_DEV uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
@@ -323,11 +333,10 @@ QM_DEV bool chunk_odd(const uint8_t* meta, int lane) {
 }
 // Puts such a half page right, in LDS.  A scale that takes the group past
 // f16's largest value becomes the next lower one.  V that is NaN becomes 0, and
-// its tokens (a bit each, a word per group) are noted in nan[4]: the rows that
-// see them are given the NaN beside the product, as a weight of 0 times it
-// would give it to the others too.
-QM_DEV void chunk_mend(uint8_t* meta, uint32_t* nan, int lane) {
-    if (lane < 4) nan[lane] = 0;
+// is returned: the rows that see it are given the NaN beside the product, as a
+// weight of 0 times it would give it to the others too.
+QM_DEV ChunkNan chunk_mend(uint8_t* meta, int lane) {
+    uint64_t nan[2];
 #pragma unroll
     for (int is_v = 0; is_v < 2; ++is_v)
 #pragma unroll
@@ -337,12 +346,11 @@ QM_DEV void chunk_mend(uint8_t* meta, uint32_t* nan, int lane) {
             uint16_t* lo = reinterpret_cast<uint16_t*>(meta + 512 * is_v + 256) + kv4_lo_at(t, group);
             const float top = fmaf(15.0f, f16_to_f32(*s), f16_to_f32(*lo));
             if (top >= 65520.0f) *s = *s - 1;
-            if (is_v && top != top) {
-                *s = *lo = 0;
-                atomicOr(nan + group, 1u << t);
-            }
+            nan[k] = __ballot(is_v && top != top);
+            if (is_v && top != top) *s = *lo = 0;
         }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read again as other types
+    asm volatile("" ::: "memory");                         // read again as other types
+    return ChunkNan{nan[0], nan[1]};
 }
 
 // The wave's part of a tile of which `left` tokens are the row's (64 and more:
@@ -352,12 +360,9 @@ QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
     uint8_t* meta = sh.raw[w][2];
     const int half = w >> 2, i = w & 3, c = lane & 15, g = lane >> 4;
     const int run = i >> 1, dims = i & 1;
-    uint32_t nan = 0;
-    if (chunk_odd(meta, lane)) {
-        chunk_mend(meta, sh.odd[w], lane);
-        nan = sh.odd[w][i];
-    }
-    if (lane == 0) sh.nan[buf][half][i] = nan;
+    ChunkNan nan{0, 0};
+    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
+    if (i == 0 && lane == 0) sh.nan[buf][half] = nan;
     {
         const uintx4 k = *reinterpret_cast<const uintx4*>(raw + 16 * lane);
         const half2_t s = as_half2(*reinterpret_cast<const uint32_t*>(meta + 2 * kv4_s_at(16 * run + c, 2 * dims)));
@@ -421,87 +426,74 @@ QM_DEV uint32_t chunk_pair(ChunkSum& s, float a, float b) {
     s.l = __builtin_amdgcn_fdot2(h, ones, s.l, false);     // of what is multiplied
     return __builtin_bit_cast(uint32_t, h);
 }
-// Whether a row at pos sees one of the half page's tokens (from k0 on) in the mask.
-QM_DEV bool chunk_sees(uint32_t mask, int pos, int k0) {
-    const int seen = pos - k0;                             // the last of them that it sees
-    return seen >= 0 && (mask & (seen >= 31 ? ~0u : (2u << seen) - 1)) != 0;
-}
-
 QM_DEV float4 bf16x4(uint2 u) {
     return make_float4(bf16_to_f32((uint16_t)(u.x & 0xffffu)), bf16_to_f32((uint16_t)(u.x >> 16)),
                        bf16_to_f32((uint16_t)(u.y & 0xffffu)), bf16_to_f32((uint16_t)(u.y >> 16)));
 }
-QM_DEV void unpack8(uint4 v, float (&x)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// Sum of squares of the bf16 pairs of four words.
+QM_DEV float chunk_squares(uint4 u, float ss) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[2 * e] = bf16_to_f32((uint16_t)(w[e] & 0xffffu));
-        x[2 * e + 1] = bf16_to_f32((uint16_t)(w[e] >> 16));
+    for (int i = 0; i < 4; ++i) {
+        const bf16x2_t x = __builtin_bit_cast(bf16x2_t, w[i]);
+        ss = __builtin_amdgcn_fdot2_f32_bf16(x, x, ss, false);
+    }
+    return ss;
+}
+// Eight bf16 values times inv (1 + gamma).
+QM_DEV void chunk_normed(float (&x)[8], uint4 u, uint4 gamma, float inv) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w}, gw[4] = {gamma.x, gamma.y, gamma.z, gamma.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2_t gv = as_half2(gw[i]);
+        const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+        x[2 * i] = fmaf(a, (float)gv[0], a);
+        x[2 * i + 1] = fmaf(b, (float)gv[1], b);
     }
 }
+// 1 / rms of a row, and the softmax's scale in base 2 as well: the scores come
+// out of the product in log2 units.
+QM_DEV float chunk_inv(float ss) {
+    return (1.4426950408889634f / 16.0f) * __builtin_amdgcn_rsqf(ss * (1.0f / QM_GQA_HD) + 1e-6f);
+}
 
-// A row's query, token i of batch row r: RMSNorm (1 + gamma, eps 1e-6) and RoPE
-// straight into the operand, in which lane group g of N has dims
-// 8 N s + 8 g .. + 7 (N 4: 16 rows, lane c + 16 g; N 2: 32 rows, c + 32 g).  A
-// row's sum of squares is over its lanes, and the pairs (i, i + 32) of a
-// rotation are in one.
-template <int N>
-QM_DEV void chunk_query(const GqaChunkArgs& A, half8 (&q)[32 / N], const ChunkRow& r, int i, int head, int g) {
-    constexpr int kSteps = 32 / N, kTurned = 4 / N;        // operands of 32 dims
-    const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + 8 * g;
-    const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 8 * g;
-    uint4 u[kSteps], gq[kSteps];
+// The queries of a block's columns, RMSNorm (1 + gamma, eps 1e-6) and RoPE: 16
+// lanes have a row, lane j dims 16 j .. + 15, so that a wave does four of them
+// and the rotation's pairs (i, i + 32) are two lanes apart.
+template <int NF>
+QM_DEV void few_queries(const GqaChunkArgs& A, uint8_t (&q)[NF][8][1024], const ChunkRow& r, int i0, int kvh, int w, int lane) {
+    const int j = lane & 15, col = 4 * w + (lane >> 4);
+    if (col >= 16 * NF) return;                            // uniform
+    const int i = min(i0 + (col >> 2), r.n - 1);           // columns past the last token: any row, never written
+    const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + 4 * kvh + (col & 3)) * (2 * QM_GQA_HD) + 16 * j;
+    const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 16 * (j & 1);
+    uint4 u[2], gq[2];
+    float4 cs[4], sn[4];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 8 * N * s);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 8 * N * s + 8 * g);
-    float4 cs[2 * kTurned], sn[2 * kTurned];
-#pragma unroll
-    for (int j = 0; j < 2 * kTurned; ++j) {
-        cs[j] = ld4(A.rope_cos + at + 8 * N * (j >> 1) + 4 * (j & 1));
-        sn[j] = ld4(A.rope_sin + at + 8 * N * (j >> 1) + 4 * (j & 1));
+    for (int k = 0; k < 2; ++k) {
+        u[k] = reinterpret_cast<const uint4*>(row)[k];
+        gq[k] = reinterpret_cast<const uint4*>(A.q_norm + 16 * j)[k];
     }
-    float ss = 0.0f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
+    for (int k = 0; k < 4; ++k) {
+        cs[k] = ld4(A.rope_cos + at + 4 * k);
+        sn[k] = ld4(A.rope_sin + at + 4 * k);
+    }
+    const float inv = chunk_inv(row_sum16(chunk_squares(u[1], chunk_squares(u[0], 0.0f))));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
         float x[8];
-        unpack8(u[s], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    }
-    if (N == 4) ss = sum_xor16(ss);
-    ss = sum_xor32(ss);
-    // the softmax's scale in base 2 as well, so that the scores come out of the product in log2 units
-    const float inv = (1.4426950408889634f / 16.0f) / sqrtf(ss / (float)QM_GQA_HD + 1e-6f);
-    auto normed = [&](int s, float (&x)[8]) {
-        unpack8(u[s], x);
-        const uint32_t gv[4] = {gq[s].x, gq[s].y, gq[s].z, gq[s].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[2 * e] = x[2 * e] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] & 0xffffu)));
-            x[2 * e + 1] = x[2 * e + 1] * inv * (1.0f + f16_to_f32((uint16_t)(gv[e] >> 16)));
-        }
-    };
-#pragma unroll
-    for (int s = 0; s < kTurned; ++s) {
-        float x1[8], x2[8];
-        normed(s, x1);
-        normed(s + kTurned, x2);
-        const float4 c0 = cs[2 * s], c1 = cs[2 * s + 1], s0 = sn[2 * s], s1 = sn[2 * s + 1];
-        const float c8[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        chunk_normed(x, u[k], gq[k], inv);
+        const float c8[8] = {cs[2 * k].x, cs[2 * k].y, cs[2 * k].z, cs[2 * k].w, cs[2 * k + 1].x, cs[2 * k + 1].y, cs[2 * k + 1].z, cs[2 * k + 1].w};
+        const float s8[8] = {sn[2 * k].x, sn[2 * k].y, sn[2 * k].z, sn[2 * k].w, sn[2 * k + 1].x, sn[2 * k + 1].y, sn[2 * k + 1].z, sn[2 * k + 1].w};
+        half8 out;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            q[s][e] = (_Float16)(x1[e] * c8[e] - x2[e] * s8[e]);
-            q[s + kTurned][e] = (_Float16)(x2[e] * c8[e] + x1[e] * s8[e]);
+            const float p = dpp_f32<0x4E>(x[e]);
+            out[e] = (_Float16)(j >= 4 ? x[e] : x[e] * c8[e] + (j < 2 ? -p : p) * s8[e]);
         }
-    }
-#pragma unroll
-    for (int s = 2 * kTurned; s < kSteps; ++s) {
-        float x[8];
-        normed(s, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)x[e];
+        *reinterpret_cast<half8*>(&q[col >> 4][j >> 1][16 * ((col & 15) + 16 * (2 * (j & 1) + k))]) = out;
     }
 }
 
@@ -547,14 +539,16 @@ QM_DEV float chunk_inverse(float l) { return l != 0.0f ? __builtin_amdgcn_rcpf(l
 // column 4 tokens of the four heads.  Every wave has all columns and every
 // eighth half page, whose codes come by LDS DMA, two ahead, and become operands
 // in its registers; the waves' sums are joined at the end.
+// The queries stand in LDS as operands, block 8 f + s: entry l the 16 bytes that
+// lane l = (c, g) reads, dims 32 s + 8 g .. of column 16 f + c.
+template <int NF>
 struct FewLds {
-    __attribute__((aligned(1024))) uint8_t ring[CHUNK_WAVES][2][QMK_KV4_HALF_BYTES];      // later o: [dim group][lane][4] f32
-    float m[CHUNK_WAVES][16], l[CHUNK_WAVES][16];
-    __attribute__((aligned(16))) uint32_t odd[CHUNK_WAVES][4];
+    // later of each wave o [dim group][lane][4] f32, then m[16], l[16]
+    __attribute__((aligned(1024))) uint8_t ring[CHUNK_WAVES][2][QMK_KV4_HALF_BYTES];
+    __attribute__((aligned(1024))) uint8_t q[NF][8][1024];
 };
 template <int NF>
 struct FewWave {
-    half8 q[NF][8];
     floatx4 o[NF][16];
     ChunkSum sum[NF];
     int pos[NF];
@@ -566,36 +560,44 @@ QM_DEV void few_fetch(const uint8_t* half, uint32_t buf, int lane) {
 }
 // `left` tokens of the half page are the row's.
 template <int NF>
-QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, uint32_t* odd, int k0, int left, bool edge, int lane) {
+QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][1024], int k0, int left, bool edge, int lane) {
     const int c = lane & 15, g = lane >> 4;
     uint8_t* meta = buf + QMK_KV4_META;
-    const bool mended = chunk_odd(meta, lane);
-    if (mended) chunk_mend(meta, odd, lane);
+    ChunkNan nan{0, 0};
+    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
     floatx4 x[NF][2];
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const float base = -chunk_base(st.sum[f]);
         x[f][0] = x[f][1] = floatx4{base, base, base, base};
     }
+    half2_t s[2][2];                                       // of the lane's token of each run
+    _Float16 lo[2][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const uint2 s4 = *reinterpret_cast<const uint2*>(meta + 2 * kv4_s_at(16 * r + c, 0));
-        const half2_t s01 = as_half2(s4.x), s23 = as_half2(s4.y);
-        _Float16 lo[4];
+        s[r][0] = as_half2(s4.x), s[r][1] = as_half2(s4.y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) lo[j] = *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * r + c, j));
+        for (int j = 0; j < 4; ++j) lo[r][j] = *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * r + c, j));
+    }
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            const uintx4 k = *reinterpret_cast<const uintx4*>(buf + 1024 * (2 * r + d) + 16 * lane);
+    for (int d = 0; d < 2; ++d) {
+        uintx4 k[2];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+        for (int r = 0; r < 2; ++r) k[r] = *reinterpret_cast<const uintx4*>(buf + 1024 * (2 * r + d) + 16 * lane);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            half8 qf[NF];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) qf[f] = *reinterpret_cast<const half8*>(&q[f][4 * d + m][16 * lane]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
                 const int j = 2 * d + (m >> 1);            // the words' group
-                const _Float16 sj = j < 2 ? s01[j & 1] : s23[j & 1];
-                const half2_t s2 = {sj, sj}, l2 = {lo[j], lo[j]};
+                const half2_t s2 = {s[r][d][m >> 1], s[r][d][m >> 1]}, l2 = {lo[r][j], lo[r][j]};
                 const half2_t ss[4] = {s2, s2, s2, s2}, ll[4] = {l2, l2, l2, l2};
-                const half8 a = chunk_values(k[m], ss, ll);
+                const half8 a = chunk_values(k[r][m], ss, ll);
 #pragma unroll
-                for (int f = 0; f < NF; ++f) x[f][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.q[f][4 * d + m], x[f][r], 0, 0, 0);
+                for (int f = 0; f < NF; ++f) x[f][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[f], x[f][r], 0, 0, 0);
             }
         }
     }
@@ -624,13 +626,12 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, uint32_t* odd, int k0, int l
             for (int f = 0; f < NF; ++f) st.o[f][4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[f], st.o[f][4 * j + m], 0, 0, 0);
         }
     }
-    if (mended) {
-        const uintx4 nan = *reinterpret_cast<const uintx4*>(odd);
+    if (nan.low | nan.high) {                              // uniform
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float add = chunk_sees(nan[j], st.pos[f], k0) ? __builtin_nanf("") : 0.0f;
+                const float add = chunk_sees(nan, j, st.pos[f], k0) ? __builtin_nanf("") : 0.0f;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) st.o[f][4 * j + m] += add;
             }
@@ -638,7 +639,7 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, uint32_t* odd, int k0, int l
 }
 
 template <int NF>
-QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
+QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
     const int c = lane & 15, g = lane >> 4, head = 4 * kvh + (c & 3);
     const int i0 = 4 * NF * it.block, first_pos = it.r.len - it.r.n + i0;
     const int end = it.r.len - it.r.n + min(it.r.n, i0 + 4 * NF);             // past the block's last token
@@ -665,9 +666,9 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
         st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
     }
     bool now = fetch(0, h0);
-#pragma unroll
-    for (int f = 0; f < NF; ++f) chunk_query<4>(A, st.q[f], it.r, min(i0 + 4 * f + (c >> 2), it.r.n - 1), head, g);
+    few_queries<NF>(A, sh.q, it.r, i0, kvh, w, lane);
     bool next = fetch(1, h0 + CHUNK_WAVES);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         st.sum[f] = chunk_sum();
@@ -682,7 +683,7 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
         if (now) {
             const int k0 = QMK_KV4_HALF_TOKENS * h;
             const bool edge = k0 + QMK_KV4_HALF_TOKENS - 1 > first_pos;
-            few_half<NF>(st, buf, sh.odd[w], k0, it.r.len - k0, edge, lane);
+            few_half<NF>(st, buf, sh.q, k0, it.r.len - k0, edge, lane);
         }
         if (((round + 2) & 63) == 0) ids = load_ids(round + 2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the buffer's reads are done
@@ -694,13 +695,13 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const float l = sum_xor32(sum_xor16(st.sum[f].l));
-        if (lane < 16) {
-            sh.m[w][lane] = st.sum[f].m;
-            sh.l[w][lane] = l;
-        }
-        float* mine = reinterpret_cast<float*>(sh.ring[w][0]) + 4 * lane;
+        float* mine = reinterpret_cast<float*>(sh.ring[w][0]);
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt) = st.o[f][dt];
+        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt + 4 * lane) = st.o[f][dt];
+        if (lane < 16) {
+            mine[4096 + lane] = st.sum[f].m;
+            mine[4112 + lane] = l;
+        }
         const int i = i0 + 4 * f + (c >> 2);
         const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
         uint2 gate[2];
@@ -710,15 +711,15 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds& sh, const typename Deal<NF>:
         __syncthreads();
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, sh.m[k][c]);
+        for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, reinterpret_cast<const float*>(sh.ring[k][0])[4096 + c]);
         floatx4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int k = 0; k < CHUNK_WAVES; ++k) {
-            const float e = sh.m[k][c] == M ? 1.0f : __builtin_amdgcn_exp2f(sh.m[k][c] - M);
-            L = fmaf(sh.l[k][c], e, L);
-            const float* a = reinterpret_cast<const float*>(sh.ring[k][0]) + 4 * lane + 512 * w;
+            const float* a = reinterpret_cast<const float*>(sh.ring[k][0]);
+            const float e = a[4096 + c] == M ? 1.0f : __builtin_amdgcn_exp2f(a[4096 + c] - M);
+            L = fmaf(a[4112 + c], e, L);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const floatx4*>(a + 256 * j) * e;
+            for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const floatx4*>(a + 512 * w + 256 * j + 4 * lane) * e;
         }
         if (!whole) {
             float* to = part + f * QMK_CHUNK_COLUMN;
@@ -769,6 +770,49 @@ QM_DEV void many_product(Read read, Use use) {
     }
 }
 
+// The rows' queries, RMSNorm (1 + gamma, eps 1e-6) and RoPE straight into the
+// operand: a row is in lanes c and c + 32, and the rotation's pairs (i, i + 32)
+// in one.
+QM_DEV void many_query(const GqaChunkArgs& A, half8 (&q)[16], const ChunkRow& r, int i, int head, int h) {
+    const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + 8 * h;
+    const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 8 * h;
+    uint4 u[16], gq[16];
+    float4 cs[4], sn[4];
+#pragma unroll
+    for (int s = 0; s < 16; ++s) u[s] = *reinterpret_cast<const uint4*>(row + 16 * s);
+#pragma unroll
+    for (int s = 0; s < 16; ++s) gq[s] = *reinterpret_cast<const uint4*>(A.q_norm + 16 * s + 8 * h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        cs[j] = ld4(A.rope_cos + at + 16 * (j >> 1) + 4 * (j & 1));
+        sn[j] = ld4(A.rope_sin + at + 16 * (j >> 1) + 4 * (j & 1));
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 16; ++s) ss = chunk_squares(u[s], ss);
+    const float inv = chunk_inv(sum_xor32(ss));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        float x1[8], x2[8];
+        chunk_normed(x1, u[s], gq[s], inv);
+        chunk_normed(x2, u[s + 2], gq[s + 2], inv);
+        const float c8[8] = {cs[2 * s].x, cs[2 * s].y, cs[2 * s].z, cs[2 * s].w, cs[2 * s + 1].x, cs[2 * s + 1].y, cs[2 * s + 1].z, cs[2 * s + 1].w};
+        const float s8[8] = {sn[2 * s].x, sn[2 * s].y, sn[2 * s].z, sn[2 * s].w, sn[2 * s + 1].x, sn[2 * s + 1].y, sn[2 * s + 1].z, sn[2 * s + 1].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q[s][e] = (_Float16)(x1[e] * c8[e] - x2[e] * s8[e]);
+            q[s + 2][e] = (_Float16)(x2[e] * c8[e] + x1[e] * s8[e]);
+        }
+    }
+#pragma unroll
+    for (int s = 4; s < 16; ++s) {
+        float x[8];
+        chunk_normed(x, u[s], gq[s], inv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)x[e];
+    }
+}
+
 // Half a tile, the 32 tokens from k0 on.
 QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k0, bool edge, int lane) {
     const uint8_t* K = sh.tile[buf] + 16 * lane + 16384 * half;
@@ -806,10 +850,10 @@ QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k
     }
     many_product([&](int i) { return *reinterpret_cast<const half8*>(V + 1024 * i); },
                  [&](int i, half8 a) { st.o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[i & 1], st.o[i >> 1], 0, 0, 0); });
-    const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][half]);
-    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
+    const ChunkNan nan = sh.nan[buf][half];
+    if (__builtin_amdgcn_readfirstlane((int)((nan.low | nan.high) != 0))) {
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) st.o[dt] += chunk_sees(nan[dt >> 1], st.pos, k0) ? __builtin_nanf("") : 0.0f;
+        for (int dt = 0; dt < 8; ++dt) st.o[dt] += chunk_sees(nan, dt >> 1, st.pos, k0) ? __builtin_nanf("") : 0.0f;
     }
 }
 
@@ -824,42 +868,37 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
     const int i0 = QMK_CHUNK_TOKENS * it.block + 32 * (w >> 2), i = i0 + c;      // the wave's first row, the lane's
     const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
     auto page = [&](int t) { return t < tb ? __builtin_amdgcn_readfirstlane(table[t]) : -1; };
-    int now = page(ta), next = page(ta + 1), after = page(ta + 2);
-    if (kv4_is_page(A.c, now)) chunk_fetch(A, sh, now, kvh, w, lane);
+    int id = page(ta), next = page(ta + 1), done = -1;     // of tiles t, t + 1, t - 1
+    if (kv4_is_page(A.c, id)) chunk_fetch(A, sh, id, kvh, w, lane);
     ManyWave st;
     st.pos = i < it.r.n ? it.r.len - it.r.n + i : -1;      // rows past the last: any row, never written
-    chunk_query<2>(A, st.q, it.r, min(i, it.r.n - 1), head, h);
+    many_query(A, st.q, it.r, min(i, it.r.n - 1), head, h);
     st.sum = chunk_sum();
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) st.o[dt] = floatx16{};
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    // the row's tokens in tile t are len - 64 t
-    if (kv4_is_page(A.c, now)) chunk_expand(sh, ta & 1, it.r.len - QMK_KV4_PAGE_TOKENS * ta, w, lane);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, lane);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int first_pos = it.r.len - it.r.n + i0;
-    for (int t = ta; t < tb; ++t) {
-        // Half of the waves make the next tile's operands before their
-        // products and half after them, so that a SIMD has one of each.
-        auto prepare = [&] {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (kv4_is_page(A.c, next)) chunk_expand(sh, (t + 1) & 1, it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), w, chunk_lane(lane));
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the codes are read
-            if (kv4_is_page(A.c, after)) chunk_fetch(A, sh, after, kvh, w, chunk_lane(lane));
-        };
-        if (w < CHUNK_WAVES / 2) prepare();
-        if (kv4_is_page(A.c, now) && i0 < it.r.n) {
-            const int k0 = QMK_KV4_PAGE_TOKENS * t;
+    // Every wave makes its part of tile t and then multiplies a tile: half of
+    // them tile t - 1, before the barrier that says that tile t is made, and
+    // half tile t, after it.  So a SIMD has one of each, and a buffer is made
+    // anew only when all have read it.
+    const bool late = w >= CHUNK_WAVES / 2;
+    for (int t = ta; t <= tb; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (kv4_is_page(A.c, id)) chunk_expand(sh, t & 1, it.r.len - QMK_KV4_PAGE_TOKENS * t, w, chunk_lane(lane));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the codes are read
+        if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, chunk_lane(lane));
+        if (late) asm volatile("s_barrier" ::: "memory");
+        const int at = late ? t : t - 1;
+        if (kv4_is_page(A.c, late ? id : done) && i0 < it.r.n) {
+            const int k0 = QMK_KV4_PAGE_TOKENS * at;
             const bool edge = k0 + QMK_KV4_PAGE_TOKENS - 1 > first_pos;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) many_half(st, sh, t & 1, half, k0 + QMK_KV4_HALF_TOKENS * half, edge, chunk_lane(lane));
+#pragma clang loop unroll(disable)
+            for (int half = 0; half < 2; ++half) many_half(st, sh, at & 1, half, k0 + QMK_KV4_HALF_TOKENS * half, edge, chunk_lane(lane));
         }
-        if (w >= CHUNK_WAVES / 2) prepare();
-        now = next;
-        next = after;
-        after = page(t + 3);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        done = id;
+        id = next;
+        next = page(t + 2);
+        if (!late) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     const float l = sum_xor32(st.sum.l);
     if (tb - ta == it.tiles) {
@@ -888,7 +927,7 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
 template <int NF, bool MANY>
 QM_DEV void chunk_attention(const GqaChunkArgs& A) {
     constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;
-    constexpr size_t kBytes = MANY && sizeof(ChunkLds) > sizeof(FewLds) ? sizeof(ChunkLds) : sizeof(FewLds);
+    constexpr size_t kBytes = MANY && sizeof(ChunkLds) > sizeof(FewLds<NF>) ? sizeof(ChunkLds) : sizeof(FewLds<NF>);
     __shared__ __attribute__((aligned(1024))) uint8_t sm[kBytes];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2;
@@ -934,7 +973,7 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         // a workgroup's first block may have begun before it, its last end after it
         float* part = A.partial + (size_t)(2 * blockIdx.x + (ta == 0)) * kColumns * QMK_CHUNK_COLUMN;
         if (MANY && !few) many_item<NF>(A, *reinterpret_cast<ChunkLds*>(sm), it, ta, tb, kvh, part, w, lane);
-        else few_item<NF>(A, *reinterpret_cast<FewLds*>(sm), it, ta, tb, kvh, part, w, lane);
+        else few_item<NF>(A, *reinterpret_cast<FewLds<NF>*>(sm), it, ta, tb, kvh, part, w, lane);
     }
 }
 extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_4(GqaChunkArgs A) { chunk_attention<1, false>(A); }

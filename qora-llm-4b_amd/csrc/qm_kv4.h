@@ -44,6 +44,7 @@
 #define QMK_CHUNK_MANY_PIECE 3      // and of many
 #define QMK_CHUNK_MIN_UNITS 4       // the same where workgroups have runs of several blocks
 #define QMK_CHUNK_WHOLE 8           // a row block of so many pages falls to one
+#define QMK_CHUNK_MAX_GROUPS 64     // workgroups per kv head
 #define QMK_CHUNK_COLUMN 4128       // f32 of an operand column's partial: 16 dim groups x 256, m[16], l[16]
 
 #ifdef __HIPCC__

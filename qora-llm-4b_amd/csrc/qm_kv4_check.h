@@ -173,7 +173,7 @@ inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t
     c.split = c.many || tiles > QMK_CHUNK_WHOLE;
     // rows that are refused for their new tokens are written in blocks of many
     const int64_t blocks = c.most_few + t / QMK_CHUNK_TOKENS + with_many;
-    const int64_t most = cus / 4 > 0 ? cus / 4 : 1;
+    const int64_t quarter = cus / 4 > 0 ? cus / 4 : 1, most = quarter < QMK_CHUNK_MAX_GROUPS ? quarter : QMK_CHUNK_MAX_GROUPS;
     const int64_t parts = c.split ? tiles : 1;
     c.groups = blocks >= most || blocks * parts >= most ? most : blocks * parts;
     if (c.groups < 1) c.groups = 1;
