@@ -125,6 +125,16 @@ struct Deal {
     }
 
     QM_DEV static int cuts_of(double cost, double piece) { return (int)ceil(cost / piece); }
+    // Blocks of many tokens, cut into k pieces each: a page takes 2.1 us of a
+    // workgroup, a piece's partial sums (264 KB a kv head) 0.4 us of all, half
+    // of it where they are written and half in the merge, and that 4 us of its
+    // own.  So pages / k * 2.1 + 0.4 * blocks * k + 4 is least at pieces of
+    // sqrt(0.19 * blocks * pages) pages (700 tokens, 11 blocks of up to 11 pages:
+    // cut into 4 pieces 37 + 11 us, whole 39).
+    QM_DEV static float many_piece(float pages, float blocks) { return fmaxf(QMK_CHUNK_MANY_PIECE, __builtin_amdgcn_sqrtf(0.19f * blocks * pages)); }
+    QM_DEV static bool many_cut(float pages, float blocks, float k) {
+        return pages * (1.0f - __builtin_amdgcn_rcpf(k)) * 2.1f > 4.0f + 0.4f * blocks * k;
+    }
 
     QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), pieces(false), piece(0.0), cuts(0), total(0.0), each(0.0), incl(0.0), units(0.0) {
         mine = chunk_row(A, lane);
@@ -135,12 +145,13 @@ struct Deal {
                 // the smallest piece with which they are no more than the
                 // workgroups, from an equal share on, in steps of an eighth
                 pieces = true;
-                const double most = nb ? (double)weight(mine) * tiles(mine, nb - 1) : 0.0;
-                const double least = few(mine) ? QMK_CHUNK_FEW_PIECE : QMK_CHUNK_MANY_PIECE * QMK_CHUNK_WEIGHT;
-                const bool cut = tiles(mine, max(nb - 1, 0)) > QMK_CHUNK_WHOLE || !few(mine);
+                const int last = tiles(mine, max(nb - 1, 0));          // pages of the row's longest block
+                const double most = nb ? (double)weight(mine) * last : 0.0;
+                const double least = few(mine) ? QMK_CHUNK_FEW_PIECE : QMK_CHUNK_WEIGHT * (double)many_piece((float)last, (float)all);
                 piece = lane_of(scan(nb * most), 63) / A.groups;
                 for (;;) {
-                    cuts = !nb ? 0 : cut ? cuts_of(most, fmax(piece, least)) : 1;
+                    cuts = nb ? cuts_of(most, fmax(piece, least)) : 0;
+                    if (few(mine) ? last <= QMK_CHUNK_WHOLE : !many_cut((float)last, (float)all, (float)cuts)) cuts = min(cuts, 1);
                     if (__builtin_amdgcn_readlane((int)wave_scan((uint32_t)(nb * cuts)), 63) <= A.groups) break;
                     piece = fmax(piece, 1.0) * 1.125;
                 }
@@ -462,40 +473,49 @@ QM_DEV float chunk_inv(float ss) {
 // lanes have a row, lane j dims 16 j .. + 15, so that a wave does four of them
 // and the rotation's pairs (i, i + 32) are two lanes apart.
 template <int NF>
-QM_DEV void few_queries(const GqaChunkArgs& A, uint8_t (&q)[NF][8][1024], const ChunkRow& r, int i0, int kvh, int w, int lane) {
-    const int j = lane & 15, col = 4 * w + (lane >> 4);
-    if (col >= 16 * NF) return;                            // uniform
-    const int i = min(i0 + (col >> 2), r.n - 1);           // columns past the last token: any row, never written
-    const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + 4 * kvh + (col & 3)) * (2 * QM_GQA_HD) + 16 * j;
-    const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 16 * (j & 1);
-    uint4 u[2], gq[2];
+struct FewQuery {
+    uint4 u[2], gamma[2];
     float4 cs[4], sn[4];
+
+    QM_DEV void load(const GqaChunkArgs& A, const ChunkRow& r, int i0, int kvh, int w, int lane) {
+        const int j = lane & 15, col = 4 * w + (lane >> 4);
+        if (4 * w >= 16 * NF) return;                      // uniform
+        const int i = min(i0 + (col >> 2), r.n - 1);       // columns past the last token: any row, never written
+        const uint16_t* row = A.q_gate + ((size_t)(r.begin + i) * QM_GQA_HEADS + 4 * kvh + (col & 3)) * (2 * QM_GQA_HD) + 16 * j;
+        const size_t at = (size_t)(r.len - r.n + i) * (QM_GQA_ROT / 2) + 16 * (j & 1);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        u[k] = reinterpret_cast<const uint4*>(row)[k];
-        gq[k] = reinterpret_cast<const uint4*>(A.q_norm + 16 * j)[k];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        cs[k] = ld4(A.rope_cos + at + 4 * k);
-        sn[k] = ld4(A.rope_sin + at + 4 * k);
-    }
-    const float inv = chunk_inv(row_sum16(chunk_squares(u[1], chunk_squares(u[0], 0.0f))));
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        float x[8];
-        chunk_normed(x, u[k], gq[k], inv);
-        const float c8[8] = {cs[2 * k].x, cs[2 * k].y, cs[2 * k].z, cs[2 * k].w, cs[2 * k + 1].x, cs[2 * k + 1].y, cs[2 * k + 1].z, cs[2 * k + 1].w};
-        const float s8[8] = {sn[2 * k].x, sn[2 * k].y, sn[2 * k].z, sn[2 * k].w, sn[2 * k + 1].x, sn[2 * k + 1].y, sn[2 * k + 1].z, sn[2 * k + 1].w};
-        half8 out;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float p = dpp_f32<0x4E>(x[e]);
-            out[e] = (_Float16)(j >= 4 ? x[e] : x[e] * c8[e] + (j < 2 ? -p : p) * s8[e]);
+        for (int k = 0; k < 2; ++k) {
+            u[k] = reinterpret_cast<const uint4*>(row)[k];
+            gamma[k] = reinterpret_cast<const uint4*>(A.q_norm + 16 * j)[k];
         }
-        *reinterpret_cast<half8*>(&q[col >> 4][j >> 1][16 * ((col & 15) + 16 * (2 * (j & 1) + k))]) = out;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            cs[k] = ld4(A.rope_cos + at + 4 * k);
+            sn[k] = ld4(A.rope_sin + at + 4 * k);
+        }
+        // here before the DMA that follows: the compiler's waits would take that for its own
+        asm volatile("" ::"v"(u[1].x), "v"(gamma[1].x), "v"(cs[3].x), "v"(sn[3].x));
     }
-}
+    QM_DEV void store(uint8_t (&q)[NF][8][1024], int w, int lane) const {
+        const int j = lane & 15, col = 4 * w + (lane >> 4);
+        if (4 * w >= 16 * NF) return;
+        const float inv = chunk_inv(row_sum16(chunk_squares(u[1], chunk_squares(u[0], 0.0f))));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float x[8];
+            chunk_normed(x, u[k], gamma[k], inv);
+            const float c8[8] = {cs[2 * k].x, cs[2 * k].y, cs[2 * k].z, cs[2 * k].w, cs[2 * k + 1].x, cs[2 * k + 1].y, cs[2 * k + 1].z, cs[2 * k + 1].w};
+            const float s8[8] = {sn[2 * k].x, sn[2 * k].y, sn[2 * k].z, sn[2 * k].w, sn[2 * k + 1].x, sn[2 * k + 1].y, sn[2 * k + 1].z, sn[2 * k + 1].w};
+            half8 out;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = dpp_f32<0x4E>(x[e]);
+                out[e] = (_Float16)(j >= 4 ? x[e] : x[e] * c8[e] + (j < 2 ? -p : p) * s8[e]);
+            }
+            *reinterpret_cast<half8*>(&q[col >> 4][j >> 1][16 * ((col & 15) + 16 * (2 * (j & 1) + k))]) = out;
+        }
+    }
+};
 
 // The weights of a half page's scores (runs 0, 1 of 16 tokens), which come
 // counted from the reference: the products' sums begin at its negative.
@@ -651,6 +671,8 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
         return t < tb ? table[t] : -1;
     };
     int ids = load_ids(0);
+    FewQuery<NF> query;
+    query.load(A, it.r, i0, kvh, w, lane);
     const uint32_t ring = lds_addr(sh.ring[w]);
     auto fetch = [&](int round, int h) {                   // the half page of that round, if there is one
         if (h >= h_end) return false;
@@ -665,9 +687,8 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
         const int i = i0 + 4 * f + (c >> 2);
         st.pos[f] = i < it.r.n ? it.r.len - it.r.n + i : -1;
     }
-    bool now = fetch(0, h0);
-    few_queries<NF>(A, sh.q, it.r, i0, kvh, w, lane);
-    bool next = fetch(1, h0 + CHUNK_WAVES);
+    bool now = fetch(0, h0), next = fetch(1, h0 + CHUNK_WAVES);
+    query.store(sh.q, w, lane);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
@@ -867,8 +888,10 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
     const int c = lane & 31, h = lane >> 5, head = 4 * kvh + (w & 3);
     const int i0 = QMK_CHUNK_TOKENS * it.block + 32 * (w >> 2), i = i0 + c;      // the wave's first row, the lane's
     const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
-    auto page = [&](int t) { return t < tb ? __builtin_amdgcn_readfirstlane(table[t]) : -1; };
-    int id = page(ta), next = page(ta + 1), done = -1;     // of tiles t, t + 1, t - 1
+    // page ids, one a lane, 64 at a time
+    auto load_ids = [&](int t) { return t + lane < tb ? table[t + lane] : -1; };
+    int ids = load_ids(ta);
+    int id = __builtin_amdgcn_readlane(ids, 0), done = -1;             // of tiles t, t - 1
     if (kv4_is_page(A.c, id)) chunk_fetch(A, sh, id, kvh, w, lane);
     ManyWave st;
     st.pos = i < it.r.n ? it.r.len - it.r.n + i : -1;      // rows past the last: any row, never written
@@ -886,6 +909,8 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (kv4_is_page(A.c, id)) chunk_expand(sh, t & 1, it.r.len - QMK_KV4_PAGE_TOKENS * t, w, chunk_lane(lane));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the codes are read
+        if (((t + 1 - ta) & 63) == 0) ids = load_ids(t + 1);
+        const int next = __builtin_amdgcn_readlane(ids, (t + 1 - ta) & 63);
         if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, chunk_lane(lane));
         if (late) asm volatile("s_barrier" ::: "memory");
         const int at = late ? t : t - 1;
@@ -897,7 +922,6 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
         }
         done = id;
         id = next;
-        next = page(t + 2);
         if (!late) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     const float l = sum_xor32(st.sum.l);
@@ -981,76 +1005,80 @@ extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_3
 extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_many(GqaChunkArgs A) { chunk_attention<2, true>(A); }
 
 // The partial sums of a row block that several workgroups share, joined: a
-// workgroup per (row block, kv head, operand column or wave's rows, eight quads
-// of dims), a wave two of them.  N partials' loads are in flight at a time.
-struct Joined {
-    float m, l;
-    floatx4 o[2];
-};
-template <int N>
-QM_DEV void chunk_join(Joined& x, const float* first, const float* others, int n, size_t stride, int quad, int sums, int rows, int lane) {
+// workgroup per (row block, kv head, operand column or wave's rows, quarter of
+// the dims), a wave Q quads of dims.  N partials' loads are in flight at a time.
+template <int N, int Q>
+QM_DEV void chunk_join(float& m, float& l, floatx4 (&o)[Q], const float* first, const float* others, int n, size_t stride, int quad, int sums,
+                       int rows, int lane) {
     const int c = lane & (rows - 1);
     for (int s0 = 0; s0 < n; s0 += N) {                    // uniform
-        floatx4 a[N][2];
+        floatx4 a[N][Q];
         float pm[N], pl[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) {                      // past the last: the last again, with weight 0
             const int i = min(s0 + k, n - 1);
             const float* part = i == 0 ? first : others + i * stride;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (quad + j) + 4 * lane);
+            for (int j = 0; j < Q; ++j) a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (quad + j) + 4 * lane);
             pm[k] = part[sums + c];
             pl[k] = part[sums + rows + c];
         }
-        float top = x.m;
+        float top = m;
 #pragma unroll
         for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k]);
-        const float corr = x.m == top ? 1.0f : __builtin_amdgcn_exp2f(x.m - top);
-        x.l *= corr;
+        const float corr = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        l *= corr;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) x.o[j] *= corr;
+        for (int j = 0; j < Q; ++j) o[j] *= corr;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             // a partial of no weight counts all the same: a NaN in it reaches the output (the last again has no other)
             const float f = s0 + k >= n ? 0.0f : pm[k] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - top);
-            x.l = fmaf(pl[k], f, x.l);
+            l = fmaf(pl[k], f, l);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) x.o[j] += a[k][j] * f;
+            for (int j = 0; j < Q; ++j) o[j] += a[k][j] * f;
         }
-        x.m = top;
+        m = top;
+    }
+}
+// FEW: of a block of few tokens, else of many.
+template <int NF, bool MANY, bool FEW>
+QM_DEV void chunk_merge_one(const GqaChunkArgs& A, int k) {
+    constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;  // of a workgroup's partial
+    constexpr int kUnits = FEW ? NF : CHUNK_WAVES, kRows = FEW ? 16 : 32, kStep = FEW ? 16 : 8, kSums = FEW ? 4096 : 8192, Q = FEW ? 1 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quad = (4 * (k & 3) + wave) * Q, unit = (k >> 2) % kUnits, kvh = (k >> 2) / kUnits & 3, number = k / (16 * kUnits);
+    const int count = A.counts[FEW];
+    const ChunkRecord rec = A.records[(FEW ? A.many : 0) + number];
+    if (number >= count || rec.from == rec.to) return;     // uniform
+    // row of the block, and first dim, of the lane's quads
+    const int c = lane & (kRows - 1), g = lane / kRows, head = 4 * kvh + (FEW ? c & 3 : unit & 3);
+    const int i = FEW ? 4 * NF * rec.block + 4 * unit + (c >> 2) : QMK_CHUNK_TOKENS * rec.block + 32 * (unit >> 2) + c;
+    const int d0 = kStep * quad + 4 * g;
+    const size_t at = (size_t)(rec.begin + min(i, rec.n - 1)) * QM_GQA_HEADS + head;
+    uint2 gate[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + d0 + j * kStep);
+    float m = -INFINITY, l = 0.0f;
+    floatx4 o[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) o[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    // the first workgroup's part ends its run, the others' begin theirs
+    const size_t slot = (size_t)kColumns * QMK_CHUNK_COLUMN;
+    const float* base = A.partial + (size_t)(2 * (4 * rec.from + kvh)) * slot + (size_t)(FEW ? 1 : 2) * unit * QMK_CHUNK_COLUMN;
+    const int n = rec.to - rec.from + 1;
+    if (n <= 4) chunk_join<4, Q>(m, l, o, base + slot, base, n, 8 * slot, quad, kSums, kRows, lane);
+    else chunk_join<32 / Q, Q>(m, l, o, base + slot, base, n, 8 * slot, quad, kSums, kRows, lane);
+    if (i < rec.n) {
+#pragma unroll
+        for (int j = 0; j < Q; ++j) chunk_out(A.out + at * QM_GQA_HD + d0 + j * kStep, o[j], chunk_inverse(l), gate[j]);
     }
 }
 template <int NF, bool MANY>
 QM_DEV void chunk_merge(const GqaChunkArgs& A) {
-    constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;  // of a workgroup's partial
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int before = MANY ? A.many * 4 * CHUNK_WAVES * 4 : 0;       // workgroups for blocks of many tokens
-    const bool few = (int)blockIdx.x >= before;
-    const int k = few ? blockIdx.x - before : blockIdx.x, units = few ? NF : CHUNK_WAVES, parts = few ? 2 : 4;
-    const int quad = 8 * (k % parts) + 2 * wave, unit = k / parts % units, kvh = k / (parts * units) & 3, number = k / (4 * parts * units);
-    const int count = A.counts[few];
-    const ChunkRecord rec = A.records[(few ? A.many : 0) + number];
-    if (number >= count || rec.from == rec.to) return;     // uniform
-    // row of the block, and first dim, of the lane's quads
-    const int rows = few ? 16 : 32, c = lane & (rows - 1), g = lane / rows;
-    const int head = 4 * kvh + (few ? c & 3 : unit & 3);
-    const int i = few ? 4 * NF * rec.block + 4 * unit + (c >> 2) : QMK_CHUNK_TOKENS * rec.block + 32 * (unit >> 2) + c;
-    const int d0 = (few ? 16 : 8) * quad + 4 * g, step = few ? 16 : 8;
-    const size_t at = (size_t)(rec.begin + min(i, rec.n - 1)) * QM_GQA_HEADS + head;
-    uint2 gate[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + d0 + j * step);
-    Joined x{-INFINITY, 0.0f, {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}};
-    // the first workgroup's part ends its run, the others' begin theirs
-    const size_t slot = (size_t)kColumns * QMK_CHUNK_COLUMN;
-    const float* base = A.partial + (size_t)(2 * (4 * rec.from + kvh)) * slot + (size_t)(few ? 1 : 2) * unit * QMK_CHUNK_COLUMN;
-    const int n = rec.to - rec.from + 1;
-    if (n <= 4) chunk_join<4>(x, base + slot, base, n, 8 * slot, quad, few ? 4096 : 8192, rows, lane);
-    else chunk_join<16>(x, base + slot, base, n, 8 * slot, quad, few ? 4096 : 8192, rows, lane);
-    if (i < rec.n) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) chunk_out(A.out + at * QM_GQA_HD + d0 + j * step, x.o[j], chunk_inverse(x.l), gate[j]);
-    }
+    if (MANY && (int)blockIdx.x < before) chunk_merge_one<NF, MANY, false>(A, blockIdx.x);
+    else chunk_merge_one<NF, MANY, true>(A, blockIdx.x - before);
 }
 extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_4(GqaChunkArgs A) { chunk_merge<1, false>(A); }
 extern "C" __global__ __launch_bounds__(256) void qm_gqa_chunk_merge_32(GqaChunkArgs A) { chunk_merge<2, false>(A); }

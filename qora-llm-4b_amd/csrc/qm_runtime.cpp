@@ -1396,7 +1396,7 @@ int32_t qm_gqa_chunk_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* ca
     const int form = shape.many ? 2 : shape.columns - 1;
     st = launch(c, c->f_gqa_chunk[form], static_cast<uint32_t>(shape.groups * QM_GQA_KV_HEADS), 512, a, s, "qm_gqa_chunk");
     if (st != QM_OK || !shape.split) return st;
-    const int64_t merge = (shape.most_many * 8 * 4 + shape.most_few * shape.columns * 2) * QM_GQA_KV_HEADS;
+    const int64_t merge = (shape.most_many * 8 * 4 + shape.most_few * shape.columns * 4) * QM_GQA_KV_HEADS;
     return launch(c, c->f_gqa_chunk_merge[form], static_cast<uint32_t>(merge), 256, a, s, "qm_gqa_chunk_merge");
 }
 
