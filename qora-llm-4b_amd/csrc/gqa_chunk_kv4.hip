@@ -266,24 +266,27 @@ QM_DEV bool chunk_sees(const ChunkNan& nan, int group, int pos, int k0) {
 //   K block h, s (16 h + s):             dims 16 s + 8 (l >> 5) .. + 7 of token many_token(l & 31) of half page h
 //   V block h, dt, k (32 + 16 h + 2 dt + k): dim 32 dt + (l & 31), tokens 16 (e >> 2) + 4 (2 k + (l >> 5)) + (e & 3),
 //                                        e < 8, of half page h
-// and a wave's own part of the next tile's codes, with its half page's scales
-// and minima.  Wave w has half page w >> 2 and pieces i = w & 3: K's run i >> 1,
-// dims 128 (i & 1) .., and V's group i.
+// and a wave's own part of the next tile's codes, K's and V's, each with its
+// half page's scales and minima.  Wave w has half page w >> 2 and pieces
+// i = w & 3: K's run i >> 1, dims 128 (i & 1) .., and V's group i.
 #define CHUNK_TILE 65536
+#define CHUNK_RAW 1536
 struct ChunkLds {
     __attribute__((aligned(1024))) uint8_t tile[2][CHUNK_TILE];
-    __attribute__((aligned(1024))) uint8_t raw[CHUNK_WAVES][3][1024];
-    ChunkNan nan[2][2];                // [buffer][half]
+    __attribute__((aligned(1024))) uint8_t raw[CHUNK_WAVES][2][CHUNK_RAW];
+    __attribute__((aligned(16))) uint32_t nan[2][2][4];      // [buffer][half][group]: tokens whose V is NaN there
 };
 
 QM_DEV uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
-QM_DEV void chunk_fetch(const GqaChunkArgs& A, ChunkLds& sh, int id, int head, int w, int lane) {
+// The wave's K (is_v 0) or V codes of page id, and their scales and minima.
+#define CHUNK_DMA 2
+template <int IS_V>
+QM_DEV void many_fetch(const GqaChunkArgs& A, ChunkLds& sh, int id, int head, int w, int lane) {
     const uint8_t* half = kv4_half(A.c, A.layer, id, head, w >> 2);
-    const uint32_t raw = lds_addr(sh.raw[w][0]);
-    dma16_off(half + 1024 * (w & 3), 16 * lane, raw);
-    dma16_off(half + 4 * QMK_KV4_V_WORDS + 1024 * (w & 3), 16 * lane, raw + 1024);
-    dma16_off(half + QMK_KV4_META, 16 * lane, raw + 2048);
+    const uint32_t raw = lds_addr(sh.raw[w][IS_V]);
+    dma16_off(half + 4 * QMK_KV4_V_WORDS * IS_V + 1024 * (w & 3), 16 * lane, raw);
+    if (lane < 32) dma16_off(half + QMK_KV4_META + 512 * IS_V, 16 * lane, raw + 1024);
 }
 
 // Token of score e of run r in lane group g.
@@ -329,82 +332,124 @@ QM_DEV void chunk_cut(half2_t (&s)[4], half2_t (&lo)[4], int left, int g) {
         if (chunk_token(e >> 2, g, e & 3) >= left) s[e >> 1][e & 1] = lo[e >> 1][e & 1] = (_Float16)0.0f;
 }
 
-// Whether some of a half page's scales or minima (at `meta`) are NaN, or so
-// large that its values may not be finite (2^10 and 2^14: lo + 15 s is under
-// 2^15).
+// Whether some of K's, or V's, scales and minima of a half page (at `meta`, 512
+// bytes) are NaN, or so large that its values may not be finite (2^10 and 2^14:
+// lo + 15 s is under 2^15).
+QM_DEV bool chunk_odd(uint32_t s, uint32_t lo) {
+    const uint32_t x = s & 0x7c007c00u, y = lo & 0x7c007c00u;
+    return (x & 0xffffu) >= 0x6400u || x >= 0x64000000u || (y & 0xffffu) >= 0x7400u || y >= 0x74000000u;
+}
 QM_DEV bool chunk_odd(const uint8_t* meta, int lane) {
     const uint32_t* m = reinterpret_cast<const uint32_t*>(meta) + lane;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t x = m[64 * i] & 0x7c007c00u, most = i & 1 ? 0x7400u : 0x6400u;
-        odd = odd || (x & 0xffffu) >= most || x >= most << 16;
-    }
-    return __any(odd);
+    return __any(chunk_odd(m[0], m[64]));
 }
-// Puts such a half page right, in LDS.  A scale that takes the group past
-// f16's largest value becomes the next lower one.  V that is NaN becomes 0, and
-// is returned: the rows that see it are given the NaN beside the product, as a
-// weight of 0 times it would give it to the others too.
+// Puts such scales right, in LDS.  One that takes the group past f16's largest
+// value becomes the next lower one.  V that is NaN becomes 0, and is returned:
+// the rows that see it are given the NaN beside the product, as a weight of 0
+// times it would give it to the others too.
+template <bool IS_V>
 QM_DEV ChunkNan chunk_mend(uint8_t* meta, int lane) {
     uint64_t nan[2];
 #pragma unroll
-    for (int is_v = 0; is_v < 2; ++is_v)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int t = 16 * k + (lane >> 2), group = lane & 3;
-            uint16_t* s = reinterpret_cast<uint16_t*>(meta + 512 * is_v) + kv4_s_at(t, group);
-            uint16_t* lo = reinterpret_cast<uint16_t*>(meta + 512 * is_v + 256) + kv4_lo_at(t, group);
-            const float top = fmaf(15.0f, f16_to_f32(*s), f16_to_f32(*lo));
-            if (top >= 65520.0f) *s = *s - 1;
-            nan[k] = __ballot(is_v && top != top);
-            if (is_v && top != top) *s = *lo = 0;
-        }
+    for (int k = 0; k < 2; ++k) {
+        const int t = 16 * k + (lane >> 2), group = lane & 3;
+        uint16_t* s = reinterpret_cast<uint16_t*>(meta) + kv4_s_at(t, group);
+        uint16_t* lo = reinterpret_cast<uint16_t*>(meta + 256) + kv4_lo_at(t, group);
+        const float top = fmaf(15.0f, f16_to_f32(*s), f16_to_f32(*lo));
+        if (top >= 65520.0f) *s = *s - 1;
+        nan[k] = __ballot(IS_V && top != top);
+        if (IS_V && top != top) *s = *lo = 0;
+    }
     asm volatile("" ::: "memory");                         // read again as other types
     return ChunkNan{nan[0], nan[1]};
 }
 
-// The wave's part of a tile of which `left` tokens are the row's (64 and more:
-// all; V of the others is 0), from its codes into buffer `buf`.
-QM_DEV void chunk_expand(ChunkLds& sh, int buf, int left, int w, int lane) {
-    const uint8_t* raw = sh.raw[w][0];
-    uint8_t* meta = sh.raw[w][2];
-    const int half = w >> 2, i = w & 3, c = lane & 15, g = lane >> 4;
-    const int run = i >> 1, dims = i & 1;
-    ChunkNan nan{0, 0};
-    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
-    if (i == 0 && lane == 0) sh.nan[buf][half] = nan;
-    {
-        const uintx4 k = *reinterpret_cast<const uintx4*>(raw + 16 * lane);
-        const half2_t s = as_half2(*reinterpret_cast<const uint32_t*>(meta + 2 * kv4_s_at(16 * run + c, 2 * dims)));
-        const half2_t lo = {*reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims)),
-                            *reinterpret_cast<const _Float16*>(meta + 256 + 2 * kv4_lo_at(16 * run + c, 2 * dims + 1))};
-        // dims 128 dims + 32 m + 8 g .. of token 16 run + c: block 2 (4 dims + m) + (g >> 1), entry of its row and g & 1
-        const int row = 16 * (c >> 3) + 8 * run + (c & 7);
-        uint8_t* to = sh.tile[buf] + (16 * half + 8 * dims + (g >> 1)) * 1024 + 16 * (row + 32 * (g & 1));
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const half2_t s2 = {s[m >> 1], s[m >> 1]}, l2 = {lo[m >> 1], lo[m >> 1]};
-            const half2_t ss[4] = {s2, s2, s2, s2}, ll[4] = {l2, l2, l2, l2};
-            *reinterpret_cast<half8*>(to + 2048 * m) = chunk_values(k[m], ss, ll);
+// The wave's part of a tile, from its codes into buffer `buf`, K and V each in
+// steps that can stand between matrix instructions: the reads, then what is
+// seldom, then a word at a time.
+struct ManyK {
+    uintx4 k;
+    uint32_t s, lo;                    // of the lane's token, groups 2 dims and + 1
+
+    QM_DEV void reads(const ChunkLds& sh, int w, int lane) {
+        const uint8_t* raw = sh.raw[w][0];
+        const int run = (w & 3) >> 1, dims = w & 1, c = lane & 15;
+        k = *reinterpret_cast<const uintx4*>(raw + 16 * lane);
+        scales(raw + 1024, 16 * run + c, 2 * dims);
+    }
+    QM_DEV void scales(const uint8_t* meta, int t, int group) {
+        s = *reinterpret_cast<const uint32_t*>(meta + 2 * kv4_s_at(t, group));
+        lo = (uint32_t)*reinterpret_cast<const uint16_t*>(meta + 256 + 2 * kv4_lo_at(t, group)) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(meta + 256 + 2 * kv4_lo_at(t, group + 1)) << 16;
+    }
+    QM_DEV void seldom(ChunkLds& sh, int, int, int w, int lane) {
+        if (__any(chunk_odd(s, lo))) {
+            uint8_t* meta = sh.raw[w][0] + 1024;
+            chunk_mend<false>(meta, lane);
+            scales(meta, 16 * ((w & 3) >> 1) + (lane & 15), 2 * (w & 1));
         }
     }
-    {
-        const uintx4 v = *reinterpret_cast<const uintx4*>(raw + 1024 + 16 * lane);
-        const uintx4 lo4 = *reinterpret_cast<const uintx4*>(meta + 768 + (4 * i + g) * 16);
-        half2_t s[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            s[e >> 1][e & 1] = *reinterpret_cast<const _Float16*>(meta + 512 + 2 * (g * 32 + (e >> 2) * 16 + (e & 3) * 4 + i));
-#pragma unroll
-        for (int n = 0; n < 4; ++n) lo[n] = as_half2(lo4[n]);
-        if (left < QMK_KV4_PAGE_TOKENS) chunk_cut(s, lo, left - 32 * half, g);      // uniform
-        // dim 64 i + 16 m + c, tokens of g: block of dims 32 (2 i + (m >> 1)) .. and g >> 1
-        uint8_t* to = sh.tile[buf] + 32768 + (16 * half + 4 * i + (g >> 1)) * 1024 + 16 * (c + 32 * (g & 1));
-#pragma unroll
-        for (int m = 0; m < 4; ++m) *reinterpret_cast<half8*>(to + 2048 * (m >> 1) + 256 * (m & 1)) = chunk_values(v[m], s, lo);
+    QM_DEV void word(ChunkLds& sh, int buf, int m, int w, int lane) const {
+        // dims 128 dims + 32 m + 8 g .. of token 16 run + c: block 2 (4 dims + m) + (g >> 1), entry of its row and g & 1
+        const int half = w >> 2, run = (w & 3) >> 1, dims = w & 1, c = lane & 15, g = lane >> 4, row = 16 * (c >> 3) + 8 * run + (c & 7);
+        const half2_t ss = as_half2(s), ll = as_half2(lo), s2 = {ss[m >> 1], ss[m >> 1]}, l2 = {ll[m >> 1], ll[m >> 1]};
+        const half2_t s4[4] = {s2, s2, s2, s2}, l4[4] = {l2, l2, l2, l2};
+        *reinterpret_cast<half8*>(sh.tile[buf] + (16 * half + 8 * dims + (g >> 1)) * 1024 + 16 * (row + 32 * (g & 1)) + 2048 * m) = chunk_values(k[m], s4, l4);
     }
-}
+};
+struct ManyV {
+    uintx4 v, s, lo;                   // of the lane's eight tokens, in pairs
+
+    QM_DEV void reads(const ChunkLds& sh, int w, int lane) {
+        const uint8_t* raw = sh.raw[w][1];
+        v = *reinterpret_cast<const uintx4*>(raw + 16 * lane);
+        scales(raw + 1024, w & 3, lane >> 4);
+    }
+    QM_DEV void scales(const uint8_t* meta, int i, int g) {
+        lo = *reinterpret_cast<const uintx4*>(meta + 256 + (4 * i + g) * 16);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(meta) + g * 32 + (n >> 1) * 16 + (n & 1) * 8 + i;
+            s[n] = (uint32_t)at[0] | (uint32_t)at[4] << 16;
+        }
+    }
+    // `left`: the row's tokens in the tile (64 and more: all); V of the others is 0.
+    QM_DEV void seldom(ChunkLds& sh, int buf, int left, int w, int lane) {
+        const int half = w >> 2, i = w & 3, g = lane >> 4;
+        uint32_t nan = 0;
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 ms = {0, 0}, ml = {0, 0};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            ms = __builtin_elementwise_max(ms, __builtin_bit_cast(u16x2, s[n]));
+            ml = __builtin_elementwise_max(ml, __builtin_bit_cast(u16x2, lo[n] & 0x7fff7fffu));
+        }
+        if (__any(chunk_odd(__builtin_bit_cast(uint32_t, ms), __builtin_bit_cast(uint32_t, ml)))) {
+            uint8_t* meta = sh.raw[w][1] + 1024;
+            const ChunkNan all = chunk_mend<true>(meta, lane);
+#pragma clang loop unroll(disable)
+            for (int t = 0; t < QMK_KV4_HALF_TOKENS; ++t) nan |= (uint32_t)((t < 16 ? all.low : all.high) >> (4 * (t & 15) + i) & 1) << t;
+            scales(meta, i, g);
+        }
+        if (lane == 0) sh.nan[buf][half][i] = nan;
+        if (left < QMK_KV4_PAGE_TOKENS) {                  // uniform
+            half2_t a[4], b[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) a[n] = as_half2(s[n]), b[n] = as_half2(lo[n]);
+            chunk_cut(a, b, left - 32 * half, g);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) s[n] = __builtin_bit_cast(uint32_t, a[n]), lo[n] = __builtin_bit_cast(uint32_t, b[n]);
+        }
+    }
+    QM_DEV void word(ChunkLds& sh, int buf, int m, int w, int lane) const {
+        // dim 64 i + 16 m + c, tokens of g: block of dims 32 (2 i + (m >> 1)) .. and g >> 1
+        const int half = w >> 2, i = w & 3, c = lane & 15, g = lane >> 4;
+        const half2_t s4[4] = {as_half2(s[0]), as_half2(s[1]), as_half2(s[2]), as_half2(s[3])};
+        const half2_t l4[4] = {as_half2(lo[0]), as_half2(lo[1]), as_half2(lo[2]), as_half2(lo[3])};
+        *reinterpret_cast<half8*>(sh.tile[buf] + 32768 + (16 * half + 4 * i + (g >> 1)) * 1024 + 16 * (c + 32 * (g & 1)) + 2048 * (m >> 1) + 256 * (m & 1)) =
+            chunk_values(v[m], s4, l4);
+    }
+};
 
 // ---- a wave's rows ---------------------------------------------------------------
 // A row's softmax: the reference m (-inf: none yet), from which its scores are
@@ -584,7 +629,8 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][10
     const int c = lane & 15, g = lane >> 4;
     uint8_t* meta = buf + QMK_KV4_META;
     ChunkNan nan{0, 0};
-    if (chunk_odd(meta, lane)) nan = chunk_mend(meta, lane);
+    if (chunk_odd(meta, lane)) chunk_mend<false>(meta, lane);
+    if (chunk_odd(meta + 512, lane)) nan = chunk_mend<true>(meta + 512, lane);
     floatx4 x[NF][2];
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
@@ -834,8 +880,10 @@ QM_DEV void many_query(const GqaChunkArgs& A, half8 (&q)[16], const ChunkRow& r,
     }
 }
 
-// Half a tile, the 32 tokens from k0 on.
-QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k0, bool edge, int lane) {
+// Half a tile, the 32 tokens from k0 on; meanwhile a part E of the next tile is
+// made, for buffer buf ^ 1 of which `left` tokens are the row's.
+template <class E>
+QM_DEV void many_half(ManyWave& st, ChunkLds& sh, int buf, int half, int k0, bool edge, int left, int w, int lane) {
     const uint8_t* K = sh.tile[buf] + 16 * lane + 16384 * half;
     const uint8_t* V = K + 32768;
     const int h = lane >> 5;
@@ -845,6 +893,8 @@ QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k
     for (int i = 0; i < 16; ++i) x[i] = base;
     many_product([&](int s) { return *reinterpret_cast<const half8*>(K + 1024 * s); },
                  [&](int s, half8 a) { x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, st.q[s], x, 0, 0, 0); });
+    E part;
+    part.reads(sh, w, lane);
     if (edge) {                                            // uniform: some row does not see all of it
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = k0 + many_token(i, h) > st.pos ? -INFINITY : x[i];
@@ -864,18 +914,33 @@ QM_DEV void many_half(ManyWave& st, const ChunkLds& sh, int buf, int half, int k
     half8 p[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        uintx4 w;
+        uintx4 w4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = chunk_pair(st.sum, x[8 * k + 2 * i], x[8 * k + 2 * i + 1]);
-        p[k] = __builtin_bit_cast(half8, w);
+        for (int i = 0; i < 4; ++i) w4[i] = chunk_pair(st.sum, x[8 * k + 2 * i], x[8 * k + 2 * i + 1]);
+        p[k] = __builtin_bit_cast(half8, w4);
     }
+    part.seldom(sh, buf ^ 1, left, w, lane);
     many_product([&](int i) { return *reinterpret_cast<const half8*>(V + 1024 * i); },
-                 [&](int i, half8 a) { st.o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[i & 1], st.o[i >> 1], 0, 0, 0); });
-    const ChunkNan nan = sh.nan[buf][half];
-    if (__builtin_amdgcn_readfirstlane((int)((nan.low | nan.high) != 0))) {
+                 [&](int i, half8 a) {
+                     st.o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[i & 1], st.o[i >> 1], 0, 0, 0);
+                     if ((i & 3) == 1) part.word(sh, buf ^ 1, i >> 2, w, lane);
+                 });
+    const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][half]);
+    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
+        const int seen = st.pos - k0;                      // the last of the half's tokens that the row sees
+        const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) st.o[dt] += chunk_sees(nan, dt >> 1, st.pos, k0) ? __builtin_nanf("") : 0.0f;
+        for (int dt = 0; dt < 8; ++dt) st.o[dt] += nan[dt >> 1] & mask ? __builtin_nanf("") : 0.0f;
     }
+}
+// A part of a tile by itself.
+template <class E>
+QM_DEV void many_make(ChunkLds& sh, int buf, int left, int w, int lane) {
+    E part;
+    part.reads(sh, w, lane);
+    part.seldom(sh, buf, left, w, lane);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) part.word(sh, buf, m, w, lane);
 }
 
 QM_DEV floatx4 many_four(const ManyWave& st, int j) {
@@ -891,8 +956,12 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
     // page ids, one a lane, 64 at a time
     auto load_ids = [&](int t) { return t + lane < tb ? table[t + lane] : -1; };
     int ids = load_ids(ta);
-    int id = __builtin_amdgcn_readlane(ids, 0), done = -1;             // of tiles t, t - 1
-    if (kv4_is_page(A.c, id)) chunk_fetch(A, sh, id, kvh, w, lane);
+    auto page_of = [&](int t) { return __builtin_amdgcn_readlane(ids, (t - ta) & 63); };
+    int id = -1, next = page_of(ta);                       // of tiles t, t + 1
+    if (kv4_is_page(A.c, next)) {
+        many_fetch<0>(A, sh, next, kvh, w, lane);
+        many_fetch<1>(A, sh, next, kvh, w, lane);
+    }
     ManyWave st;
     st.pos = i < it.r.n ? it.r.len - it.r.n + i : -1;      // rows past the last: any row, never written
     many_query(A, st.q, it.r, min(i, it.r.n - 1), head, h);
@@ -900,29 +969,32 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) st.o[dt] = floatx16{};
     const int first_pos = it.r.len - it.r.n + i0;
-    // Every wave makes its part of tile t and then multiplies a tile: half of
-    // them tile t - 1, before the barrier that says that tile t is made, and
-    // half tile t, after it.  So a SIMD has one of each, and a buffer is made
-    // anew only when all have read it.
-    const bool late = w >= CHUNK_WAVES / 2;
-    for (int t = ta; t <= tb; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (kv4_is_page(A.c, id)) chunk_expand(sh, t & 1, it.r.len - QMK_KV4_PAGE_TOKENS * t, w, chunk_lane(lane));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the codes are read
-        if (((t + 1 - ta) & 63) == 0) ids = load_ids(t + 1);
-        const int next = __builtin_amdgcn_readlane(ids, (t + 1 - ta) & 63);
-        if (kv4_is_page(A.c, next)) chunk_fetch(A, sh, next, kvh, w, chunk_lane(lane));
-        if (late) asm volatile("s_barrier" ::: "memory");
-        const int at = late ? t : t - 1;
-        if (kv4_is_page(A.c, late ? id : done) && i0 < it.r.n) {
-            const int k0 = QMK_KV4_PAGE_TOKENS * at;
-            const bool edge = k0 + QMK_KV4_PAGE_TOKENS - 1 > first_pos;
-#pragma clang loop unroll(disable)
-            for (int half = 0; half < 2; ++half) many_half(st, sh, at & 1, half, k0 + QMK_KV4_HALF_TOKENS * half, edge, chunk_lane(lane));
+    // Tile t is multiplied while tile t + 1 is made of its codes, and those of
+    // tile t + 2 come as soon as theirs are read.  A tile that is none (a page
+    // that is none of the pool, past the last) is made of whatever stands there
+    // and not multiplied.
+    for (int t = ta - 1; t < tb; ++t) {
+        if (t >= ta && ((t + 2 - ta) & 63) == 0) ids = load_ids(t + 2);
+        const int after = t + 2 < tb ? page_of(t + 2) : -1;
+        const int left = it.r.len - QMK_KV4_PAGE_TOKENS * (t + 1), k0 = QMK_KV4_PAGE_TOKENS * t, ln = chunk_lane(lane);
+        const bool active = kv4_is_page(A.c, id) && i0 < it.r.n, more = kv4_is_page(A.c, after);
+        const bool edge = k0 + QMK_KV4_PAGE_TOKENS - 1 > first_pos;
+        // K's codes are here when only V's, which came after, are out
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CHUNK_DMA) : "memory");
+        if (active) many_half<ManyK>(st, sh, t & 1, 0, k0, edge, left, w, ln);
+        else many_make<ManyK>(sh, (t + 1) & 1, left, w, ln);
+        if (more) {
+            many_fetch<0>(A, sh, after, kvh, w, ln);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CHUNK_DMA) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        done = id;
+        if (active) many_half<ManyV>(st, sh, t & 1, 1, k0 + QMK_KV4_HALF_TOKENS, edge, left, w, ln);
+        else many_make<ManyV>(sh, (t + 1) & 1, left, w, ln);
+        if (more) many_fetch<1>(A, sh, after, kvh, w, ln);
         id = next;
-        if (!late) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        next = after;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     const float l = sum_xor32(st.sum.l);
     if (tb - ta == it.tiles) {
