@@ -33,6 +33,10 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 // A row's reference moves only where a score passes it by this (log2 units):
 // weights up to 2^8 are exact enough in f16, and outputs are seldom rescaled.
 #define CHUNK_SLACK 8.0f
+// What is seldom true stands away from the code that each workgroup runs: code
+// comes from memory once a launch, and a short call waits for little else (700
+// tokens 43.1 / 41.9 us).
+#define CHUNK_SELDOM(x) __builtin_expect(!!(x), 0)
 
 // ---- how the work is dealt --------------------------------------------------
 // A batch row of the call.  A row that has no tokens to read (its slot is
@@ -125,23 +129,22 @@ struct Deal {
     }
 
     QM_DEV static int cuts_of(double cost, double piece) { return (int)ceil(cost / piece); }
-    // Blocks of many tokens, cut into k pieces each: a page takes 2.1 us of a
-    // workgroup, a piece's partial sums (264 KB a kv head) 0.4 us of all, half
-    // of it where they are written and half in the merge, and that 4 us of its
-    // own.  So pages / k * 2.1 + 0.4 * blocks * k + 4 is least at pieces of
-    // sqrt(0.19 * blocks * pages) pages (700 tokens, 11 blocks of up to 11 pages:
-    // cut into 4 pieces 37 + 11 us, whole 39).
-    QM_DEV static float many_piece(float pages, float blocks) { return fmaxf(QMK_CHUNK_MANY_PIECE, __builtin_amdgcn_sqrtf(0.19f * blocks * pages)); }
-    QM_DEV static bool many_cut(float pages, float blocks, float k) {
-        return pages * (1.0f - __builtin_amdgcn_rcpf(k)) * 2.1f > 4.0f + 0.4f * blocks * k;
-    }
+    // Blocks of many tokens, cut into k pieces each: a page takes 3.4 us of a
+    // workgroup, a piece's partial sums (264 KB a kv head, written and read by
+    // the merge) 0.3 us of all.  3.4 * pages / k + 0.3 * blocks * k is least at
+    // pieces of sqrt(0.09 * blocks * pages) pages.  Measured, whole and cut so:
+    // 64 tokens of 1000 80 / 34 us, 256 of 256 41 / 34, 700 of 700 63 / 43;
+    // where it says whole, cut in two: 4 x 200 of 200 39 / 41, 16 x 128 of 400
+    // 60 / 70.
+    QM_DEV static float many_piece(float pages, float blocks) { return fmaxf(1.0f, __builtin_amdgcn_sqrtf(0.09f * blocks * pages)); }
+    QM_DEV static bool many_cut(float pages, float blocks, float k) { return 3.4f * (pages - ceilf(pages / k)) > 0.3f * blocks * k; }
 
     QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), pieces(false), piece(0.0), cuts(0), total(0.0), each(0.0), incl(0.0), units(0.0) {
         mine = chunk_row(A, lane);
-        if (A.batch <= 64) {
+        if (!CHUNK_SELDOM(A.batch > 64)) {
             const int nb = blocks(mine);
             const uint32_t all = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)min(nb, 1 << 20)), 63);
-            if (all <= (uint32_t)A.groups) {
+            if (!CHUNK_SELDOM(all > (uint32_t)A.groups)) {
                 // the smallest piece with which they are no more than the
                 // workgroups, from an equal share on, in steps of an eighth
                 pieces = true;
@@ -590,12 +593,13 @@ QM_DEV half8 few_weights(floatx4 (&x)[2], floatx4 (&o)[16], ChunkSum& s, int pos
 }
 
 // Four outputs, gated.
-QM_DEV void chunk_out(uint16_t* to, floatx4 o, float inv, uint2 gate) {
+QM_DEV uint2 chunk_gated(floatx4 o, uint2 gate) {
     const float4 x = bf16x4(gate);
-    uint2 r;
-    r.x = pack_bf16x2(o[0] * inv * sigmoid_fast(x.x), o[1] * inv * sigmoid_fast(x.y));
-    r.y = pack_bf16x2(o[2] * inv * sigmoid_fast(x.z), o[3] * inv * sigmoid_fast(x.w));
-    *reinterpret_cast<uint2*>(to) = r;
+    return make_uint2(pack_bf16x2(o[0] * sigmoid_fast(x.x), o[1] * sigmoid_fast(x.y)), pack_bf16x2(o[2] * sigmoid_fast(x.z), o[3] * sigmoid_fast(x.w)));
+}
+QM_DEV uint4 chunk_gated8(floatx4 a, floatx4 b, uint4 gate) {
+    const uint2 x = chunk_gated(a, make_uint2(gate.x, gate.y)), y = chunk_gated(b, make_uint2(gate.z, gate.w));
+    return make_uint4(x.x, x.y, y.x, y.y);
 }
 QM_DEV float chunk_inverse(float l) { return l != 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f; }      // 0: nothing to see
 
@@ -629,8 +633,8 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][10
     const int c = lane & 15, g = lane >> 4;
     uint8_t* meta = buf + QMK_KV4_META;
     ChunkNan nan{0, 0};
-    if (chunk_odd(meta, lane)) chunk_mend<false>(meta, lane);
-    if (chunk_odd(meta + 512, lane)) nan = chunk_mend<true>(meta + 512, lane);
+    if (CHUNK_SELDOM(chunk_odd(meta, lane))) chunk_mend<false>(meta, lane);
+    if (CHUNK_SELDOM(chunk_odd(meta + 512, lane))) nan = chunk_mend<true>(meta + 512, lane);
     floatx4 x[NF][2];
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
@@ -692,7 +696,7 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][10
             for (int f = 0; f < NF; ++f) st.o[f][4 * j + m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[f], st.o[f][4 * j + m], 0, 0, 0);
         }
     }
-    if (nan.low | nan.high) {                              // uniform
+    if (CHUNK_SELDOM(nan.low | nan.high)) {                              // uniform
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -706,7 +710,7 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][10
 
 template <int NF>
 QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
-    const int c = lane & 15, g = lane >> 4, head = 4 * kvh + (c & 3);
+    const int c = lane & 15, g = lane >> 4;
     const int i0 = 4 * NF * it.block, first_pos = it.r.len - it.r.n + i0;
     const int end = it.r.len - it.r.n + min(it.r.n, i0 + 4 * NF);             // past the block's last token
     const int h0 = 2 * ta + w, h_end = min(2 * tb, (end + QMK_KV4_HALF_TOKENS - 1) / QMK_KV4_HALF_TOKENS);
@@ -757,49 +761,58 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
         now = next;
         next = fetch(round + 2, h + 2 * CHUNK_WAVES);
     }
-    // The waves' sums: dim groups 2 w, 2 w + 1 of all columns are this wave's to join.
+    // The waves' sums, by way of LDS: columns 2 w, 2 w + 1 are this wave's to
+    // join, 4 dims a lane.  (Entries are turned over so that neither the writes,
+    // a dim group's, nor the reads, a column's, meet in a bank.)
     const bool whole = tb - ta == it.tiles;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const float l = sum_xor32(sum_xor16(st.sum[f].l));
         float* mine = reinterpret_cast<float*>(sh.ring[w][0]);
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt + 4 * lane) = st.o[f][dt];
+        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt + 4 * ((c ^ (g + 4 * (dt & 1))) + 16 * g)) = st.o[f][dt];
         if (lane < 16) {
             mine[4096 + lane] = st.sum[f].m;
             mine[4112 + lane] = l;
         }
-        const int i = i0 + 4 * f + (c >> 2);
-        const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
         uint2 gate[2];
+        uint16_t* out[2];
+        bool there[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 16 * (2 * w + j) + 4 * g);
-        __syncthreads();
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, reinterpret_cast<const float*>(sh.ring[k][0])[4096 + c]);
-        floatx4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-        for (int k = 0; k < CHUNK_WAVES; ++k) {
-            const float* a = reinterpret_cast<const float*>(sh.ring[k][0]);
-            const float e = a[4096 + c] == M ? 1.0f : __builtin_amdgcn_exp2f(a[4096 + c] - M);
-            L = fmaf(a[4112 + c], e, L);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const floatx4*>(a + 512 * w + 256 * j + 4 * lane) * e;
+        for (int j = 0; j < 2; ++j) {
+            const int col = 2 * w + j, i = i0 + 4 * f + (col >> 2);
+            there[j] = i < it.r.n;                         // uniform
+            const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + 4 * kvh + (col & 3);
+            gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
+            out[j] = A.out + at * QM_GQA_HD + 4 * lane;
         }
-        if (!whole) {
-            float* to = part + f * QMK_CHUNK_COLUMN;
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 2; ++j) *reinterpret_cast<floatx4*>(to + 256 * (2 * w + j) + 4 * lane) = o[j];
-            if (w == 0 && lane < 16) {
-                to[4096 + lane] = M;
-                to[4112 + lane] = L;
+        for (int j = 0; j < 2; ++j) {
+            if (!there[j]) continue;
+            const int col = 2 * w + j;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, reinterpret_cast<const float*>(sh.ring[k][0])[4096 + col]);
+            floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < CHUNK_WAVES; ++k) {
+                const float* a = reinterpret_cast<const float*>(sh.ring[k][0]);
+                const float e = a[4096 + col] == M ? 1.0f : __builtin_amdgcn_exp2f(a[4096 + col] - M);
+                L = fmaf(a[4112 + col], e, L);
+                // dims 4 lane ..: group lane >> 2, entry of the column and lane & 3
+                o += *reinterpret_cast<const floatx4*>(a + 256 * (lane >> 2) + 4 * ((col ^ ((lane & 3) + (lane & 4))) + 16 * (lane & 3))) * e;
             }
-        } else if (i < it.r.n) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                chunk_out(A.out + at * QM_GQA_HD + 16 * (2 * w + j) + 4 * g, o[j], chunk_inverse(L), gate[j]);
+            if (whole) {
+                *reinterpret_cast<uint2*>(out[j]) = chunk_gated(o * chunk_inverse(L), gate[j]);
+            } else {
+                float* to = part + f * QMK_CHUNK_COLUMN;
+                *reinterpret_cast<floatx4*>(to + 256 * col + 4 * lane) = o;
+                if (lane == 0) {
+                    to[4096 + col] = M;
+                    to[4112 + col] = L;
+                }
+            }
         }
         __syncthreads();                                   // before the next column's, or the next block's pages
     }
@@ -926,7 +939,7 @@ QM_DEV void many_half(ManyWave& st, ChunkLds& sh, int buf, int half, int k0, boo
                      if ((i & 3) == 1) part.word(sh, buf ^ 1, i >> 2, w, lane);
                  });
     const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][half]);
-    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
+    if (CHUNK_SELDOM(__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3])))) {
         const int seen = st.pos - k0;                      // the last of the half's tokens that the row sees
         const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
 #pragma unroll
@@ -996,26 +1009,55 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
         next = after;
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
+    // The rows by way of LDS (the tiles are read), 128 dims at a time, so that
+    // memory sees whole runs of them.  Quad k of a row stands at k ^ row.
     const float l = sum_xor32(st.sum.l);
-    if (tb - ta == it.tiles) {
-        const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + head;
-        const uint16_t* gate = A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * h;
-        uint2 x[32];
+    const bool whole = tb - ta == it.tiles;
+    const float inv = whole ? chunk_inverse(l) : 1.0f;
+    const int ln = chunk_lane(lane), col = ln & 31;
+    uint4 gate[2][8];                                      // in place of the queries: their latency passes once
+    if (whole) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = *reinterpret_cast<const uint2*>(gate + 8 * j);
-        if (i < it.r.n) {
+        for (int j = 0; j < 8; ++j) {
+            const int row = min(i0 + 4 * j + (ln >> 4), it.r.n - 1);
+            const uint16_t* at = A.q_gate + ((size_t)(it.r.begin + row) * QM_GQA_HEADS + head) * (2 * QM_GQA_HD) + QM_GQA_HD + 8 * (ln & 15);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) chunk_out(A.out + at * QM_GQA_HD + 8 * j + 4 * h, many_four(st, j), chunk_inverse(l), x[j]);
+            for (int p = 0; p < 2; ++p) gate[p][j] = *reinterpret_cast<const uint4*>(at + 128 * p);
         }
-        return;
     }
+    uint8_t* mine = sh.tile[0] + 16384 * w;
     part += w * 2 * QMK_CHUNK_COLUMN;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) *reinterpret_cast<floatx4*>(part + 256 * j + 4 * lane) = many_four(st, j);
-    if (lane < 32) {
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) *reinterpret_cast<floatx4*>(mine + 512 * col + 16 * ((2 * j + (ln >> 5)) ^ col)) = many_four(st, 16 * p + j) * inv;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (whole) {
+            // 16 lanes a row, 8 dims a lane
+            const int k = ln & 15, d = 128 * p + 8 * k;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = 4 * j + (ln >> 4), row = i0 + at;
+                const floatx4 a = *reinterpret_cast<const floatx4*>(mine + 512 * at + 16 * ((2 * k) ^ at));
+                const floatx4 b = *reinterpret_cast<const floatx4*>(mine + 512 * at + 16 * ((2 * k + 1) ^ at));
+                if (row < it.r.n)
+                    *reinterpret_cast<uint4*>(A.out + ((size_t)(it.r.begin + row) * QM_GQA_HEADS + head) * QM_GQA_HD + d) = chunk_gated8(a, b, gate[p][j]);
+            }
+        } else {
+            // 32 lanes a row, 4 dims a lane
+#pragma unroll 4
+            for (int j = 0; j < 16; ++j) {
+                const int at = 2 * j + (ln >> 5);
+                *reinterpret_cast<floatx4*>(part + 256 * at + 128 * p + 4 * col) = *reinterpret_cast<const floatx4*>(mine + 512 * at + 16 * (col ^ at));
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // read, before it is written again
+    }
+    if (!whole && lane < 32) {
         part[8192 + lane] = st.sum.m;
         part[8224 + lane] = l;
     }
+    asm volatile("s_barrier" ::: "memory");                // before the next block's tiles
 }
 
 // MANY: rows of more than QMK_CHUNK_FEW tokens as well (max_new says whether
@@ -1028,7 +1070,7 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2;
     const Deal<NF> deal(A, lane);
-    if (blockIdx.x == 0 && w == 0) {                       // for the merge
+    if (CHUNK_SELDOM(blockIdx.x == 0 && w == 0)) {                       // for the merge
         int many = 0, few = 0;
         for (int b = lane; b < A.batch; b += 64) {
             const ChunkRow r = chunk_row(A, b);
@@ -1038,11 +1080,18 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
         if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
     }
-    const double end = deal.pieces ? 0.0 : deal.begin(index + 1);
-    for (double u = deal.pieces ? -1.0 : deal.begin(index); u < end;) {      // uniform, as all of it
+    double u = -1.0, end = 0.0;
+    if (CHUNK_SELDOM(!deal.pieces)) {
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {                      // the code once
+            u = end;
+            end = deal.begin(index + i);
+        }
+    }
+    while (u < end) {                                      // uniform, as all of it
         typename Deal<NF>::Item it;
         int ta, tb, last;                                  // the block's last workgroup
-        if (deal.pieces) {
+        if (!CHUNK_SELDOM(!deal.pieces)) {
             int n;
             if (!deal.find_piece(index, it, ta, tb, n)) return;
             last = index + n - 1;
@@ -1077,74 +1126,83 @@ extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_3
 extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_many(GqaChunkArgs A) { chunk_attention<2, true>(A); }
 
 // The partial sums of a row block that several workgroups share, joined: a
-// workgroup per (row block, kv head, operand column or wave's rows, quarter of
-// the dims), a wave Q quads of dims.  N partials' loads are in flight at a time.
+// wave per Q rows of an operand column's 16, or of a wave's 32, 4 dims a lane.
+// N partials' loads are in flight at a time.
 template <int N, int Q>
-QM_DEV void chunk_join(float& m, float& l, floatx4 (&o)[Q], const float* first, const float* others, int n, size_t stride, int quad, int sums,
-                       int rows, int lane) {
-    const int c = lane & (rows - 1);
+QM_DEV void chunk_join(float (&m)[Q], float (&l)[Q], floatx4 (&o)[Q], const float* first, const float* others, int n, size_t stride, int row,
+                       int sums, int rows, int lane) {
     for (int s0 = 0; s0 < n; s0 += N) {                    // uniform
         floatx4 a[N][Q];
-        float pm[N], pl[N];
+        float pm[N][Q], pl[N][Q];
 #pragma unroll
         for (int k = 0; k < N; ++k) {                      // past the last: the last again, with weight 0
             const int i = min(s0 + k, n - 1);
             const float* part = i == 0 ? first : others + i * stride;
 #pragma unroll
-            for (int j = 0; j < Q; ++j) a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (quad + j) + 4 * lane);
-            pm[k] = part[sums + c];
-            pl[k] = part[sums + rows + c];
+            for (int j = 0; j < Q; ++j) {
+                a[k][j] = *reinterpret_cast<const floatx4*>(part + 256 * (row + j) + 4 * lane);
+                pm[k][j] = part[sums + row + j];
+                pl[k][j] = part[sums + rows + row + j];
+            }
         }
-        float top = m;
 #pragma unroll
-        for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k]);
-        const float corr = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        l *= corr;
+        for (int j = 0; j < Q; ++j) {
+            float top = m[j];
 #pragma unroll
-        for (int j = 0; j < Q; ++j) o[j] *= corr;
+            for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k][j]);
+            const float corr = m[j] == top ? 1.0f : __builtin_amdgcn_exp2f(m[j] - top);
+            l[j] *= corr;
+            o[j] *= corr;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            // a partial of no weight counts all the same: a NaN in it reaches the output (the last again has no other)
-            const float f = s0 + k >= n ? 0.0f : pm[k] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - top);
-            l = fmaf(pl[k], f, l);
-#pragma unroll
-            for (int j = 0; j < Q; ++j) o[j] += a[k][j] * f;
+            for (int k = 0; k < N; ++k) {
+                // a partial of no weight counts all the same: a NaN in it reaches the output (the last again has no other)
+                const float f = s0 + k >= n ? 0.0f : pm[k][j] == top ? 1.0f : __builtin_amdgcn_exp2f(pm[k][j] - top);
+                l[j] = fmaf(pl[k][j], f, l[j]);
+                o[j] += a[k][j] * f;
+            }
+            m[j] = top;
         }
-        m = top;
     }
 }
 // FEW: of a block of few tokens, else of many.
 template <int NF, bool MANY, bool FEW>
 QM_DEV void chunk_merge_one(const GqaChunkArgs& A, int k) {
     constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;  // of a workgroup's partial
-    constexpr int kUnits = FEW ? NF : CHUNK_WAVES, kRows = FEW ? 16 : 32, kStep = FEW ? 16 : 8, kSums = FEW ? 4096 : 8192, Q = FEW ? 1 : 2;
+    constexpr int kUnits = FEW ? NF : CHUNK_WAVES, kRows = FEW ? 16 : 32, kSums = FEW ? 4096 : 8192, Q = FEW ? 1 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int quad = (4 * (k & 3) + wave) * Q, unit = (k >> 2) % kUnits, kvh = (k >> 2) / kUnits & 3, number = k / (16 * kUnits);
+    const int row = (4 * (k & 3) + wave) * Q, unit = (k >> 2) % kUnits, kvh = (k >> 2) / kUnits & 3, number = k / (16 * kUnits);
     const int count = A.counts[FEW];
     const ChunkRecord rec = A.records[(FEW ? A.many : 0) + number];
     if (number >= count || rec.from == rec.to) return;     // uniform
-    // row of the block, and first dim, of the lane's quads
-    const int c = lane & (kRows - 1), g = lane / kRows, head = 4 * kvh + (FEW ? c & 3 : unit & 3);
-    const int i = FEW ? 4 * NF * rec.block + 4 * unit + (c >> 2) : QMK_CHUNK_TOKENS * rec.block + 32 * (unit >> 2) + c;
-    const int d0 = kStep * quad + 4 * g;
-    const size_t at = (size_t)(rec.begin + min(i, rec.n - 1)) * QM_GQA_HEADS + head;
+    // tokens of the block, and heads, of the rows
+    const int i = FEW ? 4 * NF * rec.block + 4 * unit + (row >> 2) : QMK_CHUNK_TOKENS * rec.block + 32 * (unit >> 2) + row;
+    const int head = 4 * kvh + (FEW ? row & 3 : unit & 3);
+    if (i >= rec.n) return;
     uint2 gate[Q];
+    uint16_t* out[Q];
 #pragma unroll
-    for (int j = 0; j < Q; ++j) gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + d0 + j * kStep);
-    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < Q; ++j) {
+        const size_t at = (size_t)(rec.begin + min(i + j, rec.n - 1)) * QM_GQA_HEADS + head;
+        gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
+        out[j] = A.out + at * QM_GQA_HD + 4 * lane;
+    }
+    float m[Q], l[Q];
     floatx4 o[Q];
 #pragma unroll
-    for (int j = 0; j < Q; ++j) o[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < Q; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+        o[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     // the first workgroup's part ends its run, the others' begin theirs
     const size_t slot = (size_t)kColumns * QMK_CHUNK_COLUMN;
     const float* base = A.partial + (size_t)(2 * (4 * rec.from + kvh)) * slot + (size_t)(FEW ? 1 : 2) * unit * QMK_CHUNK_COLUMN;
     const int n = rec.to - rec.from + 1;
-    if (n <= 4) chunk_join<4, Q>(m, l, o, base + slot, base, n, 8 * slot, quad, kSums, kRows, lane);
-    else chunk_join<32 / Q, Q>(m, l, o, base + slot, base, n, 8 * slot, quad, kSums, kRows, lane);
-    if (i < rec.n) {
+    if (n <= 4) chunk_join<4, Q>(m, l, o, base + slot, base, n, 8 * slot, row, kSums, kRows, lane);
+    else chunk_join<8, Q>(m, l, o, base + slot, base, n, 8 * slot, row, kSums, kRows, lane);
 #pragma unroll
-        for (int j = 0; j < Q; ++j) chunk_out(A.out + at * QM_GQA_HD + d0 + j * kStep, o[j], chunk_inverse(l), gate[j]);
-    }
+    for (int j = 0; j < Q; ++j)
+        if (i + j < rec.n) *reinterpret_cast<uint2*>(out[j]) = chunk_gated(o[j] * chunk_inverse(l[j]), gate[j]);
 }
 template <int NF, bool MANY>
 QM_DEV void chunk_merge(const GqaChunkArgs& A) {

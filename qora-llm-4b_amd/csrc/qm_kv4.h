@@ -41,11 +41,10 @@
 #define QMK_CHUNK_TOKENS 64         // others in blocks of so many
 #define QMK_CHUNK_WEIGHT 7          // what a page costs a block of many tokens, against one of few
 #define QMK_CHUNK_FEW_PIECE 4       // pages of a block of few tokens that are worth a workgroup
-#define QMK_CHUNK_MANY_PIECE 3      // and of many
 #define QMK_CHUNK_MIN_UNITS 4       // the same where workgroups have runs of several blocks
 #define QMK_CHUNK_WHOLE 8           // a row block of so many pages falls to one
 #define QMK_CHUNK_MAX_GROUPS 64     // workgroups per kv head
-#define QMK_CHUNK_COLUMN 4128       // f32 of an operand column's partial: 16 dim groups x 256, m[16], l[16]
+#define QMK_CHUNK_COLUMN 4128       // f32 of 16 rows' partial sums: [16][256], m[16], l[16] (32 rows: twice each)
 
 #ifdef __HIPCC__
 #define QMK_HD __host__ __device__ inline
