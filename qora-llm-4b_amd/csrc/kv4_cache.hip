@@ -263,41 +263,66 @@ QM_DEV double xor16_sum_f64(double x) {
     const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
     return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
 }
-// The value four lanes on (lanes 0..3 of a row of 16) or back (4..7).
-QM_DEV uint32_t partner4(uint32_t x) {
-    const int on = __builtin_amdgcn_update_dpp(0, (int)x, 0x104, 0xF, 0x1, false);
-    return (uint32_t)__builtin_amdgcn_update_dpp(on, (int)x, 0x114, 0xF, 0x2, false);
+// x where the row and bank (of four lanes) are none of the masks', else y moved by CTRL.
+template <int CTRL, int ROWS, int BANKS>
+QM_DEV uint32_t take_dpp(uint32_t x, uint32_t y) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)y, CTRL, ROWS, BANKS, false); }
+template <int CTRL, int ROWS, int BANKS>
+QM_DEV double take_dpp(double x, double y) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x), v = __builtin_bit_cast(uint64_t, y);
+    return __builtin_bit_cast(double, (uint64_t)take_dpp<CTRL, ROWS, BANKS>((uint32_t)(u >> 32), (uint32_t)(v >> 32)) << 32 |
+                                          take_dpp<CTRL, ROWS, BANKS>((uint32_t)u, (uint32_t)v));
 }
-QM_DEV double partner4(double x) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    return __builtin_bit_cast(double, (uint64_t)partner4((uint32_t)(u >> 32)) << 32 | partner4((uint32_t)u));
+// Rows 0 of x and y, and 2, side by side.
+QM_DEV double rows_f64(double x, double y) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x), v = __builtin_bit_cast(uint64_t, y);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)v, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(v >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]);
 }
 
-// Dims 8 i .. of a token's row, as f32.
-struct Row8 {
-    float x[8];
-};
-QM_DEV Row8 row8(const uint16_t* p) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    Row8 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        r.x[2 * e] = bf16_to_f32((uint16_t)(w[e] & 0xffffu));
-        r.x[2 * e + 1] = bf16_to_f32((uint16_t)(w[e] >> 16));
+// Eight dims of a token's row, as they come.
+struct RowBf16 {
+    uint4 u;
+    QM_DEV void load(const uint16_t* p) { u = *reinterpret_cast<const uint4*>(p); }
+    QM_DEV float at(int e) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     }
-    return r;
+};
+struct RowF32 {
+    float4 a, b;
+    QM_DEV void load(const float* p) { a = ld4(p), b = ld4(p + 4); }
+    QM_DEV float at(int e) const {
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        return x[e];
+    }
+};
+
+QM_DEV uint4 pack_f64(const double (&y)[8]) {
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = f64_to_f16_by_f32(y[e]);
+    return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
 }
-QM_DEV Row8 row8(const float* p) {
-    const float4 a = ld4(p), b = ld4(p + 4);
-    return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
-QM_DEV uint4 pack8(const uint16_t (&h)[8]) {
-    return make_uint4((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16,
-                      (uint32_t)h[4] | (uint32_t)h[5] << 16, (uint32_t)h[6] | (uint32_t)h[7] << 16);
+// A token's row normed, eight dims a lane of 32.
+template <class Row>
+QM_DEV void append_norm(double (&y)[8], const Row& x, const double (&gamma)[8]) {
+    double ss = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        y[e] = (double)x.at(e);
+        ss = __builtin_fma(y[e], y[e], ss);
+    }
+    ss += dpp_f64<0xB1>(ss);
+    ss += dpp_f64<0x4E>(ss);
+    ss += dpp_f64<0x141>(ss);
+    ss += dpp_f64<0x140>(ss);
+    const double inv = inverse_root_f64(xor16_sum_f64(ss) * (1.0 / QM_GQA_HD) + 1e-6);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * gamma[e];
 }
 
-template <class T>
+template <class T, class Row>
 QM_DEV void kv4_append(const Kv4AppendArgs& A) {
     __shared__ __attribute__((aligned(16))) uint32_t image[QMK_KV4_HALF_BYTES / 4];
     const int tid = threadIdx.x, head = blockIdx.x & 3;
@@ -308,62 +333,75 @@ QM_DEV void kv4_append(const Kv4AppendArgs& A) {
     if ((h.t0 >> 6) >= A.c.max_pages) return;
     const int id = A.c.table[(size_t)h.row * A.c.max_pages + (h.t0 >> 6)];
     const HalfLane at = half_lane(tid);
-    const T* from = reinterpret_cast<const T*>(at.is_v ? A.v : A.k);
-    Row8 x[4];
-    float cs[4][8], sn[4][8];
+    const T* from = reinterpret_cast<const T*>(at.is_v ? A.v : A.k) + ((ptrdiff_t)(h.begin + (h.t0 - h.first)) * 4 + head) * 256 + 8 * at.i;
+    auto token = [&](int k) { return min(max(16 * at.u + 4 * at.g + k, lo), hi - 1); };      // any new one for the others
+    Row x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int t = min(max(16 * at.u + 4 * at.g + k, lo), hi - 1);          // any new token for the others
-        x[k] = row8(from + ((size_t)(h.begin + (h.t0 - h.first) + t) * 4 + head) * 256 + 8 * at.i);
-        if (!at.is_v) {                                 // uniform per wave
-            const size_t r = (size_t)(h.t0 + t) * (QM_GQA_ROT / 2) + 8 * (at.i & 3);
-            const Row8 c = row8(A.rope_cos + r), s = row8(A.rope_sin + r);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) cs[k][e] = c.x[e], sn[k][e] = s.x[e];
-        }
-    }
-    if (!kv4_is_page(A.c, id)) return;
-    const int holders = A.c.refs[id];
+    for (int k = 0; k < 4; ++k) x[k].load(from + (ptrdiff_t)token(k) * 1024);
     uint4 raw[4];
-    if (at.is_v) {
+    int holders;
+    if (at.is_v) {                                      // uniform per wave
+        if (!kv4_is_page(A.c, id)) return;
+        holders = A.c.refs[id];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            uint16_t out[8];
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out[e] = f32_to_f16(x[k].x[e]);
-            raw[k] = pack8(out);
+            for (int e = 0; e < 8; ++e) w[e] = f32_to_f16(x[k].at(e));
+            raw[k] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
         }
     } else {
+        // Only dims 0 .. 63 turn, lanes 0 .. 7 of a token's 32: those of the four
+        // tokens turn together, token k's in lanes 8 k .. (each by itself, a
+        // quarter of the lanes at work, 37 us where this takes 34).
+        RowF32 c, s;
+        const size_t r = (size_t)(h.t0 + token(at.i >> 3)) * (QM_GQA_ROT / 2) + 8 * (at.i & 3);
+        c.load(A.rope_cos + r);
+        s.load(A.rope_sin + r);
         const uint4 gw = *reinterpret_cast<const uint4*>(A.k_norm + 8 * at.i);
+        if (!kv4_is_page(A.c, id)) return;
+        holders = A.c.refs[id];
         const uint32_t g[4] = {gw.x, gw.y, gw.z, gw.w};
+        double gamma[8], turn[2][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gamma[e] = 1.0 + (double)f16_to_f32((uint16_t)(g[e >> 1] >> (16 * (e & 1))));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            double y[8], ss = 0.0;
+            double y[8];
+            append_norm(y, x[k], gamma);
+            raw[k] = pack_f64(y);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[e] = (double)x[k].x[e];
-                ss = __builtin_fma(y[e], y[e], ss);
-            }
-            ss += dpp_f64<0xB1>(ss);
-            ss += dpp_f64<0x4E>(ss);
-            ss += dpp_f64<0x141>(ss);
-            ss += dpp_f64<0x140>(ss);
-            const double inv = inverse_root_f64(xor16_sum_f64(ss) * (1.0 / QM_GQA_HD) + 1e-6);
-            uint16_t out[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[e] = y[e] * inv * (1.0 + (double)f16_to_f32((uint16_t)(g[e >> 1] >> (16 * (e & 1)))));
-                const double p = partner4(y[e]);        // 32 dims on or back
-                const double turned = at.i < 4 ? y[e] * cs[k][e] - p * sn[k][e] : y[e] * cs[k][e] + p * sn[k][e];
-                out[e] = f64_to_f16_by_f32(at.i < 8 ? turned : y[e]);
-            }
-            raw[k] = pack8(out);
+            for (int e = 0; e < 8; ++e) turn[k >> 1][e] = k & 1 ? take_dpp<0x118, 0xF, 0xC>(turn[k >> 1][e], y[e]) : y[e];
         }
+        double y[8];
+        const uint32_t minus = at.i & 4 ? 0u : 0x80000000u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            y[e] = rows_f64(turn[0][e], turn[1][e]);
+            const double p = take_dpp<0x114, 0xF, 0xA>(take_dpp<0x104, 0xF, 0x5>(y[e], y[e]), y[e]);       // 32 dims on or back
+            y[e] = y[e] * (double)c.at(e) + p * (double)__uint_as_float(__float_as_uint(s.at(e)) ^ minus);
+        }
+        const uint4 rot = pack_f64(y);
+        auto back = [&](uint32_t (&to)[4], uint32_t from) {
+            const auto odd = __builtin_amdgcn_permlane16_swap(from, from, false, false);
+            to[0] = take_dpp<0xE4, 0x5, 0x3>(to[0], from);
+            to[1] = take_dpp<0x108, 0x5, 0x3>(to[1], from);
+            to[2] = take_dpp<0xE4, 0x5, 0x3>(to[2], odd[1]);
+            to[3] = take_dpp<0x108, 0x5, 0x3>(to[3], odd[1]);
+        };
+        uint32_t w[4][4] = {{raw[0].x, raw[1].x, raw[2].x, raw[3].x}, {raw[0].y, raw[1].y, raw[2].y, raw[3].y},
+                            {raw[0].z, raw[1].z, raw[2].z, raw[3].z}, {raw[0].w, raw[1].w, raw[2].w, raw[3].w}};
+        back(w[0], rot.x);
+        back(w[1], rot.y);
+        back(w[2], rot.z);
+        back(w[3], rot.w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[k] = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
     }
     write_half(image, kv4_half(A.c, A.layer, id, head, (h.t0 >> 5) & 1), raw, lo, hi, holders, tid);
 }
-extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_append_f32(Kv4AppendArgs A) { kv4_append<float>(A); }
-extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_append_bf16(Kv4AppendArgs A) { kv4_append<uint16_t>(A); }
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS, 4) void qm_kv4_append_f32(Kv4AppendArgs A) { kv4_append<float, RowF32>(A); }
+extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS, 4) void qm_kv4_append_bf16(Kv4AppendArgs A) { kv4_append<uint16_t, RowBf16>(A); }
 
 // lo + s q of the code in bits `shift` .., rounded to f32 and then to f16.  In
 // one step (v_fma_mixlo_f16, which the compiler takes otherwise) it would be
