@@ -66,16 +66,32 @@ QM_DEV uint64_t ordered(double x) {
 QM_DEV double unordered(uint64_t u) { return __builtin_bit_cast(double, u >> 63 ? u & ~(1ull << 63) : ~u); }
 
 #define BEAM_THREADS 1024
-#define BEAM_LIST 128              // keys that are sorted by counting
+#define BEAM_LIST 512              // keys that are sorted by counting
+// A slice that is looked through: its row, first token, and the logit below
+// which none of its tokens is chosen.
+struct BeamLead {
+    int32_t row, t0;
+    float cut;
+    int32_t ended;                 // the row's one continuation
+};
 struct BeamLds {
     double base[QMK_BEAM_MAX];     // score - log-sum of a row, or an ended one's score; not finite: takes no part
     int32_t ended[QMK_BEAM_MAX];
     int32_t hist[256];
+    uint32_t tops[BEAM_THREADS / 16], bound;
     BeamKey list[BEAM_LIST], sorted[QMK_BEAM_MAX];
     BeamKey leaders[QMK_BEAM_MAX];
-    int32_t n, digit, above, inside;
+    BeamLead lead[QMK_BEAM_MAX];
+    int32_t n, digit, above;
 };
 
+template <int CTRL>
+QM_DEV uint64_t max_dpp(uint64_t x) {
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)x, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(x >> 32), CTRL, 0xF, 0xF, false);
+    const uint64_t y = (uint64_t)hi << 32 | lo;
+    return x > y ? x : y;
+}
 // Digit d of a key, from the top: eight of the value, then four of the index
 // (from the other end: the lower is before).
 QM_DEV int key_digit(const BeamKey& k, int d) {
@@ -92,32 +108,79 @@ QM_DEV int key_against(const BeamKey& k, const BeamKey& prefix, int d) {
     return ki == pi ? 0 : ki > pi ? 1 : -1;
 }
 
+QM_DEV void beam_list(BeamLds& sh, const BeamKey& k) {
+    const int at = atomicAdd(&sh.n, 1);
+    if (at < BEAM_LIST) sh.list[at] = k;
+}
+// The list's best `take`, in order, into `out`; their number.
+QM_DEV int beam_sort(BeamLds& sh, int take, BeamKey* out) {
+    const int tid = threadIdx.x, found = min(sh.n, BEAM_LIST);
+    if (tid < found) {
+        const BeamKey k = sh.list[tid];
+        int rank = 0;
+        for (int i = 0; i < found; ++i) rank += before(sh.list[i], k);
+        if (rank < take) out[rank] = k;
+    }
+    __syncthreads();
+    return min(found, take);
+}
+
 // The best `take` of keys key(0 .. n - 1), in order, into `out`; their number.
-// A radix select narrows them, from the top digit on, until BEAM_LIST are left
-// that may be among them (keys differ, so in the end there are).
-template <class F>
+// 64 groups of threads have a largest key each, and the take-th of those is a
+// bound: what is not below is sorted by counting.  Where that is more than
+// BEAM_LIST (equal values), a radix select narrows it, from the top digit on
+// (keys differ, so in the end there are no more).  A thread keeps its first KEEP
+// keys.
+template <int KEEP, class F>
 QM_DEV int beam_best(BeamLds& sh, int n, int take, BeamKey* out, F key) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (n == 0) return 0;                                  // uniform
+    BeamKey kept[KEEP];
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+        kept[r] = key(min(tid + BEAM_THREADS * r, n - 1));
+        if (tid + BEAM_THREADS * r >= n) kept[r].value = 0;
+    }
+    auto each = [&](auto use) {
+#pragma unroll
+        for (int r = 0; r < KEEP; ++r) use(kept[r]);
+        for (int i = tid + BEAM_THREADS * KEEP; i < n; i += BEAM_THREADS) use(key(i));
+    };
+    if (tid == 0) sh.n = 0;
+    uint64_t top = 0;
+    each([&](const BeamKey& k) { top = max(top, k.value); });
+    top = max_dpp<0xB1>(top);
+    top = max_dpp<0x4E>(top);
+    top = max_dpp<0x141>(top);
+    top = max_dpp<0x140>(top);
+    // (the upper halves, but for six bits that make them differ: a bound all the same)
+    if ((lane & 15) == 0) sh.tops[tid >> 4] = ((uint32_t)(top >> 32) & ~63u) | (uint32_t)(63 - (tid >> 4));
+    __syncthreads();
+    if (tid < 64) {
+        const uint32_t mine = sh.tops[lane];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine;
+        if (rank == take - 1) sh.bound = mine & ~63u;
+    }
+    __syncthreads();
+    const uint64_t least = max((uint64_t)sh.bound << 32, (uint64_t)1);       // value 0: none
     BeamKey prefix{0, ~0u};
     int digits = 0, above = 0;
     for (;;) {
         // those at or above the prefix
-        if (tid == 0) sh.n = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += BEAM_THREADS) {
-            const BeamKey k = key(i);
-            if (k.value == 0 || key_against(k, prefix, digits) < 0) continue;
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < BEAM_LIST) sh.list[at] = k;
-        }
+        each([&](const BeamKey& k) {
+            if (k.value < least || (digits && key_against(k, prefix, digits) < 0)) return;
+            beam_list(sh, k);
+        });
         __syncthreads();
         if (sh.n <= BEAM_LIST || digits == 12) break;      // uniform
-        for (int i = tid; i < 256; i += BEAM_THREADS) sh.hist[i] = 0;
+        if (tid < 256) sh.hist[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += BEAM_THREADS) {
-            const BeamKey k = key(i);
-            if (k.value != 0 && key_against(k, prefix, digits) == 0) atomicAdd(&sh.hist[key_digit(k, digits)], 1);
-        }
+        if (tid == 0) sh.n = 0;                            // all have looked at it
+        each([&](const BeamKey& k) {
+            if (k.value >= least && key_against(k, prefix, digits) == 0) atomicAdd(&sh.hist[key_digit(k, digits)], 1);
+        });
         __syncthreads();
         // the digit at which `take` are reached: a wave, lane l with bins 255 - 4 l ..
         if (tid < 64) {
@@ -149,15 +212,7 @@ QM_DEV int beam_best(BeamLds& sh, int n, int take, BeamKey* out, F key) {
         else prefix.index = ~(~prefix.index | (uint32_t)sh.digit << (24 - 8 * (digits - 8)));
         ++digits;
     }
-    const int found = min(sh.n, BEAM_LIST);
-    if (tid < found) {
-        const BeamKey k = sh.list[tid];
-        int rank = 0;
-        for (int i = 0; i < found; ++i) rank += before(sh.list[i], k);
-        if (rank < take) out[rank] = k;
-    }
-    __syncthreads();
-    return min(found, take);
+    return beam_sort(sh, take, out);
 }
 
 extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs A) {
@@ -172,16 +227,19 @@ extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs
             base = score;
         } else if (beam_finite(score)) {
             const BeamSlice* s = A.slices + (size_t)(row0 + b) * A.ns;
+            BeamSlice x[QMK_BEAM_VOCAB / QMK_BEAM_SLICE / 64];
             float top = -INFINITY;
-            for (int i = lane; i < A.ns; i += 64) top = fmaxf(top, s[i].top);
+#pragma unroll
+            for (int i = 0; i < QMK_BEAM_VOCAB / QMK_BEAM_SLICE / 64; ++i) {
+                x[i] = s[min(lane + 64 * i, A.ns - 1)];
+                top = fmaxf(top, x[i].top);
+            }
             top = max_xor32(max_xor16(row_max16(top)));
             double sum = 0.0;
-            for (int i = lane; i < A.ns; i += 64) {
-                const BeamSlice x = s[i];
-                if (x.sum != 0.0f) sum += (double)x.sum * exp((double)(x.top == -INFINITY ? 0.0f : x.top) - (double)top);
-            }
 #pragma unroll
-            for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+            for (int i = 0; i < QMK_BEAM_VOCAB / QMK_BEAM_SLICE / 64; ++i)
+                if (lane + 64 * i < A.ns && x[i].sum != 0.0f) sum += (double)x[i].sum * exp((double)(x[i].top == -INFINITY ? 0.0f : x[i].top) - (double)top);
+            sum = wave_sum64(sum);
             base = (double)score - ((double)top + log(sum));           // NaN, infinite: takes no part
         }
         if (lane == 0) {
@@ -195,24 +253,58 @@ extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs
         return __builtin_isfinite(v) ? ordered(v) : 0ull;
     };
     // the best slices, by their best tokens; a row at its end has one continuation
-    const int leaders = beam_best(sh, A.beams * A.ns, A.take, sh.leaders, [&](int i) {
+    const int leaders = beam_best<2>(sh, A.beams * A.ns, A.take, sh.leaders, [&](int i) {
         const int b = i / A.ns, j = i - b * A.ns;
         if (sh.ended[b]) return BeamKey{j == 0 ? value(b, 0.0f) : 0ull, (uint32_t)(b * A.vocab + A.end_id)};
         if (!__builtin_isfinite(sh.base[b])) return BeamKey{0ull, 0u};
         const BeamSlice s = A.slices[(size_t)(row0 + b) * A.ns + j];
         return BeamKey{value(b, s.top), (uint32_t)(b * A.vocab + s.token)};
     });
-    // and the best of those slices' tokens: where the slices are `take`, none is worth less than the last one's best
-    const uint64_t least = leaders == A.take ? sh.leaders[leaders - 1].value : 0ull;
-    const int found = beam_best(sh, leaders * QMK_BEAM_SLICE, A.take, sh.sorted, [&](int i) {
-        const BeamKey lead = sh.leaders[i / QMK_BEAM_SLICE];
-        const int b = lead.index / A.vocab, at = i % QMK_BEAM_SLICE;
-        if (sh.ended[b]) return BeamKey{at == 0 ? lead.value : 0ull, lead.index};
-        const int t = (int)(lead.index - b * A.vocab) / QMK_BEAM_SLICE * QMK_BEAM_SLICE + at;
-        if (t >= A.vocab) return BeamKey{0ull, 0u};
-        const uint64_t v = value(b, A.logits[(size_t)(row0 + b) * A.vocab + t]);
-        return BeamKey{v >= least ? v : 0ull, (uint32_t)(b * A.vocab + t)};
-    });
+    // And the best of those slices' tokens.  Where the slices are `take`, none is
+    // worth less than the last one's best: what passes in f32 is compared in f64.
+    const uint64_t least = leaders == A.take ? sh.leaders[leaders - 1].value : 1ull;
+    if (tid < leaders) {
+        const int index = (int)sh.leaders[tid].index, b = index / A.vocab;
+        // less what the sum's rounding to 64 bits, the difference's and the cut's own can be
+        const double base = sh.base[b], last = unordered(least);
+        const float cut = leaders == A.take ? (float)(last - base - (fabs(base) + fabs(last)) * 0x1p-50) : -INFINITY;
+        sh.lead[tid] = BeamLead{b, (index - b * A.vocab) / QMK_BEAM_SLICE * QMK_BEAM_SLICE, fminf(cut - fabsf(cut) * 0x1p-20f - 0x1p-100f, 0x1.fffffep127f), sh.ended[b]};
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    for (int r0 = 0; r0 < leaders; r0 += 8) {              // uniform
+        BeamLead lead[8];
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            lead[r] = sh.lead[min(r0 + r, leaders - 1)];
+            x[r] = A.logits[(size_t)(row0 + lead[r].row) * A.vocab + min(lead[r].t0 + tid, A.vocab - 1)];
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= leaders) break;                  // uniform
+            if (lead[r].ended) {
+                if (tid == 0) beam_list(sh, sh.leaders[r0 + r]);
+            } else if (x[r] >= lead[r].cut && lead[r].t0 + tid < A.vocab) {
+                const uint64_t v = value(lead[r].row, x[r]);
+                if (v >= least) beam_list(sh, BeamKey{v, (uint32_t)(lead[r].row * A.vocab + lead[r].t0 + tid)});
+            }
+        }
+    }
+    __syncthreads();
+    int found;
+    if (sh.n <= BEAM_LIST) {
+        found = beam_sort(sh, A.take, sh.sorted);
+    } else {
+        __syncthreads();                                   // all have looked at it
+        found = beam_best<1>(sh, leaders * QMK_BEAM_SLICE, A.take, sh.sorted, [&](int i) {
+            const BeamLead lead = sh.lead[i / QMK_BEAM_SLICE];
+            const int t = lead.t0 + i % QMK_BEAM_SLICE;
+            if (lead.ended) return BeamKey{i % QMK_BEAM_SLICE == 0 ? value(lead.row, 0.0f) : 0ull, (uint32_t)(lead.row * A.vocab + A.end_id)};
+            if (t >= A.vocab) return BeamKey{0ull, 0u};
+            return BeamKey{value(lead.row, A.logits[(size_t)(row0 + lead.row) * A.vocab + t]), (uint32_t)(lead.row * A.vocab + t)};
+        });
+    }
     if (tid < A.take) {
         const size_t to = (size_t)blockIdx.x * A.take + tid;
         int parent = -1, token = -1, over = 0;

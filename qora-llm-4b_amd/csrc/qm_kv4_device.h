@@ -18,13 +18,6 @@ QM_DEV uint16_t f64_to_f16_by_f32(double x) {
     return f32_to_f16(f);
 }
 
-template <int CTRL>
-QM_DEV double dpp_f64(double x) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 // 1 / sqrt(x): v_rsq_f64 is good to about 2^-24; each step of Newton's squares
 // the error.
 QM_DEV double inverse_root_f64(double x) {

@@ -144,7 +144,7 @@ def select(groups, beams, take, vocab, logits, scores, done, end_id):
             if not np.isfinite(top) or np.isnan(x).any():
                 continue
             base = score - (top + np.log(np.exp(x - top).sum()))
-            order = np.argsort(-x, kind="stable")[:take]
+            order = np.argsort(-(base + x), kind="stable")[:take]          # the values', which can be equal where the logits are not
             here += [(-(base + x[t]), r, int(t), int(t == end_id)) for t in order if np.isfinite(x[t])]
         here.sort(key=lambda c: c[:3])
         found += (here + [(np.inf, -1, -1, 0)] * take)[:take]

@@ -92,6 +92,18 @@ def test_select_of_values_of_other_sizes(ctx):
         run_select(ctx, 1, 3, 10, (scale * rng.standard_normal((3, 9000))).astype(np.float32), np.array([0.0, -0.0, -1e-3]))
 
 
+def test_select_of_scores_that_outweigh_the_logits(ctx):
+    """A sum that is its row's score in 64 bits is every token's: the lowest are chosen, whatever their logits."""
+    rng = np.random.default_rng(6)
+    for vocab in (5, 700, 6000):
+        logits = rng.standard_normal((4, vocab)).astype(np.float32)
+        got = run_select(ctx, 1, 4, 6, logits, np.array([-1e30, -2e30, -1e30, 1.5e30]))
+        assert (got[0][:5] == 3).all() and list(got[1][:5]) == [0, 1, 2, 3, 4]
+    # and one row beside the others' sums
+    logits = (1e30 * rng.standard_normal((2, 3000))).astype(np.float32)
+    run_select(ctx, 1, 2, 20, logits, np.array([-1.0, -2e30]))
+
+
 def test_select_in_place(ctx):
     rng, logits, scores = some(5, 3, 4, 2500)
     done = np.array([0, 1, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1], np.int32)
