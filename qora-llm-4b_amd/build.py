@@ -123,6 +123,13 @@ def build_kv4_reserve_test() -> None:
           str(ROOT / "tests" / "cpp" / "kv4_reserve_test.cpp"), "-o", str(LIB / "kv4_reserve_test")])
 
 
+def build_chunk_test() -> None:
+    """tests/cpp/chunk_test.cpp: the checks and workspaces of chunks of new tokens and of
+    beam search's step on the CPU (g++ only, no device code; test infrastructure)."""
+    _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-I", str(ROOT / "include"), "-I", str(CSRC),
+          str(ROOT / "tests" / "cpp" / "chunk_test.cpp"), "-o", str(LIB / "chunk_test")])
+
+
 if __name__ == "__main__":
     build()
     if "--no-oracle" not in sys.argv:
@@ -133,4 +140,5 @@ if __name__ == "__main__":
         build_dispatch_test()
         build_kv4_test()
         build_kv4_reserve_test()
+        build_chunk_test()
     print("built:", ", ".join(sorted(p.name for p in LIB.iterdir())))
