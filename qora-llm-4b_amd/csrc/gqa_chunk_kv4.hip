@@ -1105,7 +1105,8 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
             u = it.first + (double)tb * weight;
         }
         const bool few = Deal<NF>::few(it.r);
-        if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few))
+        // (ranges that overlap can have more row blocks than there are records)
+        if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few) && it.number < (few ? A.few : A.many))
             A.records[(few ? A.many : 0) + it.number] = ChunkRecord{index, last, it.r.begin, it.r.n, it.block, {0, 0, 0}};
         if (it.r.kind != CHUNK_RUN) {
             const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;

@@ -176,5 +176,5 @@ struct GqaChunkArgs {
     ChunkRecord* records;    // [most of many][most of few]
     int32_t layer, batch, tokens, max_new, max_len;
     int32_t groups;          // workgroups per kv head
-    int32_t many;            // the most row blocks of many tokens that there can be
+    int32_t many, few;       // the most row blocks of many and of few tokens that rows of `tokens` in all have
 };

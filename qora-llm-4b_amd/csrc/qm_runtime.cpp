@@ -1392,7 +1392,8 @@ int32_t qm_gqa_chunk_kv4(qm_context* c, qm_stream stream, const qm_kv4_cache* ca
     char* records = ws + qm_kv4::chunk_partial_bytes(shape);
     GqaChunkArgs a{kv4_of(*cache), slots, begins, q_gate, q_norm, rope_cos, rope_sin, result, out, reinterpret_cast<float*>(ws),
                    reinterpret_cast<int32_t*>(records), reinterpret_cast<ChunkRecord*>(records + 16), layer, batch, tokens, max_new,
-                   max_len, static_cast<int32_t>(shape.groups), static_cast<int32_t>(shape.most_many)};
+                   max_len, static_cast<int32_t>(shape.groups), static_cast<int32_t>(shape.most_many),
+                   static_cast<int32_t>(shape.most_few)};
     const int form = shape.many ? 2 : shape.columns - 1;
     st = launch(c, c->f_gqa_chunk[form], static_cast<uint32_t>(shape.groups * QM_GQA_KV_HEADS), 512, a, s, "qm_gqa_chunk");
     if (st != QM_OK || !shape.split) return st;

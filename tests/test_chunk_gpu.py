@@ -387,3 +387,79 @@ def test_a_chunk_twice_gives_the_same_bits(ctx):
     a = run_chunk(ctx, ref, [130, 80], layer=0)
     b = run_chunk(ctx, ref, [130, 80], layer=0)
     assert np.array_equal(a, b)
+
+
+# ---- more row blocks than workgroups, and few of unequal lengths ---------------------------------
+def many_rows(seed, rows, lo, hi, top, long=()):
+    rng = np.random.default_rng(seed)
+    lens = rng.integers(lo, hi + 1, rows).tolist()
+    news = [int(rng.integers(1, min(n, top) + 1)) for n in lens]
+    for at, n, new in long:
+        lens[at], news[at] = n, new
+    return lens, news
+
+
+@pytest.mark.parametrize("seed, rows, lo, hi, top, long", [
+    (50, 40, 70, 300, 129, []),                                          # runs of blocks of many tokens
+    (51, 60, 1, 200, 70, [(7, 5000, 40), (30, 2500, 70)]),               # of both kinds, long ones among them
+    (52, 100, 1, 130, 40, [(64, 6000, 100), (99, 3000, 1)]),             # more rows than lanes
+    (53, 70, 20, 200, 20, [(3, 4000, 32)]),                              # few tokens, two operand columns
+    (54, 100, 1, 100, 4, [(0, 5000, 4), (71, 2000, 3)]),                 # few tokens, one
+    (55, 3, 60, 70, 60, [(0, 4200, 500), (2, 9000, 33)])])               # few blocks, cut unevenly
+def test_chunk_of_many_row_blocks(ctx, seed, rows, lo, hi, top, long):
+    lens, news = many_rows(seed, rows, lo, hi, top, long)
+    run_chunk(ctx, cache_of(lens, layers=1, seed=seed), news, layer=0, seed=seed)
+
+
+def test_chunk_of_a_prompt_of_more_blocks_than_workgroups(ctx):
+    run_chunk(ctx, cache_of([2200, 2100], layers=1, seed=56), [2200, 2000], layer=0)
+
+
+def test_chunk_ranges_that_overlap_stay_within_the_call(ctx):
+    """Ranges have to ascend; of ones that do not, nothing but their own rows is written."""
+    ref = cache_of([50] * 9, layers=1, seed=57)
+    q, gamma = queries(np.random.default_rng(57), 60)
+    cos, sin = rope(50)
+    c, out = upload(ctx, ref), ctx.upload(np.full((60, 16, 256), FILL, np.uint16))
+    for max_new in (3, 20, 50):
+        ctx.gqa_chunk_kv4(c, 0, 9, None, ints(ctx, [4, 50, 3, 49, 4, 50, 4, 50, 4, 50]), 50, max_new, ctx.upload(q), ctx.upload(gamma.view(np.uint16)),
+                          ctx.upload(cos), ctx.upload(sin), len(cos), 50, None, out)
+    got = ctx.download(out, (60, 16, 256), np.uint16)
+    assert (got[50:] == FILL).all() and (got[:3] == FILL).all()
+    assert_same(ctx, c, ref)
+    run_chunk(ctx, ref, [5] * 9, layer=0)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_two_graphs_share_the_workspace(new):
+    """Captured one after the other, replayed in turn with eager calls between: each as if alone."""
+    own = M.Context(0)
+    own.reserve(2, 5000, 100)
+    lens = [[3000, 700], [450, 4900]]
+    refs = [cache_of(n, layers=1, seed=58 + i, room=5000 - max(n)) for i, n in enumerate(lens)]
+    caches = [upload(own, r) for r in refs]
+    q, gamma = queries(np.random.default_rng(59), 2 * new)
+    cos, sin = rope(5000)
+    up = [own.upload(x) for x in (q, gamma.view(np.uint16), cos, sin)]
+    begins = ints(own, [0, new, 2 * new])
+    outs = [own.alloc(2 * new * 8192) for _ in refs]
+
+    def call(i):
+        own.gqa_chunk_kv4(caches[i], 0, 2, None, begins, 2 * new, new, *up, len(cos), 5000, None, outs[i])
+
+    graphs = []
+    for i in range(2):
+        own.graph_begin()
+        call(i)
+        graphs.append(own.graph_end())
+    wants = [CR.attend(r, 0, 2, None, [0, new, 2 * new], 2 * new, new, CR.bf16_value(q), gamma, cos, sin, 5000) for r in refs]
+    for i in (0, 1, 1, 0, 1):
+        for o in outs:
+            own.upload(np.full((2 * new, 16, 256), FILL, np.uint16), o)
+        call(1 - i)
+        graphs[i].launch()
+        for o, (want, bound, _) in zip(outs, wants):
+            assert_near(CR.bf16_value(own.download(o, (2 * new, 16, 256), np.uint16)), want, bound)
+    for g in graphs:
+        g.close()
+    own.close()
