@@ -764,7 +764,16 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
     // The waves' sums, by way of LDS: columns 2 w, 2 w + 1 are this wave's to
     // join, 4 dims a lane.  (Entries are turned over so that neither the writes,
     // a dim group's, nor the reads, a column's, meet in a bank.)
-    const bool whole = tb - ta == it.tiles;
+    const bool whole = tb - ta == it.tiles;                // uniform
+    auto row_of = [&](int f, int j) { return i0 + 4 * f + ((2 * w + j) >> 2); };
+    auto at_of = [&](int f, int j) { return (size_t)(it.r.begin + min(row_of(f, j), it.r.n - 1)) * QM_GQA_HEADS + 4 * kvh + ((2 * w + j) & 3); };
+    uint2 gate[NF][2];
+    if (whole) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) gate[f][j] = *reinterpret_cast<const uint2*>(A.q_gate + at_of(f, j) * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
+    }
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const float l = sum_xor32(sum_xor16(st.sum[f].l));
@@ -775,36 +784,34 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
             mine[4096 + lane] = st.sum[f].m;
             mine[4112 + lane] = l;
         }
-        uint2 gate[2];
-        uint16_t* out[2];
-        bool there[2];
+        // (LDS only: no wave waits for another's stores)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int col = 2 * w + j, i = i0 + 4 * f + (col >> 2);
-            there[j] = i < it.r.n;                         // uniform
-            const size_t at = (size_t)(it.r.begin + min(i, it.r.n - 1)) * QM_GQA_HEADS + 4 * kvh + (col & 3);
-            gate[j] = *reinterpret_cast<const uint2*>(A.q_gate + at * (2 * QM_GQA_HD) + QM_GQA_HD + 4 * lane);
-            out[j] = A.out + at * QM_GQA_HD + 4 * lane;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (!there[j]) continue;
+            if (row_of(f, j) >= it.r.n) continue;          // uniform
             const int col = 2 * w + j;
-            float M = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int k = 0; k < CHUNK_WAVES; ++k) M = fmaxf(M, reinterpret_cast<const float*>(sh.ring[k][0])[4096 + col]);
-            floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            float m[CHUNK_WAVES], l[CHUNK_WAVES];
+            floatx4 part_o[CHUNK_WAVES];
 #pragma unroll
             for (int k = 0; k < CHUNK_WAVES; ++k) {
                 const float* a = reinterpret_cast<const float*>(sh.ring[k][0]);
-                const float e = a[4096 + col] == M ? 1.0f : __builtin_amdgcn_exp2f(a[4096 + col] - M);
-                L = fmaf(a[4112 + col], e, L);
+                m[k] = a[4096 + col];
+                l[k] = a[4112 + col];
                 // dims 4 lane ..: group lane >> 2, entry of the column and lane & 3
-                o += *reinterpret_cast<const floatx4*>(a + 256 * (lane >> 2) + 4 * ((col ^ ((lane & 3) + (lane & 4))) + 16 * (lane & 3))) * e;
+                part_o[k] = *reinterpret_cast<const floatx4*>(a + 256 * (lane >> 2) + 4 * ((col ^ ((lane & 3) + (lane & 4))) + 16 * (lane & 3)));
+            }
+            float M = m[0], L = 0.0f;
+#pragma unroll
+            for (int k = 1; k < CHUNK_WAVES; ++k) M = fmaxf(M, m[k]);
+            floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < CHUNK_WAVES; ++k) {
+                const float e = m[k] == M ? 1.0f : __builtin_amdgcn_exp2f(m[k] - M);
+                L = fmaf(l[k], e, L);
+                o += part_o[k] * e;
             }
             if (whole) {
-                *reinterpret_cast<uint2*>(out[j]) = chunk_gated(o * chunk_inverse(L), gate[j]);
+                *reinterpret_cast<uint2*>(A.out + at_of(f, j) * QM_GQA_HD + 4 * lane) = chunk_gated(o * chunk_inverse(L), gate[f][j]);
             } else {
                 float* to = part + f * QMK_CHUNK_COLUMN;
                 *reinterpret_cast<floatx4*>(to + 256 * col + 4 * lane) = o;
@@ -814,7 +821,8 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
                 }
             }
         }
-        __syncthreads();                                   // before the next column's, or the next block's pages
+        // before the next column's, or the next block's pages
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 }
 
@@ -1069,7 +1077,6 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
     __shared__ __attribute__((aligned(1024))) uint8_t sm[kBytes];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kvh = blockIdx.x & 3, index = blockIdx.x >> 2;
-    const Deal<NF> deal(A, lane);
     if (CHUNK_SELDOM(blockIdx.x == 0 && w == 0)) {                       // for the merge
         int many = 0, few = 0;
         for (int b = lane; b < A.batch; b += 64) {
@@ -1080,30 +1087,31 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
         if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
     }
-    double u = -1.0, end = 0.0;
-    if (CHUNK_SELDOM(!deal.pieces)) {
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {                      // the code once
-            u = end;
-            end = deal.begin(index + i);
+    for (double u = -1.0;;) {                              // uniform, as all of it
+        // (made anew for each block: nothing of it takes registers while one is attended)
+        const Deal<NF> deal(A, chunk_lane(lane));
+        double end = 0.0;
+        if (CHUNK_SELDOM(!deal.pieces)) {
+            end = deal.begin(index + 1);
+            if (u < 0.0) u = deal.begin(index);
+            if (u >= end) return;
         }
-    }
-    while (u < end) {                                      // uniform, as all of it
         typename Deal<NF>::Item it;
         int ta, tb, last;                                  // the block's last workgroup
         if (!CHUNK_SELDOM(!deal.pieces)) {
             int n;
             if (!deal.find_piece(index, it, ta, tb, n)) return;
             last = index + n - 1;
-            u = end;
+            u = -1.0;
         } else {
             it = deal.find(u, true);
             const int weight = Deal<NF>::weight(it.r);
             ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
             tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
             last = tb == it.tiles ? index : (int)((it.first + (double)it.tiles * weight - 1.0) / deal.each);
-            u = it.first + (double)tb * weight;
+            u = Deal<NF>::lane_of(it.first + (double)tb * weight, 0);
         }
+        const bool more = u >= 0.0 && u < end;
         const bool few = Deal<NF>::few(it.r);
         // (ranges that overlap can have more row blocks than there are records)
         if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few) && it.number < (few ? A.few : A.many))
@@ -1114,12 +1122,14 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
             uint16_t* out = A.out + (size_t)(it.r.begin + i0) * QM_GQA_HEADS * QM_GQA_HD + (size_t)4 * kvh * QM_GQA_HD + 4 * lane;
             for (int j = w; j < 4 * count; j += CHUNK_WAVES)
                 *reinterpret_cast<uint2*>(out + ((size_t)(j >> 2) * QM_GQA_HEADS + (j & 3)) * QM_GQA_HD) = make_uint2(fill, fill);
+            if (!more) return;
             continue;
         }
         // a workgroup's first block may have begun before it, its last end after it
         float* part = A.partial + (size_t)(2 * blockIdx.x + (ta == 0)) * kColumns * QMK_CHUNK_COLUMN;
         if (MANY && !few) many_item<NF>(A, *reinterpret_cast<ChunkLds*>(sm), it, ta, tb, kvh, part, w, lane);
         else few_item<NF>(A, *reinterpret_cast<FewLds<NF>*>(sm), it, ta, tb, kvh, part, w, lane);
+        if (!more) return;
     }
 }
 extern "C" __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void qm_gqa_chunk_4(GqaChunkArgs A) { chunk_attention<1, false>(A); }
