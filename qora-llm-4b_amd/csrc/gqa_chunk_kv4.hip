@@ -9,18 +9,36 @@
 // rounded to f16 once.  q, p (relative to a running maximum, in base 2) and
 // the operands are f16, all sums f32.
 //
-// A workgroup (8 waves) owns a row block of 64 new tokens of the four query
-// heads of a kv head: wave w has head w & 3 and 32 tokens, the columns of a
-// 32 x 32 x 16 matrix instruction.  Both products run transposed, S^T = K Q^T
-// and O^T = V^T P^T, so that a lane's scores, its running maximum and its
-// outputs are all of one row, and its scores are, as they stand, the eight keys
-// that a word of V codes holds.  A page of the kv head (64 tokens) is a tile:
-// its codes come by LDS DMA, each wave makes f16 operands of an eighth of them,
-// and the tile before it is multiplied meanwhile.
+// Both products run transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane's
+// scores, its running maximum and its outputs are all of one row, and its
+// scores are, as they stand, the keys that a word of V codes holds: between the
+// products nothing changes lanes.  The scores come out counted from the row's
+// reference (the product begins at its negative), so that a weight is one exp2;
+// the reference moves, and outputs are rescaled, only where a score passes it by
+// CHUNK_SLACK.
 //
-// The pages of all row blocks of a kv head are dealt to the workgroups in equal
-// runs; where a block's pages fall to several, they leave partial sums and
-// qm_gqa_chunk_merge joins them.
+// Two forms, by a row's new tokens, one workgroup of 8 waves a CU in both:
+//   few   (up to 32) blocks of 4 NF tokens x 4 heads, the columns of a 16 x 16 x
+//         32 product.  A wave has half pages of its own, their codes by LDS DMA
+//         two ahead, and makes operands of them in registers; the waves' sums
+//         are joined at the end.  Bound by HBM once there is enough to read: 24
+//         rows of up to 12001 tokens 44 us with the merge, 22 of it while the
+//         codes stream (6 TB/s), 8 before the first of them (lengths -> deal ->
+//         table -> page), the joins 9.  Vector unit 60% busy, matrix unit 11%.
+//   many  blocks of 64 tokens: wave w has head w & 3 and 32 of them, the columns
+//         of a 32 x 32 x 16 product.  A page is a tile: its codes come by LDS
+//         DMA, each wave makes f16 operands of an eighth of them, which all
+//         waves read, in between the second product's matrix instructions of the
+//         tile before; a barrier a tile.  Bound by the matrix unit and what
+//         issues beside it: 2048 tokens of 32768 1035 us, 1.05 PFLOP/s (a large
+//         f16 product 1.19), matrix unit 51% busy at the clock that this load
+//         leaves, vector unit 43%; a tile takes 3.3 us, 4.2 with every CU at it.
+//         An operand a wave for itself, as above, would be made eight times over.
+//         64 tokens of 64 take 21 us of it in one workgroup, nearly all of them
+//         the latency of code and data that come once.
+//
+// Row blocks are dealt over the workgroups, in pieces where one has too many
+// pages (Deal); pieces leave partial sums, which qm_gqa_chunk_merge joins.
 #include "qm_kv4_device.h"
 #include "qm_kernel_args.h"
 
@@ -78,6 +96,10 @@ struct Deal {
     double total, each;
     double incl, units;
 
+    // Pages that a block of few tokens is not cut below: more where no block of the
+    // call is, for then there is no merge (500 tokens whole 14 us without and 17
+    // with the merge's launch, cut 14).
+    QM_DEV int whole() const { return A.max_len <= QMK_CHUNK_WHOLE * QMK_KV4_PAGE_TOKENS ? QMK_CHUNK_WHOLE : QMK_CHUNK_FEW_PIECE; }
     QM_DEV static bool few(const ChunkRow& r) { return r.n <= QMK_CHUNK_FEW; }
     QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
     QM_DEV static int blocks(const ChunkRow& r) { return (r.n + tokens(r) - 1) / tokens(r); }
@@ -154,7 +176,7 @@ struct Deal {
                 piece = lane_of(scan(nb * most), 63) / A.groups;
                 for (;;) {
                     cuts = nb ? cuts_of(most, fmax(piece, least)) : 0;
-                    if (few(mine) ? last <= QMK_CHUNK_WHOLE : !many_cut((float)last, (float)all, (float)cuts)) cuts = min(cuts, 1);
+                    if (few(mine) ? last <= whole() : !many_cut((float)last, (float)all, (float)cuts)) cuts = min(cuts, 1);
                     if (__builtin_amdgcn_readlane((int)wave_scan((uint32_t)(nb * cuts)), 63) <= A.groups) break;
                     piece = fmax(piece, 1.0) * 1.125;
                 }
@@ -248,7 +270,7 @@ struct Deal {
         const Item it = find(u, false);
         const int w = weight(it.r);
         int t = (int)((u - it.first) / w);
-        if (it.tiles <= QMK_CHUNK_WHOLE) t = 2 * (u - it.first) < (double)it.tiles * w ? 0 : it.tiles;
+        if (it.tiles <= whole()) t = 2 * (u - it.first) < (double)it.tiles * w ? 0 : it.tiles;
         return it.first + (double)t * w;
     }
 };

@@ -37,12 +37,20 @@
 #define QMK_KV4_ROUNDS 64           // full rounds of decode workgroups that are dealt evenly
 #define QMK_KV4_LEN_PAGES 33554431  // pages of a row: its length is an int32
 #define QMK_CHUNK_MAX_TOKENS (1 << 20)     // new tokens of a call
-#define QMK_CHUNK_FEW 32            // a row of up to so many is attended in blocks of few tokens
+// A row of up to so many new tokens is attended in blocks of few (in blocks of
+// few / of many, us: 32 tokens of 300 20 / 24, of 4000 23 / 34, of 32000 45 / 57,
+// 8 x 32 of 4000 46 / 53; there they grow by 3 a row and block, so no further).
+#define QMK_CHUNK_FEW 32
 #define QMK_CHUNK_TOKENS 64         // others in blocks of so many
-#define QMK_CHUNK_WEIGHT 7          // what a page costs a block of many tokens, against one of few
-#define QMK_CHUNK_FEW_PIECE 4       // pages of a block of few tokens that are worth a workgroup
+// What a page costs a block of many tokens, against one of few: 3.4 us, and 1.9
+// for the eight half pages of a round.
+#define QMK_CHUNK_WEIGHT 7
+// Pages of a block of few tokens that are worth a workgroup (2 / 3 / 4 / 6, us: 1
+// token of 2000 13.9 / 15.3 / 14.4 / 15.7, of 8000 21.0 / 19.7 / 18.0 / 18.2, 5 of
+// 4000 18.9 / 18.5 / 17.3 / 18.7).
+#define QMK_CHUNK_FEW_PIECE 4
 #define QMK_CHUNK_MIN_UNITS 4       // the same where workgroups have runs of several blocks
-#define QMK_CHUNK_WHOLE 8           // a row block of so many pages falls to one
+#define QMK_CHUNK_WHOLE 8           // lengths of up to so many pages: no block of few tokens is cut
 #define QMK_CHUNK_MAX_GROUPS 64     // workgroups per kv head
 #define QMK_CHUNK_COLUMN 4128       // f32 of 16 rows' partial sums: [16][256], m[16], l[16] (32 rows: twice each)
 
