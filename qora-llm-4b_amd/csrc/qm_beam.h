@@ -9,8 +9,8 @@
 #define QMK_STATE_BUFFERS 64        // buffers of one call
 #define QMK_STATE_ROWS 65536        // rows of a buffer: the LDS bitmap of the destinations
 #define QMK_STATE_COUNT 1024        // rows of one call
-#define QMK_STATE_COLUMN 4096       // bytes of a row that a workgroup takes at a time, few rows
-#define QMK_STATE_LDS 65536         // bytes that it holds of all rows, many rows
+#define QMK_STATE_COLUMN 4096       // bytes of a row that a workgroup takes at a time, up to 32 rows
+#define QMK_STATE_LDS 65536         // bytes that it holds of all rows, more than 128
 
 // A slice's largest logit, the lowest token that has it, and the sum of
 // exp(logit - largest).

@@ -58,9 +58,13 @@ inline Fault check_fork(int32_t buffers, const qm_state_rows* list, int32_t rows
     }
     return Fault{};
 }
-// Bytes of a row that a workgroup takes at a time: all rows' fit what it holds.
+// The kernel: rows in registers, up to 8, 32, 64 and 128, or in LDS.
+inline int32_t fork_form(int32_t count) { return count <= 8 ? 0 : count <= 32 ? 1 : count <= 64 ? 2 : count <= 128 ? 3 : 4; }
+// Bytes of a row that a workgroup takes at a time: what its 256 lanes hold, or
+// all rows' fit its LDS.
 inline int32_t fork_column(int32_t count) {
-    if (count <= 32) return QMK_STATE_COLUMN;
+    const int32_t form = fork_form(count);
+    if (form < 4) return form < 2 ? QMK_STATE_COLUMN : QMK_STATE_COLUMN >> (form - 1);
     int32_t wide = QMK_STATE_COLUMN;
     while (wide * count > QMK_STATE_LDS) wide /= 2;
     return wide;

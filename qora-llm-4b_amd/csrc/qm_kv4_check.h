@@ -155,7 +155,9 @@ inline int64_t append_halves(int32_t tokens, int32_t batch) {
 // The chunk attention's shape: operand columns of a block of few tokens (4 new
 // tokens each), whether rows can have more than few, the most row blocks of
 // both kinds, workgroups per kv head (one a CU, or fewer where the blocks'
-// pages are fewer) and whether blocks may be split over them.
+// pages are fewer) and whether blocks may be split over them.  One column where
+// it has all of a row's new tokens (one / two, us: 1 token of 260 11.7 / 13.9, 4
+// of 4000 14.1 / 16.7, 24 x 4 of 12001 82 / 94).
 struct Chunk {
     int32_t columns;
     bool many, split;

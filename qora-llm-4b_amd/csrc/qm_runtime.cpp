@@ -73,7 +73,7 @@ struct qm_context {
     hipFunction_t f_kv4_append[2] = {};      // k and v f32, bf16
     hipFunction_t f_gqa_chunk[3] = {}, f_gqa_chunk_merge[3] = {};      // rows of up to 4 new tokens, up to 32, more
     hipFunction_t f_beam_slices = nullptr, f_beam_draw = nullptr;
-    hipFunction_t f_state_fork[3] = {};      // up to 8 rows, up to 32, more
+    hipFunction_t f_state_fork[5] = {};      // up to 8 rows, up to 32, 64, 128, more
     int lm_head_hidden = 0;              // the hidden size lm_head_wg_per_cu was computed for
     int lm_head_wg_per_cu = 1;
     int dnp_chunk_threads = 0;     // the DeltaNet prefill chunk kernel's workgroup size (its launch bounds)
@@ -419,7 +419,9 @@ int32_t qm_create(qm_context** out, const qm_config* cfg, const char* code_objec
     if (st == QM_OK) st = load_function(c, mods[11], "qm_beam_draw", &c->f_beam_draw);
     if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_8", &c->f_state_fork[0]);
     if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_32", &c->f_state_fork[1]);
-    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_many", &c->f_state_fork[2]);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_64", &c->f_state_fork[2]);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_128", &c->f_state_fork[3]);
+    if (st == QM_OK) st = load_function(c, mods[12], "qm_state_fork_many", &c->f_state_fork[4]);
     if (st == QM_OK &&
         (hipFuncGetAttribute(&c->q4_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gemv) != hipSuccess ||
          hipFuncGetAttribute(&c->q4_gu_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, c->f_q4_gate_up) !=
@@ -1435,7 +1437,7 @@ int32_t qm_state_fork(qm_context* c, qm_stream stream, int32_t n_buffers, const 
         a.first[i + 1] = a.first[i] + (buffers[i].row_bytes + a.column - 1) / a.column;
     }
     const int64_t grid = std::min<int64_t>(a.first[n_buffers], 8 * c->num_cu);
-    return launch(c, c->f_state_fork[count <= 8 ? 0 : count <= 32 ? 1 : 2], static_cast<uint32_t>(grid), 256, a,
+    return launch(c, c->f_state_fork[qm_beam::fork_form(count)], static_cast<uint32_t>(grid), 256, a,
                   pick(c, stream), "qm_state_fork");
 }
 

@@ -10,6 +10,7 @@
 #include "qm_beam.h"
 
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
 // The pairs whose rows differ, packed; -1: the list is refused (a row outside
 // the buffers, a destination listed twice).  Every workgroup finds the same.
@@ -52,28 +53,33 @@ QM_DEV int buffer_of(const StateForkArgs& A, int64_t at) {
     return lo;
 }
 
-// Up to N rows: a lane holds its 16 bytes of all of them.
-template <int N>
+// Up to N rows: a lane holds its 16 bytes of all of them, or 8 or 4 of more (in
+// registers / by way of LDS, us, 24 layers' states: 8 rows 170 / 379, 16 348 /
+// 715; 8 layers': 40 rows 280 / 630, 64 456 / 976, 128 952 / 1917; where 2 rows
+// move, registers for 8 / for 32 34 / 54).
+template <int N, class V>
 QM_DEV void fork_few(const StateForkArgs& A) {
     __shared__ Moves m;
     const int n = __builtin_amdgcn_readfirstlane(find_moves(A, m, 256));
     if (n <= 0) return;
     for (int64_t at = blockIdx.x; at < A.first[A.buffers]; at += gridDim.x) {
         const int k = buffer_of(A, at);
-        const int64_t stride = A.buffer[k].stride, off = (at - A.first[k]) * QMK_STATE_COLUMN + 16 * (int64_t)threadIdx.x;
+        const int64_t stride = A.buffer[k].stride, off = (at - A.first[k]) * (256 * (int)sizeof(V)) + (int)sizeof(V) * (int64_t)threadIdx.x;
         if (off >= A.buffer[k].bytes) continue;
         uint8_t* base = A.buffer[k].rows + off;
-        uintx4 x[N];
+        V x[N];
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (i < n) x[i] = *reinterpret_cast<const uintx4*>(base + (int64_t)__builtin_amdgcn_readfirstlane(m.src[i]) * stride);
+            if (i < n) x[i] = *reinterpret_cast<const V*>(base + (int64_t)__builtin_amdgcn_readfirstlane(m.src[i]) * stride);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (i < n) *reinterpret_cast<uintx4*>(base + (int64_t)__builtin_amdgcn_readfirstlane(m.dst[i]) * stride) = x[i];
+            if (i < n) *reinterpret_cast<V*>(base + (int64_t)__builtin_amdgcn_readfirstlane(m.dst[i]) * stride) = x[i];
     }
 }
-extern "C" __global__ __launch_bounds__(256) void qm_state_fork_8(StateForkArgs A) { fork_few<8>(A); }
-extern "C" __global__ __launch_bounds__(256) void qm_state_fork_32(StateForkArgs A) { fork_few<32>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_state_fork_8(StateForkArgs A) { fork_few<8, uintx4>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_state_fork_32(StateForkArgs A) { fork_few<32, uintx4>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_state_fork_64(StateForkArgs A) { fork_few<64, uintx2>(A); }
+extern "C" __global__ __launch_bounds__(256) void qm_state_fork_128(StateForkArgs A) { fork_few<128, uint32_t>(A); }
 
 // More: in LDS.
 extern "C" __global__ __launch_bounds__(256) void qm_state_fork_many(StateForkArgs A) {

@@ -131,7 +131,7 @@ def run_state_fork(ctx, rows, src, dst, sizes, seed=0, refused=False):
 SIZES = [(16, 16), (4096, 4096), (4112, 8192), (98304, 98304), (49152, 49168)]
 
 
-@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 31, 32, 33, 64, 65, 96, 200])
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 31, 32, 33, 64, 65, 96, 128, 129, 200])
 def test_state_fork(ctx, rows):
     """Parents at random: chains, cycles, rows that stay, several children of one."""
     rng = np.random.default_rng(rows)

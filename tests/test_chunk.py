@@ -119,9 +119,10 @@ def test_a_reserve_covers_the_calls_within_it():
 def test_selections_workspaces_and_the_states_columns():
     got = [int(x) for x in ask(["slices 1 1", "slices 4 1024", "slices 4 1025", "slices 65536 262144"])]
     assert got == [16, 64, 128, 65536 * 256 * 16]
-    for n, got in zip((1, 32, 33, 64, 100, 1024), ask([f"column {n}" for n in (1, 32, 33, 64, 100, 1024)])):
+    for n, got in zip((1, 32, 33, 64, 65, 128, 129, 300, 1024), ask([f"column {n}" for n in (1, 32, 33, 64, 65, 128, 129, 300, 1024)])):
         wide = int(got)
-        assert wide % 16 == 0 and 16 <= wide <= 4096 and (n <= 32 or n * wide <= 65536)
+        assert wide % 16 == 0 and 16 <= wide <= 4096 and (n <= 128 or n * wide <= 65536)
+        assert n > 128 or wide == 256 * (16 if n <= 32 else 8 if n <= 64 else 4)
 
 
 def test_rust_struct_matches_the_header():
