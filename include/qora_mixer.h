@@ -445,8 +445,8 @@ int32_t qm_kv4_append(qm_context* ctx, qm_stream stream, const qm_kv4_cache* cac
  * sigmoid(gate): qm_gqa_prefill's attention, behind any context.  K and V are
  * what the pages stand for, in f16 (a scale whose rounding takes its group past
  * f16's largest value counts as the next lower one); q and the softmax's
- * weights enter the products in f16, sums are f32, as in qm_gqa_prefill.  A token that stands in a group of NaN does so for the
- * queries that see it only.
+ * weights enter the products in f16, sums are f32, as in qm_gqa_prefill.  A
+ * token's group of NaN reaches the queries that see it only.
  * q_gate_dev   bf16 [tokens][16][512]; q_norm_dev f16 [256]
  * out_dev      bf16 [tokens][16][256]; rows of no batch row stay as they were
  * max_new      upper bound of a row's new tokens
@@ -670,8 +670,8 @@ int32_t qm_sample(qm_context* ctx, qm_stream stream, int32_t vocab, float* logit
  * tokens_dev   int32 [groups][take]
  * scores_out_dev  f32 [groups][take]: its worth
  * done_out_dev NULL, or int32 [groups][take]: whether it is at its end
- * Where there are fewer, the rest have parent -1, token -1, score -infinity
- * and done 0.  With take = beams the scores and flags may be written where
+ * Where there are fewer, the rest have parent -1 (which the forks refuse),
+ * token -1, score -infinity and done 0.  With take = beams the scores and flags may be written where
  * they were read.  Pointers need 4-byte alignment.  Uses 16 bytes of the
  * context's workspace per row and 1024 logits (reserved by qm_reserve for
  * groups * beams up to max_batch). */
