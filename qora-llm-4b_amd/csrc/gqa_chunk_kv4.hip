@@ -161,7 +161,19 @@ struct Deal {
     QM_DEV static float many_piece(float pages, float blocks) { return fmaxf(1.0f, __builtin_amdgcn_sqrtf(0.09f * blocks * pages)); }
     QM_DEV static bool many_cut(float pages, float blocks, float k) { return 3.4f * (pages - ceilf(pages / k)) > 0.3f * blocks * k; }
 
-    QM_DEV Deal(const GqaChunkArgs& args, int l) : A(args), lane(l), pieces(false), piece(0.0), cuts(0), total(0.0), each(0.0), incl(0.0), units(0.0) {
+    // sums: what the first one of a workgroup found, null for that one.
+    struct Sums {
+        double total, each;
+    };
+    QM_DEV Deal(const GqaChunkArgs& args, int l, const Sums* sums) : A(args), lane(l), pieces(false), piece(0.0), cuts(0), total(0.0), each(0.0), incl(0.0), units(0.0) {
+        if (sums) {
+            total = sums->total, each = sums->each;
+            if (A.batch > 64) return;
+            mine = chunk_row(A, lane);
+            units = row_units(mine);
+            incl = scan(units);
+            return;
+        }
         mine = chunk_row(A, lane);
         if (!CHUNK_SELDOM(A.batch > 64)) {
             const int nb = blocks(mine);
@@ -199,14 +211,20 @@ struct Deal {
         int block, tiles, number;
         double first;
     };
-    // The row block that unit u (< total) falls into.
-    QM_DEV Item find(double u, bool numbered) const {
+    // Where to look from: the units and blocks of the batch rows before b0.
+    struct Place {
+        int b0, number[2];
+        double past;
+    };
+    // The row block that unit u (< total) falls into, at `from` or behind it.
+    QM_DEV Item find(double u, bool numbered, Place& from) const {
         Item it;
-        double past = 0.0;
-        int number[2] = {0, 0};
+        double past = from.past;
+        int number[2] = {from.number[0], from.number[1]};
         ChunkRow r = mine;
         double n = units, in = incl;
-        for (int b0 = 0;; b0 += 64) {                      // uniform
+        for (int b0 = from.b0;; b0 += 64) {                // uniform
+            from = Place{b0, {number[0], number[1]}, lane_of(past, 0)};
             if (A.batch > 64) {
                 r = chunk_row(A, b0 + lane);
                 n = row_units(r);
@@ -262,12 +280,12 @@ struct Deal {
         tb = __builtin_amdgcn_readfirstlane((int)((uint32_t)it.tiles * (uint32_t)(q + 1) / (uint32_t)n));
         return q < n;
     }
-    // Where workgroup i begins: a multiple of `each`, but whole pages, and none
-    // inside a block of few pages.
-    QM_DEV double begin(int i) const {
+    // Where workgroup i begins (at `from` or behind it): a multiple of `each`, but
+    // whole pages, and none inside a block of few pages.
+    QM_DEV double begin(int i, Place from) const {
         const double u = each * i;
         if (u >= total) return total;
-        const Item it = find(u, false);
+        const Item it = find(u, false, from);
         const int w = weight(it.r);
         int t = (int)((u - it.first) / w);
         if (it.tiles <= whole()) t = 2 * (u - it.first) < (double)it.tiles * w ? 0 : it.tiles;
@@ -1109,13 +1127,16 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
         if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
     }
+    typename Deal<NF>::Sums sums{0.0, 0.0};
+    typename Deal<NF>::Place from{0, {0, 0}, 0.0};
     for (double u = -1.0;;) {                              // uniform, as all of it
-        // (made anew for each block: nothing of it takes registers while one is attended)
-        const Deal<NF> deal(A, chunk_lane(lane));
+        // (made anew for each block: little of it takes registers while one is attended)
+        const Deal<NF> deal(A, chunk_lane(lane), u < 0.0 ? nullptr : &sums);
         double end = 0.0;
         if (CHUNK_SELDOM(!deal.pieces)) {
-            end = deal.begin(index + 1);
-            if (u < 0.0) u = deal.begin(index);
+            sums = typename Deal<NF>::Sums{Deal<NF>::lane_of(deal.total, 0), Deal<NF>::lane_of(deal.each, 0)};
+            end = deal.begin(index + 1, from);
+            if (u < 0.0) u = deal.begin(index, from);
             if (u >= end) return;
         }
         typename Deal<NF>::Item it;
@@ -1126,7 +1147,7 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
             last = index + n - 1;
             u = -1.0;
         } else {
-            it = deal.find(u, true);
+            it = deal.find(u, true, from);
             const int weight = Deal<NF>::weight(it.r);
             ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
             tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
