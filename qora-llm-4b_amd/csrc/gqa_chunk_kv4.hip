@@ -201,7 +201,8 @@ struct Deal {
             incl = scan(units);
             total += lane_of(incl, 63);
         }
-        each = fmax(ceil(total / A.groups), (double)QMK_CHUNK_MIN_UNITS);
+        // (a page of many tokens at least: less, and shares inside a block would be empty)
+        each = fmax(ceil(total / A.groups), (double)max(QMK_CHUNK_MIN_UNITS, QMK_CHUNK_WEIGHT));
     }
 
     // A row block: its row, number among the row's, pages, the units before it,

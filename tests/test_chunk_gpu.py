@@ -411,6 +411,14 @@ def test_chunk_of_many_row_blocks(ctx, seed, rows, lo, hi, top, long):
     run_chunk(ctx, cache_of(lens, layers=1, seed=seed), news, layer=0, seed=seed)
 
 
+@pytest.mark.parametrize("n, new", [(600, 64), (1100, 40), (700, 300)])
+def test_chunk_of_one_longer_row_among_many_of_a_token(ctx, n, new):
+    """An even share that is less than a page of the longer row's blocks: no share of a block is empty, and what an
+    earlier call left in the workspace is not joined."""
+    run_chunk(ctx, cache_of([6001], layers=1, seed=61), [70], layer=0)
+    run_chunk(ctx, cache_of([50] * 69 + [n], layers=1, seed=60), [1] * 69 + [new], layer=0)
+
+
 def test_chunk_of_a_prompt_of_more_blocks_than_workgroups(ctx):
     run_chunk(ctx, cache_of([2200, 2100], layers=1, seed=56), [2200, 2000], layer=0)
 
