@@ -17,9 +17,9 @@
 // the reference moves, and outputs are rescaled, only where a score passes it by
 // CHUNK_SLACK.
 //
-// Two forms, by a row's new tokens, one workgroup of 8 waves a CU in both:
-//   few   (up to 32) blocks of 4 NF tokens x 4 heads, the columns of a 16 x 16 x
-//         32 product.  A wave has half pages of its own, their codes by LDS DMA
+// Two forms, by the call's and a row's new tokens (QMK_CHUNK_FEW, _SHORT), one
+// workgroup of 8 waves a CU in both:
+//   few   blocks of 4 NF tokens x 4 heads, the columns of a 16 x 16 x 32 product.  A wave has half pages of its own, their codes by LDS DMA
 //         two ahead, and makes operands of them in registers; the waves' sums
 //         are joined at the end.  Bound by HBM once there is enough to read: 24
 //         rows of up to 12001 tokens 44 us with the merge, 22 of it while the
@@ -34,8 +34,8 @@
 //         f16 product 1.19), matrix unit 51% busy at the clock that this load
 //         leaves, vector unit 43%; a tile takes 3.3 us, 4.2 with every CU at it.
 //         An operand a wave for itself, as above, would be made eight times over.
-//         64 tokens of 64 take 21 us of it in one workgroup, nearly all of them
-//         the latency of code and data that come once.
+//         A block costs 18 us beside its pages, the latency of code and data that
+//         come once (64 tokens of 64 27 us; few, in eight workgroups, 12).
 //
 // Row blocks are dealt over the workgroups, in pieces where one has too many
 // pages (Deal); pieces leave partial sums, which qm_gqa_chunk_merge joins.
@@ -81,7 +81,7 @@ QM_DEV ChunkRow chunk_row(const GqaChunkArgs& A, int b) {
 }
 
 // NF: operand columns of a row block of few tokens (4 NF tokens of four heads).
-template <int NF>
+template <int NF, bool MANY>
 struct Deal {
     static constexpr int kFew = 4 * NF;
     const GqaChunkArgs& A;
@@ -100,7 +100,7 @@ struct Deal {
     // call is, for then there is no merge (500 tokens whole 14 us without and 17
     // with the merge's launch, cut 14).
     QM_DEV int whole() const { return A.max_len <= QMK_CHUNK_WHOLE * QMK_KV4_PAGE_TOKENS ? QMK_CHUNK_WHOLE : QMK_CHUNK_FEW_PIECE; }
-    QM_DEV static bool few(const ChunkRow& r) { return r.n <= QMK_CHUNK_FEW; }
+    QM_DEV static bool few(const ChunkRow& r) { return !MANY || r.n <= QMK_CHUNK_FEW; }
     QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
     QM_DEV static int blocks(const ChunkRow& r) { return (r.n + tokens(r) - 1) / tokens(r); }
     QM_DEV static int weight(const ChunkRow& r) { return few(r) ? 1 : QMK_CHUNK_WEIGHT; }
@@ -111,17 +111,22 @@ struct Deal {
     }
     QM_DEV static double before(const ChunkRow& r, int j) {
         if (r.kind != CHUNK_RUN) return j;
-        if (!few(r)) {                 // block j, but the row's last, ends 64 j + 63 tokens after the first new one
-            const double first = (r.len - r.n + 63) / QMK_KV4_PAGE_TOKENS + 1;
-            return j * first + (double)j * (j - 1) * 0.5;
-        }
-        int sum = 0;
-        for (int i = 0; i < j; ++i) sum += tiles(r, i);    // a few blocks of at most 2^25 pages
-        return sum;
+        // block i of T tokens, but the row's last, reads page (len - n + T (i + 1) - 1) / 64
+        // and those before it: floor((c + i) / d) of them with d = 64 / T
+        const int d = QMK_KV4_PAGE_TOKENS / tokens(r), c = (r.len - r.n + tokens(r) - 1) / tokens(r);
+        auto sum = [&](int m) {                            // of floor(k / d), k < m
+            const double q = m / d;
+            return 0.5 * q * (q - 1.0) * d + q * (m % d);
+        };
+        return sum(c + j) - sum(c) + j;
     }
+    // What a block costs beside its pages, in units; where block j begins among the
+    // row's units, and its pages.
+    QM_DEV static int entry(const ChunkRow& r) { return few(r) ? QMK_CHUNK_FEW_ENTRY : QMK_CHUNK_MANY_ENTRY; }
+    QM_DEV static double start(const ChunkRow& r, int j) { return weight(r) * before(r, j) + (double)entry(r) * j; }
     QM_DEV static double row_units(const ChunkRow& r) {
         const int nb = blocks(r);
-        return nb ? weight(r) * (before(r, nb - 1) + tiles(r, nb - 1)) : 0.0;
+        return nb ? start(r, nb - 1) + entry(r) + (double)weight(r) * tiles(r, nb - 1) : 0.0;
     }
     template <int CTRL, int ROWS>
     QM_DEV static double step(double x) {
@@ -205,12 +210,12 @@ struct Deal {
         each = fmax(ceil(total / A.groups), (double)max(QMK_CHUNK_MIN_UNITS, QMK_CHUNK_WEIGHT));
     }
 
-    // A row block: its row, number among the row's, pages, the units before it,
-    // and its number among the blocks of few tokens, or of many.
+    // A row block: its row, number among the row's, pages, number among the blocks
+    // of few tokens, or of many, and the units before it and before its pages.
     struct Item {
         ChunkRow r;
         int block, tiles, number;
-        double first;
+        double first, pages;
     };
     // Where to look from: the units and blocks of the batch rows before b0.
     struct Place {
@@ -248,17 +253,17 @@ struct Deal {
             past += all;
         }
         // the last block that begins at or before u
-        const int w = weight(it.r);
         const double rest = u - it.first;
         int lo = 0, hi = blocks(it.r) - 1;
         while (lo < hi) {
             const int mid = lo + (hi - lo + 1) / 2;
-            if (before(it.r, mid) * w <= rest) lo = mid;
+            if (start(it.r, mid) <= rest) lo = mid;
             else hi = mid - 1;
         }
         it.block = __builtin_amdgcn_readfirstlane(lo);
         it.tiles = __builtin_amdgcn_readfirstlane(tiles(it.r, it.block));
-        it.first = lane_of(it.first + before(it.r, it.block) * w, 0);
+        it.first = lane_of(it.first + start(it.r, it.block), 0);
+        it.pages = it.first + entry(it.r);
         it.number = number[few(it.r)] + it.block;
         return it;
     }
@@ -271,7 +276,7 @@ struct Deal {
         const int k = __builtin_amdgcn_readlane(cuts, at), rest = i - __builtin_amdgcn_readlane(in - all, at);
         it.block = __builtin_amdgcn_readfirstlane((int)((uint32_t)rest / (uint32_t)k));
         it.tiles = __builtin_amdgcn_readfirstlane(tiles(it.r, it.block));
-        it.first = 0.0;
+        it.first = it.pages = 0.0;
         const uint32_t same = lane < at && few(mine) == few(it.r) ? (uint32_t)nb : 0u;
         it.number = __builtin_amdgcn_readlane((int)wave_scan(same), 63) + it.block;
         const int q = rest - it.block * k;
@@ -288,9 +293,9 @@ struct Deal {
         if (u >= total) return total;
         const Item it = find(u, false, from);
         const int w = weight(it.r);
-        int t = (int)((u - it.first) / w);
-        if (it.tiles <= whole()) t = 2 * (u - it.first) < (double)it.tiles * w ? 0 : it.tiles;
-        return it.first + (double)t * w;
+        int t = max(0, (int)floor((u - it.pages) / w));
+        if (it.tiles <= whole()) t = 2 * (u - it.pages) < (double)it.tiles * w ? 0 : it.tiles;
+        return t == 0 ? it.first : it.pages + (double)t * w;
     }
 };
 
@@ -749,8 +754,8 @@ QM_DEV void few_half(FewWave<NF>& st, uint8_t* buf, const uint8_t (&q)[NF][8][10
     }
 }
 
-template <int NF>
-QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
+template <int NF, bool MANY>
+QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<NF, MANY>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
     const int c = lane & 15, g = lane >> 4;
     const int i0 = 4 * NF * it.block, first_pos = it.r.len - it.r.n + i0;
     const int end = it.r.len - it.r.n + min(it.r.n, i0 + 4 * NF);             // past the block's last token
@@ -1010,8 +1015,8 @@ QM_DEV floatx4 many_four(const ManyWave& st, int j) {
     return floatx4{st.o[j >> 2][i], st.o[j >> 2][i + 1], st.o[j >> 2][i + 2], st.o[j >> 2][i + 3]};
 }
 
-template <int NF>
-QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<NF>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
+template <int NF, bool MANY>
+QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<NF, MANY>::Item& it, int ta, int tb, int kvh, float* part, int w, int lane) {
     const int c = lane & 31, h = lane >> 5, head = 4 * kvh + (w & 3);
     const int i0 = QMK_CHUNK_TOKENS * it.block + 32 * (w >> 2), i = i0 + c;      // the wave's first row, the lane's
     const int32_t* table = A.c.table + (size_t)it.r.row * A.c.max_pages;
@@ -1122,25 +1127,25 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         int many = 0, few = 0;
         for (int b = lane; b < A.batch; b += 64) {
             const ChunkRow r = chunk_row(A, b);
-            (Deal<NF>::few(r) ? few : many) += Deal<NF>::blocks(r);
+            (Deal<NF, MANY>::few(r) ? few : many) += Deal<NF, MANY>::blocks(r);
         }
         many = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)many), 63);
         few = __builtin_amdgcn_readlane((int)wave_scan((uint32_t)few), 63);
         if (lane == 0) *reinterpret_cast<int2*>(A.counts) = make_int2(many, few);
     }
-    typename Deal<NF>::Sums sums{0.0, 0.0};
-    typename Deal<NF>::Place from{0, {0, 0}, 0.0};
+    typename Deal<NF, MANY>::Sums sums{0.0, 0.0};
+    typename Deal<NF, MANY>::Place from{0, {0, 0}, 0.0};
     for (double u = -1.0;;) {                              // uniform, as all of it
         // (made anew for each block: little of it takes registers while one is attended)
-        const Deal<NF> deal(A, chunk_lane(lane), u < 0.0 ? nullptr : &sums);
+        const Deal<NF, MANY> deal(A, chunk_lane(lane), u < 0.0 ? nullptr : &sums);
         double end = 0.0;
         if (CHUNK_SELDOM(!deal.pieces)) {
-            sums = typename Deal<NF>::Sums{Deal<NF>::lane_of(deal.total, 0), Deal<NF>::lane_of(deal.each, 0)};
+            sums = typename Deal<NF, MANY>::Sums{Deal<NF, MANY>::lane_of(deal.total, 0), Deal<NF, MANY>::lane_of(deal.each, 0)};
             end = deal.begin(index + 1, from);
             if (u < 0.0) u = deal.begin(index, from);
             if (u >= end) return;
         }
-        typename Deal<NF>::Item it;
+        typename Deal<NF, MANY>::Item it;
         int ta, tb, last;                                  // the block's last workgroup
         if (!CHUNK_SELDOM(!deal.pieces)) {
             int n;
@@ -1149,20 +1154,20 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
             u = -1.0;
         } else {
             it = deal.find(u, true, from);
-            const int weight = Deal<NF>::weight(it.r);
-            ta = __builtin_amdgcn_readfirstlane((int)((u - it.first) / weight));
-            tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.first) / weight));
-            last = tb == it.tiles ? index : (int)((it.first + (double)it.tiles * weight - 1.0) / deal.each);
-            u = Deal<NF>::lane_of(it.first + (double)tb * weight, 0);
+            const int weight = Deal<NF, MANY>::weight(it.r);
+            ta = __builtin_amdgcn_readfirstlane(max(0, (int)((u - it.pages) / weight)));
+            tb = __builtin_amdgcn_readfirstlane((int)fmin((double)it.tiles, (end - it.pages) / weight));
+            last = tb == it.tiles ? index : (int)((it.pages + (double)it.tiles * weight - 1.0) / deal.each);
+            u = Deal<NF, MANY>::lane_of(it.pages + (double)tb * weight, 0);
         }
         const bool more = u >= 0.0 && u < end;
-        const bool few = Deal<NF>::few(it.r);
+        const bool few = Deal<NF, MANY>::few(it.r);
         // (ranges that overlap can have more row blocks than there are records)
         if (kvh == 0 && threadIdx.x == 0 && ta == 0 && (MANY || few) && it.number < (few ? A.few : A.many))
             A.records[(few ? A.many : 0) + it.number] = ChunkRecord{index, last, it.r.begin, it.r.n, it.block, {0, 0, 0}};
         if (it.r.kind != CHUNK_RUN) {
             const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;
-            const int i0 = Deal<NF>::tokens(it.r) * it.block, count = min(Deal<NF>::tokens(it.r), it.r.n - i0);
+            const int i0 = Deal<NF, MANY>::tokens(it.r) * it.block, count = min(Deal<NF, MANY>::tokens(it.r), it.r.n - i0);
             uint16_t* out = A.out + (size_t)(it.r.begin + i0) * QM_GQA_HEADS * QM_GQA_HD + (size_t)4 * kvh * QM_GQA_HD + 4 * lane;
             for (int j = w; j < 4 * count; j += CHUNK_WAVES)
                 *reinterpret_cast<uint2*>(out + ((size_t)(j >> 2) * QM_GQA_HEADS + (j & 3)) * QM_GQA_HD) = make_uint2(fill, fill);
@@ -1171,8 +1176,8 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
         }
         // a workgroup's first block may have begun before it, its last end after it
         float* part = A.partial + (size_t)(2 * blockIdx.x + (ta == 0)) * kColumns * QMK_CHUNK_COLUMN;
-        if (MANY && !few) many_item<NF>(A, *reinterpret_cast<ChunkLds*>(sm), it, ta, tb, kvh, part, w, lane);
-        else few_item<NF>(A, *reinterpret_cast<FewLds<NF>*>(sm), it, ta, tb, kvh, part, w, lane);
+        if (MANY && !few) many_item<NF, MANY>(A, *reinterpret_cast<ChunkLds*>(sm), it, ta, tb, kvh, part, w, lane);
+        else few_item<NF, MANY>(A, *reinterpret_cast<FewLds<NF>*>(sm), it, ta, tb, kvh, part, w, lane);
         if (!more) return;
     }
 }

@@ -42,9 +42,19 @@
 // 8 x 32 of 4000 46 / 53; there they grow by 3 a row and block, so no further).
 #define QMK_CHUNK_FEW 32
 #define QMK_CHUNK_TOKENS 64         // others in blocks of so many
+// Up to so many new tokens, and so many times the longest length, a call has
+// blocks of few only, one a workgroup (blocks of many / of few, us: 64 tokens of 64
+// 27 / 12, of 4000 42 / 25, of 32000 73 / 66; 512 of 512 37 / 18, of 4000 69 / 64,
+// of 8000 100 / 111; 4 x 128 of 1000 46 / 27; more blocks than workgroups: 700 of
+// 700 43 / 42, 1500 of 1500 77 / 86).
+#define QMK_CHUNK_SHORT_TOKENS 512
+#define QMK_CHUNK_SHORT (2ll << 20)
 // What a page costs a block of many tokens, against one of few: 3.4 us, and 1.9
-// for the eight half pages of a round.
+// for the four of a round.
 #define QMK_CHUNK_WEIGHT 7
+// And what each block costs beside its pages, in the same (12 and 18 us).
+#define QMK_CHUNK_FEW_ENTRY 20
+#define QMK_CHUNK_MANY_ENTRY 32
 // Pages of a block of few tokens that are worth a workgroup (2 / 3 / 4 / 6, us: 1
 // token of 2000 13.9 / 15.3 / 14.4 / 15.7, of 8000 21.0 / 19.7 / 18.0 / 18.2, 5 of
 // 4000 18.9 / 18.5 / 17.3 / 18.7).

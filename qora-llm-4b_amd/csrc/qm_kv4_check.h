@@ -153,34 +153,38 @@ inline int64_t append_halves(int32_t tokens, int32_t batch) {
     return (static_cast<int64_t>(tokens) + 30ll * batch) / QMK_KV4_HALF_TOKENS + batch;
 }
 // The chunk attention's shape: operand columns of a block of few tokens (4 new
-// tokens each), whether rows can have more than few, the most row blocks of
-// both kinds, workgroups per kv head (one a CU, or fewer where the blocks'
-// pages are fewer) and whether blocks may be split over them.  One column where
-// it has all of a row's new tokens (one / two, us: 1 token of 260 11.7 / 13.9, 4
-// of 4000 14.1 / 16.7, 24 x 4 of 12001 82 / 94).
+// tokens each), whether there are blocks of many, the most row blocks of both
+// kinds, workgroups per kv head (one a CU, or fewer where the blocks' pages are
+// fewer) and whether blocks may be split over them.  One column where it has all
+// of a row's new tokens (one / two, us: 1 token of 260 11.7 / 13.9, 4 of 4000
+// 14.1 / 16.7, 24 x 4 of 12001 82 / 94).
 struct Chunk {
     int32_t columns;
     bool many, split;
     int64_t most_many, most_few, groups;
 };
-inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus) {
+inline Chunk chunk_shape_of(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus, bool many) {
     Chunk c{};
     c.columns = max_new <= 4 ? 1 : 2;
-    c.many = max_new > QMK_CHUNK_FEW;
+    c.many = many;
     // a row of n: ceil(n / tokens of a block) <= n / that + 1, and many is FEW + 1 at least
     const int64_t t = tokens, b = batch, block = 4 * c.columns, with_many = t / (QMK_CHUNK_FEW + 1);
-    c.most_many = c.many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
-    c.most_few = t / block + b < b * (QMK_CHUNK_FEW / block) ? t / block + b : b * (QMK_CHUNK_FEW / block);
+    c.most_many = many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
+    c.most_few = t / block + b;
+    if (many && c.most_few > b * (QMK_CHUNK_FEW / block)) c.most_few = b * (QMK_CHUNK_FEW / block);
     const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
     c.split = c.many || tiles > QMK_CHUNK_WHOLE;
-    // rows that are refused for their new tokens are written in blocks of many
-    const int64_t blocks = c.most_few + t / QMK_CHUNK_TOKENS + with_many;
+    const int64_t blocks = c.most_few + c.most_many;
     const int64_t quarter = cus / 4 > 0 ? cus / 4 : 1, most = quarter < QMK_CHUNK_MAX_GROUPS ? quarter : QMK_CHUNK_MAX_GROUPS;
     const int64_t parts = c.split ? tiles : 1;
     c.groups = blocks >= most || blocks * parts >= most ? most : blocks * parts;
     if (c.groups < 1) c.groups = 1;
     c.split = c.split && c.groups > 1;
     return c;
+}
+inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus) {
+    const bool few = tokens <= QMK_CHUNK_SHORT_TOKENS && static_cast<int64_t>(tokens) * max_len <= QMK_CHUNK_SHORT;
+    return chunk_shape_of(tokens, batch, max_new, max_len, cus, max_new > QMK_CHUNK_FEW && !few);
 }
 inline size_t chunk_partial_bytes(const Chunk& c) {
     const int64_t columns = c.many ? 16 : c.columns;
@@ -192,8 +196,8 @@ inline size_t chunk_ws(const Chunk& c) {
 // A bound of it for up to so many tokens and rows, whatever max_new is.
 inline size_t chunk_reserve_ws(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
     size_t ws = 0;
-    for (int32_t max_new : {4, QMK_CHUNK_FEW, QMK_CHUNK_FEW + 1}) {
-        const size_t one = chunk_ws(chunk_shape(tokens, batch, max_new, max_len, cus));
+    for (int form = 0; form < 3; ++form) {
+        const size_t one = chunk_ws(chunk_shape_of(tokens, batch, form ? QMK_CHUNK_FEW : 4, max_len, cus, form == 2));
         if (one > ws) ws = one;
     }
     return ws;

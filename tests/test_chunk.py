@@ -86,16 +86,16 @@ def test_row_blocks_and_half_pages_stay_within_what_the_host_counts():
         if not any(news):
             news[0] = 1
         tokens, max_new = sum(news) + rng.choice([0, 0, 5]), max(news)
-        shapes.append(f"shape {tokens} {batch} {max_new} 5000 256")
+        shapes.append(f"shape {tokens} {batch} {max_new} {rng.choice([300, 5000, 1 << 20])} 256")
         wants.append((news, max_new))
         firsts = [rng.randrange(1000) for _ in news]
         halves.append(f"halves {tokens} {batch}")
         touched.append(sum((f + n - 1) // 32 - f // 32 + 1 for f, n in zip(firsts, news) if n))
     for (news, max_new), got in zip(wants, ask(shapes)):
         columns, many, split, most_many, most_few, groups, ws = (int(x) for x in got.split())
-        assert columns == (1 if max_new <= 4 else 2) and many == (max_new > 32)
-        assert sum(-(-n // 64) for n in news if n > 32) <= most_many
-        assert sum(-(-n // (4 * columns)) for n in news if n <= 32) <= most_few
+        assert columns == (1 if max_new <= 4 else 2) and (not many or max_new > 32)
+        assert sum(-(-n // 64) for n in news if n > 32 and many) <= most_many
+        assert sum(-(-n // (4 * columns)) for n in news if n <= 32 or not many) <= most_few
         assert 1 <= groups <= 64
         assert ws >= 16 + 32 * (most_many + most_few) + (split and groups * 4 * 2 * (16 if many else columns) * 4128 * 4)
     for want, got in zip(touched, ask(halves)):
