@@ -59,7 +59,7 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 // ---- how the work is dealt --------------------------------------------------
 // A batch row of the call.  A row that has no tokens to read (its slot is
 // outside the table, or empty) or is refused (longer than max_len, more new
-// tokens than max_new or than its length) takes one page's units a block, in
+// tokens than max_new or than its length) is one block of a page's units, in
 // which its outputs, 0 or NaN, are written.
 enum { CHUNK_RUN = 0, CHUNK_NONE = 1, CHUNK_REFUSED = 2 };
 struct ChunkRow {
@@ -102,7 +102,7 @@ struct Deal {
     QM_DEV int whole() const { return A.max_len <= QMK_CHUNK_WHOLE * QMK_KV4_PAGE_TOKENS ? QMK_CHUNK_WHOLE : QMK_CHUNK_FEW_PIECE; }
     QM_DEV static bool few(const ChunkRow& r) { return !MANY || r.n <= QMK_CHUNK_FEW; }
     QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
-    QM_DEV static int blocks(const ChunkRow& r) { return (r.n + tokens(r) - 1) / tokens(r); }
+    QM_DEV static int blocks(const ChunkRow& r) { return r.kind != CHUNK_RUN ? min(r.n, 1) : (r.n + tokens(r) - 1) / tokens(r); }
     QM_DEV static int weight(const ChunkRow& r) { return few(r) ? 1 : QMK_CHUNK_WEIGHT; }
     // Pages that block j reads, and that the blocks before it do.
     QM_DEV static int tiles(const ChunkRow& r, int j) {
@@ -1167,9 +1167,8 @@ QM_DEV void chunk_attention(const GqaChunkArgs& A) {
             A.records[(few ? A.many : 0) + it.number] = ChunkRecord{index, last, it.r.begin, it.r.n, it.block, {0, 0, 0}};
         if (it.r.kind != CHUNK_RUN) {
             const uint32_t fill = it.r.kind == CHUNK_NONE ? 0u : 0x7fc07fc0u;
-            const int i0 = Deal<NF, MANY>::tokens(it.r) * it.block, count = min(Deal<NF, MANY>::tokens(it.r), it.r.n - i0);
-            uint16_t* out = A.out + (size_t)(it.r.begin + i0) * QM_GQA_HEADS * QM_GQA_HD + (size_t)4 * kvh * QM_GQA_HD + 4 * lane;
-            for (int j = w; j < 4 * count; j += CHUNK_WAVES)
+            uint16_t* out = A.out + (size_t)it.r.begin * QM_GQA_HEADS * QM_GQA_HD + (size_t)4 * kvh * QM_GQA_HD + 4 * lane;
+            for (int j = w; j < 4 * it.r.n; j += CHUNK_WAVES)
                 *reinterpret_cast<uint2*>(out + ((size_t)(j >> 2) * QM_GQA_HEADS + (j & 3)) * QM_GQA_HD) = make_uint2(fill, fill);
             if (!more) return;
             continue;

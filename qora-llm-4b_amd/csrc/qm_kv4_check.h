@@ -167,11 +167,12 @@ inline Chunk chunk_shape_of(int32_t tokens, int32_t batch, int32_t max_new, int3
     Chunk c{};
     c.columns = max_new <= 4 ? 1 : 2;
     c.many = many;
-    // a row of n: ceil(n / tokens of a block) <= n / that + 1, and many is FEW + 1 at least
+    // a row of n: ceil(n / tokens of a block) <= n / that + 1, and many is FEW + 1 at least;
+    // one that is refused, whatever its n, is one block
     const int64_t t = tokens, b = batch, block = 4 * c.columns, with_many = t / (QMK_CHUNK_FEW + 1);
+    const int64_t row = ((many ? QMK_CHUNK_FEW : max_new) + block - 1) / block;
     c.most_many = many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
-    c.most_few = t / block + b;
-    if (many && c.most_few > b * (QMK_CHUNK_FEW / block)) c.most_few = b * (QMK_CHUNK_FEW / block);
+    c.most_few = t / block + b < b * row ? t / block + b : b * row;
     const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
     c.split = c.many || tiles > QMK_CHUNK_WHOLE;
     const int64_t blocks = c.most_few + c.most_many;
@@ -197,7 +198,7 @@ inline size_t chunk_ws(const Chunk& c) {
 inline size_t chunk_reserve_ws(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
     size_t ws = 0;
     for (int form = 0; form < 3; ++form) {
-        const size_t one = chunk_ws(chunk_shape_of(tokens, batch, form ? QMK_CHUNK_FEW : 4, max_len, cus, form == 2));
+        const size_t one = chunk_ws(chunk_shape_of(tokens, batch, form ? INT32_MAX : 4, max_len, cus, form == 2));
         if (one > ws) ws = one;
     }
     return ws;

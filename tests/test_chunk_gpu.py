@@ -411,6 +411,14 @@ def test_chunk_of_many_row_blocks(ctx, seed, rows, lo, hi, top, long):
     run_chunk(ctx, cache_of(lens, layers=1, seed=seed), news, layer=0, seed=seed)
 
 
+@pytest.mark.parametrize("news, max_new", [([300, 3, 2, 40], 3), ([300, 30, 2, 40], 32), ([900, 130, 2, 700], 200), ([900, 130, 2, 700], 131)])
+def test_chunk_refused_rows_beside_long_ones(ctx, news, max_new):
+    """Refused and idle rows of any number of tokens: theirs are NaN and 0, the others' shares are joined as ever."""
+    ref = cache_of([1000, 5000, 3000, 800], layers=1, seed=62)
+    run_chunk(ctx, ref, news, layer=0, max_new=max_new)
+    run_chunk(ctx, ref, news, layer=0, max_new=max_new, slots=[-1, 1, 2, 7])
+
+
 @pytest.mark.parametrize("n, new", [(600, 64), (1100, 40), (700, 300)])
 def test_chunk_of_one_longer_row_among_many_of_a_token(ctx, n, new):
     """An even share that is less than a page of the longer row's blocks: no share of a block is empty, and what an
