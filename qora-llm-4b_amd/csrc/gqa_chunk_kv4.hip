@@ -993,7 +993,7 @@ QM_DEV void many_half(ManyWave& st, ChunkLds& sh, int buf, int half, int k0, boo
                      if ((i & 3) == 1) part.word(sh, buf ^ 1, i >> 2, w, lane);
                  });
     const uintx4 nan = *reinterpret_cast<const uintx4*>(sh.nan[buf][half]);
-    if (CHUNK_SELDOM(__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3])))) {
+    if (__builtin_amdgcn_readfirstlane((int)(nan[0] | nan[1] | nan[2] | nan[3]))) {
         const int seen = st.pos - k0;                      // the last of the half's tokens that the row sees
         const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1;
 #pragma unroll
