@@ -96,10 +96,14 @@ struct Deal {
     double total, each;
     double incl, units;
 
-    // Pages that a block of few tokens is not cut below: more where no block of the
-    // call is, for then there is no merge (500 tokens whole 14 us without and 17
-    // with the merge's launch, cut 14).
-    QM_DEV int whole() const { return A.max_len <= QMK_CHUNK_WHOLE * QMK_KV4_PAGE_TOKENS ? QMK_CHUNK_WHOLE : QMK_CHUNK_FEW_PIECE; }
+    // Short rows' calls have no merge, and no block is cut (few tokens, 500 of them
+    // cached: whole 14 us without a merge and 17 with its launch, cut 14; many
+    // tokens: 12 x 60 of 291 whole without 39, cut where it pays 43, 9 x 64 of 512,
+    // 8 pages, 49 and 40).
+    static constexpr int kShort = MANY ? QMK_CHUNK_MANY_WHOLE : QMK_CHUNK_WHOLE;
+    QM_DEV bool split() const { return A.max_len > kShort * QMK_KV4_PAGE_TOKENS; }
+    // Pages below which a block of few tokens is not cut, where others are.
+    QM_DEV int whole() const { return split() ? QMK_CHUNK_FEW_PIECE : kShort; }
     QM_DEV static bool few(const ChunkRow& r) { return !MANY || r.n <= QMK_CHUNK_FEW; }
     QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
     QM_DEV static int blocks(const ChunkRow& r) { return r.kind != CHUNK_RUN ? min(r.n, 1) : (r.n + tokens(r) - 1) / tokens(r); }
@@ -193,7 +197,8 @@ struct Deal {
                 piece = lane_of(scan(nb * most), 63) / A.groups;
                 for (;;) {
                     cuts = nb ? cuts_of(most, fmax(piece, least)) : 0;
-                    if (few(mine) ? last <= whole() : !many_cut((float)last, (float)all, (float)cuts)) cuts = min(cuts, 1);
+                    if (last <= whole() && (few(mine) || !split())) cuts = min(cuts, 1);
+                    else if (!few(mine) && !many_cut((float)last, (float)all, (float)cuts)) cuts = min(cuts, 1);
                     if (__builtin_amdgcn_readlane((int)wave_scan((uint32_t)(nb * cuts)), 63) <= A.groups) break;
                     piece = fmax(piece, 1.0) * 1.125;
                 }

@@ -60,7 +60,9 @@
 // 4000 18.9 / 18.5 / 17.3 / 18.7).
 #define QMK_CHUNK_FEW_PIECE 4
 #define QMK_CHUNK_MIN_UNITS 4       // the same where workgroups have runs of several blocks
-#define QMK_CHUNK_WHOLE 8           // lengths of up to so many pages: no block of few tokens is cut
+// Lengths of up to so many pages: no block is cut, and there is no merge.
+#define QMK_CHUNK_WHOLE 8
+#define QMK_CHUNK_MANY_WHOLE 6      // where there are blocks of many tokens
 #define QMK_CHUNK_MAX_GROUPS 64     // workgroups per kv head
 #define QMK_CHUNK_COLUMN 4128       // f32 of 16 rows' partial sums: [16][256], m[16], l[16] (32 rows: twice each)
 

@@ -174,7 +174,7 @@ inline Chunk chunk_shape_of(int32_t tokens, int32_t batch, int32_t max_new, int3
     c.most_many = many ? t / QMK_CHUNK_TOKENS + (b < with_many ? b : with_many) : 0;
     c.most_few = t / block + b < b * row ? t / block + b : b * row;
     const int64_t tiles = (static_cast<int64_t>(max_len) + QMK_KV4_PAGE_TOKENS - 1) / QMK_KV4_PAGE_TOKENS;
-    c.split = c.many || tiles > QMK_CHUNK_WHOLE;
+    c.split = tiles > (many ? QMK_CHUNK_MANY_WHOLE : QMK_CHUNK_WHOLE);
     const int64_t blocks = c.most_few + c.most_many;
     const int64_t quarter = cus / 4 > 0 ? cus / 4 : 1, most = quarter < QMK_CHUNK_MAX_GROUPS ? quarter : QMK_CHUNK_MAX_GROUPS;
     const int64_t parts = c.split ? tiles : 1;

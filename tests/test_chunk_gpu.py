@@ -405,7 +405,11 @@ def many_rows(seed, rows, lo, hi, top, long=()):
     (52, 100, 1, 130, 40, [(64, 6000, 100), (99, 3000, 1)]),             # more rows than lanes
     (53, 70, 20, 200, 20, [(3, 4000, 32)]),                              # few tokens, two operand columns
     (54, 100, 1, 100, 4, [(0, 5000, 4), (71, 2000, 3)]),                 # few tokens, one
-    (55, 3, 60, 70, 60, [(0, 4200, 500), (2, 9000, 33)])])               # few blocks, cut unevenly
+    (55, 3, 60, 70, 60, [(0, 4200, 500), (2, 9000, 33)]),                # few blocks, cut unevenly
+    (56, 14, 150, 290, 150, []),                                         # blocks of many tokens, none cut
+    (57, 9, 400, 512, 250, []),                                          # and where they are
+    (58, 8, 33, 64, 64, []),                                             # a call of blocks of few only
+    (59, 2, 300, 400, 60, [(0, 4000, 440)])])
 def test_chunk_of_many_row_blocks(ctx, seed, rows, lo, hi, top, long):
     lens, news = many_rows(seed, rows, lo, hi, top, long)
     run_chunk(ctx, cache_of(lens, layers=1, seed=seed), news, layer=0, seed=seed)
