@@ -831,36 +831,31 @@ QM_DEV void few_item(const GqaChunkArgs& A, FewLds<NF>& sh, const typename Deal<
         float* mine = reinterpret_cast<float*>(sh.ring[w][0]);
 #pragma unroll
         for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<floatx4*>(mine + 256 * dt + 4 * ((c ^ (g + 4 * (dt & 1))) + 16 * g)) = st.o[f][dt];
-        if (lane < 16) {
-            mine[4096 + lane] = st.sum[f].m;
-            mine[4112 + lane] = l;
-        }
+        if (lane < 16) *reinterpret_cast<float2*>(mine + 4096 + 2 * lane) = make_float2(st.sum[f].m, l);
         // (LDS only: no wave waits for another's stores)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (row_of(f, j) >= it.r.n) continue;          // uniform
             const int col = 2 * w + j;
-            float m[CHUNK_WAVES], l[CHUNK_WAVES];
+            // lane k, and every eighth from it: wave k's reference and sum
+            const float2 ml = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(sh.ring[lane & 7][0]) + 4096 + 2 * col);
             floatx4 part_o[CHUNK_WAVES];
 #pragma unroll
-            for (int k = 0; k < CHUNK_WAVES; ++k) {
-                const float* a = reinterpret_cast<const float*>(sh.ring[k][0]);
-                m[k] = a[4096 + col];
-                l[k] = a[4112 + col];
-                // dims 4 lane ..: group lane >> 2, entry of the column and lane & 3
-                part_o[k] = *reinterpret_cast<const floatx4*>(a + 256 * (lane >> 2) + 4 * ((col ^ ((lane & 3) + (lane & 4))) + 16 * (lane & 3)));
-            }
-            float M = m[0], L = 0.0f;
-#pragma unroll
-            for (int k = 1; k < CHUNK_WAVES; ++k) M = fmaxf(M, m[k]);
+            for (int k = 0; k < CHUNK_WAVES; ++k)          // dims 4 lane ..: group lane >> 2, entry of the column and lane & 3
+                part_o[k] = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(sh.ring[k][0]) + 256 * (lane >> 2) +
+                                                              4 * ((col ^ ((lane & 3) + (lane & 4))) + 16 * (lane & 3)));
+            float M = fmaxf(ml.x, dpp_f32<0xB1>(ml.x));
+            M = fmaxf(M, dpp_f32<0x4E>(M));
+            M = fmaxf(M, dpp_f32<0x141>(M));
+            const float e = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            float L = ml.y * e;
+            L += dpp_f32<0xB1>(L);
+            L += dpp_f32<0x4E>(L);
+            L += dpp_f32<0x141>(L);
             floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < CHUNK_WAVES; ++k) {
-                const float e = m[k] == M ? 1.0f : __builtin_amdgcn_exp2f(m[k] - M);
-                L = fmaf(l[k], e, L);
-                o += part_o[k] * e;
-            }
+            for (int k = 0; k < CHUNK_WAVES; ++k) o += part_o[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), k));
             if (whole) {
                 *reinterpret_cast<uint2*>(A.out + at_of(f, j) * QM_GQA_HD + 4 * lane) = chunk_gated(o * chunk_inverse(L), gate[f][j]);
             } else {
@@ -893,8 +888,9 @@ QM_DEV int many_token(int i, int h) { return 16 * ((i >> 2) & 1) + 8 * (i >> 3) 
 
 // A product's 16 operand reads, CHUNK_AHEAD ahead of their use, so that LDS's
 // latency passes under the matrix instructions before.  The order is pinned:
-// the compiler's own had none ahead, where registers are short.
-#define CHUNK_AHEAD 3
+// the compiler's own had none ahead, where registers are short.  (Three ahead are
+// no faster, and may cost a spill in the loop: 2048 tokens of 32768 1072 / 1039.)
+#define CHUNK_AHEAD 2
 template <class Read, class Use>
 QM_DEV void many_product(Read read, Use use) {
     half8 a[CHUNK_AHEAD + 1];
