@@ -102,7 +102,7 @@ struct Deal {
     // 8 pages, 49 and 40).
     static constexpr int kShort = MANY ? QMK_CHUNK_MANY_WHOLE : QMK_CHUNK_WHOLE;
     QM_DEV bool split() const { return A.max_len > kShort * QMK_KV4_PAGE_TOKENS; }
-    // Pages below which a block of few tokens is not cut, where others are.
+    // Pages up to which a block of few tokens is not cut, where others are.
     QM_DEV int whole() const { return split() ? QMK_CHUNK_FEW_PIECE : kShort; }
     QM_DEV static bool few(const ChunkRow& r) { return !MANY || r.n <= QMK_CHUNK_FEW; }
     QM_DEV static int tokens(const ChunkRow& r) { return few(r) ? kFew : QMK_CHUNK_TOKENS; }
@@ -212,7 +212,7 @@ struct Deal {
             total += lane_of(incl, 63);
         }
         // (a page of many tokens at least: less, and shares inside a block would be empty)
-        each = fmax(ceil(total / A.groups), (double)max(QMK_CHUNK_MIN_UNITS, QMK_CHUNK_WEIGHT));
+        each = fmax(ceil(total / A.groups), (double)QMK_CHUNK_WEIGHT);
     }
 
     // A row block: its row, number among the row's, pages, number among the blocks

@@ -59,7 +59,6 @@
 // token of 2000 13.9 / 15.3 / 14.4 / 15.7, of 8000 21.0 / 19.7 / 18.0 / 18.2, 5 of
 // 4000 18.9 / 18.5 / 17.3 / 18.7).
 #define QMK_CHUNK_FEW_PIECE 4
-#define QMK_CHUNK_MIN_UNITS 4       // the same where workgroups have runs of several blocks
 // Lengths of up to so many pages: no block is cut, and there is no merge.
 #define QMK_CHUNK_WHOLE 8
 #define QMK_CHUNK_MANY_WHOLE 6      // where there are blocks of many tokens
