@@ -104,6 +104,28 @@ def test_select_of_scores_that_outweigh_the_logits(ctx):
     run_select(ctx, 1, 2, 20, logits, np.array([-1.0, -2e30]))
 
 
+def test_select_of_logits_past_4_gib(ctx):
+    """4480 rows of the largest vocabulary, all but the last request's without a score."""
+    groups, beams, vocab = 70, 64, 262144
+    rng = np.random.default_rng(8)
+    logits = rng.standard_normal((beams, vocab)).astype(np.float32)
+    scores = np.full(groups * beams, -np.inf, np.float32)
+    scores[-beams:] = -np.abs(rng.standard_normal(beams))
+    x = ctx.alloc(groups * beams * vocab * 4)
+    try:
+        ctx.upload_to(x.offset((groups - 1) * beams * vocab * 4), logits)
+        parents, tokens, out = (ctx.upload(np.full(groups * 5, -9, np.int32)) for _ in range(3))
+        ctx.beam_select(groups, beams, 5, vocab, x, ctx.upload(scores), None, -1, parents, tokens, out, None)
+        want = CR.select(1, beams, 5, vocab, logits, scores[-beams:], None, -1)
+        got = [ctx.download(b, (groups, 5), t) for b, t in ((parents, np.int32), (tokens, np.int32), (out, np.float32))]
+        assert np.array_equal(got[0][-1], want[0] + (groups - 1) * beams) and np.array_equal(got[1][-1], want[1])
+        assert (np.abs(got[2][-1] - want[2]) <= 2.0 ** -24 * np.abs(want[2]) + 2.0 ** -19).all()
+        assert (got[0][:-1] == -1).all() and (got[1][:-1] == -1).all() and (got[2][:-1] == -np.inf).all()
+    finally:
+        ctx.sync()
+        x.close()
+
+
 def test_select_in_place(ctx):
     rng, logits, scores = some(5, 3, 4, 2500)
     done = np.array([0, 1, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1], np.int32)
@@ -149,6 +171,23 @@ def test_state_fork_of_listed_rows(ctx):
 
 def test_state_fork_of_many_buffers(ctx):
     run_state_fork(ctx, 5, [4, 4, 0, 3, 1], None, [(16 * (i + 1), 16 * (i + 2)) for i in range(64)])
+
+
+def test_state_fork_of_rows_past_4_gib(ctx):
+    stride, size = 2 ** 31 + 4096, 8208
+    rng = np.random.default_rng(9)
+    rows = rng.integers(0, 256, (3, size), dtype=np.uint8)
+    buf = ctx.alloc(2 * stride + size)
+    try:
+        for r in range(3):
+            ctx.upload_to(buf.offset(r * stride), rows[r])
+        res = ints(ctx, [-77])
+        ctx.state_fork([(buf, size, stride)], 3, 3, ints(ctx, [2, 0, 1]), None, res)
+        assert result(ctx, res) == 0
+        assert np.array_equal([ctx.download(buf.offset(r * stride), (size,), np.uint8) for r in range(3)], rows[[2, 0, 1]])
+    finally:
+        ctx.sync()
+        buf.close()
 
 
 @pytest.mark.parametrize("src, dst", [([0, 5], [1, 2]), ([0, -1], [1, 2]), ([0, 1], [5, 2]), ([0, 1], [2, 2]), ([0, 1], [-1, 2]),

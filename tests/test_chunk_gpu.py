@@ -483,3 +483,35 @@ def test_two_graphs_share_the_workspace(new):
     for g in graphs:
         g.close()
     own.close()
+
+
+def test_pages_past_4_gib(ctx):
+    """A pool of 4.5 GB, the row's pages at its end: what is appended and attended is as in a small one."""
+    small = cache_of([700], layers=1, seed=63)
+    pages, base = small.pages.shape[1], 61000 - small.pages.shape[1]
+    c = M.Kv4Cache(ctx, 1, 61000, 1, small.table.shape[1])
+    try:
+        at = c.pages.offset(base * R.PAGE)
+        assert at - c.pages.ptr > 2 ** 32
+        refs = np.zeros(61000, np.int32)
+        refs[base:] = small.refs
+        ctx.upload_to(at, small.pages)
+        for buf, arr in ((c.table, np.where(small.table >= 0, small.table + base, -1).astype(np.int32)), (c.lens, small.lens), (c.refs, refs)):
+            ctx.upload(arr, buf)
+        rng = np.random.default_rng(64)
+        cos, sin = rope(700)
+        rc, rs = ctx.upload(cos), ctx.upload(sin)
+        for new in (3, 20, 600):
+            k, v = (CR.bf16(rng.standard_normal((new, 4, 256))) for _ in range(2))
+            q, gamma = queries(rng, new)
+            norm, begins, out = ctx.upload(gamma.view(np.uint16)), ints(ctx, [0, new]), ctx.alloc(new * 8192)
+            print(f"case: 4 GiB new={new}", flush=True)
+            ctx.kv4_append(c, 0, 1, None, begins, new, ctx.upload(k), ctx.upload(v), norm, rc, rs, len(cos), 700, None, dtype=M.QM_BF16)
+            ctx.gqa_chunk_kv4(c, 0, 1, None, begins, new, new, ctx.upload(q), norm, rc, rs, len(cos), 700, None, out)
+            CR.append(small, 0, 1, None, [0, new], new, CR.bf16_value(k), CR.bf16_value(v), gamma, cos, sin, 700)
+            assert np.array_equal(ctx.download(at, small.pages.shape, np.uint8), small.pages)
+            want, bound, _ = CR.attend(small, 0, 1, None, [0, new], new, new, CR.bf16_value(q), gamma, cos, sin, 700)
+            assert_near(CR.bf16_value(ctx.download(out, (new, 16, 256), np.uint16)), want, bound)
+    finally:
+        ctx.sync()
+        c.pages.close()
