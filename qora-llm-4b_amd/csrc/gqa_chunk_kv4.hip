@@ -655,15 +655,14 @@ QM_DEV uint4 chunk_gated8(floatx4 a, floatx4 b, uint4 gate) {
 QM_DEV float chunk_inverse(float l) { return l != 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f; }      // 0: nothing to see
 
 // ---- few tokens ------------------------------------------------------------------
-// A row of up to QMK_CHUNK_FEW new tokens: blocks of 4 NF of them, an operand
-// column 4 tokens of the four heads.  Every wave has all columns and every
+// Blocks of 4 NF tokens, an operand column 4 of them of the four heads.  Every wave has all columns and every
 // eighth half page, whose codes come by LDS DMA, two ahead, and become operands
 // in its registers; the waves' sums are joined at the end.
 // The queries stand in LDS as operands, block 8 f + s: entry l the 16 bytes that
 // lane l = (c, g) reads, dims 32 s + 8 g .. of column 16 f + c.
 template <int NF>
 struct FewLds {
-    // later of each wave o [dim group][lane][4] f32, then m[16], l[16]
+    // later of each wave o [dim group][entry][4] f32, then (m, l)[16]
     __attribute__((aligned(1024))) uint8_t ring[CHUNK_WAVES][2][QMK_KV4_HALF_BYTES];
     __attribute__((aligned(1024))) uint8_t q[NF][8][1024];
 };
@@ -1115,8 +1114,8 @@ QM_DEV void many_item(const GqaChunkArgs& A, ChunkLds& sh, const typename Deal<N
     asm volatile("s_barrier" ::: "memory");                // before the next block's tiles
 }
 
-// MANY: rows of more than QMK_CHUNK_FEW tokens as well (max_new says whether
-// there can be any).
+// MANY: rows of more than QMK_CHUNK_FEW tokens are in blocks of many (otherwise
+// the call has none of those, or is a short one).
 template <int NF, bool MANY>
 QM_DEV void chunk_attention(const GqaChunkArgs& A) {
     constexpr int kColumns = MANY ? 2 * CHUNK_WAVES : NF;
