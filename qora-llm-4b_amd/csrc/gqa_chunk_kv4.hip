@@ -6,8 +6,8 @@
 // pos = len - n + i.  With q its RMSNorm'd, rotated query (gemv.rs:586-627),
 //   out = sigmoid(gate) sum_t p_t V_t / sum_t p_t,  p_t = exp(q . K_t / 16),
 // over the cached tokens t <= pos, K and V as the cache keeps them: lo + s c,
-// rounded to f16 once.  q, p (relative to a running maximum, in base 2) and
-// the operands are f16, all sums f32.
+// rounded to f16 once.  q, p (in base 2, counted from CHUNK_HEAD below a running
+// maximum) and the operands are f16, all sums f32.
 //
 // Both products run transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane's
 // scores, its running maximum and its outputs are all of one row, and its
@@ -15,7 +15,7 @@
 // products nothing changes lanes.  The scores come out counted from the row's
 // reference (the product begins at its negative), so that a weight is one exp2;
 // the reference moves, and outputs are rescaled, only where a score passes it by
-// CHUNK_SLACK.
+// CHUNK_HEAD + CHUNK_SLACK.
 //
 // Two forms, by the call's and a row's new tokens (QMK_CHUNK_FEW, _SHORT), one
 // workgroup of 8 waves a CU in both:
@@ -48,8 +48,13 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 #define CHUNK_WAVES 8
-// A row's reference moves only where a score passes it by this (log2 units):
-// weights up to 2^8 are exact enough in f16, and outputs are seldom rescaled.
+// A row's reference is its largest score less CHUNK_HEAD (log2 units), and moves
+// only where a score passes that by CHUNK_SLACK more, so that outputs are seldom
+// rescaled.  Weights are thus up to 2^15 (f16's largest is 65504), and a key's
+// is 2^-11 of itself off down to 2^-21 of the largest, and 2^-32 of that below
+// (6000 keys 18 nats below one whose V is 0: outputs off by 0.2%, bf16's own
+// rounding; with weights of 1 at most by 15%).
+#define CHUNK_HEAD 7.0f
 #define CHUNK_SLACK 8.0f
 // What is seldom true stands away from the code that each workgroup runs: code
 // comes from memory once a launch, and a short call waits for little else (700
@@ -521,10 +526,11 @@ QM_DEV float chunk_base(const ChunkSum& s) { return s.m == -INFINITY ? 0.0f : s.
 // returned: what its scores drop by, and the factor of its sums.
 QM_DEV float chunk_raise(ChunkSum& s, float mx, float& corr) {
     const bool first = s.m == -INFINITY;                   // sums there may be only of NaN scores
-    const float up = first ? (mx == -INFINITY ? 0.0f : mx) : mx >= CHUNK_SLACK ? mx : 0.0f;
+    const float to = mx - CHUNK_HEAD;
+    const float up = first ? (mx == -INFINITY ? 0.0f : to) : mx >= CHUNK_HEAD + CHUNK_SLACK ? to : 0.0f;
     corr = first ? 1.0f : __builtin_amdgcn_exp2f(-up);
-    s.m = first ? mx : s.m + up;
-    s.due = s.m == -INFINITY ? (int)0x80000000 : __float_as_int(CHUNK_SLACK);
+    s.m = first ? to : s.m + up;
+    s.due = s.m == -INFINITY ? (int)0x80000000 : __float_as_int(CHUNK_HEAD + CHUNK_SLACK);
     s.l *= corr;
     return up;
 }
