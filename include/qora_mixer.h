@@ -670,9 +670,13 @@ int32_t qm_sample(qm_context* ctx, qm_stream stream, int32_t vocab, float* logit
  * tokens_dev   int32 [groups][take]
  * scores_out_dev  f32 [groups][take]: its worth
  * done_out_dev NULL, or int32 [groups][take]: whether it is at its end
- * Where there are fewer, the rest have parent -1 (which the forks refuse),
- * token -1, score -infinity and done 0.  With take = beams the scores and flags may be written where
- * they were read.  Pointers need 4-byte alignment.  Uses 16 bytes of the
+ * Where there are fewer, the rest have token -1, score -infinity and done 0.
+ * Their parent is, with take = beams, the row in whose place they stand: the
+ * forks leave it as it is and move the other requests' rows, and with its score
+ * it takes no part in the steps that follow.  Otherwise it is -1, which the
+ * forks refuse (the whole list, every request's).  With take = beams the scores
+ * and flags may be written where they were read.  Pointers need 4-byte
+ * alignment.  Uses 16 bytes of the
  * context's workspace per row and 1024 logits (reserved by qm_reserve for
  * groups * beams up to max_batch). */
 int32_t qm_beam_select(qm_context* ctx, qm_stream stream, int32_t groups, int32_t beams,

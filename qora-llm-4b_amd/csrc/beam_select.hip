@@ -313,7 +313,10 @@ extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs
     }
     if (tid < A.take) {
         const size_t to = (size_t)blockIdx.x * A.take + tid;
-        int parent = -1, token = -1, over = 0;
+        // A place that no continuation takes: where the places are the request's
+        // rows, it stays the row that it is, so that parents is a list for the
+        // forks whatever the requests have.
+        int parent = A.take == A.beams ? row0 + tid : -1, token = -1, over = 0;
         float score = -INFINITY;
         if (tid < found) {
             const BeamKey k = sh.sorted[tid];

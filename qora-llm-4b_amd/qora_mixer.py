@@ -483,7 +483,8 @@ class Context:
     def beam_select(self, groups, beams, take, vocab, logits, scores, done, end_id, parents, tokens, scores_out,
                     done_out=None):
         """The take best continuations of each request's beams sequences by scores + log-softmax(logits): parent rows,
-        tokens, summed scores and whether they are at their end ([groups][take] each)."""
+        tokens, summed scores and whether they are at their end ([groups][take] each).  A place without one: token -1,
+        score -inf, and its own row as parent where take is beams (the forks leave that row), else -1."""
         self._check(self.lib.qm_beam_select(
             self.h, self.stream, groups, beams, take, vocab, _addr(logits), _addr(scores), _addr(done), end_id, _addr(parents),
             _addr(tokens), _addr(scores_out), _addr(done_out)))

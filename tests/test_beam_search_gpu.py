@@ -123,3 +123,67 @@ def test_beam_search(captured):
     if captured:
         graph.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_request_that_runs_short_leaves_the_others_alone(captured):
+    """Four requests: one as ever, one without a sequence (no score is finite), one whose logits hold a NaN from some
+    step on, one whose mask leaves a single token.  Their places without a continuation stay the rows that they are,
+    and the forks move the others' rows and states."""
+    groups, rows, vocab, state_bytes = 4, 12, 700, 208
+    rng = np.random.default_rng(80)
+    ctx = M.Context(0)
+    ctx.reserve(rows, 256)
+    ref = R.Cache(1, 60, rows, 4, seed=81)
+    assert ref.resize(None, [70, 70, 70, 1, 1, 1, 64, 64, 64, 130, 130, 130]) == 0
+    c = upload(ctx, ref)
+    scores = np.where(np.arange(rows) % BEAMS == 0, 0, -np.inf).astype(np.float32)
+    scores[3:6] = -np.inf
+    done = np.zeros(rows, np.int32)
+    state = rng.integers(0, 2 ** 32, (rows, state_bytes // 4), dtype=np.uint32)
+    x, s, d, st = ctx.alloc(rows * vocab * 4), ctx.upload(scores), ctx.upload(done), ctx.upload(state)
+    parents, tokens, res = ctx.alloc(4 * rows), ctx.alloc(4 * rows), [ints(ctx, [-77]) for _ in range(3)]
+    identity, add = ints(ctx, list(range(rows))), ints(ctx, [1] * rows)
+
+    def step():
+        ctx.beam_select(groups, BEAMS, BEAMS, vocab, x, s, d, END, parents, tokens, s, d)
+        ctx.kv4_fork(c, rows, parents, identity, res[0])
+        ctx.state_fork([(st, state_bytes, state_bytes)], rows, rows, parents, None, res[1])
+        ctx.kv4_resize(c, rows, None, add, res[2], M.QM_KV4_ADD)
+
+    if captured:
+        ctx.graph_begin()
+        step()
+        graph = ctx.graph_end()
+    moved = short = 0
+    for i in range(8):
+        print(f"case: requests that run short, step {i}", flush=True)
+        logits = (2 * rng.standard_normal((rows, vocab))).astype(np.float32)
+        if i >= 3:
+            logits[6 + i % 2, 11] = np.nan
+        logits[9:, np.arange(vocab) != 5] = -np.inf
+        if i == 5:
+            logits[6:9] = np.nan
+        ctx.upload(logits, x)
+        if captured and i != 4:
+            graph.launch()
+        else:
+            step()
+        want = CR.select(groups, BEAMS, BEAMS, vocab, logits, scores, done, END)
+        none = want[0] < 0
+        source = np.where(none, np.arange(rows), want[0])
+        got = [ctx.download(b, (rows,), t) for b, t in ((parents, np.int32), (tokens, np.int32), (s, np.float32), (d, np.int32))]
+        assert np.array_equal(got[0], source) and np.array_equal(got[1], want[1]) and np.array_equal(got[3], want[3])
+        assert (got[2][none] == -np.inf).all() and np.isfinite(got[2][~none]).all()
+        scores, done = got[2], got[3]
+        assert [result(ctx, r) for r in res] == [0, 0, 0]
+        assert ref.fork(source, list(range(rows))) == 0 and ref.resize(None, [1] * rows, add=True) == 0
+        state = state[source]
+        assert np.array_equal(ctx.download(st, state.shape, np.uint32), state)
+        assert_same(ctx, c, ref)
+        moved += int((source[:3] != np.arange(3)).sum())
+        short += int(none.sum())
+    assert moved and short > 8 * 3 and ref.consistent()
+    if captured:
+        graph.close()
+    ctx.close()
