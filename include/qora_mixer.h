@@ -420,8 +420,9 @@ int32_t qm_gqa_decode_kv4(qm_context* ctx, qm_stream stream, const qm_kv4_cache*
  * qm_kv4_append writes their keys and values into a layer's pages: k RMSNorm'd
  * (1 + gamma, eps 1e-6) and rotated, in 64 bits, rounded to f32 and f16 as
  * qm_gqa_decode_kv4's new row is, v rounded to f16, both in 4 bits.  Nothing is
- * written of a batch row whose slot is outside the table or an earlier batch
- * row's, or that has more new tokens than its length or a length over max_len;
+ * written of a batch row whose slot is outside the table or that of an earlier
+ * batch row with new tokens (one without may name any), or that has more new
+ * tokens than its length or a length over max_len;
  * nor to pages that other rows hold too, or by refs none, or that are none of
  * the pool.
  * dtype        of k_dev and v_dev: QM_F32 or QM_BF16 [tokens][4][256]

@@ -248,10 +248,11 @@ QM_DEV bool append_at(const Kv4AppendArgs& A, int index, int lane, AppendAt& at)
             at.first = at.len - __builtin_amdgcn_readlane(n, from);
             at.begin = __builtin_amdgcn_readlane(begin, from);
             at.t0 = ((at.first >> 5) + index - before - __builtin_amdgcn_readlane(incl - halves, from)) << 5;
-            if (A.slots)                                // a table row that an earlier batch row has: left out
+            if (A.slots)                                // a table row that an earlier batch row with tokens has: left out
                 for (int j0 = 0; j0 < b0 + from; j0 += 64) {
-                    const int j = j0 + lane;
-                    if (__ballot(j < b0 + from && A.slots[min(j, b0 + from - 1)] == at.row)) return false;
+                    const int j = j0 + lane, k = min(j, b0 + from - 1);
+                    const int begin = A.begins[k], end = A.begins[k + 1];
+                    if (__ballot(j < b0 + from && A.slots[k] == at.row && begin >= 0 && end > begin && end <= A.tokens)) return false;
                 }
             return true;
         }
