@@ -655,8 +655,8 @@ int32_t qm_sample(qm_context* ctx, qm_stream stream, int32_t vocab, float* logit
 
 /* The `take` best continuations of each request, best first.  Continuation t
  * of a sequence is worth its score + logits[t] - log(sum exp logits), the
- * summed log-probability, compared in 64 bits (the log-sum is good to about
- * 2^-23); of equal ones the lower sequence and then the lower token is first.
+ * summed log-probability, compared in 64 bits (the log-sum is good to
+ * 2^-19); of equal ones the lower sequence and then the lower token is first.
  * A sequence at its end (done not 0) has one continuation: end_id, worth its
  * score.  One whose score is not finite takes no part, nor one whose logits
  * hold a NaN or +infinity or nothing but -infinity; a logit of -infinity is no

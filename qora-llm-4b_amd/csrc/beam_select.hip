@@ -13,8 +13,11 @@
 // The slices are bound by HBM: 87 rows of 248320 logits in 15 us, 5.8 TB/s.  The
 // draw is one workgroup's chain of loads and barriers, 11 us for 12 requests of
 // 8 rows and 7 for one of 4: log-sums 2, the leaders 3, the rest their logits.
-// Values are compared in 64 bits (the log-sum is f64 of f32 sums: off by some
-// 2^-24), ties to the lower row and then the lower token.
+// Values are compared in 64 bits, ties to the lower row and then the lower token.
+// The log-sum is off by 22 2^-24 at most: an exponential by 2 (v_exp_f32) and, of
+// a logit d below its slice's largest, by d for the difference's rounding, d for
+// its product's with log2(e) and d / 4 for that constant's own; weighted as the
+// terms are d is ln 1024 at most; and a lane's sum by 4.
 #include "qm_device.h"
 #include "qm_beam.h"
 
@@ -47,11 +50,18 @@ extern "C" __global__ __launch_bounds__(256) void qm_beam_slices(BeamArgs A) {
         if (have) token = t0 - lane + 64 * i + __builtin_ctzll(have);
     }
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;                                      // NaN where a logit is, or an infinity
+    // The sum: NaN where a logit is, or an infinity.  By halves, four roundings of
+    // f32 and not 16, and then in 64 bits (the log-sum of many equal logits is off
+    // by 3.6 2^-24, in order and in f32 by 14).
+    float e[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += exp_fast(v[i] - base);
-    sum = wave_sum64(sum);
-    if (lane == 0) A.slices[at] = BeamSlice{top, sum, token, 0};
+    for (int i = 0; i < 16; ++i) e[i] = exp_fast(v[i] - base);
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+#pragma unroll
+        for (int i = 0; i < d; ++i) e[i] += e[i + d];
+    const double sum = wave_sum64((double)e[0]);
+    if (lane == 0) A.slices[at] = BeamSlice{sum, top, token};
 }
 
 // ---- the request's choice ------------------------------------------------------
@@ -241,7 +251,7 @@ extern "C" __global__ __launch_bounds__(BEAM_THREADS) void qm_beam_draw(BeamArgs
             double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < QMK_BEAM_VOCAB / QMK_BEAM_SLICE / 64; ++i)
-                if (lane + 64 * i < A.ns && x[i].sum != 0.0f) sum += (double)x[i].sum * exp((double)(x[i].top == -INFINITY ? 0.0f : x[i].top) - (double)top);
+                if (lane + 64 * i < A.ns && x[i].sum != 0.0) sum += x[i].sum * exp((double)(x[i].top == -INFINITY ? 0.0f : x[i].top) - (double)top);
             sum = wave_sum64(sum);
             base = (double)score - ((double)top + log(sum));           // NaN, infinite: takes no part
         }

@@ -15,9 +15,9 @@
 // A slice's largest logit, the lowest token that has it, and the sum of
 // exp(logit - largest).
 struct BeamSlice {
-    float top, sum;
+    double sum;
+    float top;
     int32_t token;
-    int32_t pad;
 };
 struct BeamArgs {
     const float* logits;     // [groups * beams][vocab]

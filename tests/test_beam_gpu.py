@@ -132,6 +132,31 @@ def test_select_in_place(ctx):
     run_select(ctx, 3, 4, 4, logits, scores, done, end_id=3, in_place=True)
 
 
+def test_select_log_sums_of_many_equal_logits(ctx):
+    """A token in every 1024 leads equal ones d below: what a term and a sum are off by does not average out.
+
+    In units of 2^-24: an exponential is off by 2 (1 ulp of 2^t), by d of the difference's rounding, d of its product's
+    and d / 4 of log2(e)'s; equal terms, summed by halves, by nothing more, the sum of the leader's lane by 4; the rest is
+    64 bits.  Scores about as large as the log-sums, so that the results are small and their own rounding, half a step,
+    is next to nothing."""
+    rng = np.random.default_rng(10)
+    top = np.concatenate([np.zeros(9), np.round(rng.uniform(-30, 30, 40), 1), [0.1, -1.4, 1.7, 2.2, 0, 1e4]]).astype(np.float32)
+    rest = top - np.concatenate([[0.01, 0.018, 0.053, 0.078, 0.107, 0.15, 0.173, 0.371, 0.6], rng.uniform(0, 9, 40),
+                                 [8.8, 8.8, 7.5, 7.5, 8, 7]]).astype(np.float32)
+    logits = np.repeat(rest[:, None], 262144, 1)
+    logits[:, ::1024] = top[:, None]
+    d = top.astype(np.float64) - rest
+    sums = np.log(256 + (262144 - 256) * np.exp(-d))
+    scores = sums.astype(np.float32)
+    got = run_select(ctx, len(top), 1, 1, logits, scores)
+    want = scores.astype(np.float64) - sums
+    off = np.abs(got[2] - want) * 2 ** 24
+    w, lane = 1023 * np.exp(-d) / (1 + 1023 * np.exp(-d)), (1 + 15 * np.exp(-d)) / (1 + 1023 * np.exp(-d))
+    room = w * (2 + 2.25 * d) + 4 * lane + np.abs(want)
+    print("largest, in 2^-24:", off.max(), "of the room:", (off / room).max())
+    assert (off <= room).all()
+
+
 # ---- states --------------------------------------------------------------------------------------
 def run_state_fork(ctx, rows, src, dst, sizes, seed=0, refused=False):
     """sizes: (row bytes, stride) of each buffer; everything beside the rows has to stay."""
