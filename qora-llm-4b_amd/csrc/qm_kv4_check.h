@@ -183,9 +183,14 @@ inline Chunk chunk_shape_of(int32_t tokens, int32_t batch, int32_t max_new, int3
     c.split = c.split && c.groups > 1;
     return c;
 }
-inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus) {
+// Whether a call has blocks of many tokens; max_new may be a loose bound, and no
+// row has more new tokens than the call.
+inline bool chunk_many(int32_t tokens, int32_t max_new, int32_t max_len) {
     const bool few = tokens <= QMK_CHUNK_SHORT_TOKENS && static_cast<int64_t>(tokens) * max_len <= QMK_CHUNK_SHORT;
-    return chunk_shape_of(tokens, batch, max_new, max_len, cus, max_new > QMK_CHUNK_FEW && !few);
+    return max_new > QMK_CHUNK_FEW && tokens > QMK_CHUNK_FEW && !few;
+}
+inline Chunk chunk_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int cus) {
+    return chunk_shape_of(tokens, batch, max_new < tokens ? max_new : tokens, max_len, cus, chunk_many(tokens, max_new, max_len));
 }
 inline size_t chunk_partial_bytes(const Chunk& c) {
     const int64_t columns = c.many ? 16 : c.columns;
@@ -194,11 +199,13 @@ inline size_t chunk_partial_bytes(const Chunk& c) {
 inline size_t chunk_ws(const Chunk& c) {
     return chunk_partial_bytes(c) + 16 + static_cast<size_t>(c.most_many + c.most_few) * sizeof(ChunkRecord);
 }
-// A bound of it for up to so many tokens and rows, whatever max_new is.
+// A bound of it for up to so many tokens, rows and lengths, whatever max_new is.
+// Where the largest such call has no blocks of many tokens, no other has.
 inline size_t chunk_reserve_ws(int32_t tokens, int32_t batch, int32_t max_len, int cus) {
     size_t ws = 0;
-    for (int form = 0; form < 3; ++form) {
-        const size_t one = chunk_ws(chunk_shape_of(tokens, batch, form ? INT32_MAX : 4, max_len, cus, form == 2));
+    const int forms = chunk_many(tokens, tokens, max_len) ? 3 : tokens > 4 ? 2 : 1;
+    for (int form = 0; form < forms; ++form) {
+        const size_t one = chunk_ws(chunk_shape_of(tokens, batch, form ? tokens : 4, max_len, cus, form == 2));
         if (one > ws) ws = one;
     }
     return ws;

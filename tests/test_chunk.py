@@ -116,6 +116,24 @@ def test_a_reserve_covers_the_calls_within_it():
                 assert int(got.split()[-1]) <= reserve, line
 
 
+def test_a_loose_bound_of_a_rows_new_tokens_is_the_calls():
+    """No row has more new tokens than the call: max_new past that picks no other kernel and no larger workspace."""
+    for tokens, batch, max_len in [(1, 1, 100), (3, 2, 20000), (4, 1, 5000), (5, 1, 5000), (20, 4, 300000), (32, 1, 1 << 20), (33, 2, 1 << 20), (700, 3, 9000)]:
+        tight, *loose = ask([f"shape {tokens} {batch} {m} {max_len} 256" for m in (tokens, tokens + 1, 64, 4096, 2147483647) if m >= tokens])
+        assert all(x == tight for x in loose), (tokens, tight, loose)
+
+
+def test_a_reserve_for_few_tokens_takes_no_more_than_they_need():
+    """Blocks of many tokens leave 135 MB of partial sums; a reserve whose calls have none does not ask for them."""
+    of = {k: int(x) for k, x in zip([(1, 32768), (4, 1 << 20), (16, 32768), (32, 1 << 20), (33, 32768), (512, 4096), (513, 4096), (33, 65536)], ask(
+        ["reserve 1 1 32768 256", "reserve 4 1 1048576 256", "reserve 16 1 32768 256", "reserve 32 1 1048576 256", "reserve 33 1 32768 256",
+         "reserve 512 1 4096 256", "reserve 513 1 4096 256", "reserve 33 1 65536 256"]))}
+    column = 64 * 4 * 2 * 4128 * 4
+    for key, columns in {(1, 32768): 1, (4, 1 << 20): 1, (16, 32768): 2, (32, 1 << 20): 2, (33, 32768): 2, (512, 4096): 2}.items():
+        assert of[key] <= columns * column + 16 + 32 * 600, key
+    assert of[513, 4096] >= 16 * column and of[33, 65536] >= 16 * column
+
+
 def test_selections_workspaces_and_the_states_columns():
     got = [int(x) for x in ask(["slices 1 1", "slices 4 1024", "slices 4 1025", "slices 65536 262144"])]
     assert got == [16, 64, 128, 65536 * 256 * 16]

@@ -215,6 +215,13 @@ def test_chunk_slots(ctx):
     run_chunk(ctx, ref, None, slots=[3, -1, 1, 3, 0, 7], begins=[2, 22, 25, 30, 95, 100, 103], tokens=110)
 
 
+@pytest.mark.parametrize("lens, news", [([900], [1]), ([900, 70], [2, 2]), ([1500, 600], [20, 5]), ([3000, 64], [32, 1]), ([1200], [33])])
+def test_chunk_with_a_loose_bound_of_the_rows_new_tokens(ctx, lens, news):
+    """A bound past the call's tokens, as a captured call has it: the same bits as with the least that is true."""
+    ref = cache_of(lens, layers=1, seed=sum(lens))
+    assert np.array_equal(run_chunk(ctx, ref, news, layer=0, max_new=4096), run_chunk(ctx, ref, news, layer=0, max_new=sum(news)))
+
+
 def test_chunk_refused_rows(ctx):
     """More new tokens than max_new or than the length, a length over max_len: NaN; ranges that are none: nothing."""
     ref = cache_of([10, 90, 20, 30, 60], seed=22)
