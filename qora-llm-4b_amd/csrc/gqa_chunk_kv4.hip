@@ -153,11 +153,7 @@ struct Deal {
         x = step<0x142, 0xA>(x);
         return step<0x143, 0xC>(x);
     }
-    QM_DEV static double lane_of(double x, int lane) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, x);
-        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
-        return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-    }
+    QM_DEV static double lane_of(double x, int lane) { return readlane_f64(x, lane); }
     QM_DEV static ChunkRow lane_of(const ChunkRow& r, int lane) {
         return ChunkRow{__builtin_amdgcn_readlane(r.row, lane), __builtin_amdgcn_readlane(r.len, lane),
                         __builtin_amdgcn_readlane(r.n, lane), __builtin_amdgcn_readlane(r.begin, lane),

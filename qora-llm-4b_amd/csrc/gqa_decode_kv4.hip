@@ -169,20 +169,6 @@ QM_DEV bool deal_split(const GqaKv4Args& A, Deal& d, int k, bool note, int lane)
     return found;
 }
 
-QM_DEV double readlane_f64(double x, int lane) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-// Sum over the wave in 64 bits.
-QM_DEV double wave_sum64_f64(double x) {
-    x += dpp_f64<0xB1>(x);
-    x += dpp_f64<0x4E>(x);
-    x += dpp_f64<0x141>(x);
-    x += dpp_f64<0x140>(x);
-    return (readlane_f64(x, 0) + readlane_f64(x, 16)) + (readlane_f64(x, 32) + readlane_f64(x, 48));
-}
-
 // A head's row, lane l with dims 4 l .. 4 l + 3: RMSNorm (1 + gamma, eps
 // 1e-6), and the rotation of dims 0..63 (gemv.rs:586-627).  Apart, so that the
 // norm is done by the time the RoPE rows arrive.
@@ -204,7 +190,7 @@ QM_DEV void rotate_head(float (&x)[4], const float (&c)[4], const float (&s)[4],
 // on the order of a sum.
 QM_DEV void norm_new_k(double (&x)[4], uint2 gw) {
     const uint16_t g[4] = {(uint16_t)(gw.x & 0xffffu), (uint16_t)(gw.x >> 16), (uint16_t)(gw.y & 0xffffu), (uint16_t)(gw.y >> 16)};
-    const double mean = wave_sum64_f64((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) * (1.0 / QM_GQA_HD) + 1e-6;
+    const double mean = wave_sum64((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) * (1.0 / QM_GQA_HD) + 1e-6;
     const double inv = inverse_root_f64(mean);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (1.0 + (double)f16_to_f32(g[i]));

@@ -71,19 +71,17 @@ QM_DEV double dpp_f64(double x) {
     const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+QM_DEV double readlane_f64(double x, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 QM_DEV double wave_sum64(double x) {
     x += dpp_f64<0xB1>(x);
     x += dpp_f64<0x4E>(x);
     x += dpp_f64<0x141>(x);
     x += dpp_f64<0x140>(x);
-    uint64_t u = __builtin_bit_cast(uint64_t, x);
-    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
-    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
-    x = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
-    u = __builtin_bit_cast(uint64_t, x);
-    lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
-    hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
-    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+    return (readlane_f64(x, 0) + readlane_f64(x, 16)) + (readlane_f64(x, 32) + readlane_f64(x, 48));
 }
 
 // ---- f16 / bf16 ----------------------------------------------------------
