@@ -30,7 +30,7 @@
 //         DMA, each wave makes f16 operands of an eighth of them, which all
 //         waves read, in between the second product's matrix instructions of the
 //         tile before; a barrier a tile.  Bound by the matrix unit and what
-//         issues beside it: 2048 tokens of 32768 1039 us, 1.02 PFLOP/s (a large
+//         issues beside it: 2048 tokens of 32768 1075 us, 0.99 PFLOP/s (a large
 //         f16 product 1.19), matrix unit 51% busy at the clock that this load
 //         leaves, vector unit 43%; a tile takes 3.3 us, 4.2 with every CU at it.
 //         An operand a wave for itself, as above, would be made eight times over.

@@ -217,9 +217,9 @@ extern "C" __global__ __launch_bounds__(KV4_STORE_THREADS) void qm_kv4_store(Kv4
 // half a wave (32 lanes x 8 dims).  A workgroup takes half a page of one batch
 // row and head, as a store does; the half pages that the rows touch are dealt
 // in list order.  Bound by the vector unit, busy 88% of the time that a CU
-// works: 14113 tokens of 5 rows, bf16, 34 us (the bytes alone would be 15).  108
-// registers, so two workgroups a CU; with 201 and one 59 us.  One token 8.8 us:
-// the chain slots -> length -> table -> page, and the code.
+// works: 14113 tokens of 5 rows, bf16, 32 to 34 us, f32 34 (the bytes alone 15
+// and 27).  108 registers, so two workgroups a CU; with 201 and one 59 us.  One
+// token 8.8 us: the chain slots -> length -> table -> page, and the code.
 struct AppendAt {
     int row, first, len, begin;          // table row, its first new token's position, length, packed row
     int t0;                              // token 0 of the half page
